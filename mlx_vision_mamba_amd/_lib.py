@@ -89,6 +89,35 @@ class GemmDesc(ctypes.Structure):
     ]
 
 
+class SeqDesc(ctypes.Structure):
+    """Mirror of ``mvm_seq_desc`` (include/mvm_seq.h)."""
+
+    _fields_ = [
+        ("tokens", _i64), ("nseq", _i64), ("seqlen", _i64), ("dim", _i64), ("state_rows", _i64),
+        ("offsets", _vp), ("slots", _vp), ("fresh", _vp),
+    ]
+
+
+class SeqScanDesc(ctypes.Structure):
+    """Mirror of ``mvm_seq_scan_desc`` (include/mvm_seq.h)."""
+
+    _fields_ = [
+        ("seq", SeqDesc), ("dstate", _i64),
+        ("u_stride", _i64), ("delta_stride", _i64), ("bc_stride", _i64), ("y_stride", _i64), ("z_stride", _i64),
+        ("max_len", _i64), ("dtype", _i32), ("delta_dtype", _i32), ("delta_softplus", _i32), ("a_is_log", _i32),
+        ("chunk_len", _i32), ("reserved", _i32),
+    ]
+
+
+class SeqConvDesc(ctypes.Structure):
+    """Mirror of ``mvm_seq_conv_desc`` (include/mvm_seq.h)."""
+
+    _fields_ = [
+        ("seq", SeqDesc), ("kwidth", _i64), ("x_stride", _i64), ("y_stride", _i64),
+        ("dtype", _i32), ("reserved", _i32),
+    ]
+
+
 class AdamwTensor(ctypes.Structure):
     """Mirror of ``mvm_adamw_tensor`` (include/mvm_optim.h)."""
 
@@ -146,6 +175,21 @@ GEMM_SIGNATURES = {
     "mvm_gemm_f32": (ctypes.c_int, [ctypes.POINTER(GemmDesc)] + [_vp] * 5 + [ctypes.c_size_t, _vp]),
 }
 
+# symbol -> (restype, argtypes) of include/mvm_seq.h
+SEQ_SIGNATURES = {
+    "mvm_seq_scan_validate": (ctypes.c_int, [ctypes.POINTER(SeqScanDesc)]),
+    "mvm_seq_scan_ckpt_elems": (_i64, [ctypes.POINTER(SeqScanDesc)]),
+    "mvm_seq_scan_workspace_bytes": (_i64, [ctypes.POINTER(SeqScanDesc), ctypes.c_int]),
+    "mvm_seq_scan_fwd": (ctypes.c_int, [ctypes.POINTER(SeqScanDesc)] + [_vp] * 13 + [ctypes.c_size_t, _vp]),
+    "mvm_seq_scan_bwd": (ctypes.c_int, [ctypes.POINTER(SeqScanDesc)] + [_vp] * 21 + [ctypes.c_size_t, _vp]),
+    "mvm_seq_scan_step": (ctypes.c_int, [ctypes.POINTER(SeqScanDesc)] + [_vp] * 11),
+    "mvm_seq_conv_validate": (ctypes.c_int, [ctypes.POINTER(SeqConvDesc)]),
+    "mvm_seq_conv_workspace_bytes": (_i64, [ctypes.POINTER(SeqConvDesc)]),
+    "mvm_seq_conv_fwd": (ctypes.c_int, [ctypes.POINTER(SeqConvDesc)] + [_vp] * 7),
+    "mvm_seq_conv_bwd": (ctypes.c_int, [ctypes.POINTER(SeqConvDesc)] + [_vp] * 11 + [ctypes.c_size_t, _vp]),
+    "mvm_seq_conv_step": (ctypes.c_int, [ctypes.POINTER(SeqConvDesc)] + [_vp] * 6),
+}
+
 _lib = None
 
 
@@ -166,7 +210,7 @@ def lib():
                 f"{LIB_PATH} is missing: build it with `python -m mlx_vision_mamba_amd.build` "
                 "(the HIP extension is required; there is no CPU fallback)")
         handle = ctypes.CDLL(LIB_PATH)
-        for name, (res, args) in {**SIGNATURES, **GEMM_SIGNATURES}.items():
+        for name, (res, args) in {**SIGNATURES, **GEMM_SIGNATURES, **SEQ_SIGNATURES}.items():
             fn = getattr(handle, name)
             fn.restype = res
             fn.argtypes = args

@@ -26,12 +26,14 @@
 #include "mvm_testing.h"
 #include "scan_common.h"
 #include "scan_kernels.h"
+#include "status.h"
 
 namespace {
-
 thread_local char g_err[512] = "";
+}  // namespace
 
-int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+namespace mvm {
+
 int fail(int code, const char* fmt, ...) {
   va_list ap;
   va_start(ap, fmt);
@@ -44,6 +46,19 @@ int ok() {
   g_err[0] = '\0';
   return MVM_OK;
 }
+
+int hip_status(hipError_t e, const char* what) {
+  if (e != hipSuccess) return fail(MVM_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
+  return ok();
+}
+
+}  // namespace mvm
+
+namespace {
+
+using mvm::fail;
+using mvm::hip_status;
+using mvm::ok;
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -217,11 +232,6 @@ BwdWs bwd_ws(const mvm::Geom& g, bool recompute_ckpt) {
   }
   w.total = w.agg_mu + w.agg_s + w.part_dA + w.part_dD + w.part_bc + w.ckpt + w.fwd;
   return w;
-}
-
-int hip_status(hipError_t e, const char* what) {
-  if (e != hipSuccess) return fail(MVM_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
-  return ok();
 }
 
 }  // namespace

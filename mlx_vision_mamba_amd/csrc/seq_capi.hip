@@ -1,0 +1,341 @@
+// C ABI of the packed and served forms (include/mvm_seq.h): validation, the
+// cut into time chunks, and the split of the caller's workspace.
+#include <algorithm>
+
+#include "mvm_conv.h"
+#include "mvm_scan.h"
+#include "mvm_seq.h"
+#include "seq_kernels.h"
+#include "status.h"
+
+namespace {
+
+using mvm::fail;
+using mvm::hip_status;
+using mvm::ok;
+
+// positions are int32, and formed up to a chunk's tile past the last
+constexpr int64_t kMaxTokens = INT32_MAX - 64;
+constexpr int64_t kMaxBlocks = INT32_MAX;
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+constexpr size_t kAlign = 256;
+size_t align_up(size_t x) { return (x + kAlign - 1) / kAlign * kAlign; }
+
+int check_seq(const mvm_seq_desc& q) {
+  if (q.tokens < 0 || q.nseq < 0 || q.seqlen < 0 || q.dim < 0 || q.state_rows < 0)
+    return fail(MVM_ERR_INVALID_ARG, "negative size (tokens=%lld nseq=%lld seqlen=%lld dim=%lld state_rows=%lld)",
+                (long long)q.tokens, (long long)q.nseq, (long long)q.seqlen, (long long)q.dim,
+                (long long)q.state_rows);
+  if (q.tokens > kMaxTokens || q.nseq > kMaxTokens || q.state_rows > kMaxTokens || q.dim > kMaxTokens)
+    return fail(MVM_ERR_UNSUPPORTED, "tokens, nseq, dim and state_rows must be at most %lld", (long long)kMaxTokens);
+  // (seqlen <= tokens where there are sequences, so the product cannot overflow)
+  if (q.offsets == nullptr && (q.nseq > 0 ? q.seqlen > q.tokens || q.nseq * q.seqlen != q.tokens : q.tokens != 0))
+    return fail(MVM_ERR_INVALID_ARG, "without offsets tokens=%lld must be nseq=%lld * seqlen=%lld",
+                (long long)q.tokens, (long long)q.nseq, (long long)q.seqlen);
+  if (q.slots == nullptr && q.state_rows < q.nseq)
+    return fail(MVM_ERR_INVALID_ARG, "state_rows=%lld < nseq=%lld without slots", (long long)q.state_rows,
+                (long long)q.nseq);
+  return MVM_OK;
+}
+
+int check_rows(const char* name, int64_t stride, int64_t tokens, int64_t cols, bool written) {
+  if (stride < 0 || (written && tokens > 1 && stride < cols))
+    return fail(MVM_ERR_INVALID_ARG, "%s=%lld: rows of %lld values %s", name, (long long)stride, (long long)cols,
+                written ? "must not overlap" : "need a stride >= 0");
+  return MVM_OK;
+}
+
+int check_scan(const mvm_seq_scan_desc* d) {
+  if (d == nullptr) return fail(MVM_ERR_INVALID_ARG, "desc is NULL");
+  int rc = check_seq(d->seq);
+  if (rc != MVM_OK) return rc;
+  if (d->dstate < 1 || d->dstate > MVM_MAX_DSTATE)
+    return fail(MVM_ERR_UNSUPPORTED, "dstate=%lld unsupported (1..%d)", (long long)d->dstate, MVM_MAX_DSTATE);
+  if (d->dtype != MVM_F32 && d->dtype != MVM_BF16)
+    return fail(MVM_ERR_UNSUPPORTED, "dtype=%d unsupported", d->dtype);
+  if (d->delta_dtype != MVM_F32 && d->delta_dtype != d->dtype)
+    return fail(MVM_ERR_UNSUPPORTED, "delta_dtype=%d must be MVM_F32 or dtype", d->delta_dtype);
+  if (d->reserved != 0) return fail(MVM_ERR_INVALID_ARG, "reserved must be 0");
+  if (d->max_len < 0) return fail(MVM_ERR_INVALID_ARG, "max_len=%lld is negative", (long long)d->max_len);
+  if (d->chunk_len != 0 && (d->chunk_len < 16 || (d->chunk_len & (d->chunk_len - 1)) != 0))
+    return fail(MVM_ERR_INVALID_ARG, "chunk_len=%d must be 0 or a power of two >= 16", d->chunk_len);
+  const int64_t t = d->seq.tokens, c = d->seq.dim;
+  if ((rc = check_rows("u_stride", d->u_stride, t, c, false)) || (rc = check_rows("delta_stride", d->delta_stride, t, c, false)) ||
+      (rc = check_rows("bc_stride", d->bc_stride, t, d->dstate, false)) ||
+      (rc = check_rows("z_stride", d->z_stride, t, c, false)) || (rc = check_rows("y_stride", d->y_stride, t, c, true)))
+    return rc;
+  const int64_t ncb = ceil_div(c, 64);
+  if (ncb * std::max((t >> 4) + d->seq.nseq + 1, d->seq.nseq) > kMaxBlocks)
+    return fail(MVM_ERR_UNSUPPORTED, "tokens=%lld, nseq=%lld and dim=%lld are too many for one launch", (long long)t,
+                (long long)d->seq.nseq, (long long)c);
+  return MVM_OK;
+}
+
+mvm::SeqGeom seq_geom(const mvm_seq_desc& q) {
+  mvm::SeqGeom g;
+  g.T = static_cast<int32_t>(q.tokens);
+  g.S = static_cast<int32_t>(q.nseq);
+  g.M = static_cast<int32_t>(q.state_rows);
+  g.L = static_cast<int32_t>(q.seqlen);
+  g.D = q.dim;
+  g.off = q.offsets;
+  g.slots = q.slots;
+  g.fresh = q.fresh;
+  return g;
+}
+
+int log2_ceil(int64_t n) {
+  int k = 0;
+  while ((int64_t{1} << k) < n) ++k;
+  return k;
+}
+
+// The cut into time chunks, a power of two long.  A pass over chunks repeats
+// the recurrence for their end states, so sequences stay whole when they fill
+// the card by themselves; else they are cut until the main pass has `waves`
+// waves of 64 channels, four (backward: two) on each of the 1024 SIMDs.
+void pick_chunk(const mvm_seq_scan_desc* d, int64_t waves, mvm::SeqScanGeom& g) {
+  const int64_t T = d->seq.tokens, ncb = std::max<int64_t>(1, ceil_div(d->seq.dim, 64));
+  int64_t longest = d->seq.offsets == nullptr ? d->seq.seqlen : T;
+  if (d->max_len > 0) longest = std::min(longest, d->max_len);
+  int64_t len = d->chunk_len;
+  if (len == 0) {
+    len = 16;
+    while (len < longest && ceil_div(T, len * 2) * ncb >= waves) len *= 2;
+  }
+  g.multi = len < longest;
+  // Whole sequences: one chunk whatever max_len says
+  g.shift = g.multi ? log2_ceil(len) : std::max(4, log2_ceil(T + 1));
+}
+
+mvm::SeqScanGeom scan_geom(const mvm_seq_scan_desc* d, bool backward) {
+  mvm::SeqScanGeom g;
+  g.q = seq_geom(d->seq);
+  g.us = d->u_stride;
+  g.ds = d->delta_stride;
+  g.bs = d->bc_stride;
+  g.ys = d->y_stride;
+  g.zs = d->z_stride;
+  g.N = static_cast<int32_t>(d->dstate);
+  g.a_log = d->a_is_log != 0;
+  g.softplus = d->delta_softplus != 0;
+  pick_chunk(d, backward ? 2048 : 4096, g);
+  return g;
+}
+
+int64_t ckpt_elems(const mvm_seq_scan_desc* d) {
+  return ((d->seq.tokens >> mvm::kSeqTileShift) + d->seq.nseq + 1) * d->seq.dim * 16;
+}
+
+struct ScanWs {
+  size_t agg_h = 0, agg_s = 0, bc = 0, part = 0, part_bc = 0, total = 0;
+};
+ScanWs scan_ws(const mvm_seq_scan_desc* d, const mvm::SeqScanGeom& g, bool backward) {
+  ScanWs w;
+  const size_t slots = static_cast<size_t>(mvm::chunk_slots(g.q, g.shift)), D = static_cast<size_t>(g.q.D);
+  const size_t T = static_cast<size_t>(g.q.T);
+  if (g.multi) {
+    w.agg_h = align_up(slots * D * 16 * sizeof(float));
+    w.agg_s = align_up(slots * D * sizeof(float));
+  }
+  if (d->dtype != MVM_F32 || d->dstate != 16) w.bc = align_up(T * 32 * sizeof(float));
+  if (backward) {
+    w.part = align_up(slots * D * 18 * sizeof(float));
+    w.part_bc = align_up(static_cast<size_t>(ceil_div(g.q.D, 64)) * T * 32 * sizeof(float));
+  }
+  w.total = w.agg_h + w.agg_s + w.bc + w.part + w.part_bc;
+  return w;
+}
+
+struct Take {
+  char* at;
+  float* operator()(size_t n) {
+    float* p = n > 0 ? reinterpret_cast<float*>(at) : nullptr;
+    at += n;
+    return p;
+  }
+};
+
+int check_ws(const char* what, const void* ws, size_t have, size_t need) {
+  if (need > 0 && (ws == nullptr || have < need))
+    return fail(MVM_ERR_WORKSPACE, "%s: workspace %zu bytes < %zu needed", what, have, need);
+  return MVM_OK;
+}
+
+// Operands that are read wherever there are tokens.
+bool missing(const mvm::SeqScanIn& in) { return !in.u || !in.delta || !in.A || !in.Bm || !in.Cm || !in.Dv; }
+
+int check_conv(const mvm_seq_conv_desc* d) {
+  if (d == nullptr) return fail(MVM_ERR_INVALID_ARG, "desc is NULL");
+  int rc = check_seq(d->seq);
+  if (rc != MVM_OK) return rc;
+  if (d->kwidth < 1 || d->kwidth > MVM_CONV_MAX_KWIDTH)
+    return fail(MVM_ERR_UNSUPPORTED, "kwidth=%lld unsupported (1..%d)", (long long)d->kwidth, MVM_CONV_MAX_KWIDTH);
+  if (d->dtype != MVM_F32 && d->dtype != MVM_BF16)
+    return fail(MVM_ERR_UNSUPPORTED, "dtype=%d unsupported", d->dtype);
+  if (d->reserved != 0) return fail(MVM_ERR_INVALID_ARG, "reserved must be 0");
+  const int64_t t = d->seq.tokens, c = d->seq.dim;
+  if ((rc = check_rows("x_stride", d->x_stride, t, c, false)) || (rc = check_rows("y_stride", d->y_stride, t, c, true)))
+    return rc;
+  if (ceil_div(c, 64) * std::max((t >> mvm::kSeqConvShift) + d->seq.nseq + 1, d->seq.nseq) > kMaxBlocks)
+    return fail(MVM_ERR_UNSUPPORTED, "tokens=%lld, nseq=%lld and dim=%lld are too many for one launch", (long long)t,
+                (long long)d->seq.nseq, (long long)c);
+  return MVM_OK;
+}
+
+mvm::SeqConvGeom conv_geom(const mvm_seq_conv_desc* d) {
+  mvm::SeqConvGeom g;
+  g.q = seq_geom(d->seq);
+  g.xs = d->x_stride;
+  g.ys = d->y_stride;
+  g.kc = static_cast<int32_t>(d->kwidth);
+  return g;
+}
+
+int check_step(const mvm_seq_desc& q) {
+  if (q.offsets != nullptr || q.tokens != q.nseq || (q.nseq > 0 && q.seqlen != 1))
+    return fail(MVM_ERR_INVALID_ARG, "a step takes one token for each sequence (tokens == nseq, seqlen 1, no offsets)");
+  return MVM_OK;
+}
+
+int check_plain(const mvm_seq_desc& q) {
+  if (q.slots != nullptr || q.fresh != nullptr)
+    return fail(MVM_ERR_INVALID_ARG, "a backward takes neither slots nor fresh");
+  return MVM_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int mvm_seq_scan_validate(const mvm_seq_scan_desc* desc) {
+  const int rc = check_scan(desc);
+  return rc == MVM_OK ? ok() : rc;
+}
+
+int64_t mvm_seq_scan_ckpt_elems(const mvm_seq_scan_desc* desc) {
+  const int rc = check_scan(desc);
+  return rc == MVM_OK ? ckpt_elems(desc) : rc;
+}
+
+int64_t mvm_seq_scan_workspace_bytes(const mvm_seq_scan_desc* desc, int which) {
+  const int rc = check_scan(desc);
+  if (rc != MVM_OK) return rc;
+  if (which != 0 && which != 1) return fail(MVM_ERR_INVALID_ARG, "which=%d must be 0 or 1", which);
+  return static_cast<int64_t>(scan_ws(desc, scan_geom(desc, which == 1), which == 1).total);
+}
+
+int mvm_seq_scan_fwd(const mvm_seq_scan_desc* desc, const void* u, const void* delta, const float* delta_bias,
+                     const float* A, const void* Bm, const void* Cm, const float* Dv, const void* z, const float* h0,
+                     float* h1, void* y, float* ckpt, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_scan(desc);
+  if (rc != MVM_OK) return rc;
+  const mvm::SeqScanGeom g = scan_geom(desc, false);
+  if (g.q.D == 0 || (g.q.T == 0 && g.q.S == 0)) return ok();
+  const mvm::SeqScanIn in{u, delta, delta_bias, A, Bm, Cm, Dv, z};
+  if (!A || !Dv || (g.q.T > 0 && (missing(in) || !y)))
+    return fail(MVM_ERR_INVALID_ARG, "mvm_seq_scan_fwd: NULL pointer");
+  const ScanWs w = scan_ws(desc, g, false);
+  if ((rc = check_ws("mvm_seq_scan_fwd", workspace, workspace_bytes, w.total)) != MVM_OK) return rc;
+  Take take{static_cast<char*>(workspace)};
+  mvm::SeqScanFwd b{h0, h1, y, ckpt, take(w.agg_h), take(w.agg_s), take(w.bc)};
+  if (mvm::seq_bc_in_place(g, in, desc->dtype)) b.bc = nullptr;
+  return hip_status(mvm::launch_seq_scan_fwd(g, in, b, desc->dtype, desc->delta_dtype, static_cast<hipStream_t>(stream)),
+                    "mvm_seq_scan_fwd launch");
+}
+
+int mvm_seq_scan_bwd(const mvm_seq_scan_desc* desc, const void* u, const void* delta, const float* delta_bias,
+                     const float* A, const void* Bm, const void* Cm, const float* Dv, const void* z, const float* ckpt,
+                     const void* dy, const float* dh1, void* du, void* ddelta, float* ddelta_bias, float* dA, void* dB,
+                     void* dC, float* dD, void* dz, float* dh0, void* workspace, size_t workspace_bytes,
+                     void* stream) {
+  int rc = check_scan(desc);
+  if (rc != MVM_OK || (rc = check_plain(desc->seq)) != MVM_OK) return rc;
+  const mvm::SeqScanGeom g = scan_geom(desc, true);
+  if (g.q.D == 0) return ok();
+  const mvm::SeqScanIn in{u, delta, delta_bias, A, Bm, Cm, Dv, z};
+  if (!A || !Dv || !dA || !dD ||
+      (g.q.T > 0 && (missing(in) || !ckpt || !dy || !du || !ddelta || !dB || !dC || (z != nullptr) != (dz != nullptr))))
+    return fail(MVM_ERR_INVALID_ARG, "mvm_seq_scan_bwd: NULL pointer");
+  const ScanWs w = scan_ws(desc, g, true);
+  if ((rc = check_ws("mvm_seq_scan_bwd", workspace, workspace_bytes, w.total)) != MVM_OK) return rc;
+  Take take{static_cast<char*>(workspace)};
+  mvm::SeqScanBwd b{};
+  b.ckpt = ckpt; b.dy = dy; b.dh1 = dh1; b.du = du; b.ddelta = ddelta; b.ddbias = ddelta_bias; b.dA = dA;
+  b.dB = dB; b.dC = dC; b.dD = dD; b.dz = dz; b.dh0 = dh0;
+  b.agg_h = take(w.agg_h);
+  b.agg_s = take(w.agg_s);
+  b.bc = take(w.bc);
+  b.part = take(w.part);
+  b.part_bc = take(w.part_bc);
+  if (mvm::seq_bc_in_place(g, in, desc->dtype)) b.bc = nullptr;
+  return hip_status(mvm::launch_seq_scan_bwd(g, in, b, desc->dtype, desc->delta_dtype, static_cast<hipStream_t>(stream)),
+                    "mvm_seq_scan_bwd launch");
+}
+
+int mvm_seq_scan_step(const mvm_seq_scan_desc* desc, const void* u, const void* delta, const float* delta_bias,
+                      const float* A, const void* Bm, const void* Cm, const float* Dv, const void* z, float* states,
+                      void* y, void* stream) {
+  int rc = check_scan(desc);
+  if (rc != MVM_OK || (rc = check_step(desc->seq)) != MVM_OK) return rc;
+  const mvm::SeqScanGeom g = scan_geom(desc, false);
+  if (g.q.D == 0 || g.q.S == 0) return ok();
+  const mvm::SeqScanIn in{u, delta, delta_bias, A, Bm, Cm, Dv, z};
+  if (missing(in) || !states || !y) return fail(MVM_ERR_INVALID_ARG, "mvm_seq_scan_step: NULL pointer");
+  return hip_status(mvm::launch_seq_scan_step(g, in, states, y, desc->dtype, desc->delta_dtype,
+                                              static_cast<hipStream_t>(stream)),
+                    "mvm_seq_scan_step launch");
+}
+
+int mvm_seq_conv_validate(const mvm_seq_conv_desc* desc) {
+  const int rc = check_conv(desc);
+  return rc == MVM_OK ? ok() : rc;
+}
+
+int64_t mvm_seq_conv_workspace_bytes(const mvm_seq_conv_desc* desc) {
+  const int rc = check_conv(desc);
+  if (rc != MVM_OK) return rc;
+  return static_cast<int64_t>(align_up(sizeof(float) * mvm::seq_conv_partial_floats(conv_geom(desc))));
+}
+
+int mvm_seq_conv_fwd(const mvm_seq_conv_desc* desc, const void* x, const float* w, const float* bias, const void* c0,
+                     void* c1, void* y, void* stream) {
+  const int rc = check_conv(desc);
+  if (rc != MVM_OK) return rc;
+  const mvm::SeqConvGeom g = conv_geom(desc);
+  if (g.q.D == 0 || (g.q.T == 0 && g.q.S == 0)) return ok();
+  if (!w || (g.q.T > 0 && (!x || !y))) return fail(MVM_ERR_INVALID_ARG, "mvm_seq_conv_fwd: NULL pointer");
+  return hip_status(mvm::launch_seq_conv_fwd(g, x, w, bias, c0, c1, y, desc->dtype, static_cast<hipStream_t>(stream)),
+                    "mvm_seq_conv_fwd launch");
+}
+
+int mvm_seq_conv_bwd(const mvm_seq_conv_desc* desc, const void* x, const float* w, const float* bias, const void* c0,
+                     const void* dy, const void* dc1, void* dx, float* dw, float* dbias, void* dc0, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  int rc = check_conv(desc);
+  if (rc != MVM_OK || (rc = check_plain(desc->seq)) != MVM_OK) return rc;
+  const mvm::SeqConvGeom g = conv_geom(desc);
+  if (g.q.D == 0) return ok();
+  if (!w || !dw || (g.q.T > 0 && (!x || !dy || !dx)))
+    return fail(MVM_ERR_INVALID_ARG, "mvm_seq_conv_bwd: NULL pointer");
+  const size_t need = align_up(sizeof(float) * mvm::seq_conv_partial_floats(g));
+  if ((rc = check_ws("mvm_seq_conv_bwd", workspace, workspace_bytes, need)) != MVM_OK) return rc;
+  return hip_status(mvm::launch_seq_conv_bwd(g, x, w, bias, c0, dy, dc1, dx, dw, dbias, dc0,
+                                             static_cast<float*>(workspace), desc->dtype,
+                                             static_cast<hipStream_t>(stream)),
+                    "mvm_seq_conv_bwd launch");
+}
+
+int mvm_seq_conv_step(const mvm_seq_conv_desc* desc, const void* x, const float* w, const float* bias, void* states,
+                      void* y, void* stream) {
+  int rc = check_conv(desc);
+  if (rc != MVM_OK || (rc = check_step(desc->seq)) != MVM_OK) return rc;
+  const mvm::SeqConvGeom g = conv_geom(desc);
+  if (g.q.D == 0 || g.q.S == 0) return ok();
+  if (!x || !w || !y || (!states && g.kc > 1)) return fail(MVM_ERR_INVALID_ARG, "mvm_seq_conv_step: NULL pointer");
+  return hip_status(mvm::launch_seq_conv_step(g, x, w, bias, states, y, desc->dtype, static_cast<hipStream_t>(stream)),
+                    "mvm_seq_conv_step launch");
+}
+
+}  // extern "C"

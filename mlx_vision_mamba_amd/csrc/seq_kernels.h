@@ -1,0 +1,107 @@
+// Packed sequences with states: parameter blocks and launch entry points of
+// the scan (seq_scan.hip) and the conv (seq_conv.hip), used by the C ABI
+// (seq_capi.hip).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace mvm {
+
+// The cut of the token rows into sequences, and their state rows.  Work is
+// handed out in chunks of 2^shift positions of one sequence.  The chunk slots
+// of sequence i start at (offset(i) >> shift) + i: floor(a) + 1 >= ceil(a)
+// keeps the ranges apart, so a chunk finds its sequence by a search over the
+// offsets, without a table made before the launch, and every sequence, an
+// empty one too, has at least one slot.  Sequence S stands for the rows past
+// the last offset, whose outputs are zero.
+struct SeqGeom {
+  int32_t T, S, M, L;    // token rows, sequences, state rows, length (off == nullptr)
+  int64_t D;
+  const int32_t* off;    // (S + 1) or nullptr
+  const int32_t* slots;  // (S) or nullptr
+  const uint8_t* fresh;  // (S) or nullptr
+};
+inline int64_t chunk_slots(const SeqGeom& g, int shift) {
+  return (static_cast<int64_t>(g.T) >> shift) + g.S + 1;
+}
+
+constexpr int kSeqTile = 8;       // positions per tile, and between checkpoints
+constexpr int kSeqTileShift = 3;
+
+struct SeqScanGeom {
+  SeqGeom q;
+  int64_t us, ds, bs, ys, zs;  // row strides
+  int32_t N;
+  int32_t shift;     // log2 of the chunk length
+  int32_t multi;     // 0: every sequence is one chunk, no carries
+  int32_t a_log, softplus;
+};
+
+struct SeqScanIn {
+  const void* u;
+  const void* delta;
+  const float* dbias;  // or null
+  const float* A;
+  const void* Bm;
+  const void* Cm;
+  const float* Dv;
+  const void* z;       // or null
+};
+struct SeqScanFwd {
+  const float* h0;  // or null; may be h1
+  float* h1;        // or null
+  void* y;
+  float* ckpt;      // or null
+  float* agg_h;     // (slots, 4, D, 4): end states from zero, then carry-ins
+  float* agg_s;     // (slots, D): sum of delta
+  float* bc;        // (T, 32) float32 copies of B | C, or null: read in place
+};
+struct SeqScanBwd {
+  const float* ckpt;
+  const void* dy;
+  const float* dh1;  // or null
+  void* du;
+  void* ddelta;
+  float* ddbias;     // or null
+  float* dA;
+  void* dB;
+  void* dC;
+  float* dD;
+  void* dz;          // or null
+  float* dh0;        // or null
+  float* agg_h;      // adjoint aggregates, then carry-ins
+  float* agg_s;
+  float* part;       // (slots, 18, D): dA | dD | ddelta_bias of each chunk
+  float* part_bc;    // (channel blocks, T, 32)
+  float* bc;
+};
+
+// true when B and C rows are read where they lie by scalar loads: 16 states,
+// rows that start on 4 bytes.  Others are first copied to float32 rows of 32.
+bool seq_bc_in_place(const SeqScanGeom& g, const SeqScanIn& in, int dtype);
+hipError_t launch_seq_scan_fwd(const SeqScanGeom& g, const SeqScanIn& in, const SeqScanFwd& b, int dtype,
+                               int delta_dtype, hipStream_t s);
+hipError_t launch_seq_scan_bwd(const SeqScanGeom& g, const SeqScanIn& in, const SeqScanBwd& b, int dtype,
+                               int delta_dtype, hipStream_t s);
+hipError_t launch_seq_scan_step(const SeqScanGeom& g, const SeqScanIn& in, float* states, void* y, int dtype,
+                                int delta_dtype, hipStream_t s);
+
+struct SeqConvGeom {
+  SeqGeom q;
+  int64_t xs, ys;
+  int32_t kc;
+};
+constexpr int kSeqConvShift = 6;  // positions per conv chunk: 4 waves of 16
+inline int64_t seq_conv_partial_floats(const SeqConvGeom& g) {
+  return chunk_slots(g.q, kSeqConvShift) * g.q.D * (g.kc + 1);
+}
+hipError_t launch_seq_conv_fwd(const SeqConvGeom& g, const void* x, const float* w, const float* b, const void* c0,
+                               void* c1, void* y, int dtype, hipStream_t s);
+hipError_t launch_seq_conv_bwd(const SeqConvGeom& g, const void* x, const float* w, const float* b, const void* c0,
+                               const void* dy, const void* dc1, void* dx, float* dw, float* db, void* dc0,
+                               float* part, int dtype, hipStream_t s);
+hipError_t launch_seq_conv_step(const SeqConvGeom& g, const void* x, const float* w, const float* b, void* states,
+                                void* y, int dtype, hipStream_t s);
+
+}  // namespace mvm

@@ -14,6 +14,12 @@ All of them compute the same function with the same six gradients; they run
 the HIP kernels of libmvm_scan.so and differ only in how the sequence is cut
 into time chunks.  CPU tensors raise: there is no CPU fallback.
 
+``selective_scan_packed``, ``selective_scan_prefill`` and
+``selective_scan_step`` have no counterpart in the reference: they start from
+states and leave them, over sequences of different lengths packed without
+padding, for training, for the prompts of a serving loop and for its single
+tokens.
+
 ``selective_scan_directions`` is the index-remapped multi-direction form
 used by the direction blocks: K scans over (B, L, K, D) token-order tensors,
 where scan position s of direction k reads and writes token row
@@ -282,6 +288,114 @@ def selective_scan_metal_trainable(x, delta, A, B, C, D):
 def selective_scan_metal_fused(x, delta, A, B, C, D):
     """mamba_metal_fused.py:253 ``metal_fused`` mode."""
     return _scan3(x, delta, A, B, C, D, 0)
+
+
+# ------------------------------------------------- packed and served forms
+
+def sequence_offsets(offsets, x):
+    """``offsets`` of the sequences packed in the rows of ``x``, as the kernels
+    take it: an int32 tensor on its device.  One on the host (a list, or a CPU
+    tensor) is checked: it must start at 0, not decrease and not pass the rows.  One on the GPU is
+    taken as it is, since looking would wait for the GPU: there the kernels
+    clamp it into [0, tokens]."""
+    if offsets is None or (isinstance(offsets, torch.Tensor) and offsets.is_cuda):
+        return offsets
+    if x.dim() != 2:
+        raise ValueError(f"rows must be (T, D) with offsets; got {tuple(x.shape)}")
+    tokens = x.shape[0]
+    offsets = torch.as_tensor(offsets)
+    if offsets.dim() != 1 or offsets.numel() < 1 or offsets.is_floating_point():
+        raise ValueError(f"offsets must hold S + 1 whole numbers; got {tuple(offsets.shape)} of {offsets.dtype}")
+    if int(offsets[0]) != 0 or bool((offsets[1:] < offsets[:-1]).any()) or int(offsets[-1]) > tokens:
+        raise ValueError(f"offsets must start at 0, not decrease and end at {tokens} at most; got {offsets.tolist()}")
+    return offsets.to(device=x.device, dtype=torch.int32)
+
+
+def sequence_slots(slots, rows, device):
+    """``slots`` (or None) as an int32 tensor on ``device``; one on the host is
+    checked for rows named twice."""
+    if slots is None or (isinstance(slots, torch.Tensor) and slots.is_cuda):
+        return slots
+    slots = torch.as_tensor(slots)
+    if slots.dim() != 1 or slots.is_floating_point():
+        raise ValueError(f"slots must be whole numbers, one a sequence; got {tuple(slots.shape)} of {slots.dtype}")
+    used = slots[(slots >= 0) & (slots < rows)]
+    if used.unique().numel() != used.numel():
+        raise ValueError(f"two sequences share a slot: {slots.tolist()}")
+    return slots.to(device=device, dtype=torch.int32)
+
+
+def _chunk_pow2(chunk_len):
+    chunk_len = int(chunk_len)
+    if chunk_len and (chunk_len < 16 or chunk_len & (chunk_len - 1)):
+        raise ValueError(f"chunk_len must be 0 or a power of two >= 16; got {chunk_len}")
+    return chunk_len
+
+
+def _packed(*args):
+    return _lib.native().seq_scan(*args)
+
+
+def selective_scan_packed(u, delta, A, B, C, D, offsets=None, *, z=None, delta_bias=None, delta_softplus=False,
+                          a_is_log=False, initial_states=None, max_len=None, chunk_len=0):
+    """Selective scan of packed sequences that start from states: (y, final_states).
+
+    u, delta, z: (T, D_inner), and B, C: (T, N), the rows of all sequences one
+    after the other; sequence i holds the rows offsets[i] .. offsets[i+1]-1
+    (``offsets``: S + 1 int32, see ``sequence_offsets``; sequences may be empty,
+    rows past the last offset belong to none and give zero).  Without offsets
+    the tensors are (B, L, ...), one sequence a batch row.  Any row stride, the
+    last dimension contiguous.  u, z, B, C, y share a type, float32 or bfloat16;
+    delta has it too or is float32.  A: (D_inner, N), D, delta_bias: (D_inner,).
+
+        delta' = softplus(delta + delta_bias) if delta_softplus else delta + delta_bias
+        h_t = exp(delta'_t A) h_{t-1} + delta'_t B_t u_t      (A = -exp(A) if a_is_log)
+        y_t = (C_t h_t + D u_t) * silu(z_t)                   (without z: no gate)
+
+    initial_states (default zero) and final_states: (S, D_inner, N), float32.
+    Gradients reach every argument, final_states' gradient included; second
+    derivatives are refused.  ``max_len``: an upper bound of the lengths where
+    the caller knows one; only the cut into time chunks goes by it.
+    ``chunk_len``: 0, or a power of two >= 16 to set the cut.
+    """
+    off = sequence_offsets(offsets, u)
+    args = (u, delta, A, B, C, D, z, delta_bias, initial_states, off, bool(delta_softplus), bool(a_is_log),
+            int(max_len or 0), _chunk_pow2(chunk_len))
+    return tuple(_lib.traced(_packed, *args) if _lib.is_tracing() else _packed(*args))
+
+
+def _no_trace(name):
+    if _lib.is_tracing():
+        raise RuntimeError(f"{name} advances its states in place and cannot be traced; capture it in a HIP graph")
+
+
+def selective_scan_prefill(u, delta, A, B, C, D, states, offsets=None, *, slots=None, fresh=None, z=None,
+                           delta_bias=None, delta_softplus=False, a_is_log=False, max_len=None, chunk_len=0):
+    """``selective_scan_packed`` on a cache: returns y, no gradients.
+
+    Sequence i starts from row slots[i] of ``states`` ((rows, D_inner, N)
+    float32, contiguous) and leaves its final state there; without slots row i
+    is sequence i's.  fresh[i] (bool) starts sequence i from zero whatever the
+    row holds: a new prompt's first piece.  A slot outside the cache means none:
+    the sequence starts from zero and its final state is dropped.  Sequences of
+    one call must have different rows.
+    """
+    _no_trace("selective_scan_prefill")
+    off = sequence_offsets(offsets, u)
+    return _lib.native().seq_scan_prefill(
+        u, delta, A, B, C, D, states, off, sequence_slots(slots, states.shape[0], u.device), fresh, z, delta_bias,
+        bool(delta_softplus), bool(a_is_log), int(max_len or 0), _chunk_pow2(chunk_len))
+
+
+def selective_scan_step(u, delta, A, B, C, D, states, *, slots=None, z=None, delta_bias=None, delta_softplus=False,
+                        a_is_log=False):
+    """One token for each of S sequences: y (S, D_inner), ``states`` advanced in
+    place.  Arguments as in ``selective_scan_prefill`` with one row a sequence;
+    a row whose slot lies outside the cache is padding: its y is zero."""
+    _no_trace("selective_scan_step")
+    return _lib.native().seq_scan_step(u, delta, A, B, C, D, states,
+                                       sequence_slots(slots, states.shape[0], u.device), z, delta_bias,
+                                       bool(delta_softplus), bool(a_is_log))
 
 
 _MODE_FNS = {
