@@ -16,7 +16,7 @@ using mvm::ok;
 
 // positions are int32, and formed up to a chunk's tile past the last
 constexpr int64_t kMaxTokens = INT32_MAX - 64;
-constexpr int64_t kMaxBlocks = INT32_MAX;
+constexpr int64_t kMaxThreads = (int64_t{1} << 32) - 1024;  // of one launch
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 constexpr size_t kAlign = 256;
@@ -27,8 +27,9 @@ int check_seq(const mvm_seq_desc& q) {
     return fail(MVM_ERR_INVALID_ARG, "negative size (tokens=%lld nseq=%lld seqlen=%lld dim=%lld state_rows=%lld)",
                 (long long)q.tokens, (long long)q.nseq, (long long)q.seqlen, (long long)q.dim,
                 (long long)q.state_rows);
-  if (q.tokens > kMaxTokens || q.nseq > kMaxTokens || q.state_rows > kMaxTokens || q.dim > kMaxTokens)
-    return fail(MVM_ERR_UNSUPPORTED, "tokens, nseq, dim and state_rows must be at most %lld", (long long)kMaxTokens);
+  if (q.tokens > kMaxTokens || q.nseq > kMaxTokens || q.state_rows > kMaxTokens || q.dim > (kMaxTokens >> 2))
+    return fail(MVM_ERR_UNSUPPORTED, "tokens, nseq and state_rows must be at most %lld, dim %lld",
+                (long long)kMaxTokens, (long long)(kMaxTokens >> 2));
   // (seqlen <= tokens where there are sequences, so the product cannot overflow)
   if (q.offsets == nullptr && (q.nseq > 0 ? q.seqlen > q.tokens || q.nseq * q.seqlen != q.tokens : q.tokens != 0))
     return fail(MVM_ERR_INVALID_ARG, "without offsets tokens=%lld must be nseq=%lld * seqlen=%lld",
@@ -40,13 +41,15 @@ int check_seq(const mvm_seq_desc& q) {
 }
 
 int check_rows(const char* name, int64_t stride, int64_t tokens, int64_t cols, bool written) {
+  if (stride > (INT32_MAX >> 2))
+    return fail(MVM_ERR_UNSUPPORTED, "%s=%lld: strides of at most %d values", name, (long long)stride, INT32_MAX >> 2);
   if (stride < 0 || (written && tokens > 1 && stride < cols))
     return fail(MVM_ERR_INVALID_ARG, "%s=%lld: rows of %lld values %s", name, (long long)stride, (long long)cols,
                 written ? "must not overlap" : "need a stride >= 0");
   return MVM_OK;
 }
 
-int check_scan(const mvm_seq_scan_desc* d) {
+int check_scan_fields(const mvm_seq_scan_desc* d) {
   if (d == nullptr) return fail(MVM_ERR_INVALID_ARG, "desc is NULL");
   int rc = check_seq(d->seq);
   if (rc != MVM_OK) return rc;
@@ -65,10 +68,13 @@ int check_scan(const mvm_seq_scan_desc* d) {
       (rc = check_rows("bc_stride", d->bc_stride, t, d->dstate, false)) ||
       (rc = check_rows("z_stride", d->z_stride, t, c, false)) || (rc = check_rows("y_stride", d->y_stride, t, c, true)))
     return rc;
-  const int64_t ncb = ceil_div(c, 64);
-  if (ncb * std::max((t >> 4) + d->seq.nseq + 1, d->seq.nseq) > kMaxBlocks)
-    return fail(MVM_ERR_UNSUPPORTED, "tokens=%lld, nseq=%lld and dim=%lld are too many for one launch", (long long)t,
-                (long long)d->seq.nseq, (long long)c);
+  return MVM_OK;
+}
+
+int check_threads(const mvm_seq_desc& q, int64_t blocks, int64_t threads) {
+  if (threads > 0 && blocks > kMaxThreads / threads)
+    return fail(MVM_ERR_UNSUPPORTED, "tokens=%lld, nseq=%lld and dim=%lld are too many for one launch",
+                (long long)q.tokens, (long long)q.nseq, (long long)q.dim);
   return MVM_OK;
 }
 
@@ -85,28 +91,41 @@ mvm::SeqGeom seq_geom(const mvm_seq_desc& q) {
   return g;
 }
 
-int log2_ceil(int64_t n) {
-  int k = 0;
-  while ((int64_t{1} << k) < n) ++k;
-  return k;
-}
+// The cut into time chunks.  A wave is 64 channels of one chunk; the passes
+// run at the rate of the SIMDs' instruction issue once each of the 1024 SIMDs
+// has a few waves.  Chunks need an aggregate pass and a carry before the main
+// pass, which repeat most of the recurrence.  In cycles (measured on MI355X
+// at 2.4 GHz; lone: a wave by itself on its SIMD):
+struct Cost {
+  int64_t waves;     // that the card holds at once
+  int64_t lone;      // main pass, cycles a token and wave
+  int64_t main_, agg;  // per token and wave, issued by a full SIMD
+};
+constexpr Cost kFwdCost = {4096, 800, 520, 420};
+constexpr Cost kBwdCost = {3072, 2000, 1500, 430};
+constexpr int64_t kPassCycles = 24000;  // launches and start-up of the two extra passes
 
-// The cut into time chunks, a power of two long.  A pass over chunks repeats
-// the recurrence for their end states, so sequences stay whole when they fill
-// the card by themselves; else they are cut until the main pass has `waves`
-// waves of 64 channels, four (backward: two) on each of the 1024 SIMDs.
-void pick_chunk(const mvm_seq_scan_desc* d, int64_t waves, mvm::SeqScanGeom& g) {
-  const int64_t T = d->seq.tokens, ncb = std::max<int64_t>(1, ceil_div(d->seq.dim, 64));
+void pick_chunk(const mvm_seq_scan_desc* d, const Cost& k, mvm::SeqScanGeom& g) {
+  const int64_t T = d->seq.tokens, S = d->seq.nseq, ncb = std::max<int64_t>(1, ceil_div(d->seq.dim, 64));
   int64_t longest = d->seq.offsets == nullptr ? d->seq.seqlen : T;
   if (d->max_len > 0) longest = std::min(longest, d->max_len);
   int64_t len = d->chunk_len;
   if (len == 0) {
-    len = 16;
-    while (len < longest && ceil_div(T, len * 2) * ncb >= waves) len *= 2;
+    // Chunks that fill the card once; a sequence's last one is half a chunk on
+    // average
+    const int64_t budget = std::max<int64_t>(1, k.waves / ncb), chunks = std::max(budget - S / 2, ceil_div(budget, 4));
+    len = std::max<int64_t>(16, ceil_div(ceil_div(T, chunks), mvm::kSeqTile) * mvm::kSeqTile);
+    // Whole sequences where the longest one by itself takes no longer
+    const int64_t work = T * ncb / 1024;
+    const int64_t whole = std::max(longest * k.lone, work * k.main_);
+    const int64_t cut = std::max(2 * len * k.lone, work * (k.main_ + k.agg)) + kPassCycles;
+    if (whole <= cut) len = longest;
   }
   g.multi = len < longest;
   // Whole sequences: one chunk whatever max_len says
-  g.shift = g.multi ? log2_ceil(len) : std::max(4, log2_ceil(T + 1));
+  if (!g.multi) len = std::max<int64_t>(16, T + 1);
+  g.cut = mvm::seq_cut(len);
+  g.max_chunks = g.multi ? static_cast<int32_t>(ceil_div(longest, len)) : 1;
 }
 
 mvm::SeqScanGeom scan_geom(const mvm_seq_scan_desc* d, bool backward) {
@@ -120,8 +139,21 @@ mvm::SeqScanGeom scan_geom(const mvm_seq_scan_desc* d, bool backward) {
   g.N = static_cast<int32_t>(d->dstate);
   g.a_log = d->a_is_log != 0;
   g.softplus = d->delta_softplus != 0;
-  pick_chunk(d, backward ? 2048 : 4096, g);
+  pick_chunk(d, backward ? kBwdCost : kFwdCost, g);
   return g;
+}
+
+// Everything that a call of either direction would be refused for.
+int check_scan(const mvm_seq_scan_desc* d) {
+  int rc = check_scan_fields(d);
+  if (rc == MVM_OK) rc = check_threads(d->seq, d->seq.tokens, ceil_div(d->seq.dim, 64));
+  for (int backward = 0; rc == MVM_OK && backward < 2; ++backward) {
+    const mvm::SeqScanGeom g = scan_geom(d, backward != 0);
+    const int64_t carry = g.multi ? ceil_div(g.q.D, 16) * g.q.S : 0;
+    if ((rc = check_threads(d->seq, mvm::chunk_slots(g.q, g.cut), ceil_div(g.q.D, 64) * 64)) == MVM_OK)
+      rc = check_threads(d->seq, carry, 64 * mvm::carry_waves(g));
+  }
+  return rc;
 }
 
 int64_t ckpt_elems(const mvm_seq_scan_desc* d) {
@@ -133,7 +165,7 @@ struct ScanWs {
 };
 ScanWs scan_ws(const mvm_seq_scan_desc* d, const mvm::SeqScanGeom& g, bool backward) {
   ScanWs w;
-  const size_t slots = static_cast<size_t>(mvm::chunk_slots(g.q, g.shift)), D = static_cast<size_t>(g.q.D);
+  const size_t slots = static_cast<size_t>(mvm::chunk_slots(g.q, g.cut)), D = static_cast<size_t>(g.q.D);
   const size_t T = static_cast<size_t>(g.q.T);
   if (g.multi) {
     w.agg_h = align_up(slots * D * 16 * sizeof(float));
@@ -178,10 +210,7 @@ int check_conv(const mvm_seq_conv_desc* d) {
   const int64_t t = d->seq.tokens, c = d->seq.dim;
   if ((rc = check_rows("x_stride", d->x_stride, t, c, false)) || (rc = check_rows("y_stride", d->y_stride, t, c, true)))
     return rc;
-  if (ceil_div(c, 64) * std::max((t >> mvm::kSeqConvShift) + d->seq.nseq + 1, d->seq.nseq) > kMaxBlocks)
-    return fail(MVM_ERR_UNSUPPORTED, "tokens=%lld, nseq=%lld and dim=%lld are too many for one launch", (long long)t,
-                (long long)d->seq.nseq, (long long)c);
-  return MVM_OK;
+  return check_threads(d->seq, t / mvm::kSeqConvCut.len + d->seq.nseq + 1, ceil_div(c, 64) * 256);
 }
 
 mvm::SeqConvGeom conv_geom(const mvm_seq_conv_desc* d) {
@@ -280,6 +309,7 @@ int mvm_seq_scan_step(const mvm_seq_scan_desc* desc, const void* u, const void* 
   int rc = check_scan(desc);
   if (rc != MVM_OK || (rc = check_step(desc->seq)) != MVM_OK) return rc;
   const mvm::SeqScanGeom g = scan_geom(desc, false);
+  if ((rc = check_threads(desc->seq, g.q.S, ceil_div(g.q.D, 64) * 256)) != MVM_OK) return rc;
   if (g.q.D == 0 || g.q.S == 0) return ok();
   const mvm::SeqScanIn in{u, delta, delta_bias, A, Bm, Cm, Dv, z};
   if (missing(in) || !states || !y) return fail(MVM_ERR_INVALID_ARG, "mvm_seq_scan_step: NULL pointer");

@@ -34,36 +34,48 @@ __device__ __forceinline__ bool seq_fresh(const SeqGeom& g, int32_t i) {
   return g.fresh != nullptr && g.fresh[i] != 0;
 }
 
+__device__ __forceinline__ int32_t cut_div(const SeqCut& cut, int32_t n) {
+  return static_cast<int32_t>(__umulhi(static_cast<uint32_t>(n), cut.magic) >> cut.shift);
+}
+
 // The chunk that a slot stands for: rows [t0, t1) of sequence seq, which
 // holds rows [start, end).  t0 < 0: none.  An empty sequence has one chunk,
 // with t0 == t1 == start == end.
 struct SeqChunk {
   int32_t seq, start, end, t0, t1, slot;
 };
-__device__ __forceinline__ SeqChunk seq_chunk(const SeqGeom& g, int32_t slot, int shift, int lane) {
-  // the last i in [0, S] with (offset(i) >> shift) + i <= slot: each round 64
-  // lanes probe the range at even steps
-  int32_t lo = 0, hi = g.S;
-  while (hi > lo) {
-    const int32_t step = (hi - lo + 63) / 64;
-    const int32_t i = lo + (lane + 1) * step;
-    const bool in = i <= hi;
-    const bool le = in && (seq_off(g, in ? i : lo) >> shift) + i <= slot;
-    const int32_t cnt = __popcll(__ballot(le));
-    lo += cnt * step;
-    const int32_t last = lo + step - 1;
-    hi = hi < last ? hi : last;
-  }
+__device__ __forceinline__ SeqChunk seq_chunk(const SeqGeom& g, int32_t slot, const SeqCut& cut, int lane) {
+  // the last i in [0, S] with offset(i) / len + i <= slot: each round 64 lanes
+  // probe the range at even steps
   SeqChunk c;
   c.slot = slot;
-  c.seq = __builtin_amdgcn_readfirstlane(lo);
-  c.start = seq_off_u(g, c.seq);
-  const int32_t next = c.seq == g.S ? g.T : seq_off_u(g, c.seq + 1);
+  int32_t next;
+  if (g.S <= 64) {  // one round, whose lanes hold the bounds too
+    const int32_t i = lane + 1, off = seq_off(g, i <= g.S ? i : 0);
+    c.seq = __popcll(__ballot(i <= g.S && cut_div(cut, off) + i <= slot));
+    c.start = c.seq > 0 ? __builtin_amdgcn_readlane(off, c.seq - 1) : 0;
+    next = c.seq < g.S ? __builtin_amdgcn_readlane(off, c.seq) : g.T;
+  } else {
+    int32_t lo = 0, hi = g.S;
+    while (hi > lo) {
+      const int32_t step = (hi - lo + 63) / 64;
+      const int32_t i = lo + (lane + 1) * step;
+      const bool in = i <= hi;
+      const bool le = in && cut_div(cut, seq_off(g, in ? i : lo)) + i <= slot;
+      const int32_t cnt = __popcll(__ballot(le));
+      lo += cnt * step;
+      const int32_t last = lo + step - 1;
+      hi = hi < last ? hi : last;
+    }
+    c.seq = __builtin_amdgcn_readfirstlane(lo);
+    c.start = seq_off_u(g, c.seq);
+    next = c.seq == g.S ? g.T : seq_off_u(g, c.seq + 1);
+  }
   c.end = next < c.start ? c.start : next;
-  const int32_t nth = slot - (c.start >> shift) - c.seq;
-  const int64_t t0 = c.start + (static_cast<int64_t>(nth) << shift);
+  const int32_t nth = slot - cut_div(cut, c.start) - c.seq;
+  const int64_t t0 = c.start + static_cast<int64_t>(nth) * cut.len;
   c.t0 = static_cast<int32_t>(t0 < c.end ? t0 : c.end);
-  const int64_t t1 = t0 + (int64_t{1} << shift);
+  const int64_t t1 = t0 + cut.len;
   c.t1 = static_cast<int32_t>(t1 < c.end ? t1 : c.end);
   // a slot past the sequence's last chunk (or before its first, which only
   // offsets that decrease give)

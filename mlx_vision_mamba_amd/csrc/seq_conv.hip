@@ -57,7 +57,7 @@ seq_conv_fwd_kernel(SeqConvGeom g, uint32_t ncb, const T* __restrict__ x, const 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const BlockPos pos = block_pos(ncb);
-  const SeqChunk c = seq_chunk(g.q, pos.slot, kSeqConvShift, lane);
+  const SeqChunk c = seq_chunk(g.q, pos.slot, kSeqConvCut, lane);
   const int64_t D = g.q.D, d = (static_cast<int64_t>(pos.cb) * 64 + lane) * V;
   if (c.t0 < 0 || d >= D) return;
   const int32_t s0 = c.t0 + wave * kPos;
@@ -122,7 +122,7 @@ seq_conv_bwd_kernel(SeqConvGeom g, uint32_t ncb, const T* __restrict__ x, const 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const BlockPos pos = block_pos(ncb);
-  const SeqChunk c = seq_chunk(g.q, pos.slot, kSeqConvShift, lane);
+  const SeqChunk c = seq_chunk(g.q, pos.slot, kSeqConvCut, lane);
   const int64_t D = g.q.D, d = (static_cast<int64_t>(pos.cb) * 64 + lane) * V;
   const bool valid = d < D;
   const int64_t dd = valid ? d : 0;
@@ -335,7 +335,7 @@ template <typename T, int V, int KC>
 hipError_t fwd_v(const SeqConvGeom& g, const void* x, const float* w, const float* b, const void* c0, void* c1, void* y,
                  hipStream_t s) {
   const uint32_t ncb = conv_blocks<V>(g);
-  hipLaunchKernelGGL((seq_conv_fwd_kernel<T, V, KC>), dim3(static_cast<unsigned>(chunk_slots(g.q, kSeqConvShift) * ncb)),
+  hipLaunchKernelGGL((seq_conv_fwd_kernel<T, V, KC>), dim3(static_cast<unsigned>(chunk_slots(g.q, kSeqConvCut) * ncb)),
                      dim3(256), 0, s, g, ncb, static_cast<const T*>(x), w, b, static_cast<const T*>(c0),
                      static_cast<T*>(c1), static_cast<T*>(y));
   return hipGetLastError();
@@ -345,7 +345,7 @@ template <typename T, int V, int KC>
 hipError_t bwd_v(const SeqConvGeom& g, const void* x, const float* w, const float* b, const void* c0, const void* dy,
                  const void* dc1, void* dx, float* dw, float* db, void* dc0, float* part, hipStream_t s) {
   const uint32_t ncb = conv_blocks<V>(g);
-  const int64_t slots = chunk_slots(g.q, kSeqConvShift), ncols = g.q.D * (KC + 1);
+  const int64_t slots = chunk_slots(g.q, kSeqConvCut), ncols = g.q.D * (KC + 1);
   hipLaunchKernelGGL((seq_conv_bwd_kernel<T, V, KC>), dim3(static_cast<unsigned>(slots * ncb)), dim3(256), 0, s, g, ncb,
                      static_cast<const T*>(x), w, b, static_cast<const T*>(c0), static_cast<const T*>(dy),
                      static_cast<const T*>(dc1), static_cast<T*>(dx), static_cast<T*>(dc0), part);

@@ -8,9 +8,23 @@
 
 namespace mvm {
 
+// Lengths of chunks that positions are cut by.  n / len for 0 <= n < 2^31 is
+// (n * magic) >> (32 + shift): magic = ceil(2^(32 + shift) / len), shift =
+// ceil(log2(len)) - 1, exact there because the error of magic, below len <=
+// 2^(shift + 1), times n stays below 2^(32 + shift).
+struct SeqCut {
+  uint32_t len, magic, shift;  // len in [8, 2^31]
+};
+inline SeqCut seq_cut(int64_t len) {
+  uint32_t l = 3;
+  while ((uint64_t{1} << l) < static_cast<uint64_t>(len)) ++l;
+  const uint64_t two = uint64_t{1} << (31 + l);
+  return {static_cast<uint32_t>(len), static_cast<uint32_t>((two + len - 1) / len), l - 1};
+}
+
 // The cut of the token rows into sequences, and their state rows.  Work is
-// handed out in chunks of 2^shift positions of one sequence.  The chunk slots
-// of sequence i start at (offset(i) >> shift) + i: floor(a) + 1 >= ceil(a)
+// handed out in chunks of positions of one sequence.  The chunk slots of
+// sequence i start at offset(i) / len + i: floor(a) + 1 >= ceil(a)
 // keeps the ranges apart, so a chunk finds its sequence by a search over the
 // offsets, without a table made before the launch, and every sequence, an
 // empty one too, has at least one slot.  Sequence S stands for the rows past
@@ -22,8 +36,8 @@ struct SeqGeom {
   const int32_t* slots;  // (S) or nullptr
   const uint8_t* fresh;  // (S) or nullptr
 };
-inline int64_t chunk_slots(const SeqGeom& g, int shift) {
-  return (static_cast<int64_t>(g.T) >> shift) + g.S + 1;
+inline int64_t chunk_slots(const SeqGeom& g, const SeqCut& cut) {
+  return static_cast<int64_t>(g.T) / cut.len + g.S + 1;
 }
 
 constexpr int kSeqTile = 8;       // positions per tile, and between checkpoints
@@ -33,10 +47,18 @@ struct SeqScanGeom {
   SeqGeom q;
   int64_t us, ds, bs, ys, zs;  // row strides
   int32_t N;
-  int32_t shift;     // log2 of the chunk length
-  int32_t multi;     // 0: every sequence is one chunk, no carries
+  SeqCut cut;
+  int32_t multi;       // 0: every sequence is one chunk, no carries
+  int32_t max_chunks;  // of a sequence, as far as the caller's max_len holds
   int32_t a_log, softplus;
 };
+
+// Chunks whose aggregates a wave of the carry pass holds, and its waves.
+constexpr int kCarryRun = 8;
+inline int carry_waves(const SeqScanGeom& g) {
+  const int w = (g.max_chunks + kCarryRun - 1) / kCarryRun;
+  return w < 1 ? 1 : (w > 16 ? 16 : w);
+}
 
 struct SeqScanIn {
   const void* u;
@@ -92,9 +114,9 @@ struct SeqConvGeom {
   int64_t xs, ys;
   int32_t kc;
 };
-constexpr int kSeqConvShift = 6;  // positions per conv chunk: 4 waves of 16
+constexpr SeqCut kSeqConvCut = {64, 1u << 31, 5};  // 4 waves of 16 positions
 inline int64_t seq_conv_partial_floats(const SeqConvGeom& g) {
-  return chunk_slots(g.q, kSeqConvShift) * g.q.D * (g.kc + 1);
+  return chunk_slots(g.q, kSeqConvCut) * g.q.D * (g.kc + 1);
 }
 hipError_t launch_seq_conv_fwd(const SeqConvGeom& g, const void* x, const float* w, const float* b, const void* c0,
                                void* c1, void* y, int dtype, hipStream_t s);
