@@ -25,7 +25,7 @@ CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 LIB = os.path.join(PKG, "libmvm_scan.so")
 SOURCES = ["capi.hip", "scan_fwd.hip", "scan_bwd.hip", "conv.hip", "layernorm.hip", "gemm.hip", "optim.hip",
-           "seq_capi.hip", "seq_scan.hip", "seq_conv.hip"]
+           "seq_capi.hip", "seq_scan.hip", "seq_scan_bwd.hip", "seq_conv.hip"]
 NATIVE = os.path.join(PKG, "_native.so")
 ARCH = "gfx950"
 

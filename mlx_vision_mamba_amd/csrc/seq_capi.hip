@@ -103,6 +103,7 @@ struct Cost {
 };
 constexpr Cost kFwdCost = {4096, 800, 520, 420};
 constexpr Cost kBwdCost = {3072, 2000, 1500, 430};
+constexpr int64_t kFoldChunks = 16;
 constexpr int64_t kPassCycles = 24000;  // launches and start-up of the two extra passes
 
 void pick_chunk(const mvm_seq_scan_desc* d, const Cost& k, mvm::SeqScanGeom& g) {
@@ -125,6 +126,7 @@ void pick_chunk(const mvm_seq_scan_desc* d, const Cost& k, mvm::SeqScanGeom& g) 
   // Whole sequences: one chunk whatever max_len says
   if (!g.multi) len = std::max<int64_t>(16, T + 1);
   g.cut = mvm::seq_cut(len);
+  g.fold = g.multi && ceil_div(longest, len) <= kFoldChunks;
   g.max_chunks = g.multi ? static_cast<int32_t>(ceil_div(longest, len)) : 1;
 }
 
@@ -296,9 +298,9 @@ int mvm_seq_scan_bwd(const mvm_seq_scan_desc* desc, const void* u, const void* d
   b.agg_h = take(w.agg_h);
   b.agg_s = take(w.agg_s);
   b.bc = take(w.bc);
+  if (mvm::seq_bc_in_place(g, in, desc->dtype)) b.bc = nullptr;
   b.part = take(w.part);
   b.part_bc = take(w.part_bc);
-  if (mvm::seq_bc_in_place(g, in, desc->dtype)) b.bc = nullptr;
   return hip_status(mvm::launch_seq_scan_bwd(g, in, b, desc->dtype, desc->delta_dtype, static_cast<hipStream_t>(stream)),
                     "mvm_seq_scan_bwd launch");
 }

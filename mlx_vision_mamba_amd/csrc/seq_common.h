@@ -83,6 +83,14 @@ __device__ __forceinline__ SeqChunk seq_chunk(const SeqGeom& g, int32_t slot, co
   return c;
 }
 
+// a pointer to global memory that the compiler knows nothing about
+template <typename T>
+__device__ __forceinline__ T* opaque(T* p) {
+  uint64_t v = reinterpret_cast<uint64_t>(p);
+  asm volatile("" : "+v"(v));
+  return (T*)(__attribute__((address_space(1))) T*)v;
+}
+
 // V consecutive values, one access
 template <typename T, int V>
 struct alignas(sizeof(T) * V) Pack {

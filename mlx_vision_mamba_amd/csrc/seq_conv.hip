@@ -37,16 +37,39 @@ __device__ __forceinline__ Pack<T, V> row_of_seq(const T* x, int64_t xs, const S
   return r;
 }
 
+// The taps and biases of a lane's V channels.  Sixteen bytes a load where the
+// channels' taps are whole multiples of that (vec: and the buffers aligned):
+// one value a load would be more loads than the rows themselves.
 template <int V, int KC>
 struct Taps {
   float w[KC][V], b[V];
-  __device__ __forceinline__ void load(const float* wp, const float* bp, int64_t d) {
+  __device__ __forceinline__ void load(const float* wp, const float* bp, int64_t d, int vec) {
+    float t[V * KC];
+    if ((V * KC) % 4 == 0 && V % 4 == 0 && vec) {
+      wp = opaque(wp + d * KC);
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
+      for (int i = 0; i < V * KC / 4; ++i) {
+        const Pack<float, 4> p = load_pack<float, 4>(wp + 4 * i);
 #pragma unroll
-      for (int j = 0; j < KC; ++j) w[j][v] = wp[(d + v) * KC + j];
-      b[v] = bp ? bp[d + v] : 0.f;
+        for (int j = 0; j < 4; ++j) t[4 * i + j] = p.v[j];
+      }
+      if (bp) bp = opaque(bp + d);
+#pragma unroll
+      for (int i = 0; i < V / 4; ++i) {
+        const Pack<float, 4> p = bp ? load_pack<float, 4>(bp + 4 * i) : Pack<float, 4>{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) b[4 * i + j] = p.v[j];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V * KC; ++i) t[i] = wp[d * KC + i];
+#pragma unroll
+      for (int v = 0; v < V; ++v) b[v] = bp ? bp[d + v] : 0.f;
     }
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+      for (int j = 0; j < KC; ++j) w[j][v] = t[v * KC + j];
   }
 };
 
@@ -73,7 +96,7 @@ seq_conv_fwd_kernel(SeqConvGeom g, uint32_t ncb, const T* __restrict__ x, const 
   if (c.t0 == c.start && c0 != nullptr && row >= 0 && !seq_fresh(g.q, c.seq)) state = c0 + row * (KC - 1) * D;
   if (s0 < c.t1) {
     Taps<V, KC> k;
-    k.load(w, bias, d);
+    k.load(w, bias, d, g.w_vec);
     const int64_t p0 = s0 - c.start;
     Pack<T, V> win[kPos + KC - 1];
     if (p0 >= KC - 1 && s0 + kPos <= c.end) {
@@ -155,7 +178,7 @@ seq_conv_bwd_kernel(SeqConvGeom g, uint32_t ncb, const T* __restrict__ x, const 
     const bool head = c.t0 == c.start && wave == 0;
     if (s0 < c.t1 || head) {
       Taps<V, KC> k;
-      k.load(w, bias, dd);
+      k.load(w, bias, dd, g.w_vec);
       constexpr int kG = kPos + KC - 1;  // positions whose dpre is needed
       Pack<T, V> xw[kG + KC - 1], gy[kG];
 #pragma unroll
@@ -255,52 +278,69 @@ seq_conv_reduce_kernel(int64_t ncols, int32_t kc, int64_t nparts, const float* _
   });
 }
 
-// One token: the state's rows move up by one in place.
-template <typename T, int V, int KC>
+// One token: the state's rows move up by one in place.  A wave keeps its
+// channels' taps for R sequences, and has all their loads in flight together.
+template <typename T, int V, int KC, int R>
 __global__ void __launch_bounds__(64)
 seq_conv_step_kernel(SeqConvGeom g, uint32_t ncb, const T* __restrict__ x, const float* __restrict__ w,
                      const float* __restrict__ bias, T* __restrict__ states, T* __restrict__ y) {
   const BlockPos pos = block_pos(ncb);
   const int64_t D = g.q.D, d = (static_cast<int64_t>(pos.cb) * 64 + threadIdx.x) * V;
   if (d >= D) return;
-  const int32_t i = pos.slot, row = seq_slot(g.q, i);
-  Pack<T, V> o;
-  if (row < 0) {
+  const int32_t i0 = pos.slot * R;
+  int32_t row[R];
+  Pack<T, V> win[R][KC];
 #pragma unroll
-    for (int v = 0; v < V; ++v) o.v[v] = from_f32<T>(0.f);
-    store_pack(y + i * g.ys + d, o);
-    return;
+  for (int r = 0; r < R; ++r) {
+    const int32_t i = i0 + r < g.q.S ? i0 + r : g.q.S - 1;
+    row[r] = seq_slot(g.q, i);
+    const T* at = states + static_cast<int64_t>(row[r] < 0 ? 0 : row[r]) * (KC - 1) * D + d;
+    if (row[r] >= 0) {
+#pragma unroll
+      for (int k = 0; k < KC - 1; ++k) win[r][k] = load_pack<T, V>(at + k * D);
+    }
+    win[r][KC - 1] = load_pack<T, V>(x + i * g.xs + d);
   }
-  const bool fresh = seq_fresh(g.q, i);
-  T* at = states + static_cast<int64_t>(row) * (KC - 1) * D + d;
-  Pack<T, V> win[KC];
-#pragma unroll
-  for (int r = 0; r < KC - 1; ++r) win[r] = load_pack<T, V>(at + r * D);
-  win[KC - 1] = load_pack<T, V>(x + i * g.xs + d);
   Taps<V, KC> k;
-  k.load(w, bias, d);
-  if (fresh) {
+  k.load(w, bias, d, g.w_vec);
 #pragma unroll
-    for (int r = 0; r < KC - 1; ++r)
+  for (int r = 0; r < R; ++r) {
+    if (i0 + r >= g.q.S) break;
+    Pack<T, V> o;
+    if (row[r] < 0) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) win[r].v[v] = from_f32<T>(0.f);
+      for (int v = 0; v < V; ++v) o.v[v] = from_f32<T>(0.f);
+      store_pack(y + (i0 + r) * g.ys + d, o);
+      continue;
+    }
+    if (seq_fresh(g.q, i0 + r)) {
+#pragma unroll
+      for (int j = 0; j < KC - 1; ++j)
+#pragma unroll
+        for (int v = 0; v < V; ++v) win[r][j].v[v] = from_f32<T>(0.f);
+    }
+    T* at = states + static_cast<int64_t>(row[r]) * (KC - 1) * D + d;
+#pragma unroll
+    for (int j = 0; j < KC - 1; ++j) store_pack(at + j * D, win[r][j + 1]);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float pre = k.b[v];
+#pragma unroll
+      for (int j = 0; j < KC; ++j) pre = fmaf(k.w[j][v], to_f32(win[r][j].v[v]), pre);
+      o.v[v] = from_f32<T>(pre * sigmoid_f(pre));
+    }
+    store_pack(y + (i0 + r) * g.ys + d, o);
   }
-#pragma unroll
-  for (int r = 0; r < KC - 1; ++r) store_pack(at + r * D, win[r + 1]);
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    float pre = k.b[v];
-#pragma unroll
-    for (int j = 0; j < KC; ++j) pre = fmaf(k.w[j][v], to_f32(win[j].v[v]), pre);
-    o.v[v] = from_f32<T>(pre * sigmoid_f(pre));
-  }
-  store_pack(y + i * g.ys + d, o);
 }
 
 // ----------------------------------------------------------------- launches
 
 // Whether rows can be accessed V values at a time: whole packs in a row, and
 // every row of every buffer aligned to them.
+SeqConvGeom with_vec(SeqConvGeom g, const float* w, const float* b) {
+  g.w_vec = ((reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(b)) & 15) == 0;
+  return g;
+}
 template <typename T, int V>
 bool packs(const SeqConvGeom& g, std::initializer_list<const void*> ptrs) {
   bool ok = g.q.D % V == 0 && g.xs % V == 0 && g.ys % V == 0;
@@ -360,15 +400,21 @@ template <typename T, int V, int KC>
 hipError_t step_v(const SeqConvGeom& g, const void* x, const float* w, const float* b, void* states, void* y,
                   hipStream_t s) {
   const uint32_t ncb = conv_blocks<V>(g);
-  hipLaunchKernelGGL((seq_conv_step_kernel<T, V, KC>), dim3(ncb * static_cast<unsigned>(g.q.S)), dim3(64), 0, s, g, ncb,
-                     static_cast<const T*>(x), w, b, static_cast<T*>(states), static_cast<T*>(y));
-  return hipGetLastError();
+  auto run = [&](auto kernel, int R) {
+    hipLaunchKernelGGL(kernel, dim3(ncb * static_cast<unsigned>((g.q.S + R - 1) / R)), dim3(64), 0, s, g, ncb,
+                       static_cast<const T*>(x), w, b, static_cast<T*>(states), static_cast<T*>(y));
+    return hipGetLastError();
+  };
+  // two sequences a wave once that leaves each SIMD a wave
+  return static_cast<int64_t>(g.q.S) * ncb >= 2 * 1024 ? run(seq_conv_step_kernel<T, V, KC, 2>, 2)
+                                                       : run(seq_conv_step_kernel<T, V, KC, 1>, 1);
 }
 
 }  // namespace
 
-hipError_t launch_seq_conv_fwd(const SeqConvGeom& g, const void* x, const float* w, const float* b, const void* c0,
+hipError_t launch_seq_conv_fwd(const SeqConvGeom& geom, const void* x, const float* w, const float* b, const void* c0,
                                void* c1, void* y, int dtype, hipStream_t s) {
+  const SeqConvGeom g = with_vec(geom, w, b);
   return by_width(dtype, g.kc, [&](auto t, auto kc) {
     using T = decltype(t);
     constexpr int KC = decltype(kc)::value, V = 16 / sizeof(T);
@@ -377,9 +423,10 @@ hipError_t launch_seq_conv_fwd(const SeqConvGeom& g, const void* x, const float*
   });
 }
 
-hipError_t launch_seq_conv_bwd(const SeqConvGeom& g, const void* x, const float* w, const float* b, const void* c0,
+hipError_t launch_seq_conv_bwd(const SeqConvGeom& geom, const void* x, const float* w, const float* b, const void* c0,
                                const void* dy, const void* dc1, void* dx, float* dw, float* db, void* dc0,
                                float* part, int dtype, hipStream_t s) {
+  const SeqConvGeom g = with_vec(geom, w, b);
   return by_width(dtype, g.kc, [&](auto t, auto kc) {
     using T = decltype(t);
     constexpr int KC = decltype(kc)::value;
@@ -390,8 +437,9 @@ hipError_t launch_seq_conv_bwd(const SeqConvGeom& g, const void* x, const float*
   });
 }
 
-hipError_t launch_seq_conv_step(const SeqConvGeom& g, const void* x, const float* w, const float* b, void* states,
+hipError_t launch_seq_conv_step(const SeqConvGeom& geom, const void* x, const float* w, const float* b, void* states,
                                 void* y, int dtype, hipStream_t s) {
+  const SeqConvGeom g = with_vec(geom, w, b);
   return by_width(dtype, g.kc, [&](auto t, auto kc) {
     using T = decltype(t);
     constexpr int KC = decltype(kc)::value, V = 16 / sizeof(T);

@@ -49,8 +49,10 @@ struct SeqScanGeom {
   int32_t N;
   SeqCut cut;
   int32_t multi;       // 0: every sequence is one chunk, no carries
+  int32_t fold;        // 1: the main pass joins the chunks before its own itself, 0: a carry pass does
   int32_t max_chunks;  // of a sequence, as far as the caller's max_len holds
   int32_t a_log, softplus;
+  int32_t a_vec, h_vec;  // rows of A, of the states, are read 16 bytes at a time
 };
 
 // Chunks whose aggregates a wave of the carry pass holds, and its waves.
@@ -113,6 +115,7 @@ struct SeqConvGeom {
   SeqGeom q;
   int64_t xs, ys;
   int32_t kc;
+  int32_t w_vec;  // taps and biases are read 16 bytes at a time
 };
 constexpr SeqCut kSeqConvCut = {64, 1u << 31, 5};  // 4 waves of 16 positions
 inline int64_t seq_conv_partial_floats(const SeqConvGeom& g) {
