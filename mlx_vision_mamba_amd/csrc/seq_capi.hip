@@ -91,43 +91,69 @@ mvm::SeqGeom seq_geom(const mvm_seq_desc& q) {
   return g;
 }
 
-// The cut into time chunks.  A wave is 64 channels of one chunk; the passes
-// run at the rate of the SIMDs' instruction issue once each of the 1024 SIMDs
-// has a few waves.  Chunks need an aggregate pass and a carry before the main
-// pass, which repeat most of the recurrence.  In cycles (measured on MI355X
-// at 2.4 GHz; lone: a wave by itself on its SIMD):
+// The cut into time chunks.  A wave is 64 channels of one chunk; chunks let
+// one sequence use more waves, but need an aggregate pass before the main one,
+// which repeats most of the recurrence, and their joining.  The cut is the
+// cheapest of those that put 1/4 to `waves` waves on each of the card's 1024
+// SIMDs, and of whole sequences, by a model of the passes in cycles (measured
+// on MI355X at 2.4 GHz): what one token more costs a SIMD of one, two, ..
+// waves.
 struct Cost {
-  int64_t waves;     // that the card holds at once
-  int64_t lone;      // main pass, cycles a token and wave
-  int64_t main_, agg;  // per token and wave, issued by a full SIMD
+  int waves;
+  int64_t agg[4], main_[4];
+  int64_t token(int64_t n) const {
+    const int64_t last = agg[waves - 1] + main_[waves - 1];
+    return n <= waves ? agg[n - 1] + main_[n - 1] : (last * n + waves - 1) / waves;
+  }
 };
-constexpr Cost kFwdCost = {4096, 800, 520, 420};
-constexpr Cost kBwdCost = {3072, 2000, 1500, 430};
-constexpr int64_t kFoldChunks = 16;
-constexpr int64_t kPassCycles = 24000;  // launches and start-up of the two extra passes
+constexpr Cost kFwdCost = {4, {540, 950, 1250, 1600}, {1100, 1420, 1900, 2090}};
+constexpr Cost kBwdCost = {3, {600, 1180, 1690}, {3000, 4300, 5400}};
+constexpr int64_t kSimds = 1024;
+constexpr int64_t kStart = 10000;  // a pass's launch and its waves' first loads,
+constexpr int64_t kStartWave = 3;  // those of many waves
+constexpr int64_t kFold = 1000;    // the main pass joins one chunk before its own
+constexpr int64_t kCarry = 9000;   // a carry pass,
+constexpr int64_t kCarryRound = 10000;  // its rounds of 128 chunks,
+constexpr int64_t kCarryWave = 3;       // and its traffic for one wave's aggregate
 
 void pick_chunk(const mvm_seq_scan_desc* d, const Cost& k, mvm::SeqScanGeom& g) {
   const int64_t T = d->seq.tokens, S = d->seq.nseq, ncb = std::max<int64_t>(1, ceil_div(d->seq.dim, 64));
   int64_t longest = d->seq.offsets == nullptr ? d->seq.seqlen : T;
   if (d->max_len > 0) longest = std::min(longest, d->max_len);
+  const auto join = [&](int64_t waves, int64_t nth, bool fold) {
+    return fold ? (nth - 1) * kFold * std::max<int64_t>(1, waves / kSimds)
+                : kCarry + ceil_div(nth, 128) * kCarryRound + waves * kCarryWave;
+  };
+  // (a sequence's last chunk is half a chunk on average)
+  const auto waves_of = [&](int64_t len) { return ncb * ceil_div(T + (S - 1) * len / 2, len); };
+  const auto cost = [&](int64_t len) {
+    const int64_t waves = waves_of(len), nth = ceil_div(longest, len);
+    return 2 * (kStart + waves * kStartWave) + len * k.token(ceil_div(waves, kSimds)) +
+           std::min(join(waves, nth, true), join(waves, nth, false));
+  };
   int64_t len = d->chunk_len;
   if (len == 0) {
-    // Chunks that fill the card once; a sequence's last one is half a chunk on
-    // average
-    const int64_t budget = std::max<int64_t>(1, k.waves / ncb), chunks = std::max(budget - S / 2, ceil_div(budget, 4));
-    len = std::max<int64_t>(16, ceil_div(ceil_div(T, chunks), mvm::kSeqTile) * mvm::kSeqTile);
-    // Whole sequences where the longest one by itself takes no longer
-    const int64_t work = T * ncb / 1024;
-    const int64_t whole = std::max(longest * k.lone, work * k.main_);
-    const int64_t cut = std::max(2 * len * k.lone, work * (k.main_ + k.agg)) + kPassCycles;
-    if (whole <= cut) len = longest;
+    // whole sequences: the longest by itself, or all the work (a SIMD's waves
+    // are of different lengths)
+    const int64_t full = k.main_[k.waves - 1] / k.waves;
+    int64_t best = kStart + std::max(longest * k.main_[0], T * ncb / kSimds * full + longest / 2 * full);
+    len = longest;
+    for (int64_t quarters = 1; quarters <= 4 * k.waves; quarters += quarters < 4 ? quarters : 4) {
+      const int64_t chunks = quarters * (kSimds / 4) / ncb - S / 2;
+      if (chunks < 1) continue;
+      const int64_t n = std::max<int64_t>(1, ceil_div(ceil_div(T, chunks), mvm::kSeqTile)) * mvm::kSeqTile;
+      if (n >= longest) continue;
+      const int64_t c = cost(n);
+      if (c < best) best = c, len = n;
+    }
   }
   g.multi = len < longest;
   // Whole sequences: one chunk whatever max_len says
   if (!g.multi) len = std::max<int64_t>(16, T + 1);
+  const int64_t nth = ceil_div(longest, len), waves = waves_of(len);
   g.cut = mvm::seq_cut(len);
-  g.fold = g.multi && ceil_div(longest, len) <= kFoldChunks;
-  g.max_chunks = g.multi ? static_cast<int32_t>(ceil_div(longest, len)) : 1;
+  g.fold = g.multi && join(waves, nth, true) <= join(waves, nth, false);
+  g.max_chunks = g.multi ? static_cast<int32_t>(nth) : 1;
 }
 
 mvm::SeqScanGeom scan_geom(const mvm_seq_scan_desc* d, bool backward) {

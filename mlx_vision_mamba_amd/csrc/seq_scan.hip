@@ -129,17 +129,16 @@ seq_scan_fwd_kernel(FwdArgs<T, DT, BT> args) {
     if (!AGG && p.ckpt != nullptr && valid)
       store_agg16(h, p.ckpt, (c.start >> kSeqTileShift) + c.seq + ((t - c.start) >> kSeqTileShift), D, d);
     float out[kSeqTile];
+    const int32_t left = c.t1 - t;
 #pragma unroll
     for (int i = 0; i < kSeqTile; ++i) {
       // B and C are on their way while the decays are formed
       float a[16];
       typename BcRows<BT>::template Raw<16> Bv, Cv;
       Bv.load(pb.at);
-      pb.next(t + i + 1 < c.t1);
-      if constexpr (!AGG) {
-        Cv.load(pc.at);
-        pc.next(t + i + 1 < c.t1);
-      }
+      if constexpr (!AGG) Cv.load(pc.at);
+      pb.next(i + 1 < left);
+      if constexpr (!AGG) pc.next(i + 1 < left);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int n = 0; n < 16; ++n) a[n] = fast_exp2(dl[i] * a2[n]);

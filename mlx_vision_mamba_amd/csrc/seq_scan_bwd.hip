@@ -65,9 +65,9 @@ seq_scan_bwd_agg_kernel(BwdArgs<T, DT, BT> args) {
   T ny[kSeqTile], nz[kSeqTile];
   DT nd[kSeqTile];
   auto fetch = [&](int32_t t) {
-    load_prev(nd, pd, t, c.t0, c.t1, lc);
-    load_prev(ny, py, t, c.t0, c.t1, lc);
-    if (gate) load_prev(nz, pz, t, c.t0, c.t1, lc);
+    load_prev(nd, pd, t, c.t1, lc);
+    load_prev(ny, py, t, c.t1, lc);
+    if (gate) load_prev(nz, pz, t, c.t1, lc);
   };
   const int32_t last = c.t0 + ((c.t1 - 1 - c.t0) & ~(kSeqTile - 1));
   fetch(last);
@@ -108,7 +108,7 @@ seq_scan_bwd_agg_kernel(BwdArgs<T, DT, BT> args) {
       float a[16];
       typename BcRows<BT>::template Raw<16> Cv;
       Cv.load(pc.at);
-      pc.prev(t + i < c.t1 && t + i > c.t0);
+      pc.prev(t + i < c.t1);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int n = 0; n < 16; ++n) a[n] = fast_exp2(dl[i] * a2[n]);
@@ -196,10 +196,10 @@ seq_scan_bwd_kernel(BwdArgs<T, DT, BT> args) {
   T nu[kSeqTile], ny[kSeqTile], nz[kSeqTile];
   DT nd[kSeqTile];
   auto fetch = [&](int32_t t) {
-    load_prev(nd, pd, t, c.t0, c.t1, lc);
-    load_prev(nu, pu, t, c.t0, c.t1, lc);
-    load_prev(ny, py, t, c.t0, c.t1, lc);
-    if (gate) load_prev(nz, pz, t, c.t0, c.t1, lc);
+    load_prev(nd, pd, t, c.t1, lc);
+    load_prev(nu, pu, t, c.t1, lc);
+    load_prev(ny, py, t, c.t1, lc);
+    if (gate) load_prev(nz, pz, t, c.t1, lc);
   };
   const int32_t row = seq_slot(g.q, c.seq);
   {

@@ -80,18 +80,19 @@ __device__ __forceinline__ void load_a2(float (&a)[COUNT], const float* A, int64
 template <int DIR>
 __device__ __forceinline__ void fold_chunks(float (&h)[16], const float (&a2)[16], const float* agg_h,
                                             const float* agg_s, int64_t base, int32_t nth, int64_t D, int64_t d) {
-  for (int32_t j0 = 0; j0 < nth; j0 += 2) {  // two chunks' loads in flight
-    Pack<float, 4> v[2][4];
-    float s[2];
+  constexpr int kBatch = 3;  // chunks whose loads are in flight together
+  for (int32_t j0 = 0; j0 < nth; j0 += kBatch) {
+    Pack<float, 4> v[kBatch][4];
+    float s[kBatch];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kBatch; ++i) {
       const int64_t slot = base + DIR * (j0 + i < nth ? j0 + i : j0);
 #pragma unroll
       for (int q = 0; q < 4; ++q) v[i][q] = load_pack<float, 4>(agg_h + ((slot * 4 + q) * D + d) * 4);
       s[i] = agg_s[slot * D + d];
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < kBatch; ++i)
       if (j0 + i < nth) {
 #pragma unroll
         for (int n = 0; n < 16; ++n) h[n] = fmaf(fast_exp2(a2[n] * s[i]), h[n], v[i][n >> 2].v[n & 3]);
@@ -171,7 +172,7 @@ struct RowPtr {
     at += go ? st : 0u;
     asm volatile("" : "+s"(at));
   }
-  __device__ __forceinline__ void prev(bool go) {
+  __device__ __forceinline__ void prev(bool go = true) {
     at -= go ? st : 0u;
     asm volatile("" : "+s"(at));
   }
@@ -194,21 +195,36 @@ struct RowPtr {
 // The next kSeqTile rows, from row t on; rows past the chunk read its last one.
 template <typename T>
 __device__ __forceinline__ void load_next(T (&v)[kSeqTile], RowPtr& p, int32_t t, int32_t t1, uint32_t lane) {
+  if (t + kSeqTile <= t1) {
 #pragma unroll
-  for (int i = 0; i < kSeqTile; ++i) {
-    v[i] = p.load<T>(lane);
-    p.next(t + i + 1 < t1);
+    for (int i = 0; i < kSeqTile; ++i) {
+      v[i] = p.load<T>(lane);
+      p.next();
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kSeqTile; ++i) {
+      v[i] = p.load<T>(lane);
+      p.next(t + i + 1 < t1);
+    }
   }
 }
 // The kSeqTile rows from row t on, last one first: p is at row t + 7, or at
-// the chunk's last, and comes to rest at row t - 1 (t0 at the least).
+// the chunk's last, and comes to rest at row t - 1.
 template <typename T>
-__device__ __forceinline__ void load_prev(T (&v)[kSeqTile], RowPtr& p, int32_t t, int32_t t0, int32_t t1,
-                                          uint32_t lane) {
+__device__ __forceinline__ void load_prev(T (&v)[kSeqTile], RowPtr& p, int32_t t, int32_t t1, uint32_t lane) {
+  if (t + kSeqTile <= t1) {
 #pragma unroll
-  for (int i = kSeqTile - 1; i >= 0; --i) {
-    v[i] = p.load<T>(lane);
-    p.prev(t + i < t1 && t + i > t0);
+    for (int i = kSeqTile - 1; i >= 0; --i) {
+      v[i] = p.load<T>(lane);
+      p.prev();
+    }
+  } else {
+#pragma unroll
+    for (int i = kSeqTile - 1; i >= 0; --i) {
+      v[i] = p.load<T>(lane);
+      p.prev(t + i < t1);
+    }
   }
 }
 // The first `rows` of the next kSeqTile rows.
