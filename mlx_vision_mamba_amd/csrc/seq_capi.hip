@@ -178,8 +178,9 @@ int check_scan(const mvm_seq_scan_desc* d) {
   for (int backward = 0; rc == MVM_OK && backward < 2; ++backward) {
     const mvm::SeqScanGeom g = scan_geom(d, backward != 0);
     const int64_t carry = g.multi ? ceil_div(g.q.D, 16) * g.q.S : 0;
-    if ((rc = check_threads(d->seq, mvm::chunk_slots(g.q, g.cut), ceil_div(g.q.D, 64) * 64)) == MVM_OK)
-      rc = check_threads(d->seq, carry, 64 * mvm::carry_waves(g));
+    if ((rc = check_threads(d->seq, mvm::chunk_slots(g.q, g.cut), ceil_div(g.q.D, 64) * 64)) == MVM_OK &&
+        (rc = check_threads(d->seq, carry, 64 * mvm::carry_waves(g))) == MVM_OK)
+      rc = check_threads(d->seq, g.q.D, 18 * 16);  // the reduction's workgroups of 64 columns
   }
   return rc;
 }

@@ -155,7 +155,9 @@ __device__ __forceinline__ float wave_sums16(const float (&v)[16], int lane) {
 // All of a wave's LDS is its own: no barrier.
 struct BwdLds {
   Pack<float, 4> a2[4][kWave], c[4][kWave], da[4][kWave];
-  float bc[16][17];  // the tile's sums: [token | 8 for dC][state]
+  // per state B of the 8 tokens, C of the 8; replaced, once the state is done,
+  // by the tile's sums for dB and dC
+  Pack<float, 4> bc[16][4];
 };
 
 template <typename T, typename DT, typename BT>
@@ -195,7 +197,9 @@ seq_scan_bwd_kernel(BwdArgs<T, DT, BT> args) {
   if (gate) pz.set(args.z + d0, c.t1 - 1, g.zs);
   T nu[kSeqTile], ny[kSeqTile], nz[kSeqTile];
   DT nd[kSeqTile];
+  BcTile<BT> nbc;
   auto fetch = [&](int32_t t) {
+    nbc.fetch(args.bc.B, args.bc.C, args.bc.st, t, c.t1, 16, lane);
     load_prev(nd, pd, t, c.t1, lc);
     load_prev(nu, pu, t, c.t1, lc);
     load_prev(ny, py, t, c.t1, lc);
@@ -234,6 +238,11 @@ seq_scan_bwd_kernel(BwdArgs<T, DT, BT> args) {
     float dl[kSeqTile], du[kSeqTile], dr[kSeqTile], qs[kSeqTile], ws[kSeqTile], rs[kSeqTile];
     float us[kSeqTile], sg[kSeqTile], gz[kSeqTile];  // for the outputs
     fetch(t);
+    lds_order();
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      reinterpret_cast<float*>(s.bc)[(4 * (lane & 3) + j) * 16 + 2 * (lane & 4) + (lane >> 3)] = nbc.value(j, 16, lane);
+    lds_order();
 #pragma unroll
     for (int i = 0; i < kSeqTile; ++i) {
       us[i] = to_f32(nu[i]);
@@ -278,22 +287,18 @@ seq_scan_bwd_kernel(BwdArgs<T, DT, BT> args) {
       const Pack<float, 4> a2 = s.a2[q][lane];
       Pack<float, 4> cs = s.c[q][lane], da = s.da[q][lane], h4 = hs;
       if (q < 3) hs = load_pack<float, 4>(ck + (q + 1) * 4 * D);
-      typename BcRows<BT>::template Raw<2> Bv[kSeqTile], Cv[kSeqTile];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         __builtin_amdgcn_sched_barrier(0);
-        if (j % 2 == 0) {  // two states at a time: what the scalar registers hold
-          RowPtr pb, pc;
-          pb.set(args.bc.B + 4 * q + j, t, args.bc.st);
-          pc.set(args.bc.C + 4 * q + j, t, args.bc.st);
+        float Bv[kSeqTile], Cv[kSeqTile];
 #pragma unroll
-          for (int i = 0; i < kSeqTile; ++i) {
-            Bv[i].load(pb.at);
-            Cv[i].load(pc.at);
-            pb.next(t + i + 1 < c.t1);
-            pc.next(t + i + 1 < c.t1);
+        for (int k = 0; k < 2; ++k) {
+          const Pack<float, 4> bk = s.bc[4 * q + j][k], ck4 = s.bc[4 * q + j][2 + k];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            Bv[4 * k + i] = bk.v[i];
+            Cv[4 * k + i] = ck4.v[i];
           }
-          __builtin_amdgcn_sched_barrier(0);
         }
         float h = valid ? h4.v[j] : 0.f;
         float a[kSeqTile], ah[kSeqTile], v[16];  // v: the terms of dB of the 8 tokens, then those of dC
@@ -301,36 +306,36 @@ seq_scan_bwd_kernel(BwdArgs<T, DT, BT> args) {
         for (int i = 0; i < kSeqTile; ++i) {
           a[i] = fast_exp2(dl[i] * a2.v[j]);
           ah[i] = a[i] * h;
-          h = fmaf(du[i], Bv[i][j & 1], ah[i]);
-          rs[i] = fmaf(h, Cv[i][j & 1], rs[i]);
+          h = fmaf(du[i], Bv[i], ah[i]);
+          rs[i] = fmaf(h, Cv[i], rs[i]);
           v[8 + i] = dr[i] * h;
         }
 #pragma unroll
         for (int i = kSeqTile - 1; i >= 0; --i) {
-          const float dh = fmaf(Cv[i][j & 1], dr[i], cs.v[j]);
-          qs[i] = fmaf(dh, Bv[i][j & 1], qs[i]);
+          const float dh = fmaf(Cv[i], dr[i], cs.v[j]);
+          qs[i] = fmaf(dh, Bv[i], qs[i]);
           v[i] = dh * du[i];
           const float w = dh * ah[i];
           da.v[j] = fmaf(w, dl[i], da.v[j]);
           ws[i] = fmaf(w, a2.v[j], ws[i]);
           cs.v[j] = dh * a[i];
         }
-        s.bc[lane >> 2][4 * q + j] = wave_sums16(v, lane);  // (four lanes, one value)
+        reinterpret_cast<float*>(s.bc[4 * q + j])[lane >> 2] = wave_sums16(v, lane);  // (four lanes, one value)
       }
       s.c[q][lane] = cs;
       s.da[q][lane] = da;
     }
     const auto& late = late_args<BwdArgs<T, DT, BT>>();
-    __builtin_amdgcn_wave_barrier();
+    lds_order();
     // rows t .. t + 7 of 32 values: dB at 0, dC at 16
     float* out = late.p.part_bc + (static_cast<int64_t>(pos.cb) * g.q.T + t) * 32;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int i = k * 2 + (lane >> 5), n = lane & 31;
-      const float v = s.bc[i + ((n >> 4) << 3)][n & 15];
+      const float v = reinterpret_cast<const float*>(s.bc)[(n & 15) * 16 + (n >> 4) * 8 + i];
       if (t + i < c.t1) out[i * 32 + n] = v;
     }
-    __builtin_amdgcn_wave_barrier();
+    lds_order();
     const int32_t rows = c.t1 - t < kSeqTile ? c.t1 - t : kSeqTile;
 #pragma unroll
     for (int i = 0; i < kSeqTile; ++i) {
@@ -366,40 +371,46 @@ seq_scan_bwd_kernel(BwdArgs<T, DT, BT> args) {
   part[17 * D] = ddb;
 }
 
-// dA, dD and ddelta_bias: the chunks' sums, added in order.
-__global__ void __launch_bounds__(1024)
-seq_reduce_params_kernel(int64_t D, int32_t N, int64_t nparts, int a_log, const float* __restrict__ A,
-                         const float* __restrict__ part, float* __restrict__ dA, float* __restrict__ dD,
-                         float* __restrict__ ddb) {
-  sum_columns(part, nparts, 18 * D, [&](int64_t col, float s) {
-    const int64_t k = col / D, d = col - k * D;
-    if (k < N)
-      dA[d * N + k] = a_log ? s * -expf(A[d * N + k]) : s;  // of A_log: A' = A
-    else if (k == 16)
-      dD[d] = s;
-    else if (k == 17 && ddb != nullptr)
-      ddb[d] = s;
-  });
-}
-
-// dB and dC: the channel blocks' sums, added in order.
+// The first `pblocks` workgroups: dA, dD and ddelta_bias, the chunks' sums added
+// in order.  The others: dB and dC, the channel blocks' sums added in order.
 template <typename T>
-__global__ void __launch_bounds__(256)
-seq_reduce_bc_kernel(int32_t rows, int32_t N, int32_t ncb, const float* __restrict__ part, T* __restrict__ dB,
-                     T* __restrict__ dC) {
-  const int64_t total = static_cast<int64_t>(rows) * 32, step = static_cast<int64_t>(gridDim.x) * 256;
+struct ReduceArgs {
+  int64_t D, nparts;
+  int32_t N, a_log, rows, ncb;
+  uint32_t pblocks;
+  const float *A, *part, *part_bc;
+  float *dA, *dD, *ddb;
+  T *dB, *dC;
+};
+template <typename T>
+__global__ void __launch_bounds__(1024)
+seq_reduce_kernel(ReduceArgs<T> r) {
+  if (blockIdx.x < r.pblocks) {
+    sum_columns(r.part, r.nparts, 18 * r.D, [&](int64_t col, float s) {
+      const int64_t k = col / r.D, d = col - k * r.D;
+      if (k < r.N)
+        r.dA[d * r.N + k] = r.a_log ? s * -expf(r.A[d * r.N + k]) : s;  // of A_log: A' = A
+      else if (k == 16)
+        r.dD[d] = s;
+      else if (k == 17 && r.ddb != nullptr)
+        r.ddb[d] = s;
+    });
+    return;
+  }
+  const int64_t total = static_cast<int64_t>(r.rows) * 32;
+  const int64_t step = static_cast<int64_t>(gridDim.x - r.pblocks) * 1024;
   const int n = threadIdx.x & 15;
-  T* out = (threadIdx.x & 16) ? dC : dB;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total; i += step) {
+  T* out = (threadIdx.x & 16) ? r.dC : r.dB;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x - r.pblocks) * 1024 + threadIdx.x; i < total; i += step) {
     float s = 0.f;
-    for (int32_t k0 = 0; k0 < ncb; k0 += 8) {
+    for (int32_t k0 = 0; k0 < r.ncb; k0 += 8) {
       float v[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = part[(k0 + k < ncb ? k0 + k : 0) * total + i];
+      for (int k = 0; k < 8; ++k) v[k] = r.part_bc[(k0 + k < r.ncb ? k0 + k : 0) * total + i];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) s += k0 + k < ncb ? v[k] : 0.f;
+      for (int k = 0; k < 8; ++k) s += k0 + k < r.ncb ? v[k] : 0.f;
     }
-    if (n < N) out[(i >> 5) * N + n] = from_f32<T>(s);
+    if (n < r.N) out[(i >> 5) * r.N + n] = from_f32<T>(s);
   }
 }
 
@@ -424,13 +435,11 @@ hipError_t bwd_t(SeqScanGeom g, const SeqScanIn& in, const SeqScanBwd& b, BcRows
   }
   hipLaunchKernelGGL((seq_scan_bwd_kernel<T, DT, BT>), grid, dim3(256), 0, s, args);
   if ((e = hipGetLastError()) != hipSuccess) return e;
-  hipLaunchKernelGGL(seq_reduce_params_kernel, dim3(static_cast<unsigned>((18 * g.q.D + 63) / 64)), dim3(1024), 0, s,
-                     g.q.D, g.N, slots, g.a_log, in.A, b.part, b.dA, b.dD, b.ddbias);
-  if ((e = hipGetLastError()) != hipSuccess) return e;
-  const int64_t n = static_cast<int64_t>(g.q.T) * 32;
-  if (n == 0) return hipSuccess;
-  hipLaunchKernelGGL(seq_reduce_bc_kernel<T>, strided_grid(n), dim3(256), 0, s, g.q.T, g.N, static_cast<int32_t>(ncb),
-                     b.part_bc, static_cast<T*>(b.dB), static_cast<T*>(b.dC));
+  const uint32_t pblocks = static_cast<uint32_t>((18 * g.q.D + 63) / 64);
+  const int64_t bblocks = std::min<int64_t>((static_cast<int64_t>(g.q.T) * 32 + 1023) / 1024, 1 << 18);
+  const ReduceArgs<T> red{g.q.D, slots, g.N, g.a_log, g.q.T, static_cast<int32_t>(ncb), pblocks, in.A, b.part, b.part_bc,
+                          b.dA, b.dD, b.ddbias, static_cast<T*>(b.dB), static_cast<T*>(b.dC)};
+  hipLaunchKernelGGL(seq_reduce_kernel<T>, dim3(pblocks + static_cast<unsigned>(bblocks)), dim3(1024), 0, s, red);
   return hipGetLastError();
 }
 

@@ -156,6 +156,30 @@ struct BcRows<bf16_t> {
 // x is computed here: the compiler would move a sum that only a branch uses
 // into the branch, and keep all its terms in registers until then
 __device__ __forceinline__ void pin(float& x) { asm volatile("" : "+v"(x)); }
+// B and C of a tile on their way: lane l asks for states 4 (l & 3) .. + 3 of
+// row l >> 3, of B or (l & 4) of C; rows past the chunk are its last one.
+template <typename T>
+struct BcTile {
+  T raw[4];
+  __device__ __forceinline__ void fetch(const T* B, const T* C, int64_t st, int32_t t, int32_t t1, int N,
+                                        uint32_t lane) {
+    const int32_t i = t + static_cast<int32_t>(lane >> 3);
+    const T* row = ((lane & 4) ? C : B) + (i < t1 ? i : t1 - 1) * st;
+    const int n0 = 4 * (lane & 3);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) raw[j] = row[state_col(n0 + j, N)];
+  }
+  __device__ __forceinline__ float value(int j, int N, uint32_t lane) const {
+    return static_cast<int>(4 * (lane & 3)) + j < N ? to_f32(raw[j]) : 0.f;
+  }
+};
+// orders a wave's own LDS accesses for the compiler (the unit keeps them in order)
+__device__ __forceinline__ void lds_order() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // A row of a tensor as a wave walks along it: a wave-uniform address that
 // moves by whole rows.  The empty asm keeps each step's sum in the scalar unit
 // where it stands: left to itself the compiler forms the addresses of all rows
