@@ -239,7 +239,7 @@ int check_conv(const mvm_seq_conv_desc* d) {
   const int64_t t = d->seq.tokens, c = d->seq.dim;
   if ((rc = check_rows("x_stride", d->x_stride, t, c, false)) || (rc = check_rows("y_stride", d->y_stride, t, c, true)))
     return rc;
-  return check_threads(d->seq, t / mvm::kSeqConvCut.len + d->seq.nseq + 1, ceil_div(c, 64) * 256);
+  return check_threads(d->seq, t / mvm::conv_cut(4).len + d->seq.nseq + 1, ceil_div(c, 64) * 256);
 }
 
 mvm::SeqConvGeom conv_geom(const mvm_seq_conv_desc* d) {
@@ -248,6 +248,13 @@ mvm::SeqConvGeom conv_geom(const mvm_seq_conv_desc* d) {
   g.xs = d->x_stride;
   g.ys = d->y_stride;
   g.kc = static_cast<int32_t>(d->kwidth);
+  // waves with 16 bytes a lane (backward: two channels) at the longer runs.
+  // MI355X, forward: 392 tokens of 1536 bf16 channels 6.4 us by runs of 8, 5.1
+  // by 4; 12000 tokens 19.5 and 21.0
+  const int64_t lanes = d->dtype == MVM_F32 ? 4 : 8, t = d->seq.tokens;
+  // (a run is at least the window's earlier positions)
+  g.fwd_pos = d->kwidth > 5 || ceil_div(d->seq.dim, 64 * lanes) * (t / 8) >= 1536 ? 8 : 4;
+  g.bwd_pos = ceil_div(d->seq.dim, 128) * (t / 16) >= 1536 ? 16 : 8;
   return g;
 }
 

@@ -6,11 +6,11 @@
 // and the final state is the last kc - 1 rows of x~.
 //
 // Bound by the rows' traffic.  A lane holds V consecutive channels (16 bytes
-// where the layout allows it), a wave 16 positions of one sequence with their
+// where the layout allows it), a wave P positions of one sequence with their
 // whole window in registers, so that all its loads are in flight together; a
-// block is four such waves, 64 positions.  The first block of a sequence is
-// the only one that reads its initial state (kc - 1 < 16 positions), and it
-// also writes the final one: both may be one buffer.
+// block is four such waves.  The first wave of a sequence is the only one that
+// reads its initial state (kc - 1 <= P), and it also writes the final one: both
+// may be one buffer.
 #include <initializer_list>
 #include <type_traits>
 
@@ -21,8 +21,6 @@
 namespace mvm {
 
 namespace {
-
-constexpr int kPos = 16;  // positions per wave
 
 // Row p of x~ of a sequence, p counted from its first token (p < 0: the
 // state's row kc - 1 + p); zero where there is none.
@@ -73,22 +71,23 @@ struct Taps {
   }
 };
 
-template <typename T, int V, int KC>
+template <typename T, int V, int KC, int P>
 __global__ void __launch_bounds__(256)
 seq_conv_fwd_kernel(SeqConvGeom g, uint32_t ncb, const T* __restrict__ x, const float* __restrict__ w,
                     const float* __restrict__ bias, const T* c0, T* c1, T* __restrict__ y) {
+  static_assert(KC - 1 <= P, "a second wave would read the state that the first one writes");
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const BlockPos pos = block_pos(ncb);
-  const SeqChunk c = seq_chunk(g.q, pos.slot, kSeqConvCut, lane);
+  const SeqChunk c = seq_chunk(g.q, pos.slot, conv_cut(P), lane);
   const int64_t D = g.q.D, d = (static_cast<int64_t>(pos.cb) * 64 + lane) * V;
   if (c.t0 < 0 || d >= D) return;
-  const int32_t s0 = c.t0 + wave * kPos;
+  const int32_t s0 = c.t0 + wave * P;
   if (c.seq == g.q.S) {  // rows of no sequence
     Pack<T, V> zero;
 #pragma unroll
     for (int v = 0; v < V; ++v) zero.v[v] = from_f32<T>(0.f);
-    for (int32_t t = s0; t < c.t1 && t < s0 + kPos; ++t) store_pack(y + t * g.ys + d, zero);
+    for (int32_t t = s0; t < c.t1 && t < s0 + P; ++t) store_pack(y + t * g.ys + d, zero);
     return;
   }
   const int32_t row = seq_slot(g.q, c.seq);
@@ -98,17 +97,17 @@ seq_conv_fwd_kernel(SeqConvGeom g, uint32_t ncb, const T* __restrict__ x, const 
     Taps<V, KC> k;
     k.load(w, bias, d, g.w_vec);
     const int64_t p0 = s0 - c.start;
-    Pack<T, V> win[kPos + KC - 1];
-    if (p0 >= KC - 1 && s0 + kPos <= c.end) {
+    Pack<T, V> win[P + KC - 1];
+    if (p0 >= KC - 1 && s0 + P <= c.end) {
 #pragma unroll
-      for (int i = 0; i < kPos + KC - 1; ++i) win[i] = load_pack<T, V>(x + (s0 - (KC - 1) + i) * g.xs + d);
+      for (int i = 0; i < P + KC - 1; ++i) win[i] = load_pack<T, V>(x + (s0 - (KC - 1) + i) * g.xs + d);
     } else {
 #pragma unroll
-      for (int i = 0; i < kPos + KC - 1; ++i)
+      for (int i = 0; i < P + KC - 1; ++i)
         win[i] = row_of_seq<T, V, KC>(x, g.xs, c, state, D, d, p0 - (KC - 1) + i);
     }
 #pragma unroll
-    for (int i = 0; i < kPos; ++i) {
+    for (int i = 0; i < P; ++i) {
       if (s0 + i < c.t1) {
         Pack<T, V> o;
 #pragma unroll
@@ -136,7 +135,7 @@ seq_conv_fwd_kernel(SeqConvGeom g, uint32_t ncb, const T* __restrict__ x, const 
   }
 }
 
-template <typename T, int V, int KC>
+template <typename T, int V, int KC, int P>
 __global__ void __launch_bounds__(256)
 seq_conv_bwd_kernel(SeqConvGeom g, uint32_t ncb, const T* __restrict__ x, const float* __restrict__ w,
                     const float* __restrict__ bias, const T* __restrict__ c0, const T* __restrict__ dy,
@@ -145,11 +144,11 @@ seq_conv_bwd_kernel(SeqConvGeom g, uint32_t ncb, const T* __restrict__ x, const 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const BlockPos pos = block_pos(ncb);
-  const SeqChunk c = seq_chunk(g.q, pos.slot, kSeqConvCut, lane);
+  const SeqChunk c = seq_chunk(g.q, pos.slot, conv_cut(P), lane);
   const int64_t D = g.q.D, d = (static_cast<int64_t>(pos.cb) * 64 + lane) * V;
   const bool valid = d < D;
   const int64_t dd = valid ? d : 0;
-  const int32_t s0 = c.t0 + wave * kPos;
+  const int32_t s0 = c.t0 + wave * P;
   float dw[KC][V], db[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
@@ -161,7 +160,7 @@ seq_conv_bwd_kernel(SeqConvGeom g, uint32_t ncb, const T* __restrict__ x, const 
     Pack<T, V> zero;
 #pragma unroll
     for (int v = 0; v < V; ++v) zero.v[v] = from_f32<T>(0.f);
-    for (int32_t t = s0; t < c.t1 && t < s0 + kPos; ++t)
+    for (int32_t t = s0; t < c.t1 && t < s0 + P; ++t)
       if (valid) store_pack(dx + static_cast<int64_t>(t) * D + d, zero);
   } else if (c.t0 >= 0) {
     const T* state = c0 != nullptr ? c0 + static_cast<int64_t>(c.seq) * (KC - 1) * D : nullptr;
@@ -179,7 +178,7 @@ seq_conv_bwd_kernel(SeqConvGeom g, uint32_t ncb, const T* __restrict__ x, const 
     if (s0 < c.t1 || head) {
       Taps<V, KC> k;
       k.load(w, bias, dd, g.w_vec);
-      constexpr int kG = kPos + KC - 1;  // positions whose dpre is needed
+      constexpr int kG = P + KC - 1;  // positions whose dpre is needed
       Pack<T, V> xw[kG + KC - 1], gy[kG];
 #pragma unroll
       for (int i = 0; i < kG + KC - 1; ++i)
@@ -205,7 +204,7 @@ seq_conv_bwd_kernel(SeqConvGeom g, uint32_t ncb, const T* __restrict__ x, const 
           gp[i][v] = p0 + i < len ? to_f32(gy[i].v[v]) * sg * fmaf(pre, 1.f - sg, 1.f) : 0.f;
         }
 #pragma unroll
-      for (int i = 0; i < kPos; ++i) {
+      for (int i = 0; i < P; ++i) {
         if (s0 + i < c.t1) {
           float a[V];
 #pragma unroll
@@ -375,21 +374,31 @@ template <typename T, int V, int KC>
 hipError_t fwd_v(const SeqConvGeom& g, const void* x, const float* w, const float* b, const void* c0, void* c1, void* y,
                  hipStream_t s) {
   const uint32_t ncb = conv_blocks<V>(g);
-  hipLaunchKernelGGL((seq_conv_fwd_kernel<T, V, KC>), dim3(static_cast<unsigned>(chunk_slots(g.q, kSeqConvCut) * ncb)),
-                     dim3(256), 0, s, g, ncb, static_cast<const T*>(x), w, b, static_cast<const T*>(c0),
-                     static_cast<T*>(c1), static_cast<T*>(y));
-  return hipGetLastError();
+  auto run = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(chunk_slots(g.q, conv_cut(g.fwd_pos)) * ncb)), dim3(256), 0,
+                       s, g, ncb, static_cast<const T*>(x), w, b, static_cast<const T*>(c0), static_cast<T*>(c1),
+                       static_cast<T*>(y));
+    return hipGetLastError();
+  };
+  if constexpr (KC - 1 <= 4) {
+    if (g.fwd_pos == 4) return run(seq_conv_fwd_kernel<T, V, KC, 4>);
+  }
+  return run(seq_conv_fwd_kernel<T, V, KC, 8>);
 }
 
 template <typename T, int V, int KC>
 hipError_t bwd_v(const SeqConvGeom& g, const void* x, const float* w, const float* b, const void* c0, const void* dy,
                  const void* dc1, void* dx, float* dw, float* db, void* dc0, float* part, hipStream_t s) {
   const uint32_t ncb = conv_blocks<V>(g);
-  const int64_t slots = chunk_slots(g.q, kSeqConvCut), ncols = g.q.D * (KC + 1);
-  hipLaunchKernelGGL((seq_conv_bwd_kernel<T, V, KC>), dim3(static_cast<unsigned>(slots * ncb)), dim3(256), 0, s, g, ncb,
-                     static_cast<const T*>(x), w, b, static_cast<const T*>(c0), static_cast<const T*>(dy),
-                     static_cast<const T*>(dc1), static_cast<T*>(dx), static_cast<T*>(dc0), part);
-  const hipError_t e = hipGetLastError();
+  const int64_t slots = chunk_slots(g.q, conv_cut(g.bwd_pos)), ncols = g.q.D * (KC + 1);
+  auto run = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(slots * ncb)), dim3(256), 0, s, g, ncb,
+                       static_cast<const T*>(x), w, b, static_cast<const T*>(c0), static_cast<const T*>(dy),
+                       static_cast<const T*>(dc1), static_cast<T*>(dx), static_cast<T*>(dc0), part);
+    return hipGetLastError();
+  };
+  const hipError_t e =
+      g.bwd_pos == 16 ? run(seq_conv_bwd_kernel<T, V, KC, 16>) : run(seq_conv_bwd_kernel<T, V, KC, 8>);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(seq_conv_reduce_kernel, dim3(static_cast<unsigned>((ncols + 63) / 64)), dim3(1024), 0, s, ncols,
                      static_cast<int32_t>(KC), slots, part, dw, db);

@@ -115,11 +115,16 @@ struct SeqConvGeom {
   SeqGeom q;
   int64_t xs, ys;
   int32_t kc;
+  int32_t fwd_pos, bwd_pos;  // 4 or 8, 8 or 16: positions of a wave
   int32_t w_vec;  // taps and biases are read 16 bytes at a time
 };
-constexpr SeqCut kSeqConvCut = {64, 1u << 31, 5};  // 4 waves of 16 positions
+// A wave takes `pos` positions, a workgroup's chunk is four such runs: short
+// ones while the card is not full, longer ones read fewer rows twice.
+constexpr SeqCut conv_cut(int pos) {
+  return {4u * pos, 1u << 31, pos == 4 ? 3u : (pos == 8 ? 4u : 5u)};
+}
 inline int64_t seq_conv_partial_floats(const SeqConvGeom& g) {
-  return chunk_slots(g.q, kSeqConvCut) * g.q.D * (g.kc + 1);
+  return chunk_slots(g.q, conv_cut(g.bwd_pos)) * g.q.D * (g.kc + 1);
 }
 hipError_t launch_seq_conv_fwd(const SeqConvGeom& g, const void* x, const float* w, const float* b, const void* c0,
                                void* c1, void* y, int dtype, hipStream_t s);
