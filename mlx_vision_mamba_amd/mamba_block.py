@@ -43,9 +43,11 @@ import torch.nn.functional as F
 
 from . import _lib
 from . import directions as _dirs
-from .conv import causal_conv_silu
+from .conv import causal_conv_silu, causal_conv_silu_packed, causal_conv_silu_prefill, causal_conv_silu_step
+from .gemm import in_proj
 from .norm import layer_norm
-from .scan import _resolve_chunk, check_permutation_table, get_scan_fn, mode_chunk_len
+from .scan import (_resolve_chunk, check_permutation_table, get_scan_fn, mode_chunk_len, selective_scan_packed,
+                   selective_scan_prefill, selective_scan_step)
 
 
 def _dt_bias_init(d_inner: int, dt_min: float = 1e-3, dt_max: float = 1e-1) -> torch.Tensor:
@@ -97,6 +99,56 @@ class MambaBlock(nn.Module):
             return _scan_fn_forward(self, x)
         return _directional_forward([self], x, None, self.scan_mode)
 
+    # ---- packed and served sequences: the same function of each sequence as
+    # ``forward``, of tokens that continue earlier ones
+
+    def init_states(self, rows: int, dtype=None, device=None):
+        """Zero states of ``rows`` sequences: the conv's last inputs, (rows,
+        d_conv - 1, d_inner) of the activations' type (default: the
+        parameters'), and the scan's states, (rows, d_inner, d_state) float32."""
+        w = self.in_proj.weight
+        device = w.device if device is None else device
+        return (torch.zeros(rows, self.d_conv - 1, self.d_inner, dtype=dtype or w.dtype, device=device),
+                torch.zeros(rows, self.d_inner, self.d_state, device=device))
+
+    def forward_packed(self, x, offsets=None, states=None, *, max_len=None):
+        """(y, states) of sequences packed without padding: x (T, d_model) with
+        ``offsets`` (see ``scan.selective_scan_packed``), or (B, L, d_model)
+        without.  ``states``: what ``forward_packed`` of the tokens before gave
+        (default: zero).  Differentiable, through both states too."""
+        conv0, scan0 = states if states is not None else (None, None)
+        out = []
+
+        def conv(xb, w, b):
+            y, c = causal_conv_silu_packed(xb, w, b, offsets, initial_states=conv0)
+            out.append(c)
+            return y
+
+        def scan(*args, **kw):
+            y, h = selective_scan_packed(*args, offsets, initial_states=scan0, max_len=max_len, **kw)
+            out.append(h)
+            return y
+
+        return _recurrent_forward(self, x, conv, scan), tuple(out)
+
+    def prefill(self, x, states, offsets=None, *, slots=None, fresh=None, max_len=None):
+        """y of prompts, or of pieces of them, packed as in ``forward_packed``:
+        sequence i continues row slots[i] of the cache ``states`` (from
+        ``init_states``) and leaves its states there; fresh[i] starts it from
+        zero.  No gradients."""
+        return _recurrent_forward(
+            self, x,
+            lambda xb, w, b: causal_conv_silu_prefill(xb, w, b, states[0], offsets, slots=slots, fresh=fresh),
+            lambda *a, **kw: selective_scan_prefill(*a, states[1], offsets, slots=slots, fresh=fresh,
+                                                    max_len=max_len, **kw))
+
+    def step(self, x, states, *, slots=None):
+        """y (S, d_model) of one token for each of S sequences, x (S, d_model);
+        ``states`` and ``slots`` as in ``prefill``.  No gradients."""
+        return _recurrent_forward(
+            self, x, lambda xb, w, b: causal_conv_silu_step(xb, w, b, states[0], slots=slots),
+            lambda *a, **kw: selective_scan_step(*a, states[1], slots=slots, **kw))
+
 
 class ResidualMambaBlock(nn.Module):
     """Pre-norm MambaBlock with a residual (mamba_block.py:195-205)."""
@@ -110,6 +162,24 @@ class ResidualMambaBlock(nn.Module):
     def forward(self, x):
         h, xr = layer_norm(x, self.norm, residual=True)
         return xr + self.mamba(h)
+
+    def init_states(self, rows: int, dtype=None, device=None):
+        return self.mamba.init_states(rows, dtype, device)
+
+    def forward_packed(self, x, offsets=None, states=None, *, max_len=None):
+        """``MambaBlock.forward_packed`` with the norm and the residual."""
+        h, xr = layer_norm(x, self.norm, residual=True)
+        y, states = self.mamba.forward_packed(h, offsets, states, max_len=max_len)
+        return xr + y, states
+
+    def prefill(self, x, states, offsets=None, *, slots=None, fresh=None, max_len=None):
+        """``MambaBlock.prefill`` with the norm and the residual."""
+        return x + self.mamba.prefill(layer_norm(x, self.norm), states, offsets, slots=slots, fresh=fresh,
+                                      max_len=max_len)
+
+    def step(self, x, states, *, slots=None):
+        """``MambaBlock.step`` with the norm and the residual."""
+        return x + self.mamba.step(layer_norm(x, self.norm), states, slots=slots)
 
 
 class BidirectionalMambaBlock(nn.Module):
@@ -284,6 +354,28 @@ def _scan_fn_forward(blk, x):
     y = blk._scan_fn(xc, delta, A, Bm, Cm, blk.D)                              # :187
     y = y * F.silu(z)                                                          # :190
     return F.linear(y, blk.out_proj.weight)                                    # :191
+
+
+def _linear(x, w):
+    """x @ w^T: float32 by the package's products, other types by the library's."""
+    return in_proj(x, w) if x.dtype == torch.float32 else F.linear(x, w)
+
+
+def _recurrent_forward(blk, x, conv, scan):
+    """MambaBlock's op sequence on rows of tokens, with the given conv and
+    scan; the latter forms softplus(delta + bias), -exp(A_log) and the gate.
+    The halves of in_proj's output and the columns of x_proj's are passed as
+    they lie."""
+    if _custom_scan(blk):
+        raise ValueError("a block whose _scan_fn was replaced has no packed or served form")
+    din, ns, R = blk.d_inner, blk.d_state, blk.dt_rank
+    xz = _linear(x, blk.in_proj.weight)
+    xc = conv(xz[..., :din], blk.conv1d.weight.reshape(din, blk.d_conv), blk.conv1d.bias)
+    dbc = _linear(xc, blk.x_proj.weight)
+    delta = _linear(dbc[..., :R], blk.dt_proj.weight)
+    y = scan(xc, delta, blk.A_log, dbc[..., R:R + ns], dbc[..., R + ns:], blk.D, z=xz[..., din:],
+             delta_bias=blk.dt_proj.bias, delta_softplus=True, a_is_log=True)
+    return _linear(y, blk.out_proj.weight)
 
 
 def _per_direction_forward(blocks, h, tok):
