@@ -273,3 +273,32 @@ def test_oracle_bound_notices_a_wrong_value():
     wrong = ref.scan([0, 24, 40], delta_softplus=True, a_is_log=True, **args)
     with pytest.raises(AssertionError):
         ref.check("y", wrong["y"].v.float(), out["y"])
+
+
+def test_long_rows_are_refused():
+    """Rows are walked in steps of 32 bits."""
+    lib, d = _lib.lib(), _scan_desc()
+    for f in ("u_stride", "delta_stride", "bc_stride", "y_stride", "z_stride"):
+        d = _scan_desc()
+        setattr(d, f, 2 ** 29)
+        assert lib.mvm_seq_scan_validate(ctypes.byref(d)) == _lib.MVM_ERR_UNSUPPORTED, f
+        assert f in _lib.last_error()
+    c = _conv_desc()
+    c.x_stride = 2 ** 29
+    assert lib.mvm_seq_conv_validate(ctypes.byref(c)) == _lib.MVM_ERR_UNSUPPORTED
+
+
+def test_sizes_of_scratch_follow_the_cut():
+    """No workspace without chunks; with them aggregates of every chunk slot."""
+    lib, d = _lib.lib(), _scan_desc(T=4096, S=2, D=128)
+    d.chunk_len = 4096
+    assert lib.mvm_seq_scan_workspace_bytes(ctypes.byref(d), 0) == 0
+    d.chunk_len = 64
+    slots = 4096 // 64 + 3
+    assert lib.mvm_seq_scan_workspace_bytes(ctypes.byref(d), 0) == slots * 128 * 17 * 4
+    assert lib.mvm_seq_scan_ckpt_elems(ctypes.byref(d)) == (4096 // 8 + 3) * 128 * 16
+    d.chunk_len, d.max_len = 0, 0
+    for t in (1, 17, 1000, 70000):  # any cut that the library picks is within its own bounds
+        d.seq.tokens = t
+        for back in (0, 1):
+            assert lib.mvm_seq_scan_workspace_bytes(ctypes.byref(d), back) >= 0
