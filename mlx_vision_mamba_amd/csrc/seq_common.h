@@ -83,6 +83,11 @@ __device__ __forceinline__ SeqChunk seq_chunk(const SeqGeom& g, int32_t slot, co
   return c;
 }
 
+// the slot of the last chunk of c's sequence
+__device__ __forceinline__ int32_t last_slot(const SeqCut& cut, const SeqChunk& c) {
+  return cut_div(cut, c.start) + c.seq + (c.end > c.start ? cut_div(cut, c.end - c.start - 1) : 0);
+}
+
 // a pointer to global memory that the compiler knows nothing about
 template <typename T>
 __device__ __forceinline__ T* opaque(T* p) {

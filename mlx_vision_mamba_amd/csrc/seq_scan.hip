@@ -63,7 +63,20 @@ seq_scan_fwd_kernel(FwdArgs<T, DT, BT> args) {
       for (int32_t t = c.t0; t < c.t1; ++t) args.y[t * g.ys + d] = from_f32<T>(0.f);
     return;
   }
-  if (AGG && c.t1 == c.end) return;
+  if (AGG && c.t1 == c.end) {
+    // Where the main pass folds the chunks, the place of the last one's
+    // aggregate takes the state that the sequence starts from: its own row may
+    // hold the final state before each chunk of the main pass has read it.
+    if (g.fold && valid) {
+      const int32_t row = seq_slot(g.q, c.seq);
+      float h[16];
+#pragma unroll
+      for (int n = 0; n < 16; ++n) h[n] = 0.f;
+      if (p.h0 != nullptr && row >= 0 && !seq_fresh(g.q, c.seq)) load_states(h, p.h0, row * D + d, 0, g.N, g.h_vec);
+      store_agg16(h, p.agg_h, c.slot, D, d);
+    }
+    return;
+  }
   const bool soft = g.softplus != 0, gate = !AGG && args.z != nullptr;
   // Everything that a chunk starts from is asked for before any of it is used
   RowPtr pu, pd, pz, py, pb, pc;
@@ -88,8 +101,8 @@ seq_scan_fwd_kernel(FwdArgs<T, DT, BT> args) {
 #pragma unroll
   for (int n = 0; n < 16; ++n) h[n] = 0.f;
   if constexpr (!AGG) {
-    if (g.multi && !g.fold)
-      load_agg16(h, p.agg_h, c.slot, D, d);
+    if (g.multi)
+      load_agg16(h, p.agg_h, g.fold ? last_slot(g.cut, c) : c.slot, D, d);
     else if (p.h0 != nullptr && row >= 0 && !seq_fresh(g.q, c.seq))
       load_states(h, p.h0, row * D + d, 0, g.N, g.h_vec);
   }

@@ -216,8 +216,8 @@ seq_scan_bwd_kernel(BwdArgs<T, DT, BT> args) {
       load_states(h, p.dh1, row * D + dc, 0, g.N, g.h_vec);
     load_a2(a2, p.A, dc, 0, g);
     if (g.multi && g.fold) {
-      const int64_t end = cut_div(g.cut, c.start) + c.seq + (c.end - c.start - 1) / static_cast<int32_t>(g.cut.len);
-      fold_chunks<-1>(h, a2, p.agg_h, p.agg_s, end, static_cast<int32_t>(end - c.slot), D, dc);
+      const int32_t end = last_slot(g.cut, c);
+      fold_chunks<-1>(h, a2, p.agg_h, p.agg_s, end, end - c.slot, D, dc);
     }
 #pragma unroll
     for (int q = 0; q < 4; ++q) {

@@ -122,3 +122,24 @@ def test_scan_inputs_of_many_alignments(cuda):
     states = off(init[:2])
     y = mvm.selective_scan_prefill(*[off(v) for v in a.values()], states, [0, 4, 6], delta_softplus=True, a_is_log=True)
     _compare({"y": y, "final": states}, want)
+
+
+@pytest.mark.parametrize("gather", [False, True])
+def test_prefill_in_place_is_the_same_as_apart(cuda, gather):
+    """Chunks that the main pass joins, many more of them than run at once: the
+    last one's final state replaces the initial state that all of them start from."""
+    lens = [60 + 40 * (i % 2) for i in range(50)]
+    off = [0] + torch.tensor(lens).cumsum(0).tolist()
+    T, D, N, S = off[-1], 1536, 16, len(lens)
+    gen = torch.Generator().manual_seed(66)
+    r = lambda *s: torch.randn(*s, generator=gen).to(cuda)
+    a = [r(T, D), 0.3 * r(T, D), 0.2 * r(D, N), r(T, N), r(T, N), r(D)]
+    kw = dict(delta_softplus=True, a_is_log=True, max_len=100, chunk_len=16)
+    init = r(S, D, N)
+    y, final = mvm.selective_scan_packed(*a, off, initial_states=init, **kw)
+    for _ in range(5):
+        slots = torch.randperm(S, generator=gen).int().to(cuda) if gather else None
+        states = init.clone() if slots is None else torch.empty_like(init).index_copy_(0, slots.long(), init)
+        ys = mvm.selective_scan_prefill(*a, states, off, slots=slots, **kw)
+        assert torch.equal(ys, y)
+        assert torch.equal(states if slots is None else states[slots.long()], final)
