@@ -34,6 +34,38 @@ __device__ __forceinline__ bool seq_fresh(const SeqGeom& g, int32_t i) {
   return g.fresh != nullptr && g.fresh[i] != 0;
 }
 
+// The state rows of sequences i0 .. i0 + R - 1 (past the last one: the last
+// one's) and whether they start from zero, all asked for at once.  fresh is read
+// from any valid address where there is none: a load in a branch would be
+// waited for there.
+template <int R>
+struct StateRows {
+  int32_t row[R];
+  uint32_t fresh[R];
+  __device__ __forceinline__ void load(const SeqGeom& g, int32_t i0, const void* any) {
+    const uint8_t* f = g.fresh != nullptr ? g.fresh : static_cast<const uint8_t*>(any);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      row[r] = i0 + r < g.S ? i0 + r : g.S - 1;
+      fresh[r] = f[g.fresh != nullptr ? row[r] : 0];
+    }
+    if (g.slots != nullptr) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) row[r] = ((const const_i32*)g.slots)[row[r]];
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) row[r] = row[r] < 0 || row[r] >= g.M ? -1 : row[r];
+  }
+  // (once the loads that are to be in flight beside it have been issued)
+  __device__ __forceinline__ void settle(const SeqGeom& g) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      asm volatile("" : "+v"(fresh[r]));
+      fresh[r] = g.fresh != nullptr ? fresh[r] : 0u;
+    }
+  }
+};
+
 __device__ __forceinline__ int32_t cut_div(const SeqCut& cut, int32_t n) {
   return static_cast<int32_t>(__umulhi(static_cast<uint32_t>(n), cut.magic) >> cut.shift);
 }

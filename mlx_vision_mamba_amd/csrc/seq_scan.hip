@@ -14,6 +14,17 @@
 // zero state for its end state, those are joined in order (the decay over a
 // chunk is one exponential of the summed delta), the main pass runs each chunk
 // from its carry.
+//
+// Bound by VALU issue.  On MI355X, 32768 bf16 tokens of 1536 channels with gate
+// and softplus: aggregate pass 138 us, carry 15, main pass 188, the VALU busy
+// 97 % of both passes (85 and 116 instructions a token and wave; 80 of
+// the main pass's are the recurrence, the 16 exponentials among them count
+// twice).  Four waves a SIMD; what kept it from that rate were row addresses
+// held (and spilled) for whole tiles, and the issue order (Pace).
+//
+// B and C are the same for a whole wave and come through scalar loads, as
+// scalar operands.  Through LDS instead (a tile at a time) the same prompt took
+// 146 + 198 us.
 #include "seq_scan_pass.h"
 
 namespace mvm {
@@ -93,20 +104,28 @@ seq_scan_fwd_kernel(FwdArgs<T, DT, BT> args) {
     load_next(nu, pu, t, c.t1, lc);
     if (gate) load_next(nz, pz, t, c.t1, lc);
   };
+  StateRows<1> rows;
+  if constexpr (!AGG) rows.load(g.q, c.seq, p.A);
   if (c.t0 < c.t1) fetch(c.t0);
   const float bias = p.dbias ? p.dbias[d] : 0.f;
   const float Dd = AGG ? 0.f : p.Dv[d];
-  const int32_t row = seq_slot(g.q, c.seq);
   float a2[16], h[16];
 #pragma unroll
   for (int n = 0; n < 16; ++n) h[n] = 0.f;
   if constexpr (!AGG) {
     if (g.multi)
       load_agg16(h, p.agg_h, g.fold ? last_slot(g.cut, c) : c.slot, D, d);
-    else if (p.h0 != nullptr && row >= 0 && !seq_fresh(g.q, c.seq))
-      load_states(h, p.h0, row * D + d, 0, g.N, g.h_vec);
+    else if (p.h0 != nullptr && rows.row[0] >= 0)
+      load_states(h, p.h0, rows.row[0] * D + d, 0, g.N, g.h_vec);
   }
   load_a2(a2, p.A, d, 0, g);
+  if constexpr (!AGG) {
+    rows.settle(g.q);
+    if (!g.multi) {
+#pragma unroll
+      for (int n = 0; n < 16; ++n) h[n] = rows.fresh[0] != 0 ? 0.f : h[n];
+    }
+  }
   if constexpr (!AGG) {
     if (g.multi && g.fold) {
       const int64_t first = cut_div(g.cut, c.start) + c.seq;
@@ -178,8 +197,8 @@ seq_scan_fwd_kernel(FwdArgs<T, DT, BT> args) {
   if constexpr (AGG) {
     store_agg16(h, late.p.agg_h, c.slot, D, d);
     late.p.agg_s[c.slot * D + d] = sum_dl;
-  } else if (c.t1 == c.end && late.p.h1 != nullptr && row >= 0) {
-    store_states(h, late.p.h1, row * D + d, 0, late.g.N, late.g.h_vec);
+  } else if (c.t1 == c.end && late.p.h1 != nullptr && rows.row[0] >= 0) {
+    store_states(h, late.p.h1, rows.row[0] * D + d, 0, late.g.N, late.g.h_vec);
   }
 }
 
@@ -188,6 +207,7 @@ seq_scan_fwd_kernel(FwdArgs<T, DT, BT> args) {
 // (lane & 15) x 4 groups of states and takes kCarryRun consecutive chunks in
 // registers, one round of loads; the waves' own aggregates are joined through
 // LDS, and the workgroup goes on with the next kCarryRun * (its waves) chunks.
+// MI355X, 164 chunks of 1536 channels: 15 us (96 chunk after chunk).
 template <bool REV>
 __global__ void __launch_bounds__(1024)
 seq_carry_kernel(SeqScanGeom g, uint32_t ncb, const float* __restrict__ A, const float* __restrict__ enter,
@@ -203,14 +223,31 @@ seq_carry_kernel(SeqScanGeom g, uint32_t ncb, const float* __restrict__ A, const
   const int32_t start = seq_off_u(g.q, seq), next = seq_off_u(g.q, seq + 1);
   const int32_t len = next > start ? next - start : 0;
   const int32_t n = cut_div(g.cut, len) + (cut_div(g.cut, len) * static_cast<int64_t>(g.cut.len) < len ? 1 : 0);
-  const int32_t row = seq_slot(g.q, seq);
-  // (waves that no run falls to only meet the others at the barrier)
-  const bool idle = wave > 0 && wave * kCarryRun >= n;
-  float a2[4] = {0.f, 0.f, 0.f, 0.f}, h[4] = {0.f, 0.f, 0.f, 0.f};
-  if (!idle) load_a2(a2, A, dc, 4 * q, g);
-  if (!idle && enter != nullptr && row >= 0 && !seq_fresh(g.q, seq)) load_states(h, enter, row * D + dc, 4 * q, g.N, g.h_vec);
+  StateRows<1> rows;
+  rows.load(g.q, seq, A);
   const int64_t base = static_cast<int64_t>(cut_div(g.cut, start)) + seq;
   auto slot_of = [&](int32_t j) { return base + (REV ? n - 1 - j : j); };  // j-th chunk in the carry's order
+  // (waves that no run falls to only meet the others at the barrier)
+  const bool idle = wave > 0 && wave * kCarryRun >= n;
+  Pack<float, 4> v[kCarryRun];
+  float s[kCarryRun];
+  auto fetch = [&](int32_t j) {
+#pragma unroll
+    for (int i = 0; i < kCarryRun; ++i) {
+      // (the last chunk in order has no aggregate, and nothing follows it)
+      const int64_t slot = slot_of(j + i < n ? j + i : n - 1);
+      v[i] = load_pack<float, 4>(agg_h + ((slot * 4 + q) * D + dc) * 4);
+      s[i] = agg_s[slot * D + dc];
+    }
+  };
+  // The first round's aggregates, the initial state and A in flight together
+  float a2[4] = {0.f, 0.f, 0.f, 0.f}, h[4] = {0.f, 0.f, 0.f, 0.f};
+  if (!idle && n > 0) fetch(wave * kCarryRun);
+  if (!idle && enter != nullptr && rows.row[0] >= 0) load_states(h, enter, rows.row[0] * D + dc, 4 * q, g.N, g.h_vec);
+  if (!idle) load_a2(a2, A, dc, 4 * q, g);
+  rows.settle(g.q);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) h[k] = rows.fresh[0] != 0 ? 0.f : h[k];
   auto put = [&](int64_t slot) {
     if (d < D) store_pack(agg_h + ((slot * 4 + q) * D + d) * 4, Pack<float, 4>{h[0], h[1], h[2], h[3]});
   };
@@ -224,15 +261,7 @@ seq_carry_kernel(SeqScanGeom g, uint32_t ncb, const float* __restrict__ A, const
       return;
     }
     const int32_t j = j0 + wave * kCarryRun;
-    Pack<float, 4> v[kCarryRun];
-    float s[kCarryRun];
-#pragma unroll
-    for (int i = 0; i < kCarryRun; ++i) {
-      // (the last chunk in order has no aggregate, and nothing follows it)
-      const int64_t slot = slot_of(j + i < n ? j + i : n - 1);
-      v[i] = load_pack<float, 4>(agg_h + ((slot * 4 + q) * D + dc) * 4);
-      s[i] = agg_s[slot * D + dc];
-    }
+    if (j0 > 0) fetch(j);
     float e[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
 #pragma unroll
     for (int i = 0; i < kCarryRun; ++i) {
@@ -284,6 +313,9 @@ seq_carry_kernel(SeqScanGeom g, uint32_t ncb, const float* __restrict__ A, const
 // little else is asked for beside it: a wave keeps its channels' A, D and bias
 // for R sequences, and has all their loads in flight together.  VEC: states,
 // and B and C, are read four at a time (N a multiple of 4, aligned rows).
+// MI355X, 1024 sequences of 1536 channels, bf16: 43 us, 5.0 TB/s (a large copy
+// reaches 4.9); 48 us while the gate's loads stood in branches, 58 at one sequence
+// a wave.
 template <typename T, typename DT, bool VEC, int R>
 __global__ void __launch_bounds__(256)
 seq_scan_step_kernel(SeqScanGeom g, uint32_t ncb, const T* __restrict__ u, const DT* __restrict__ delta,
@@ -302,11 +334,15 @@ seq_scan_step_kernel(SeqScanGeom g, uint32_t ncb, const T* __restrict__ u, const
   Pack<T, 4> b[R], c[R];
   T uv[R], zv[R];
   DT dv[R];
-  int32_t row[R];
+  StateRows<R> rows;
+  rows.load(g.q, i0, u);
+  const int32_t(&row)[R] = rows.row;
+  // (read without a gate too: a load in a branch would be waited for there)
+  const T* zp = z ? z : u;
+  const int64_t zs = z ? g.zs : g.us;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const int32_t i = i0 + r < g.q.S ? i0 + r : g.q.S - 1;
-    row[r] = seq_slot(g.q, i);
     at[r] = states + (static_cast<int64_t>(row[r] < 0 ? 0 : row[r]) * D + dc) * N + n0;
     if (row[r] >= 0) {
       if constexpr (VEC) {
@@ -318,7 +354,7 @@ seq_scan_step_kernel(SeqScanGeom g, uint32_t ncb, const T* __restrict__ u, const
     }
     uv[r] = u[i * g.us + dc];
     dv[r] = delta[i * g.ds + dc];
-    if (z) zv[r] = z[i * g.zs + dc];
+    zv[r] = zp[i * zs + dc];
     if constexpr (VEC) {
       b[r] = load_pack<T, 4>(Bm + i * g.bs + n0);
       c[r] = load_pack<T, 4>(Cm + i * g.bs + n0);
@@ -332,8 +368,14 @@ seq_scan_step_kernel(SeqScanGeom g, uint32_t ncb, const T* __restrict__ u, const
     }
   }
   const float bias = dbias ? dbias[dc] : 0.f, Dd = Dv[dc];
-  float a2[4];
+  float a2[4], zf[R];
   load_a2(a2, A, dc, 4 * q, g);
+  rows.settle(g.q);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    zf[r] = to_f32(zv[r]);
+    pin(zf[r]);
+  }
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     if (i0 + r >= g.q.S) break;
@@ -342,8 +384,8 @@ seq_scan_step_kernel(SeqScanGeom g, uint32_t ncb, const T* __restrict__ u, const
       if (valid && q == 0) yr[d] = from_f32<T>(0.f);
       continue;
     }
-    const bool fresh = seq_fresh(g.q, i0 + r);
-    const float uf = to_f32(uv[r]), zf = z ? to_f32(zv[r]) : 0.f;
+    const bool fresh = rows.fresh[r] != 0;
+    const float uf = to_f32(uv[r]);
     float dl = to_f32(dv[r]) + bias, sum = 0.f;
     if (g.softplus) dl = softplus_f(dl);
     const float du = dl * uf;
@@ -362,7 +404,7 @@ seq_scan_step_kernel(SeqScanGeom g, uint32_t ncb, const T* __restrict__ u, const
       }
     }
     float out = fmaf(Dd, uf, sum_groups(sum));
-    if (z) out *= zf * sigmoid_f(zf);
+    if (z) out *= zf[r] * sigmoid_f(zf[r]);
     if (valid && q == 0) yr[d] = from_f32<T>(out);
   }
 }
@@ -399,7 +441,7 @@ hipError_t fwd_t(SeqScanGeom g, const SeqScanIn& in, const SeqScanFwd& b, BcRows
   return hipGetLastError();
 }
 
-constexpr int kStepRows = 4;
+constexpr int kStateRows = 4;
 
 template <typename T, typename DT>
 hipError_t step_t(SeqScanGeom g, const SeqScanIn& in, float* states, void* y, hipStream_t s) {
@@ -415,9 +457,11 @@ hipError_t step_t(SeqScanGeom g, const SeqScanIn& in, float* states, void* y, hi
     return hipGetLastError();
   };
   if (!g.h_vec || !bc) return run(seq_scan_step_kernel<T, DT, false, 1>, 1);
-  // several sequences a wave once that leaves each SIMD four waves
-  const bool many = static_cast<int64_t>(g.q.S) * ncb >= 4 * kStepRows * 1024;
-  return many ? run(seq_scan_step_kernel<T, DT, true, kStepRows>, kStepRows)
+  // four sequences a wave once that leaves each SIMD two waves.  MI355X, 1536 bf16
+  // channels: 64 sequences 6.4 us by four, 6.1 by one; 128 9.7 and 10.4; 512 24.6
+  // and 30.2; 2048 82 and 110
+  const bool many = static_cast<int64_t>(g.q.S) * ncb >= 2 * 1024;
+  return many ? run(seq_scan_step_kernel<T, DT, true, kStateRows>, kStateRows)
               : run(seq_scan_step_kernel<T, DT, true, 1>, 1);
 }
 
