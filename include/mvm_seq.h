@@ -97,7 +97,7 @@ int mvm_seq_scan_fwd(const mvm_seq_scan_desc* desc, const void* u, const void* d
  * Gradients for dy (y_stride rows) and dh1 (may be NULL: zero).  slots and
  * fresh must be NULL.  du, ddelta, dz (tokens, dim) and dB, dC (tokens,
  * dstate) are contiguous, in the types of their primals; dA (of A_log with
- * a_is_log), dD, ddelta_bias and dh0 float32.  All are written in full;
+ * a_is_log), dD, ddelta_bias and dh0 (not dh1's buffer) float32.  All are written in full;
  * ddelta_bias may be NULL, dz is NULL without z, dh0 may be NULL.
  */
 int mvm_seq_scan_bwd(const mvm_seq_scan_desc* desc, const void* u, const void* delta,

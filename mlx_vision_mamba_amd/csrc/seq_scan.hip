@@ -207,7 +207,7 @@ seq_scan_fwd_kernel(FwdArgs<T, DT, BT> args) {
 // (lane & 15) x 4 groups of states and takes kCarryRun consecutive chunks in
 // registers, one round of loads; the waves' own aggregates are joined through
 // LDS, and the workgroup goes on with the next kCarryRun * (its waves) chunks.
-// MI355X, 164 chunks of 1536 channels: 15 us (96 chunk after chunk).
+// MI355X, 164 chunks of 1536 channels: 15-17 us (96 chunk after chunk).
 template <bool REV>
 __global__ void __launch_bounds__(1024)
 seq_carry_kernel(SeqScanGeom g, uint32_t ncb, const float* __restrict__ A, const float* __restrict__ enter,
