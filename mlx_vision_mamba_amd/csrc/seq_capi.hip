@@ -93,55 +93,61 @@ mvm::SeqGeom seq_geom(const mvm_seq_desc& q) {
 
 // The cut into time chunks.  A wave is 64 channels of one chunk; chunks let
 // one sequence use more waves, but need an aggregate pass before the main one,
-// which repeats most of the recurrence, and their joining.  The cut is the
-// cheapest of those that put 1/4 to `waves` waves on each of the card's 1024
-// SIMDs, and of whole sequences, by a model of the passes in cycles (measured
-// on MI355X at 2.4 GHz): what one token more costs a SIMD of one, two, ..
-// waves.
+// which repeats most of the recurrence, and their joining.  Waves are placed
+// when the launch starts, so a pass takes as long as the SIMDs with the most of
+// them: the cut is the cheapest of those that just fit 1/4, 1/2, 1, 2, .. waves
+// on each of the card's 1024 SIMDs (from `waves` on, what fits at once, in
+// rounds), and of whole sequences, by a model in cycles at 2.36 GHz.  It is
+// fitted to times of 14 packings of 1 to 60 sequences at 4 to 28 lengths each on
+// MI355X (5 % off on average), where its choices take 0.1 % longer than the best
+// length forward and 1.6 % backward.
 struct Cost {
   int waves;
-  int64_t agg[4], main_[4];
-  int64_t token(int64_t n) const {
-    const int64_t last = agg[waves - 1] + main_[waves - 1];
-    return n <= waves ? agg[n - 1] + main_[n - 1] : (last * n + waves - 1) / waves;
-  }
+  int64_t start, placed;         // the launches and first loads, and for one wave a SIMD
+  int64_t work;                  // a token of a SIMD's share of all tokens and waves
+  int64_t token[4], whole[4];    // one token of chunks, of whole sequences, on a SIMD of 1, 2, .. waves
+  int64_t whole_start;
 };
-constexpr Cost kFwdCost = {4, {540, 950, 1250, 1600}, {1100, 1420, 1900, 2090}};
-constexpr Cost kBwdCost = {3, {600, 1180, 1690}, {3000, 4300, 5400}};
+constexpr Cost kFwdCost = {4, 8000, 11500, 0, {1910, 2210, 2520, 2910}, {1280, 1540, 1900, 2270}, 3000};
+constexpr Cost kBwdCost = {3, 32000, 5800, 1000, {2600, 2940, 3400}, {2300, 3250, 5600}, 20000};
 constexpr int64_t kSimds = 1024;
-constexpr int64_t kStart = 10000;  // a pass's launch and its waves' first loads,
-constexpr int64_t kStartWave = 3;  // those of many waves
-constexpr int64_t kFold = 1000;    // the main pass joins one chunk before its own
-constexpr int64_t kCarry = 9000;   // a carry pass,
-constexpr int64_t kCarryRound = 10000;  // its rounds of 128 chunks,
-constexpr int64_t kCarryWave = 3;       // and its traffic for one wave's aggregate
+constexpr int64_t kFold = 1060;        // the main pass joins one chunk before its own
+constexpr int64_t kCarry = 9000;       // a carry pass,
+constexpr int64_t kCarryRound = 3000;  // its rounds of 128 chunks,
+constexpr int64_t kCarryWave = 12;     // and its traffic for one wave's aggregate
 
 void pick_chunk(const mvm_seq_scan_desc* d, const Cost& k, mvm::SeqScanGeom& g) {
   const int64_t T = d->seq.tokens, S = d->seq.nseq, ncb = std::max<int64_t>(1, ceil_div(d->seq.dim, 64));
   int64_t longest = d->seq.offsets == nullptr ? d->seq.seqlen : T;
   if (d->max_len > 0) longest = std::min(longest, d->max_len);
-  const auto join = [&](int64_t waves, int64_t nth, bool fold) {
-    return fold ? (nth - 1) * kFold * std::max<int64_t>(1, waves / kSimds)
-                : kCarry + ceil_div(nth, 128) * kCarryRound + waves * kCarryWave;
-  };
   // (a sequence's last chunk is half a chunk on average)
   const auto waves_of = [&](int64_t len) { return ncb * ceil_div(T + (S - 1) * len / 2, len); };
+  const auto join = [&](int64_t waves, int64_t nth, bool fold) {
+    return fold ? (nth - 1) * kFold * std::max(waves, kSimds) / kSimds
+                : kCarry + ceil_div(nth, 128) * kCarryRound + waves * kCarryWave;
+  };
+  const int64_t share = T * ncb / kSimds;
   const auto cost = [&](int64_t len) {
-    const int64_t waves = waves_of(len), nth = ceil_div(longest, len);
-    return 2 * (kStart + waves * kStartWave) + len * k.token(ceil_div(waves, kSimds)) +
+    // slots of no chunk take their places too
+    const int64_t waves = waves_of(len), nth = ceil_div(longest, len), placed = ncb * ((T - 1) / len + S);
+    const int64_t n = std::max<int64_t>(1, ceil_div(placed, kSimds));
+    const int64_t token = n <= k.waves ? k.token[n - 1] : k.token[k.waves - 1] * n / k.waves;
+    return k.start + k.placed * placed / kSimds + k.work * share + len * token +
            std::min(join(waves, nth, true), join(waves, nth, false));
   };
   int64_t len = d->chunk_len;
   if (len == 0) {
-    // whole sequences: the longest by itself, or all the work (a SIMD's waves
-    // are of different lengths)
-    const int64_t full = k.main_[k.waves - 1] / k.waves;
-    int64_t best = kStart + std::max(longest * k.main_[0], T * ncb / kSimds * full + longest / 2 * full);
+    // whole sequences: the longest, or all the work where it comes in rounds
+    const int64_t n = std::max<int64_t>(1, ceil_div(ncb * S, kSimds));
+    int64_t best = k.whole_start + (n <= k.waves ? longest * k.whole[n - 1]
+                                                 : std::max(longest * k.whole[0],
+                                                            (share + longest / 2) * k.whole[k.waves - 1] / k.waves));
     len = longest;
-    for (int64_t quarters = 1; quarters <= 4 * k.waves; quarters += quarters < 4 ? quarters : 4) {
-      const int64_t chunks = quarters * (kSimds / 4) / ncb - S / 2;
-      if (chunks < 1) continue;
-      const int64_t n = std::max<int64_t>(1, ceil_div(ceil_div(T, chunks), mvm::kSeqTile)) * mvm::kSeqTile;
+    for (int64_t quarters = 1; quarters <= 16 * k.waves;
+         quarters += quarters < 4 || quarters >= 4 * k.waves ? quarters : 4) {
+      const int64_t chunks = quarters * (kSimds / 4) / ncb - S;  // beside each sequence's first
+      if (chunks < 0) continue;
+      const int64_t n = std::max<int64_t>(1, ceil_div(ceil_div(T, chunks + 1), mvm::kSeqTile)) * mvm::kSeqTile;
       if (n >= longest) continue;
       const int64_t c = cost(n);
       if (c < best) best = c, len = n;
