@@ -308,23 +308,24 @@ seq_carry_kernel(SeqScanGeom g, uint32_t ncb, const float* __restrict__ A, const
 
 // --------------------------------------------------------------- one token
 
-// Lane 4c + q holds states 4q .. 4q + 3 of channel c: a wave reads 16
+// Lane G c + q holds states 4q .. 4q + 3 of channel c: a wave reads 64 / G
 // channels' states, 1 KB, at once.  Bound by the states' traffic, as long as
 // little else is asked for beside it: a wave keeps its channels' A, D and bias
 // for R sequences, and has all their loads in flight together.  VEC: states,
 // and B and C, are read four at a time (N a multiple of 4, aligned rows).
 // MI355X, 1024 sequences of 1536 channels, bf16: 43 us, 5.0 TB/s (a large copy
 // reaches 4.9); 48 us while the gate's loads stood in branches, 58 at one sequence
-// a wave.
-template <typename T, typename DT, bool VEC, int R>
+// a wave.  One or two lanes a channel for up to 4 or 8 states: 2048 sequences
+// 24.5 us (N 4) and 43 (N 8), against 52 and 66 by four lanes, some of them idle.
+template <typename T, typename DT, bool VEC, int R, int G>
 __global__ void __launch_bounds__(256)
 seq_scan_step_kernel(SeqScanGeom g, uint32_t ncb, const T* __restrict__ u, const DT* __restrict__ delta,
                      const float* __restrict__ dbias, const float* __restrict__ A, const T* __restrict__ Bm,
                      const T* __restrict__ Cm, const float* __restrict__ Dv, const T* __restrict__ z,
                      float* __restrict__ states, T* __restrict__ y) {
   const BlockPos pos = block_pos(ncb);
-  const int q = threadIdx.x & 3, N = g.N;
-  const int64_t D = g.q.D, d = static_cast<int64_t>(pos.cb) * 64 + (threadIdx.x >> 2);
+  const int q = threadIdx.x & (G - 1), N = g.N;
+  const int64_t D = g.q.D, d = static_cast<int64_t>(pos.cb) * (256 / G) + threadIdx.x / G;
   const bool valid = d < D, mine = valid && 4 * q < N;
   const int64_t dc = valid ? d : D - 1;
   const int n0 = 4 * q < N ? 4 * q : 0;
@@ -403,7 +404,9 @@ seq_scan_step_kernel(SeqScanGeom g, uint32_t ncb, const T* __restrict__ u, const
           if (4 * q + j < N) at[r][j] = h[r].v[j];
       }
     }
-    float out = fmaf(Dd, uf, sum_groups(sum));
+    if constexpr (G > 1) sum += dpp<kQuadXor1>(sum);
+    if constexpr (G > 2) sum += dpp<kQuadXor2>(sum);
+    float out = fmaf(Dd, uf, sum);
     if (z) out *= zf[r] * sigmoid_f(zf[r]);
     if (valid && q == 0) yr[d] = from_f32<T>(out);
   }
@@ -441,28 +444,34 @@ hipError_t fwd_t(SeqScanGeom g, const SeqScanIn& in, const SeqScanFwd& b, BcRows
   return hipGetLastError();
 }
 
-constexpr int kStateRows = 4;
+constexpr int kStepRows = 4;
 
 template <typename T, typename DT>
 hipError_t step_t(SeqScanGeom g, const SeqScanIn& in, float* states, void* y, hipStream_t s) {
-  const uint32_t ncb = static_cast<uint32_t>((g.q.D + 63) / 64);
   set_vec(g, in.A, states, nullptr);
   const bool bc = (reinterpret_cast<uintptr_t>(in.Bm) | reinterpret_cast<uintptr_t>(in.Cm) |
                    static_cast<uintptr_t>(g.bs) * sizeof(T)) % (4 * sizeof(T)) == 0;
-  auto run = [&](auto kernel, int R) {
+  auto launch = [&](auto kernel, uint32_t ncb, int R) {
     const dim3 grid(ncb * static_cast<unsigned>((g.q.S + R - 1) / R));
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, g, ncb, static_cast<const T*>(in.u),
                        static_cast<const DT*>(in.delta), in.dbias, in.A, static_cast<const T*>(in.Bm),
                        static_cast<const T*>(in.Cm), in.Dv, static_cast<const T*>(in.z), states, static_cast<T*>(y));
     return hipGetLastError();
   };
-  if (!g.h_vec || !bc) return run(seq_scan_step_kernel<T, DT, false, 1>, 1);
+  const auto blocks = [&](int G) { return static_cast<uint32_t>((g.q.D * G + 255) / 256); };
+  if (!g.h_vec || !bc) return launch(seq_scan_step_kernel<T, DT, false, 1, 4>, blocks(4), 1);
   // four sequences a wave once that leaves each SIMD two waves.  MI355X, 1536 bf16
   // channels: 64 sequences 6.4 us by four, 6.1 by one; 128 9.7 and 10.4; 512 24.6
   // and 30.2; 2048 82 and 110
-  const bool many = static_cast<int64_t>(g.q.S) * ncb >= 2 * 1024;
-  return many ? run(seq_scan_step_kernel<T, DT, true, kStateRows>, kStateRows)
-              : run(seq_scan_step_kernel<T, DT, true, 1>, 1);
+  auto run = [&](auto groups) {
+    constexpr int G = decltype(groups)::value;
+    const uint32_t ncb = blocks(G);
+    return static_cast<int64_t>(g.q.S) * ncb >= 2 * 1024
+               ? launch(seq_scan_step_kernel<T, DT, true, kStepRows, G>, ncb, kStepRows)
+               : launch(seq_scan_step_kernel<T, DT, true, 1, G>, ncb, 1);
+  };
+  return g.N <= 4 ? run(std::integral_constant<int, 1>{})
+                  : (g.N <= 8 ? run(std::integral_constant<int, 2>{}) : run(std::integral_constant<int, 4>{}));
 }
 
 }  // namespace

@@ -143,3 +143,23 @@ def test_prefill_in_place_is_the_same_as_apart(cuda, gather):
         ys = mvm.selective_scan_prefill(*a, states, off, slots=slots, **kw)
         assert torch.equal(ys, y)
         assert torch.equal(states if slots is None else states[slots.long()], final)
+
+
+@pytest.mark.parametrize("N", [4, 8, 12, 16])
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_scan_step_lanes_of_a_channel(cuda, dtype, N):
+    """One, two or four lanes a channel; several sequences a wave give the values of one a wave."""
+    S, D = 1001, 515
+    a, k, _, _ = _scan_inputs([1] * S, D, N, TYPES[dtype], 67)
+    want = ref.scan(list(range(S + 1)), **a, **k, delta_softplus=True, a_is_log=True)
+    d = {n: v.to(cuda) for n, v in {**a, "z": k["z"]}.items()}
+    whole, parts = k["initial"].to(cuda), []
+    y = mvm.selective_scan_step(*[d[n] for n in a], whole, z=d["z"], delta_bias=k["delta_bias"].to(cuda),
+                                delta_softplus=True, a_is_log=True)
+    _compare({"y": y, "final": whole}, want)
+    cut = k["initial"].to(cuda)
+    for lo in range(0, S, 90):
+        rows = lambda n: d[n] if n in ("A", "D") else d[n][lo:lo + 90]
+        parts.append(mvm.selective_scan_step(*[rows(n) for n in a], cut[lo:lo + 90], z=rows("z"), a_is_log=True,
+                                             delta_bias=k["delta_bias"].to(cuda), delta_softplus=True))
+    assert torch.equal(torch.cat(parts), y) and torch.equal(cut, whole)
