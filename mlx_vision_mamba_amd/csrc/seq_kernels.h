@@ -77,7 +77,7 @@ struct SeqScanFwd {
   float* h1;        // or null
   void* y;
   float* ckpt;      // or null
-  float* agg_h;     // (slots, 4, D, 4): end states from zero, then carry-ins; with
+  float* agg_h;     // (slots, 4, D, 4; the groups that there are): end states from zero, then carry-ins; with
                     // fold the initial state at each sequence's last chunk
   float* agg_s;     // (slots, D): sum of delta
   float* bc;        // (T, 32) float32 copies of B | C, or null: read in place

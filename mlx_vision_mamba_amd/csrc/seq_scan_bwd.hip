@@ -127,7 +127,7 @@ seq_scan_bwd_agg_kernel(BwdArgs<T, DT, BT> args) {
   }
   if (!valid) return;
   const auto& late = late_args<BwdArgs<T, DT, BT>>();
-  store_agg16(h, late.p.agg_h, c.slot, D, d);
+  store_agg(h, late.p.agg_h, c.slot, D, d);
   late.p.agg_s[c.slot * D + d] = sum_dl;
 }
 
@@ -157,8 +157,8 @@ __device__ __forceinline__ float wave_sums16(const float (&v)[16], int lane) {
 
 // The main pass.  Per tile of 8 tokens the states are taken four at a time
 // (an inner loop that is not unrolled, and ends with the states there are:
-// 16384 tokens of 1536 channels forward and backward 575 us with 16, 475 with
-// 8, 440 with 4): the tile is run forward from its
+// 16384 bf16 tokens of 1536 channels, forward and backward: 575 us with 16, 430
+// with 8, 380 with 4): the tile is run forward from its
 // checkpoint with the states and decays kept in registers, then backward.
 // What a state carries from tile to tile (its adjoint and dA) waits in LDS, and
 // the tile's B and C, from where all lanes read them.  All of a wave's LDS is
@@ -221,7 +221,7 @@ seq_scan_bwd_kernel(BwdArgs<T, DT, BT> args) {
 #pragma unroll
     for (int n = 0; n < 16; ++n) h[n] = 0.f;
     if (g.multi && !g.fold)
-      load_agg16(h, p.agg_h, c.slot, D, dc);
+      load_agg(h, p.agg_h, c.slot, D, dc);
     else if (p.dh1 != nullptr)
       load_states(h, p.dh1, row * D + dc, 0, g.N, g.h_vec);
     load_a2(a2, p.A, dc, 0, g);

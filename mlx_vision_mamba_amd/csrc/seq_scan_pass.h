@@ -77,40 +77,42 @@ __device__ __forceinline__ void load_a2(float (&a)[COUNT], const float* A, int64
 // What enters chunk nth (in order) of a sequence whose earlier chunks left their
 // aggregates in `agg_h`, `agg_s` (DIR 1: slots base, base + 1, ..; -1: base,
 // base - 1, ..), folded into h.
-template <int DIR>
-__device__ __forceinline__ void fold_chunks(float (&h)[16], const float (&a2)[16], const float* agg_h,
+template <int DIR, int COUNT>
+__device__ __forceinline__ void fold_chunks(float (&h)[COUNT], const float (&a2)[COUNT], const float* agg_h,
                                             const float* agg_s, int64_t base, int32_t nth, int64_t D, int64_t d) {
   constexpr int kBatch = 3;  // chunks whose loads are in flight together
   for (int32_t j0 = 0; j0 < nth; j0 += kBatch) {
-    Pack<float, 4> v[kBatch][4];
+    Pack<float, 4> v[kBatch][COUNT / 4];
     float s[kBatch];
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       const int64_t slot = base + DIR * (j0 + i < nth ? j0 + i : j0);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) v[i][q] = load_pack<float, 4>(agg_h + ((slot * 4 + q) * D + d) * 4);
+      for (int q = 0; q < COUNT / 4; ++q) v[i][q] = load_pack<float, 4>(agg_h + ((slot * 4 + q) * D + d) * 4);
       s[i] = agg_s[slot * D + d];
     }
 #pragma unroll
     for (int i = 0; i < kBatch; ++i)
       if (j0 + i < nth) {
 #pragma unroll
-        for (int n = 0; n < 16; ++n) h[n] = fmaf(fast_exp2(a2[n] * s[i]), h[n], v[i][n >> 2].v[n & 3]);
+        for (int n = 0; n < COUNT; ++n) h[n] = fmaf(fast_exp2(a2[n] * s[i]), h[n], v[i][n >> 2].v[n & 3]);
       }
   }
 }
-__device__ __forceinline__ void load_agg16(float (&h)[16], const float* agg_h, int64_t slot, int64_t D, int64_t d) {
+template <int COUNT>
+__device__ __forceinline__ void load_agg(float (&h)[COUNT], const float* agg_h, int64_t slot, int64_t D, int64_t d) {
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
+  for (int q = 0; q < COUNT / 4; ++q) {
     const Pack<float, 4> v = load_pack<float, 4>(agg_h + ((slot * 4 + q) * D + d) * 4);
 #pragma unroll
     for (int j = 0; j < 4; ++j) h[4 * q + j] = v.v[j];
   }
 }
-// (a channel's 16 values of a (row, 4, D, 4) array)
-__device__ __forceinline__ void store_agg16(const float (&h)[16], float* agg_h, int64_t slot, int64_t D, int64_t d) {
+// (a channel's values of a (row, 4, D, 4) array)
+template <int COUNT>
+__device__ __forceinline__ void store_agg(const float (&h)[COUNT], float* agg_h, int64_t slot, int64_t D, int64_t d) {
 #pragma unroll
-  for (int q = 0; q < 4; ++q)
+  for (int q = 0; q < COUNT / 4; ++q)
     store_pack(agg_h + ((slot * 4 + q) * D + d) * 4, Pack<float, 4>{h[4 * q], h[4 * q + 1], h[4 * q + 2], h[4 * q + 3]});
 }
 
