@@ -98,7 +98,8 @@ seq_conv_fwd_kernel(SeqConvGeom g, uint32_t ncb, const T* __restrict__ x, const 
   Taps<V, KC> k;
   if (s0 < c.t1) k.load(w, bias, d, g.w_vec);
   const T* state = nullptr;
-  if (c.t0 == c.start && c0 != nullptr && row >= 0 && !seq_fresh(g.q, c.seq)) state = c0 + row * (KC - 1) * D;
+  if (c.t0 == c.start && c0 != nullptr && row >= 0 && !seq_fresh(g.q, c.seq))
+    state = c0 + static_cast<int64_t>(row) * (KC - 1) * D;
   if (s0 < c.t1) {
     const int64_t p0 = s0 - c.start;
     Pack<T, V> win[P + KC - 1];
