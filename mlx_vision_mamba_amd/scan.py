@@ -313,16 +313,19 @@ def sequence_offsets(offsets, x):
 
 def sequence_slots(slots, rows, device):
     """``slots`` (or None) as an int32 tensor on ``device``; one on the host is
-    checked for rows named twice."""
+    checked for rows named twice, and what lies outside the cache becomes -1."""
     if slots is None or (isinstance(slots, torch.Tensor) and slots.is_cuda):
         return slots
     slots = torch.as_tensor(slots)
     if slots.dim() != 1 or slots.is_floating_point():
         raise ValueError(f"slots must be whole numbers, one a sequence; got {tuple(slots.shape)} of {slots.dtype}")
-    used = slots[(slots >= 0) & (slots < rows)]
+    slots = slots.long()
+    inside = (slots >= 0) & (slots < rows)
+    used = slots[inside]
     if used.unique().numel() != used.numel():
         raise ValueError(f"two sequences share a slot: {slots.tolist()}")
-    return slots.to(device=device, dtype=torch.int32)
+    # (32 bits of a number outside could name a row)
+    return torch.where(inside, slots, -1).to(device=device, dtype=torch.int32)
 
 
 def _chunk_pow2(chunk_len):
