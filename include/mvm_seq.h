@@ -79,7 +79,8 @@ int mvm_seq_scan_validate(const mvm_seq_scan_desc* desc);
 /* float32 elements of the checkpoints that a forward leaves for a backward. */
 int64_t mvm_seq_scan_ckpt_elems(const mvm_seq_scan_desc* desc);
 
-/* Workspace bytes: which = 0 forward, 1 backward. */
+/* Workspace bytes: which = 0 forward, 1 backward.  The workspace must be
+ * 256-byte aligned, the checkpoints 16-byte. */
 int64_t mvm_seq_scan_workspace_bytes(const mvm_seq_scan_desc* desc, int which);
 
 /*
@@ -116,7 +117,7 @@ int mvm_seq_scan_step(const mvm_seq_scan_desc* desc, const void* u, const void* 
 
 int mvm_seq_conv_validate(const mvm_seq_conv_desc* desc);
 
-/* Workspace bytes of mvm_seq_conv_bwd. */
+/* Workspace bytes of mvm_seq_conv_bwd (256-byte aligned). */
 int64_t mvm_seq_conv_workspace_bytes(const mvm_seq_conv_desc* desc);
 
 /* y = silu(bias + causal depthwise conv(x)); w (dim, kwidth) and bias (dim)

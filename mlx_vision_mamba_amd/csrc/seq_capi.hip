@@ -227,6 +227,15 @@ struct Take {
 int check_ws(const char* what, const void* ws, size_t have, size_t need) {
   if (need > 0 && (ws == nullptr || have < need))
     return fail(MVM_ERR_WORKSPACE, "%s: workspace %zu bytes < %zu needed", what, have, need);
+  if (need > 0 && (reinterpret_cast<uintptr_t>(ws) & (kAlign - 1)) != 0)
+    return fail(MVM_ERR_WORKSPACE, "%s: workspace must be %zu-byte aligned", what, kAlign);
+  return MVM_OK;
+}
+
+// (accessed 16 bytes at a time)
+int check_ckpt(const char* what, const float* ckpt) {
+  if ((reinterpret_cast<uintptr_t>(ckpt) & 15u) != 0)
+    return fail(MVM_ERR_INVALID_ARG, "%s: ckpt must be 16-byte aligned", what);
   return MVM_OK;
 }
 
@@ -307,6 +316,7 @@ int mvm_seq_scan_fwd(const mvm_seq_scan_desc* desc, const void* u, const void* d
   const mvm::SeqScanIn in{u, delta, delta_bias, A, Bm, Cm, Dv, z};
   if (!A || !Dv || (g.q.T > 0 && (missing(in) || !y)))
     return fail(MVM_ERR_INVALID_ARG, "mvm_seq_scan_fwd: NULL pointer");
+  if ((rc = check_ckpt("mvm_seq_scan_fwd", ckpt)) != MVM_OK) return rc;
   const ScanWs w = scan_ws(desc, g, false);
   if ((rc = check_ws("mvm_seq_scan_fwd", workspace, workspace_bytes, w.total)) != MVM_OK) return rc;
   Take take{static_cast<char*>(workspace)};
@@ -329,6 +339,7 @@ int mvm_seq_scan_bwd(const mvm_seq_scan_desc* desc, const void* u, const void* d
   if (!A || !Dv || !dA || !dD ||
       (g.q.T > 0 && (missing(in) || !ckpt || !dy || !du || !ddelta || !dB || !dC || (z != nullptr) != (dz != nullptr))))
     return fail(MVM_ERR_INVALID_ARG, "mvm_seq_scan_bwd: NULL pointer");
+  if ((rc = check_ckpt("mvm_seq_scan_bwd", ckpt)) != MVM_OK) return rc;
   const ScanWs w = scan_ws(desc, g, true);
   if ((rc = check_ws("mvm_seq_scan_bwd", workspace, workspace_bytes, w.total)) != MVM_OK) return rc;
   Take take{static_cast<char*>(workspace)};
