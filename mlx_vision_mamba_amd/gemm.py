@@ -20,14 +20,22 @@ from __future__ import annotations
 from . import _lib
 
 
+def _in_proj(h, W):
+    return _lib.native().in_proj(h, W)
+
+
 def in_proj(h, W):
     """h (..., E) @ W (O, E)^T."""
-    return _lib.native().in_proj(h, W)
+    return _lib.traced(_in_proj, h, W) if _lib.is_tracing() else _in_proj(h, W)
+
+
+def _out_proj(y, W):
+    return _lib.native().out_proj(y, W)
 
 
 def out_proj(y, W):
     """Sum over k of y (..., K, D)[k] @ W (K, E, D)[k]^T: (..., E)."""
-    return _lib.native().out_proj(y, W)
+    return _lib.traced(_out_proj, y, W) if _lib.is_tracing() else _out_proj(y, W)
 
 
 def batched(A, B, out=None, ta=False, tb=False, accumulate=False, stream=False):

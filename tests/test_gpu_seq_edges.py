@@ -1,10 +1,11 @@
 """The packed and served scan and conv at the edges of what they accept:
-caches of more rows than 32-bit products hold."""
+caches of more rows than 32-bit products hold, traces."""
 
 import pytest
 import torch
 
 import mlx_vision_mamba_amd as mvm
+from mlx_vision_mamba_amd import gemm
 from tests import seq_reference as ref
 
 pytestmark = pytest.mark.gpu
@@ -36,3 +37,54 @@ def test_conv_cache_past_32_bit_products(cuda):
     ref.check("y", y, want["y"])
     for i, s in enumerate(slots):
         ref.check("states", states[s], want["final"][i])
+
+
+class _Packed(torch.nn.Module):
+    def __init__(self, kind, d_model, d_state):
+        super().__init__()
+        self.width = d_model
+        self.block = getattr(mvm, kind)(d_model, d_state=d_state)
+
+    def forward(self, x, offsets):
+        y, (conv, scan) = self.block.forward_packed(x, offsets)
+        return y, conv, scan
+
+
+class _Products(torch.nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.width = 64
+        self.w = torch.nn.Parameter(torch.randn(2 * 32, 64))
+        self.v = torch.nn.Parameter(torch.randn(2, 24, 32))
+
+    def forward(self, x, offsets):
+        h = gemm.in_proj(x, self.w)
+        return h, gemm.out_proj(h.view(-1, 2, 32), self.v)
+
+
+@pytest.mark.parametrize("make", [
+    # (the first one's x_proj and dt_proj are too narrow for the package's products)
+    lambda: _Packed("MambaBlock", 32, 4), lambda: _Packed("MambaBlock", 64, 16),
+    lambda: _Packed("ResidualMambaBlock", 64, 16), _Products], ids=["narrow", "mamba", "residual", "products"])
+def test_traced_packed_blocks_compute(cuda, make):
+    """A torch.jit trace runs the block again on new tokens and another cut of
+    them: its outputs and gradients are the module's own."""
+    torch.manual_seed(0)
+    m = make().to(cuda)
+    rn = lambda seed: torch.randn(40, m.width, generator=torch.Generator().manual_seed(seed)).to(cuda)  # noqa: E731
+    off = lambda *o: torch.tensor(o, dtype=torch.int32, device=cuda)  # noqa: E731
+    t = torch.jit.trace(m, (rn(0), off(0, 7, 40)), check_trace=False)
+    x = rn(1).requires_grad_()
+    for o in (off(0, 7, 40), off(0, 25, 31)):
+        torch.full((1 << 20,), float("nan"), device=cuda)  # (what unwritten memory would hold)
+        got, want = t(x, o), m(x, o)
+        assert len(got) == len(want)
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+        g = [torch.randn(w.shape, generator=torch.Generator().manual_seed(2)).to(cuda) for w in want]
+        ps = [x, *m.parameters()]
+        for a, b in zip(torch.autograd.grad(got, ps, g), torch.autograd.grad(want, ps, g)):
+            assert torch.equal(a, b)
+    with torch.no_grad():
+        for a, b in zip(t(x, o), m(x, o)):
+            assert torch.equal(a, b) and a.grad_fn is None
