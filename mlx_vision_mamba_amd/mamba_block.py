@@ -131,6 +131,7 @@ class MambaBlock(nn.Module):
 
         return _recurrent_forward(self, x, conv, scan), tuple(out)
 
+    @torch.no_grad()
     def prefill(self, x, states, offsets=None, *, slots=None, fresh=None, max_len=None):
         """y of prompts, or of pieces of them, packed as in ``forward_packed``:
         sequence i continues row slots[i] of the cache ``states`` (from
@@ -142,6 +143,7 @@ class MambaBlock(nn.Module):
             lambda *a, **kw: selective_scan_prefill(*a, states[1], offsets, slots=slots, fresh=fresh,
                                                     max_len=max_len, **kw))
 
+    @torch.no_grad()
     def step(self, x, states, *, slots=None):
         """y (S, d_model) of one token for each of S sequences, x (S, d_model);
         ``states`` and ``slots`` as in ``prefill``.  No gradients."""
@@ -172,11 +174,13 @@ class ResidualMambaBlock(nn.Module):
         y, states = self.mamba.forward_packed(h, offsets, states, max_len=max_len)
         return xr + y, states
 
+    @torch.no_grad()
     def prefill(self, x, states, offsets=None, *, slots=None, fresh=None, max_len=None):
         """``MambaBlock.prefill`` with the norm and the residual."""
         return x + self.mamba.prefill(layer_norm(x, self.norm), states, offsets, slots=slots, fresh=fresh,
                                       max_len=max_len)
 
+    @torch.no_grad()
     def step(self, x, states, *, slots=None):
         """``MambaBlock.step`` with the norm and the residual."""
         return x + self.mamba.step(layer_norm(x, self.norm), states, slots=slots)

@@ -1,5 +1,6 @@
 """The packed and served scan and conv at the edges of what they accept:
-caches of more rows than 32-bit products hold, traces."""
+caches of more rows than 32-bit products hold, traces,
+grad mode."""
 
 import pytest
 import torch
@@ -88,3 +89,17 @@ def test_traced_packed_blocks_compute(cuda, make):
     with torch.no_grad():
         for a, b in zip(t(x, o), m(x, o)):
             assert torch.equal(a, b) and a.grad_fn is None
+
+
+@pytest.mark.parametrize("kind", ["MambaBlock", "ResidualMambaBlock"])
+def test_served_blocks_build_no_graph(cuda, kind):
+    """prefill and step in the default grad mode: values without a graph."""
+    torch.manual_seed(0)
+    blk = getattr(mvm, kind)(32, d_state=4).to(cuda)
+    x = torch.randn(2, 5, 32, device=cuda, requires_grad=True)
+    states, quiet = blk.init_states(2), blk.init_states(2)
+    for name, arg in (("prefill", x), ("step", x[:, 0])):
+        y = getattr(blk, name)(arg, states)
+        assert torch.is_grad_enabled() and not y.requires_grad and y.grad_fn is None
+        with torch.no_grad():
+            assert torch.equal(y, getattr(blk, name)(arg, quiet))

@@ -6,7 +6,7 @@ import ctypes
 import pytest
 import torch
 
-from mlx_vision_mamba_amd import _lib, scan as scan_mod
+from mlx_vision_mamba_amd import _lib, mamba_block as block_mod, scan as scan_mod
 from tests.test_seq_host import _conv_desc, _scan_desc
 
 
@@ -40,3 +40,18 @@ def test_unaligned_scratch_is_refused(off):
         assert "ckpt" in _lib.last_error()
         assert lib.mvm_seq_scan_bwd(ref, *[some] * 8, odd, *[some] * 11, some, 1 << 40, None) == _lib.MVM_ERR_INVALID_ARG
         assert "ckpt" in _lib.last_error()
+
+
+@pytest.mark.parametrize("kind", ["MambaBlock", "ResidualMambaBlock"])
+def test_served_blocks_build_no_graph(monkeypatch, kind):
+    """prefill and step in the default grad mode: no gradients, not some."""
+    for name in ("conv_silu", "selective_scan"):
+        for form in ("prefill", "step"):
+            fn = f"causal_conv_silu_{form}" if name == "conv_silu" else f"selective_scan_{form}"
+            monkeypatch.setattr(block_mod, fn, lambda u, *a, **k: u.detach() * 0.5)
+    monkeypatch.setattr(block_mod, "layer_norm", lambda x, norm, residual=False: norm(x))
+    blk = getattr(block_mod, kind)(32, d_state=4)
+    x = torch.randn(2, 5, 32, requires_grad=True)
+    states = blk.init_states(2)
+    for y in (blk.prefill(x, states), blk.step(x[:, 0], states)):
+        assert torch.is_grad_enabled() and not y.requires_grad and y.grad_fn is None
