@@ -334,8 +334,15 @@ int mvm_seq_scan_bwd(const mvm_seq_scan_desc* desc, const void* u, const void* d
   int rc = check_scan(desc);
   if (rc != MVM_OK || (rc = check_plain(desc->seq)) != MVM_OK) return rc;
   const mvm::SeqScanGeom g = scan_geom(desc, true);
-  if (g.q.D == 0) return ok();
   const mvm::SeqScanIn in{u, delta, delta_bias, A, Bm, Cm, Dv, z};
+  if (g.q.D == 0) {  // (dB and dC are sums over no channels)
+    if (g.q.T > 0 && (!dB || !dC)) return fail(MVM_ERR_INVALID_ARG, "mvm_seq_scan_bwd: NULL pointer");
+    mvm::SeqScanBwd b{};
+    b.dB = dB; b.dC = dC;
+    return hip_status(mvm::launch_seq_scan_bwd(g, in, b, desc->dtype, desc->delta_dtype,
+                                               static_cast<hipStream_t>(stream)),
+                      "mvm_seq_scan_bwd launch");
+  }
   if (!A || !Dv || !dA || !dD ||
       (g.q.T > 0 && (missing(in) || !ckpt || !dy || !du || !ddelta || !dB || !dC || (z != nullptr) != (dz != nullptr))))
     return fail(MVM_ERR_INVALID_ARG, "mvm_seq_scan_bwd: NULL pointer");

@@ -428,6 +428,18 @@ seq_reduce_kernel(ReduceArgs<T> r) {
 
 // ----------------------------------------------------------------- launches
 
+// (without channels just zeros for dB and dC)
+template <typename T>
+hipError_t launch_reduce(const SeqScanGeom& g, const SeqScanIn& in, const SeqScanBwd& b, int64_t slots, hipStream_t s) {
+  const uint32_t pblocks = static_cast<uint32_t>((18 * g.q.D + 63) / 64);
+  const int64_t bblocks = std::min<int64_t>((static_cast<int64_t>(g.q.T) * 32 + 1023) / 1024, 1 << 18);
+  if (pblocks + bblocks == 0) return hipSuccess;
+  const ReduceArgs<T> red{g.q.D, slots, g.N, g.a_log, g.q.T, static_cast<int32_t>(blocks_of(g.q.D)), pblocks, in.A,
+                          b.part, b.part_bc, b.dA, b.dD, b.ddbias, static_cast<T*>(b.dB), static_cast<T*>(b.dC)};
+  hipLaunchKernelGGL(seq_reduce_kernel<T>, dim3(pblocks + static_cast<unsigned>(bblocks)), dim3(1024), 0, s, red);
+  return hipGetLastError();
+}
+
 template <typename T, typename DT, typename BT>
 hipError_t bwd_t(SeqScanGeom g, const SeqScanIn& in, const SeqScanBwd& b, BcRows<BT> bc, hipStream_t s) {
   set_vec(g, in.A, b.dh1, b.dh0);
@@ -447,12 +459,7 @@ hipError_t bwd_t(SeqScanGeom g, const SeqScanIn& in, const SeqScanBwd& b, BcRows
   }
   hipLaunchKernelGGL((seq_scan_bwd_kernel<T, DT, BT>), grid, dim3(256), 0, s, args);
   if ((e = hipGetLastError()) != hipSuccess) return e;
-  const uint32_t pblocks = static_cast<uint32_t>((18 * g.q.D + 63) / 64);
-  const int64_t bblocks = std::min<int64_t>((static_cast<int64_t>(g.q.T) * 32 + 1023) / 1024, 1 << 18);
-  const ReduceArgs<T> red{g.q.D, slots, g.N, g.a_log, g.q.T, static_cast<int32_t>(ncb), pblocks, in.A, b.part, b.part_bc,
-                          b.dA, b.dD, b.ddbias, static_cast<T*>(b.dB), static_cast<T*>(b.dC)};
-  hipLaunchKernelGGL(seq_reduce_kernel<T>, dim3(pblocks + static_cast<unsigned>(bblocks)), dim3(1024), 0, s, red);
-  return hipGetLastError();
+  return launch_reduce<T>(g, in, b, slots, s);
 }
 
 }  // namespace
@@ -462,6 +469,7 @@ hipError_t launch_seq_scan_bwd(const SeqScanGeom& g, const SeqScanIn& in, const 
   return by_types(dtype, delta_dtype, [&](auto t, auto dt) {
     using T = decltype(t);
     using DT = decltype(dt);
+    if (g.q.D == 0) return launch_reduce<T>(g, in, b, 0, s);
     return with_bc<T>(g, in, b.bc, [&](auto bc) { return bwd_t<T, DT>(g, in, b, bc, s); }, s);
   });
 }

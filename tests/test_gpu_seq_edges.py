@@ -1,6 +1,6 @@
 """The packed and served scan and conv at the edges of what they accept:
 caches of more rows than 32-bit products hold, traces,
-grad mode."""
+grad mode, no channels."""
 
 import pytest
 import torch
@@ -103,3 +103,19 @@ def test_served_blocks_build_no_graph(cuda, kind):
         assert torch.is_grad_enabled() and not y.requires_grad and y.grad_fn is None
         with torch.no_grad():
             assert torch.equal(y, getattr(blk, name)(arg, quiet))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T", [0, 1, 4099])
+def test_gradients_of_no_channels(cuda, T, dtype):
+    """Sums over no channels: B's and C's gradients are zero."""
+    z = lambda *s: torch.zeros(*s, dtype=dtype, device=cuda, requires_grad=True)  # noqa: E731
+    f = lambda *s: torch.zeros(*s, device=cuda, requires_grad=True)  # noqa: E731
+    leaves = dict(u=z(T, 0), delta=z(T, 0), A=f(0, 13), B=z(T, 13), C=z(T, 13), D=f(0))
+    y, final = mvm.selective_scan_packed(*leaves.values(), [0, T // 2, T], z=z(T, 0), delta_softplus=True)
+    # what the allocator hands out again holds something else
+    old = [torch.full((T * 13,), 7.0, dtype=dtype, device=cuda) for _ in range(4)]
+    del old
+    grads = torch.autograd.grad([y, final], list(leaves.values()), [torch.ones_like(y), torch.ones_like(final)])
+    for (n, v), g in zip(leaves.items(), grads):
+        assert g.shape == v.shape and g.dtype == v.dtype and not g.any(), n
