@@ -43,6 +43,7 @@ struct FwdPtrs {
 };
 template <typename T, typename DT, typename BT>
 struct FwdArgs {
+  float zeros[kZeroRow];
   SeqScanGeom g;
   FwdPtrs p;
   BcRows<BT> bc;
@@ -156,7 +157,10 @@ seq_scan_fwd_kernel(FwdArgs<T, DT, BT> args) {
     }
     if (t + kSeqTile > c.t1) {  // positions past the chunk: nothing decays or enters
 #pragma unroll
-      for (int i = 0; i < kSeqTile; ++i) dl[i] = t + i < c.t1 ? dl[i] : 0.f;
+      for (int i = 0; i < kSeqTile; ++i) {
+        dl[i] = t + i < c.t1 ? dl[i] : 0.f;
+        uf[i] = t + i < c.t1 ? uf[i] : 0.f;
+      }
     }
 #pragma unroll
     for (int i = 0; i < kSeqTile; ++i) du[i] = dl[i] * uf[i];
@@ -171,8 +175,12 @@ seq_scan_fwd_kernel(FwdArgs<T, DT, BT> args) {
       typename BcRows<BT>::template Raw<NS> Bv, Cv;
       Bv.load(pb.at);
       if constexpr (!AGG) Cv.load(pc.at);
-      pb.next(i + 1 < left);
-      if constexpr (!AGG) pc.next(i + 1 < left);
+      if constexpr (AGG) {  // (whole tiles only)
+        pb.next(i + 1 < left);
+      } else {
+        pb.next_or(i + 1 < left, zero_row());
+        pc.next(i + 1 < left);
+      }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int n = 0; n < NS; ++n) a[n] = fast_exp2(dl[i] * a2[n]);
@@ -434,7 +442,7 @@ hipError_t fwd_n(SeqScanGeom g, const SeqScanIn& in, const SeqScanFwd& b, BcRows
   const uint32_t ncb = blocks_of(g.q.D);
   const dim3 grid = wave_grid(chunk_slots(g.q, g.cut), ncb);
   set_vec(g, in.A, b.h0, b.h1);
-  const FwdArgs<T, DT, BT> args{g, {in.dbias, in.A, in.Dv, b.h0, b.h1, b.ckpt, b.agg_h, b.agg_s}, bc, ncb,
+  const FwdArgs<T, DT, BT> args{{}, g, {in.dbias, in.A, in.Dv, b.h0, b.h1, b.ckpt, b.agg_h, b.agg_s}, bc, ncb,
                                 static_cast<const T*>(in.u), static_cast<const DT*>(in.delta),
                                 static_cast<const T*>(in.z), static_cast<T*>(b.y)};
   if (g.multi) {

@@ -35,6 +35,7 @@ struct BwdPtrs {
 };
 template <typename T, typename DT, typename BT>
 struct BwdArgs {
+  float zeros[kZeroRow];
   SeqScanGeom g;
   BwdPtrs p;
   BcRows<BT> bc;
@@ -114,7 +115,7 @@ seq_scan_bwd_agg_kernel(BwdArgs<T, DT, BT> args) {
     for (int i = kSeqTile - 1; i >= 0; --i) {
       float a[16];
       typename BcRows<BT>::template Raw<16> Cv;
-      Cv.load(pc.at);
+      Cv.load(t + i < c.t1 ? pc.at : zero_row());
       pc.prev(t + i < c.t1);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -208,12 +209,12 @@ seq_scan_bwd_kernel(BwdArgs<T, DT, BT> args) {
   T nu[kSeqTile], ny[kSeqTile], nz[kSeqTile];
   DT nd[kSeqTile];
   BcTile<BT> nbc;
-  auto fetch = [&](int32_t t) {
-    nbc.fetch(args.bc.B, args.bc.C, args.bc.st, t, c.t1, 16, lane);
-    load_prev(nd, pd, t, c.t1, lc);
-    load_prev(nu, pu, t, c.t1, lc);
-    load_prev(ny, py, t, c.t1, lc);
-    if (gate) load_prev(nz, pz, t, c.t1, lc);
+  auto fetch = [&](int32_t t, int32_t end) {
+    nbc.fetch(args.bc.B, args.bc.C, args.bc.st, t, end, 16, lane);
+    load_prev(nd, pd, t, end, lc);
+    load_prev(nu, pu, t, end, lc);
+    load_prev(ny, py, t, end, lc);
+    if (gate) load_prev(nz, pz, t, end, lc);
   };
   const int32_t row = seq_slot(g.q, c.seq);
   {
@@ -241,17 +242,20 @@ seq_scan_bwd_kernel(BwdArgs<T, DT, BT> args) {
   const float Dd = p.Dv[dc];
   float dD = 0.f, ddb = 0.f;
   const int64_t ck0 = (c.start >> kSeqTileShift) + c.seq;
-  const int32_t last = c.t0 + ((c.t1 - 1 - c.t0) & ~(kSeqTile - 1));
   Pace pace(c.t1 - c.t0);
-  for (int32_t t = last; c.t0 < c.t1 && t >= c.t0; t -= kSeqTile) {
+  // 8 tokens from t on; of a chunk's last tile, which is taken first, maybe fewer
+  auto tile = [&](int32_t t, auto whole) {
+    constexpr bool kWhole = decltype(whole)::value;
+    const int32_t end = kWhole ? t + kSeqTile : c.t1;
     pace.tile();
     float dl[kSeqTile], du[kSeqTile], dr[kSeqTile], qs[kSeqTile], ws[kSeqTile], rs[kSeqTile];
     float us[kSeqTile], sg[kSeqTile], gz[kSeqTile];  // for the outputs
-    fetch(t);
+    fetch(t, end);
     lds_order();
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      reinterpret_cast<float*>(s.bc)[(4 * (lane & 3) + j) * 16 + 2 * (lane & 4) + (lane >> 3)] = nbc.value(j, 16, lane);
+      reinterpret_cast<float*>(s.bc)[(4 * (lane & 3) + j) * 16 + 2 * (lane & 4) + (lane >> 3)] =
+          nbc.value(j, 16, lane, t, end);
     lds_order();
 #pragma unroll
     for (int i = 0; i < kSeqTile; ++i) {
@@ -273,12 +277,12 @@ seq_scan_bwd_kernel(BwdArgs<T, DT, BT> args) {
         gz[i] = ys * fmaf(zf, 1.f - sz, 1.f);  // dy times the derivative of silu(z)
       }
     }
-    if (t + kSeqTile > c.t1 || !all_valid) {
+    if (!kWhole || !all_valid) {
       // positions past the chunk, channels that do not exist: nothing decays,
       // enters or leaves
 #pragma unroll
       for (int i = 0; i < kSeqTile; ++i) {
-        const bool in = valid && t + i < c.t1;
+        const bool in = valid && (kWhole || t + i < end);
         dl[i] = in ? dl[i] : 0.f;
         us[i] = in ? us[i] : 0.f;
         dr[i] = in ? dr[i] : 0.f;
@@ -327,7 +331,9 @@ seq_scan_bwd_kernel(BwdArgs<T, DT, BT> args) {
           const float dh = fmaf(Cv[i], dr[i], cs.v[j]);
           qs[i] = fmaf(dh, Bv[i], qs[i]);
           v[i] = dh * du[i];
-          const float w = dh * ah[i];
+          float w = dh * ah[i];
+          // (past the chunk delta is zero, and either factor may be infinite)
+          if constexpr (!kWhole) w = t + i < end ? w : 0.f;
           da.v[j] = fmaf(w, dl[i], da.v[j]);
           ws[i] = fmaf(w, a2.v[j], ws[i]);
           cs.v[j] = dh * a[i];
@@ -345,10 +351,10 @@ seq_scan_bwd_kernel(BwdArgs<T, DT, BT> args) {
     for (int k = 0; k < 4; ++k) {
       const int i = k * 2 + (lane >> 5), n = lane & 31;
       const float v = reinterpret_cast<const float*>(s.bc)[(n & 15) * 16 + (n >> 4) * 8 + i];
-      if (t + i < c.t1) out[i * 32 + n] = v;
+      if (kWhole || t + i < end) out[i * 32 + n] = v;
     }
     lds_order();
-    const int32_t rows = c.t1 - t < kSeqTile ? c.t1 - t : kSeqTile;
+    const int32_t rows = end - t;
 #pragma unroll
     for (int i = 0; i < kSeqTile; ++i) {
       const float dd = fmaf(ws[i], kLn2, qs[i] * us[i]) * sg[i];
@@ -368,7 +374,13 @@ seq_scan_bwd_kernel(BwdArgs<T, DT, BT> args) {
         store_next<T>(o, rows, lane, rs);
       }
     }
+  };
+  int32_t t = c.t0 + ((c.t1 - 1 - c.t0) & ~(kSeqTile - 1));
+  if (c.t0 < c.t1 && t + kSeqTile > c.t1) {
+    tile(t, std::false_type{});
+    t -= kSeqTile;
   }
+  for (; c.t0 < c.t1 && t >= c.t0; t -= kSeqTile) tile(t, std::true_type{});
   if (!valid) return;
   const auto& late = late_args<BwdArgs<T, DT, BT>>();
   float* part = late.p.part + static_cast<int64_t>(c.slot) * 18 * D + d;
@@ -446,7 +458,7 @@ hipError_t bwd_t(SeqScanGeom g, const SeqScanIn& in, const SeqScanBwd& b, BcRows
   const uint32_t ncb = blocks_of(g.q.D);
   const int64_t slots = chunk_slots(g.q, g.cut);
   const dim3 grid = wave_grid(slots, ncb);
-  const BwdArgs<T, DT, BT> args{g, {in.dbias, in.A, in.Dv, b.dh1, b.dh0, b.ckpt, b.agg_h, b.agg_s, b.part, b.part_bc},
+  const BwdArgs<T, DT, BT> args{{}, g, {in.dbias, in.A, in.Dv, b.dh1, b.dh0, b.ckpt, b.agg_h, b.agg_s, b.part, b.part_bc},
                             bc, ncb, static_cast<uint32_t>(slots), static_cast<const T*>(in.u),
                             static_cast<const DT*>(in.delta), static_cast<const T*>(in.z),
                             static_cast<const T*>(b.dy), static_cast<T*>(b.du), static_cast<DT*>(b.ddelta),

@@ -159,7 +159,7 @@ struct BcRows<bf16_t> {
 // into the branch, and keep all its terms in registers until then
 __device__ __forceinline__ void pin(float& x) { asm volatile("" : "+v"(x)); }
 // B and C of a tile on their way: lane l asks for states 4 (l & 3) .. + 3 of
-// row l >> 3, of B or (l & 4) of C; rows past the chunk are its last one.
+// row l >> 3, of B or (l & 4) of C; rows past the chunk are zero.
 template <typename T>
 struct BcTile {
   T raw[4];
@@ -171,8 +171,8 @@ struct BcTile {
 #pragma unroll
     for (int j = 0; j < 4; ++j) raw[j] = row[state_col(n0 + j, N)];
   }
-  __device__ __forceinline__ float value(int j, int N, uint32_t lane) const {
-    return static_cast<int>(4 * (lane & 3)) + j < N ? to_f32(raw[j]) : 0.f;
+  __device__ __forceinline__ float value(int j, int N, uint32_t lane, int32_t t, int32_t t1) const {
+    return static_cast<int>(4 * (lane & 3)) + j < N && t + static_cast<int32_t>(lane >> 3) < t1 ? to_f32(raw[j]) : 0.f;
   }
 };
 // orders a wave's own LDS accesses for the compiler (the unit keeps them in order)
@@ -196,6 +196,11 @@ struct RowPtr {
   }
   __device__ __forceinline__ void next(bool go = true) {
     at += go ? st : 0u;
+    asm volatile("" : "+s"(at));
+  }
+  // (or another address)
+  __device__ __forceinline__ void next_or(bool go, uint64_t past) {
+    at = go ? at + st : past;
     asm volatile("" : "+s"(at));
   }
   __device__ __forceinline__ void prev(bool go = true) {
@@ -311,6 +316,12 @@ __device__ __forceinline__ const __attribute__((address_space(4))) Args& late_ar
   asm volatile("" : "+s"(at));
   return *(const __attribute__((address_space(4))) Args*)at;
 }
+
+// B and C of positions past a chunk's end: a row of zeros at the front of the
+// kernel's argument.  (What enters there is multiplied by a delta of zero, and
+// infinities of the chunk's last row would make NaN of it.)
+constexpr int kZeroRow = 16;
+__device__ __forceinline__ uint64_t zero_row() { return (uint64_t)__builtin_amdgcn_kernarg_segment_ptr(); }
 
 // f<T, DT>(): T the activations' type, DT delta's
 template <typename F>

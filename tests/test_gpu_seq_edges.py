@@ -1,6 +1,6 @@
 """The packed and served scan and conv at the edges of what they accept:
 caches of more rows than 32-bit products hold, traces,
-grad mode, no channels."""
+grad mode, no channels, infinities in a last token."""
 
 import pytest
 import torch
@@ -10,6 +10,8 @@ from mlx_vision_mamba_amd import gemm
 from tests import seq_reference as ref
 
 pytestmark = pytest.mark.gpu
+
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16}
 
 
 def test_conv_cache_past_32_bit_products(cuda):
@@ -119,3 +121,47 @@ def test_gradients_of_no_channels(cuda, T, dtype):
     grads = torch.autograd.grad([y, final], list(leaves.values()), [torch.ones_like(y), torch.ones_like(final)])
     for (n, v), g in zip(leaves.items(), grads):
         assert g.shape == v.shape and g.dtype == v.dtype and not g.any(), n
+
+
+def _check_kinds(name, got, want):
+    """The oracle's infinities and NaN where it has them, within its bound elsewhere."""
+    g, v = got.detach().double().cpu(), want.v
+    assert torch.equal(torch.isnan(g), torch.isnan(v)), (name, "NaN")
+    inf = torch.isinf(v)
+    assert torch.equal(torch.isinf(g), inf) and torch.equal(g[inf], v[inf]), (name, "infinities")
+    ok = torch.isfinite(v)
+    ref.check(name, torch.where(ok.to(got.device), got, 0), ref.E(torch.where(ok, v, 0.0), torch.where(ok, want.e, 0.0)))
+
+
+LAST = {"u": ("u", (4, 3)), "u negative": ("u", (15, 65)), "B": ("B", (4, 6)), "C": ("C", (15, 2)),
+        "all of B": ("B", (35,)), "final's gradient": ("dfinal", (0, 9, 5)), "every one": ("u", (4, 11))}
+
+
+@pytest.mark.parametrize("what", list(LAST))
+@pytest.mark.parametrize("chunk", [0, 16])
+@pytest.mark.parametrize("N", [8, 16])
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_infinite_last_tokens(cuda, dtype, N, chunk, what):
+    """A sequence ends inside a tile: what its last token makes infinite stays so,
+    and nothing else turns into NaN (tokens 4, 15 and 35 are last ones)."""
+    lens, D, t = [5, 8, 3, 20, 1], 70, TYPES[dtype]
+    off = [0, 5, 13, 16, 36, 37]
+    g = torch.Generator().manual_seed(7)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    a = dict(u=r(37, D).to(t), delta=(0.5 * r(37, D)).to(t), A=torch.log(torch.arange(1, N + 1).float()).repeat(D, 1),
+             B=r(37, N).to(t), C=r(37, N).to(t), D=1 + 0.1 * r(D))
+    k = dict(z=r(37, D).to(t), delta_bias=0.5 * r(D) - 3, initial=r(len(lens), D, N))
+    dy, df = r(37, D).to(t), r(len(lens), D, N)
+    name, at = LAST[what]
+    (df if name == "dfinal" else a[name])[at] = float("-inf") if "negative" in what else float("inf")
+    if what == "every one":
+        a["B"][15, 1] = a["C"][35, 2] = df[1, 2, 3] = float("inf")
+    leaves = {n: v.to(cuda).requires_grad_(True) for n, v in {**a, **k}.items()}
+    y, final = mvm.selective_scan_packed(*[leaves[n] for n in a], off, z=leaves["z"], delta_bias=leaves["delta_bias"],
+                                         initial_states=leaves["initial"], delta_softplus=True, a_is_log=True,
+                                         chunk_len=chunk)
+    grads = torch.autograd.grad([y, final], list(leaves.values()), [dy.to(cuda), df.to(cuda)])
+    want = ref.scan(off, **a, **k, delta_softplus=True, a_is_log=True, dy=dy, dfinal=df)
+    got = {"y": y, "final": final, **{"d" + n: v for n, v in zip(leaves, grads)}}
+    for n, v in got.items():
+        _check_kinds(n, v, want[n])
