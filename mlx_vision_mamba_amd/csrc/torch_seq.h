@@ -20,7 +20,8 @@ Tensor as_rows(const Tensor& t) {
   Tensor r = t.dim() == 3 ? t.reshape({t.size(0) * t.size(1), t.size(2)}) : t;
   return r.size(1) > 1 && r.stride(1) != 1 ? r.contiguous() : r;
 }
-int64_t row_stride(const Tensor& r) { return r.size(0) > 1 ? r.stride(0) : std::max(r.size(1), r.stride(0)); }
+// (a single row's stride is never walked)
+int64_t row_stride(const Tensor& r) { return r.size(0) > 1 ? r.stride(0) : r.size(1); }
 
 // The cut into sequences of an x of (T, D) with offsets (S + 1) or (B, L, D)
 // without, or (S, D) in a step

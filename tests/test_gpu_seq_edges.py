@@ -1,6 +1,7 @@
 """The packed and served scan and conv at the edges of what they accept:
 caches of more rows than 32-bit products hold, traces,
-grad mode, no channels, infinities in a last token."""
+grad mode, no channels, infinities in a last token,
+single rows of any stride."""
 
 import pytest
 import torch
@@ -165,3 +166,35 @@ def test_infinite_last_tokens(cuda, dtype, N, chunk, what):
     got = {"y": y, "final": final, **{"d" + n: v for n, v in zip(leaves, grads)}}
     for n, v in got.items():
         _check_kinds(n, v, want[n])
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_single_rows_of_any_stride(cuda, dtype):
+    """One row has no next one: a stride that the kernels could not walk (the last
+    token of a long history, say) is as good as any."""
+    t, D, N = TYPES[dtype], 64, 16
+    g = torch.Generator().manual_seed(5)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    a = dict(u=r(1, D).to(t), delta=r(1, D).to(t), A=-torch.rand(D, N, generator=g), B=r(1, N).to(t), C=r(1, N).to(t),
+             D=r(D))
+    z, init = r(1, D).to(t), r(1, D, N)
+    want = ref.scan([0, 1], **a, z=z, initial=init, delta_softplus=True)
+    far = lambda v: v.to(cuda).as_strided(v.shape, (2 ** 33 + 64, 1))  # noqa: E731
+    rows = [far(v) if n in ("u", "delta", "B", "C") else v.to(cuda) for n, v in a.items()]
+    states = init.to(cuda)
+    y = mvm.selective_scan_step(*rows, states, z=far(z), delta_softplus=True)
+    ref.check("y", y, want["y"])
+    ref.check("states", states, want["final"])
+    states = init.to(cuda)
+    y = mvm.selective_scan_prefill(*rows, states, [0, 1], z=far(z), delta_softplus=True)
+    ref.check("y", y, want["y"])
+    y, final = mvm.selective_scan_packed(*rows, [0, 1], z=far(z), delta_softplus=True, initial_states=init.to(cuda))
+    ref.check("y", y, want["y"])
+    ref.check("final", final, want["final"])
+    x, w, init = r(1, D).to(t), r(D, 4), r(1, 3, D).to(t)
+    want = ref.conv([0, 1], x, w, initial=init)
+    states = init.to(cuda)
+    ref.check("y", mvm.causal_conv_silu_step(far(x), w.to(cuda), None, states), want["y"])
+    ref.check("states", states, want["final"])
+    y, final = mvm.causal_conv_silu_packed(far(x), w.to(cuda), None, [0, 1], initial_states=init.to(cuda))
+    ref.check("y", y, want["y"])
