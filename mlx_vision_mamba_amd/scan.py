@@ -316,7 +316,8 @@ def sequence_slots(slots, rows, device):
     checked for rows named twice, and what lies outside the cache becomes -1."""
     if slots is None or (isinstance(slots, torch.Tensor) and slots.is_cuda):
         return slots
-    slots = torch.as_tensor(slots)
+    # (torch makes floats of an empty list)
+    slots = torch.as_tensor(slots, dtype=torch.int64 if isinstance(slots, (list, tuple)) and not len(slots) else None)
     if slots.dim() != 1 or slots.is_floating_point():
         raise ValueError(f"slots must be whole numbers, one a sequence; got {tuple(slots.shape)} of {slots.dtype}")
     slots = slots.long()

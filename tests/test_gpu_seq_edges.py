@@ -198,3 +198,17 @@ def test_single_rows_of_any_stride(cuda, dtype):
     ref.check("states", states, want["final"])
     y, final = mvm.causal_conv_silu_packed(far(x), w.to(cuda), None, [0, 1], initial_states=init.to(cuda))
     ref.check("y", y, want["y"])
+
+
+def test_calls_of_no_sequences(cuda):
+    """A scheduler's turn without any: empty outputs, an untouched cache."""
+    D, N = 64, 16
+    z = lambda *s: torch.zeros(*s, device=cuda)  # noqa: E731
+    scan_ops = (z(0, D), z(0, D), -torch.ones(D, N, device=cuda), z(0, N), z(0, N), z(D))
+    h, c = torch.randn(2, D, N, device=cuda), torch.randn(2, 3, D, device=cuda)
+    h0, c0 = h.clone(), c.clone()
+    for y in (mvm.selective_scan_step(*scan_ops, h, slots=[]), mvm.selective_scan_prefill(*scan_ops, h, [0], slots=[]),
+              mvm.causal_conv_silu_step(z(0, D), z(D, 4), None, c, slots=[]),
+              mvm.causal_conv_silu_prefill(z(0, D), z(D, 4), None, c, [0], slots=[])):
+        assert y.shape == (0, D)
+    assert torch.equal(h, h0) and torch.equal(c, c0)

@@ -55,3 +55,12 @@ def test_served_blocks_build_no_graph(monkeypatch, kind):
     states = blk.init_states(2)
     for y in (blk.prefill(x, states), blk.step(x[:, 0], states)):
         assert torch.is_grad_enabled() and not y.requires_grad and y.grad_fn is None
+
+
+def test_no_slots_in_a_list():
+    """A call of no sequences: an empty list is a list of whole numbers."""
+    got = scan_mod.sequence_slots([], 4, "cpu")
+    assert got.dtype == torch.int32 and got.shape == (0,)
+    for bad in ([0.5], torch.zeros(0), [[]]):
+        with pytest.raises(ValueError, match="whole numbers"):
+            scan_mod.sequence_slots(bad, 4, "cpu")
