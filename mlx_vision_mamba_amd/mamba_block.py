@@ -105,10 +105,13 @@ class MambaBlock(nn.Module):
     def init_states(self, rows: int, dtype=None, device=None):
         """Zero states of ``rows`` sequences: the conv's last inputs, (rows,
         d_conv - 1, d_inner) of the activations' type (default: the
-        parameters'), and the scan's states, (rows, d_inner, d_state) float32."""
+        parameters', or autocast's inside of it), and the scan's states, (rows,
+        d_inner, d_state) float32."""
         w = self.in_proj.weight
+        if dtype is None:
+            dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else w.dtype
         device = w.device if device is None else device
-        return (torch.zeros(rows, self.d_conv - 1, self.d_inner, dtype=dtype or w.dtype, device=device),
+        return (torch.zeros(rows, self.d_conv - 1, self.d_inner, dtype=dtype, device=device),
                 torch.zeros(rows, self.d_inner, self.d_state, device=device))
 
     def forward_packed(self, x, offsets=None, states=None, *, max_len=None):

@@ -1,7 +1,7 @@
 """The packed and served scan and conv at the edges of what they accept:
 caches of more rows than 32-bit products hold, traces,
 grad mode, no channels, infinities in a last token,
-single rows of any stride."""
+single rows of any stride, no sequences, autocast."""
 
 import pytest
 import torch
@@ -212,3 +212,24 @@ def test_calls_of_no_sequences(cuda):
               mvm.causal_conv_silu_prefill(z(0, D), z(D, 4), None, c, [0], slots=[])):
         assert y.shape == (0, D)
     assert torch.equal(h, h0) and torch.equal(c, c0)
+
+
+@pytest.mark.parametrize("kind", ["MambaBlock", "ResidualMambaBlock"])
+def test_served_under_autocast(cuda, kind):
+    """The states that a block makes by default fit what it computes there: a
+    prompt and single tokens give the packed form's values."""
+    torch.manual_seed(3)
+    blk = getattr(mvm, kind)(64).to(cuda)
+    x = torch.randn(2, 12, 64, device=cuda)
+    with torch.autocast("cuda", torch.bfloat16), torch.no_grad():
+        want, (conv, _) = blk.forward_packed(x)
+        states = blk.init_states(2)
+        assert states[0].dtype == conv.dtype == torch.bfloat16 and states[1].dtype == torch.float32
+        got = [blk.prefill(x[:, :9], states)] + [blk.step(x[:, t], states)[:, None] for t in range(9, 12)]
+        # the same roundings to bf16 at the same places: float32 sums in another
+        # order move a value across a border of half a step seldom, by one step
+        got = torch.cat(got, 1)
+        assert got.dtype == want.dtype and (got - want).float().norm() <= 2.0 ** -8 * want.float().norm()
+    assert blk.init_states(2)[0].dtype == torch.float32
+    with torch.autocast("cuda", torch.bfloat16):
+        assert blk.init_states(2, dtype=torch.float32)[0].dtype == torch.float32  # what is asked for
