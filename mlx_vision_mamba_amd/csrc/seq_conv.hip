@@ -12,9 +12,10 @@
 // reads its initial state (kc - 1 <= P), and it also writes the final one: both
 // may be one buffer.
 //
-// MI355X: 8191 bf16 tokens of 1536 channels in 23 sequences 14.2 us, 3.6 TB/s (a
-// large copy reaches 4.9); forward + backward of 6272 float32 tokens of 768
-// channels 10 + 16 + 4 us of kernels.
+// MI355X: 8191 bf16 tokens of 1536 channels in 23 sequences 14.1 us, 3.6 TB/s (a
+// large copy reaches 4.9), of 1535 channels, one a lane, 17.3; forward + backward
+// of 6272 tokens of 768 channels 10 + 16 + 4 us of kernels, float32 or bf16 (the
+// backward has two channels a lane).
 #include <initializer_list>
 #include <type_traits>
 
@@ -284,8 +285,8 @@ seq_conv_reduce_kernel(int64_t ncols, int32_t kc, int64_t nparts, const float* _
 
 // One token: the state's rows move up by one in place.  A wave keeps its
 // channels' taps for R sequences, and has all their loads in flight together.
-// MI355X, 1024 sequences of 1536 bf16 channels: 7.2 us, 3.5 TB/s; 8.0 at one
-// sequence a wave.
+// MI355X, 1024 sequences of 1536 bf16 channels: 6.9 us, 3.6 TB/s; 0.8 more at one
+// sequence a wave; 11.7 with 1535 channels, one a lane.
 template <typename T, int V, int KC, int R>
 __global__ void __launch_bounds__(64)
 seq_conv_step_kernel(SeqConvGeom g, uint32_t ncb, const T* __restrict__ x, const float* __restrict__ w,
@@ -425,8 +426,8 @@ hipError_t step_v(const SeqConvGeom& g, const void* x, const float* w, const flo
   };
   // bf16: the taps of a lane's eight channels are more than a sequence's rows, so
   // two sequences share them once there is a wave for each SIMD.  MI355X, 1536
-  // channels: 64 sequences 3.0 us by two, 2.6 by one; 384 4.6 and 4.6; 2048 11.4
-  // and 13.2.  float32 (four channels): 2048 20.4 and 20.1
+  // channels: 64 sequences 3.0 us by two, 2.6 by one; 384 4.6 and 4.6; 2048 10.9
+  // and 12.5.  float32 (four channels): 2048 20.4 and 20.1
   if constexpr (V == 8) {
     if (static_cast<int64_t>(g.q.S) * ncb >= 1024) return run(seq_conv_step_kernel<T, V, KC, 2>, 2);
   }

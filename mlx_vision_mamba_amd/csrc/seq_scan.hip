@@ -16,15 +16,15 @@
 // from its carry.
 //
 // Bound by VALU issue.  On MI355X, 32768 bf16 tokens of 1536 channels with gate
-// and softplus: aggregate pass 138 us, carry 15, main pass 188, the VALU busy
+// and softplus: aggregate pass 123 us, carry 16, main pass 171, the VALU busy
 // 97 % of both passes (85 and 116 instructions a token and wave; 80 of
 // the main pass's are the recurrence, the 16 exponentials among them count
 // twice).  Four waves a SIMD; what kept it from that rate were row addresses
 // held (and spilled) for whole tiles, and the issue order (Pace).
 //
 // B and C are the same for a whole wave and come through scalar loads, as
-// scalar operands.  Through LDS instead (a tile at a time) the same prompt took
-// 146 + 198 us.
+// scalar operands.  Through LDS instead (a tile at a time) both passes took
+// 5 % longer.
 #include "seq_scan_pass.h"
 
 namespace mvm {
@@ -57,7 +57,7 @@ struct FwdArgs {
 // AGG: the end state of each chunk but a sequence's last from a zero state,
 // and the sum of delta over it.  Otherwise the main pass.  NS: the states that a
 // lane holds, 8 where there are no more (16384 bf16 tokens of 1536 channels, 8
-// states: 135 us, 176 by 16).
+// states: 138 us, 178 by 16).
 template <typename T, typename DT, typename BT, bool AGG, int NS>
 __global__ void __launch_bounds__(256, 4)
 seq_scan_fwd_kernel(FwdArgs<T, DT, BT> args) {
@@ -324,10 +324,11 @@ seq_carry_kernel(SeqScanGeom g, uint32_t ncb, const float* __restrict__ A, const
 // little else is asked for beside it: a wave keeps its channels' A, D and bias
 // for R sequences, and has all their loads in flight together.  VEC: states,
 // and B and C, are read four at a time (N a multiple of 4, aligned rows).
-// MI355X, 1024 sequences of 1536 channels, bf16: 43 us, 5.0 TB/s (a large copy
-// reaches 4.9); 48 us while the gate's loads stood in branches, 58 at one sequence
-// a wave.  One or two lanes a channel for up to 4 or 8 states: 2048 sequences
-// 24.5 us (N 4) and 43 (N 8), against 52 and 66 by four lanes, some of them idle.
+// MI355X, 1024 sequences of 1536 channels, bf16: 44.4 us, 4.8 TB/s (a large copy
+// reaches 4.9); 5 us more while the gate's loads stood in branches, 10 more at one
+// sequence a wave.  One or two lanes a channel for up to 4 or 8 states: 2048
+// sequences 28 us (N 4) and 48 (N 8), against 50 and 65 by four lanes, some of
+// them idle.  Single values (N 13): 85 us, 2.1 TB/s.
 template <typename T, typename DT, bool VEC, int R, int G>
 __global__ void __launch_bounds__(256)
 seq_scan_step_kernel(SeqScanGeom g, uint32_t ncb, const T* __restrict__ u, const DT* __restrict__ delta,
@@ -480,8 +481,8 @@ hipError_t step_t(SeqScanGeom g, const SeqScanIn& in, float* states, void* y, hi
   const auto blocks = [&](int G) { return static_cast<uint32_t>((g.q.D * G + 255) / 256); };
   if (!g.h_vec || !bc) return launch(seq_scan_step_kernel<T, DT, false, 1, 4>, blocks(4), 1);
   // four sequences a wave once that leaves each SIMD two waves.  MI355X, 1536 bf16
-  // channels: 64 sequences 6.4 us by four, 6.1 by one; 128 9.7 and 10.4; 512 24.6
-  // and 30.2; 2048 82 and 110
+  // channels: 64 sequences 6.4 us by four, 6.1 by one; 128 7.8 and 8.8; 512 24.6
+  // and 30.0; 2048 89 and 109
   auto run = [&](auto groups) {
     constexpr int G = decltype(groups)::value;
     const uint32_t ncb = blocks(G);

@@ -10,11 +10,11 @@
 // initial state's.  The same passes as forward, in the other direction.
 //
 // Bound by VALU issue.  On MI355X, 16384 bf16 tokens of 1536 channels: aggregate
-// pass 88 us, carry 13, main pass 308 (VALU busy 91 %), reductions 14.  The main
-// pass issues 347 VALU instructions a token and wave: 13 a state for the
+// pass 78 us, carry 12, main pass 259 (VALU busy 93 %), reductions 14.  The main
+// pass issues 346 VALU instructions a token and wave: 13 a state for the
 // recurrence and its gradients, 4.4 for the sums of dB and dC over the wave's
-// channels.  Three waves a SIMD at 168 VGPRs; one at 275 took 689 us, and two
-// with the next tile's loads ahead no less than three.
+// channels.  Three waves a SIMD at 168 VGPRs; one at 275 took 2.2 times as long,
+// and two with the next tile's loads ahead no less than three.
 #include "seq_scan_pass.h"
 
 namespace mvm {
@@ -158,8 +158,8 @@ __device__ __forceinline__ float wave_sums16(const float (&v)[16], int lane) {
 
 // The main pass.  Per tile of 8 tokens the states are taken four at a time
 // (an inner loop that is not unrolled, and ends with the states there are:
-// 16384 bf16 tokens of 1536 channels, forward and backward: 575 us with 16, 430
-// with 8, 380 with 4): the tile is run forward from its
+// 16384 bf16 tokens of 1536 channels, forward and backward: 546 us with 16, 418
+// with 8, 370 with 4): the tile is run forward from its
 // checkpoint with the states and decays kept in registers, then backward.
 // What a state carries from tile to tile (its adjoint and dA) waits in LDS, and
 // the tile's B and C, from where all lanes read them.  All of a wave's LDS is
