@@ -243,7 +243,10 @@ seq_scan_bwd_kernel(BwdArgs<T, DT, BT> args) {
   float dD = 0.f, ddb = 0.f;
   const int64_t ck0 = (c.start >> kSeqTileShift) + c.seq;
   Pace pace(c.t1 - c.t0);
-  // 8 tokens from t on; of a chunk's last tile, which is taken first, maybe fewer
+  // 8 tokens from t on; of a chunk's last tile, which is taken first, maybe fewer:
+  // a copy of the code with masks (which in every tile would be one instruction
+  // in 13 a state; a branch inside, or two copies of the states' loop alone,
+  // spill 16 to 190 registers)
   auto tile = [&](int32_t t, auto whole) {
     constexpr bool kWhole = decltype(whole)::value;
     const int32_t end = kWhole ? t + kSeqTile : c.t1;
