@@ -28,6 +28,11 @@ from .conv import (  # noqa: F401
     causal_conv_silu_prefill,
     causal_conv_silu_step,
 )
+from .delta import (  # noqa: F401
+    gated_delta_rule_packed,
+    gated_delta_rule_prefill,
+    gated_delta_rule_step,
+)
 
 from .mamba_block import (  # noqa: F401
     BidirectionalMambaBlock,
@@ -62,6 +67,9 @@ __all__ = [
     "causal_conv_silu_packed",
     "causal_conv_silu_prefill",
     "causal_conv_silu_step",
+    "gated_delta_rule_packed",
+    "gated_delta_rule_prefill",
+    "gated_delta_rule_step",
     "SCAN_MODES",
     "get_scan_fn",
 ]

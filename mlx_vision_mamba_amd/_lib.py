@@ -118,6 +118,18 @@ class SeqConvDesc(ctypes.Structure):
     ]
 
 
+class DeltaDesc(ctypes.Structure):
+    """Mirror of ``mvm_delta_desc`` (include/mvm_delta.h)."""
+
+    _fields_ = [
+        ("seq", SeqDesc), ("key_heads", _i64), ("value_heads", _i64), ("dk", _i64), ("dv", _i64),
+        ("q_stride", _i64), ("q_stride_head", _i64), ("k_stride", _i64), ("k_stride_head", _i64),
+        ("v_stride", _i64), ("v_stride_head", _i64), ("g_stride", _i64), ("beta_stride", _i64), ("max_len", _i64),
+        ("scale", ctypes.c_float), ("dtype", _i32), ("beta_dtype", _i32), ("qk_l2norm", _i32),
+        ("split_len", _i32), ("reserved", _i32),
+    ]
+
+
 class AdamwTensor(ctypes.Structure):
     """Mirror of ``mvm_adamw_tensor`` (include/mvm_optim.h)."""
 
@@ -190,6 +202,16 @@ SEQ_SIGNATURES = {
     "mvm_seq_conv_step": (ctypes.c_int, [ctypes.POINTER(SeqConvDesc)] + [_vp] * 6),
 }
 
+# symbol -> (restype, argtypes) of include/mvm_delta.h
+DELTA_SIGNATURES = {
+    "mvm_delta_validate": (ctypes.c_int, [ctypes.POINTER(DeltaDesc)]),
+    "mvm_delta_ckpt_elems": (_i64, [ctypes.POINTER(DeltaDesc)]),
+    "mvm_delta_workspace_bytes": (_i64, [ctypes.POINTER(DeltaDesc), ctypes.c_int]),
+    "mvm_delta_fwd": (ctypes.c_int, [ctypes.POINTER(DeltaDesc)] + [_vp] * 10 + [ctypes.c_size_t, _vp]),
+    "mvm_delta_bwd": (ctypes.c_int, [ctypes.POINTER(DeltaDesc)] + [_vp] * 15 + [ctypes.c_size_t, _vp]),
+    "mvm_delta_step": (ctypes.c_int, [ctypes.POINTER(DeltaDesc)] + [_vp] * 8),
+}
+
 _lib = None
 
 
@@ -210,7 +232,7 @@ def lib():
                 f"{LIB_PATH} is missing: build it with `python -m mlx_vision_mamba_amd.build` "
                 "(the HIP extension is required; there is no CPU fallback)")
         handle = ctypes.CDLL(LIB_PATH)
-        for name, (res, args) in {**SIGNATURES, **GEMM_SIGNATURES, **SEQ_SIGNATURES}.items():
+        for name, (res, args) in {**SIGNATURES, **GEMM_SIGNATURES, **SEQ_SIGNATURES, **DELTA_SIGNATURES}.items():
             fn = getattr(handle, name)
             fn.restype = res
             fn.argtypes = args

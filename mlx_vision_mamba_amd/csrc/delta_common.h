@@ -1,0 +1,292 @@
+// Device helpers of the gated delta rule's chunk kernels.
+//
+// Products run on the bf16 matrix units (16x16x32).  A float32 operand is the
+// sum of three bf16 values, exactly (hi = bf16(x), mid = bf16(x - hi), lo = x -
+// hi - mid: the method of gemm.hip), a bfloat16 one is its own only part.  The
+// products of parts whose orders add up to less than 3 are kept: what is left
+// out is below 2^-24 of a product.  So an operand of bfloat16 activations
+// costs three instructions against a float32 state, one of float32 activations
+// six.
+//
+// Lane layout (l = lane, m = l % 16, g = l / 16):
+//   result   lane holds column m, rows 4g .. 4g + 3 of a 16 x 16 tile;
+//   operands lane holds row (A) or column (B) m, 8 values of the summed index.
+// The order of the summed index is free as long as both operands agree.  Here
+// slot e of lane group g stands for 4g + e (e < 4) and 16 + 4g + e - 4 of the
+// 32: then two result tiles one above the other are, converted, the next
+// product's B operand, and the recurrence's chain of products never leaves the
+// registers.  A operands come from LDS: rows as they lie, or columns by the
+// transposing reads.
+#pragma once
+
+#include "delta_kernels.h"
+#include "mvm_delta.h"
+#include "mvm_scan.h"
+#include "seq_common.h"
+
+namespace mvm {
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+constexpr int kC = kDeltaChunk;
+constexpr float kL2Eps = 1e-6f;
+constexpr float kMinLogDecay = -1e4f;
+
+// bf16 parts of an operand of the activations' type
+template <typename T>
+constexpr int kRawParts = std::is_same_v<T, float> ? 3 : 1;
+
+template <int P>
+struct Frag {
+  uint4 p[P];
+};
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  const f32x2 v = {a, b};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
+}
+
+// the P leading bf16 parts of 8 values
+template <int P>
+__device__ __forceinline__ Frag<P> split8(float v0, float v1, float v2, float v3, float v4, float v5, float v6,
+                                          float v7) {
+  float v[8] = {v0, v1, v2, v3, v4, v5, v6, v7};
+  Frag<P> f;
+#pragma unroll
+  for (int q = 0; q < P; ++q) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+      if (q + 1 < P) {
+        v[2 * i] -= __uint_as_float(w[i] << 16);
+        v[2 * i + 1] -= __uint_as_float(w[i] & 0xffff0000u);
+      }
+    }
+    f.p[q] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  return f;
+}
+template <int P>
+__device__ __forceinline__ Frag<P> split_tiles(const f32x4& a, const f32x4& b) {
+  return split8<P>(a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]);
+}
+
+// c + a b: the products of parts whose orders add up to less than ORD, small ones first
+template <int ORD, int PA, int PB>
+__device__ __forceinline__ f32x4 mma(const Frag<PA>& a, const Frag<PB>& b, f32x4 c) {
+#pragma unroll
+  for (int o = ORD - 1; o >= 0; --o)
+#pragma unroll
+    for (int i = 0; i < PA; ++i)
+      if (o - i >= 0 && o - i < PB)
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a.p[i]),
+                                                    __builtin_bit_cast(bf16x8, b.p[o - i]), c, 0, 0, 0);
+  return c;
+}
+
+// A tile of ROWS rows of LD values (LD a multiple of 8, not of 64: rows start in different banks) in
+// LDS, one plane for each part
+template <int ROWS, int COLS, int P>
+struct Tile {
+  static constexpr int LD = COLS + 8;
+  static constexpr int kPlane = ROWS * LD;
+  uint16_t v[P * kPlane];
+
+  // row `row`, summed index k0 .. k0 + 31 in the chained order (k0 includes 4g)
+  __device__ __forceinline__ Frag<P> rows(int row, int k0) const {
+    Frag<P> f;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const uint2 a = *reinterpret_cast<const uint2*>(v + p * kPlane + row * LD + k0);
+      const uint2 b = *reinterpret_cast<const uint2*>(v + p * kPlane + row * LD + k0 + 16);
+      f.p[p] = make_uint4(a.x, a.y, b.x, b.y);
+    }
+    return f;
+  }
+  // the same in the plain order (k0 includes 8g)
+  __device__ __forceinline__ Frag<P> rows_plain(int row, int k0) const {
+    Frag<P> f;
+#pragma unroll
+    for (int p = 0; p < P; ++p) f.p[p] = *reinterpret_cast<const uint4*>(v + p * kPlane + row * LD + k0);
+    return f;
+  }
+  // column c0 + m of the tile, summed index rows r0 .. r0 + 31 in the chained order (r0 includes 4g).  The
+  // transposing read hands lane i of 16 the i % 4-th values of the 8-byte words at the addresses of lanes
+  // i / 4, i / 4 + 4, + 8, + 12.
+  __device__ __forceinline__ Frag<P> cols(int c0, int r0, int m) const {
+    Frag<P> f;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const uint16_t* at = v + p * kPlane + (r0 + (m >> 2)) * LD + c0 + 4 * (m & 3);
+      const uint2 a = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at));
+      const uint2 b = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 16 * LD)));
+      f.p[p] = make_uint4(a.x, a.y, b.x, b.y);
+    }
+    return f;
+  }
+  __device__ __forceinline__ void put(int row, int col, const Frag<P>& f) {
+#pragma unroll
+    for (int p = 0; p < P; ++p) *reinterpret_cast<uint4*>(v + p * kPlane + row * LD + col) = f.p[p];
+  }
+  // values col .. col + 3 of a row (col a multiple of 4)
+  __device__ __forceinline__ f32x4 get4(int row, int col) const {
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int p = P - 1; p >= 0; --p) {
+      const uint2 a = *reinterpret_cast<const uint2*>(v + p * kPlane + row * LD + col);
+      s[0] += __uint_as_float(a.x << 16);
+      s[1] += __uint_as_float(a.x & 0xffff0000u);
+      s[2] += __uint_as_float(a.y << 16);
+      s[3] += __uint_as_float(a.y & 0xffff0000u);
+    }
+    return s;
+  }
+};
+
+// 8 values of a row of n from column c, zero past it
+template <typename T>
+__device__ __forceinline__ void load8f(float (&v)[8], const T* p, int c, int n, bool vec) {
+  if (vec && c + 8 <= n) {
+    if constexpr (std::is_same_v<T, float>) {
+      const float4 a = *reinterpret_cast<const float4*>(p + c), b = *reinterpret_cast<const float4*>(p + c + 4);
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+      const uint4 w = *reinterpret_cast<const uint4*>(p + c);
+      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(u[i] << 16);
+        v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c + i < n ? to_f32(p[c + i]) : 0.f;
+  }
+}
+template <int P>
+__device__ __forceinline__ Frag<P> split8(const float (&v)[8]) {
+  return split8<P>(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]);
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int c, int n, bool vec, const float (&v)[8]) {
+  if (vec && c + 8 <= n) {
+    Pack<T, 8> x;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x.v[i] = from_f32<T>(v[i]);
+    if constexpr (std::is_same_v<T, float>) {
+      reinterpret_cast<float4*>(p + c)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(p + c)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      *reinterpret_cast<Pack<T, 8>*>(p + c) = x;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + i < n) p[c + i] = from_f32<T>(v[i]);
+  }
+}
+// the same as the parts of an operand: bfloat16 as it is
+template <typename T>
+__device__ __forceinline__ Frag<kRawParts<T>> load8(const T* p, int c, int n, bool vec) {
+  if constexpr (std::is_same_v<T, float>) {
+    float v[8];
+    load8f(v, p, c, n, vec);
+    return split8<3>(v);
+  } else {
+    Frag<1> f;
+    if (vec && c + 8 <= n) {
+      f.p[0] = *reinterpret_cast<const uint4*>(p + c);
+    } else {
+      uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c + i < n) w[i >> 1] |= static_cast<uint32_t>(p[c + i].bits) << (16 * (i & 1));
+      f.p[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    return f;
+  }
+}
+
+// Rows [t0, t0 + 64) of a head's q or k as parts in LDS, zero from row n on and from column dk on
+template <typename T, int DKP>
+__device__ __forceinline__ void stage_rows(Tile<kC, DKP, kRawParts<T>>& tile, const T* p, int64_t stride, int n, int dk,
+                                           bool vec, int tid, int nthreads) {
+  constexpr int kPer = DKP / 8;
+  for (int i = tid; i < kC * kPer; i += nthreads) {
+    const int row = i / kPer, c = (i % kPer) * 8;
+    tile.put(row, c, load8<T>(p + (row < n ? row : 0) * stride, c, row < n ? dk : 0, vec));
+  }
+}
+
+// Number of the fragment of 16 rows (tile rt) and 32 columns (ks) of a lower
+// (BWD: upper) triangle of 64 x 64, or -1 where all of it is zero.
+template <bool BWD>
+constexpr int tri_frag(int rt, int ks) {
+  if (BWD) return rt < 2 ? 2 * rt + ks : (ks == 0 ? -1 : rt + 2);
+  return rt < 2 ? (ks == 0 ? rt : -1) : 2 * rt - 2 + ks;
+}
+
+// Sum over the 4 lane groups of the lanes with the same m
+__device__ __forceinline__ float sum_g(float x) {
+  x += __shfl_xor(x, 16);
+  x += __shfl_xor(x, 32);
+  return x;
+}
+
+// Lane = token of a chunk of n: the log decay summed from the chunk's start up to it, in 64 bits: the decay between
+// two tokens is the exponential of a difference, which 32 bits would leave with the rounding of the sums.
+__device__ __forceinline__ double log_decay(const DeltaGeom& g, const float* gp, int t0, int n, int h, int lane) {
+  double s = 0.0;
+  if (lane < n) {
+    const float x = gp[(t0 + static_cast<int64_t>(lane)) * g.gs + h];
+    s = x < kMinLogDecay ? kMinLogDecay : x;  // (NaN stays)
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double v = __shfl_up(s, o);
+    if (lane >= o) s += v;
+  }
+  return s;
+}
+__device__ __forceinline__ float exp_diff(double x) { return fast_exp2(static_cast<float>(x * 1.4426950408889634)); }
+
+template <typename T>
+__device__ __forceinline__ float load_beta(const DeltaGeom& g, const void* beta, int64_t t, int h) {
+  return g.beta_f32 ? static_cast<const float*>(beta)[t * g.bs + h] : to_f32(static_cast<const T*>(beta)[t * g.bs + h]);
+}
+
+// The workgroup's item (a slot and value head) and column block.  Blocks are dealt to the 8 XCDs in turn: the column
+// blocks of an item come 8 apart, so that its rows are read into one L2.
+struct DeltaPos {
+  int32_t slot, h, cb;
+  bool ok;
+};
+__device__ __forceinline__ DeltaPos delta_pos(uint32_t ncb, uint32_t nslots, uint32_t heads) {
+  const uint32_t b = blockIdx.x, r = b / (8 * ncb), in = b - r * 8 * ncb;
+  const uint32_t item = r * 8 + in % 8;
+  const uint32_t slot = item / heads;
+  return {static_cast<int32_t>(slot), static_cast<int32_t>(item - slot * heads), static_cast<int32_t>(in / 8), slot < nslots};
+}
+inline int64_t delta_blocks(int64_t ncb, int64_t nslots, int64_t heads) { return (nslots * heads + 7) / 8 * 8 * ncb; }
+
+// f(type of the activations, std::integral_constant<int, padded dk>)
+template <typename F>
+hipError_t delta_dispatch(int dtype, int dk, F&& f) {
+  const auto by_dk = [&](auto t) {
+    switch (delta_dkp(dk)) {
+      case 32: return f(t, std::integral_constant<int, 32>{});
+      case 64: return f(t, std::integral_constant<int, 64>{});
+      default: return f(t, std::integral_constant<int, 128>{});
+    }
+  };
+  return dtype == MVM_F32 ? by_dk(float{}) : by_dk(bf16_t{});
+}
+
+}  // namespace mvm

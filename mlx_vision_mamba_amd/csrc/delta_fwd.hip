@@ -1,0 +1,198 @@
+// The gated delta rule along time, by chunks of 64 tokens:
+//   R  = diag(beta) (V - diag(e^G) K S)
+//   D  = T R                                   (rows d_t)
+//   O  = scale diag(e^G) Q S + P D
+//   S' = e^Gc S + K' diag(e^(Gc - G)) D        (Gc: G of the last token)
+// with T and P of delta_prep.hip.  The columns of S are independent: a wave
+// keeps 16 of them in registers, as result tiles whose rows are the keys'
+// index, for the whole sequence, and the four waves of a workgroup share the
+// chunk's A operands in LDS.
+#include "delta_common.h"
+
+namespace mvm {
+namespace {
+
+struct FwdArgs {
+  DeltaGeom g;
+  DeltaIn in;
+  DeltaWork w;
+  const float* h0;
+  float* h1;
+  void* o;
+  float* s0;
+  float* vt;
+  uint32_t ncb, nslots;
+};
+
+template <typename T, int DKP, bool SAVE>
+__global__ void __launch_bounds__(256)
+delta_fwd_kernel(FwdArgs a) {
+  constexpr int P = kRawParts<T>, KT = DKP / 16, KS = DKP / 32;
+  constexpr int ORD = P == 3 ? 3 : 2;  // of what only the outputs see: bfloat16 keeps 8 bits of them
+  __shared__ __attribute__((aligned(16))) Tile<kC, DKP, P> sK, sQ;
+  __shared__ uint4 sTri[2 * kTriFrags * kTriParts * 64];
+  __shared__ float4 sDec[kC];
+  const DeltaGeom& g = a.g;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 15, grp = lane >> 4;
+  const DeltaPos p = delta_pos(a.ncb, a.nslots, static_cast<uint32_t>(g.HV));
+  if (!p.ok) return;
+  const int h = p.h, hk = h / g.group;
+  const int col = p.cb * kDeltaCols + 16 * wave + m;
+  const bool live = col < g.DV;
+  T* o = static_cast<T*>(a.o) + static_cast<int64_t>(h) * g.DV + col;
+  const int64_t orow = static_cast<int64_t>(g.HV) * g.DV;
+  const SeqChunk part = seq_chunk(g.q, p.slot, g.part, lane);
+  if (part.t0 < 0) return;
+  if (part.seq >= g.q.S) {  // rows of no sequence
+    if (live)
+      for (int32_t t = part.t0 + 4 * 0 + grp; t < part.t1; t += 4) o[t * orow] = from_f32<T>(0.f);
+    return;
+  }
+  const int32_t row = seq_slot(g.q, part.seq);
+  const int64_t cells = static_cast<int64_t>(g.DK) * g.DV, at_h = static_cast<int64_t>(h) * cells + col;
+  f32x4 S[KT];
+  {
+    const float* src = a.h0 != nullptr && row >= 0 && !seq_fresh(g.q, part.seq) ? a.h0 + row * (g.HV * cells) + at_h : nullptr;
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int d = 16 * t + 4 * grp + r;
+        S[t][r] = src != nullptr && live && d < g.DK ? src[static_cast<int64_t>(d) * g.DV] : 0.f;
+      }
+  }
+  const T* kp = static_cast<const T*>(a.in.k) + hk * g.kh;
+  const T* qp = static_cast<const T*>(a.in.q) + hk * g.qh;
+  const T* vp = static_cast<const T*>(a.in.v) + h * g.vh + col;
+  int32_t slot = cut_div(g.cut, part.start) + part.seq + (part.t0 - part.start) / kC;
+  for (int32_t t0 = part.t0; t0 < part.t1; t0 += kC, ++slot) {
+    const int n = part.t1 - t0 < kC ? part.t1 - t0 : kC;
+    const int64_t at = static_cast<int64_t>(slot) * g.HV + h;
+    __syncthreads();
+    stage_rows<T, DKP>(sK, kp + t0 * g.ks, g.ks, n, g.DK, g.qk_vec, tid, 256);
+    stage_rows<T, DKP>(sQ, qp + t0 * g.qs, g.qs, n, g.DK, g.qk_vec, tid, 256);
+    const uint4* tri = reinterpret_cast<const uint4*>(a.w.tri) + at * (2 * kTriFrags * kTriParts * 64);
+    for (int i = tid; i < 2 * kTriFrags * kTriParts * 64; i += 256) sTri[i] = tri[i];
+    if (tid < kC) sDec[tid] = reinterpret_cast<const float4*>(a.w.dec)[at * kC + tid];
+    const float gam = a.w.gam[at];
+    f32x4 V[4];
+#pragma unroll
+    for (int rt = 0; rt < 4; ++rt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = 16 * rt + 4 * grp + r;
+        V[rt][r] = live && i < n ? to_f32(vp[(t0 + i) * g.vs]) : 0.f;
+      }
+    if constexpr (SAVE) {
+      float* s0 = a.s0 + at * cells + col;
+      if (live)
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int d = 16 * t + 4 * grp + r;
+            if (d < g.DK) s0[static_cast<int64_t>(d) * g.DV] = S[t][r];
+          }
+    }
+    __syncthreads();
+    f32x4 R[4], O[4];
+#pragma unroll
+    for (int rt = 0; rt < 4; ++rt) R[rt] = O[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const Frag<3> sf = split_tiles<3>(S[2 * ks], S[2 * ks + 1]);
+      const int k0 = 32 * ks + 4 * grp;
+#pragma unroll
+      for (int rt = 0; rt < 4; ++rt) {
+        R[rt] = mma<3>(sK.rows(16 * rt + m, k0), sf, R[rt]);
+        O[rt] = mma<ORD>(sQ.rows(16 * rt + m, k0), sf, O[rt]);
+      }
+    }
+    float up[4][4];
+#pragma unroll
+    for (int rt = 0; rt < 4; ++rt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float4 d = sDec[16 * rt + 4 * grp + r];
+        R[rt][r] = d.w * fmaf(-d.x, R[rt][r], V[rt][r]);
+        O[rt][r] *= d.z;
+        up[rt][r] = d.y;
+      }
+    const auto tri_at = [&](int which, int f) {
+      Frag<3> x;
+#pragma unroll
+      for (int q = 0; q < 3; ++q) x.p[q] = sTri[((which * kTriFrags + f) * kTriParts + q) * 64 + lane];
+      return x;
+    };
+    f32x4 D[4];
+    {
+      const Frag<3> rf[2] = {split_tiles<3>(R[0], R[1]), split_tiles<3>(R[2], R[3])};
+#pragma unroll
+      for (int rt = 0; rt < 4; ++rt) {
+        D[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+          if (tri_frag<false>(rt, ks) >= 0) D[rt] = mma<3>(tri_at(0, tri_frag<false>(rt, ks)), rf[ks], D[rt]);
+      }
+    }
+    {
+      const Frag<3> df[2] = {split_tiles<3>(D[0], D[1]), split_tiles<3>(D[2], D[3])};
+#pragma unroll
+      for (int rt = 0; rt < 4; ++rt) {
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+          if (tri_frag<false>(rt, ks) >= 0) O[rt] = mma<ORD>(tri_at(1, tri_frag<false>(rt, ks)), df[ks], O[rt]);
+      }
+    }
+#pragma unroll
+    for (int rt = 0; rt < 4; ++rt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = 16 * rt + 4 * grp + r;
+        if (live && i < n) {
+          o[(t0 + i) * orow] = from_f32<T>(O[rt][r]);
+          if constexpr (SAVE) a.vt[(t0 + i) * orow + static_cast<int64_t>(h) * g.DV + col] = D[rt][r];
+        }
+        D[rt][r] *= up[rt][r];
+      }
+    const Frag<3> uf[2] = {split_tiles<3>(D[0], D[1]), split_tiles<3>(D[2], D[3])};
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      S[t] *= gam;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) S[t] = mma<3>(sK.cols(16 * t, 32 * ks + 4 * grp, m), uf[ks], S[t]);
+    }
+  }
+  if (a.h1 != nullptr && row >= 0 && live && part.t1 == part.end) {
+    float* dst = a.h1 + row * (g.HV * cells) + at_h;
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int d = 16 * t + 4 * grp + r;
+        if (d < g.DK) dst[static_cast<int64_t>(d) * g.DV] = S[t][r];
+      }
+  }
+}
+
+}  // namespace
+
+hipError_t launch_delta_fwd(const DeltaGeom& g, const DeltaIn& in, const DeltaWork& w, const float* h0, float* h1,
+                            void* o, float* s0, float* vt, int dtype, hipStream_t s) {
+  FwdArgs a{g, in, w, h0, h1, o, s0, vt, static_cast<uint32_t>((g.DV + kDeltaCols - 1) / kDeltaCols),
+            static_cast<uint32_t>(chunk_slots(g.q, g.part))};
+  const dim3 grid(static_cast<unsigned>(delta_blocks(a.ncb, a.nslots, g.HV)));
+  hipError_t e = launch_delta_prep(g, in, w, false, dtype, s);
+  if (e != hipSuccess) return e;
+  return delta_dispatch(dtype, g.DK, [&](auto t, auto dkp) {
+    using T = decltype(t);
+    constexpr int DKP = decltype(dkp)::value;
+    if (s0 != nullptr)
+      hipLaunchKernelGGL((delta_fwd_kernel<T, DKP, true>), grid, dim3(256), 0, s, a);
+    else
+      hipLaunchKernelGGL((delta_fwd_kernel<T, DKP, false>), grid, dim3(256), 0, s, a);
+    return hipGetLastError();
+  });
+}
+
+}  // namespace mvm

@@ -1,0 +1,77 @@
+// The gated delta rule: parameter blocks and launch entry points
+// (delta_prep.hip, delta_fwd.hip, delta_bwd.hip, delta_step.hip), used by the
+// C ABI (delta_capi.hip).
+#pragma once
+
+#include "seq_kernels.h"
+
+namespace mvm {
+
+constexpr int kDeltaChunk = 64;   // tokens of a chunk
+constexpr int kDeltaCols = 64;    // state columns of a workgroup: 16 a wave
+
+struct DeltaGeom {
+  SeqGeom q;
+  int32_t HK, HV, group;          // group = HV / HK
+  int32_t DK, DV;
+  int64_t qs, qh, ks, kh, vs, vh, gs, bs;
+  float scale;
+  int32_t l2;
+  int32_t beta_f32;               // beta is float32, else of the activations' type
+  int32_t qk_vec, v_vec;          // rows of q and k, of v are read 16 bytes at a time
+  SeqCut cut;                     // chunks
+  SeqCut part;                    // parts of the time axis, whole chunks
+  int32_t parts;                  // 1: a sequence is one part
+};
+
+struct DeltaIn {
+  const void* q;
+  const void* k;
+  const void* v;
+  const float* g;
+  const void* beta;
+};
+
+// What the chunks' own products leave for the passes along time, for every
+// chunk slot and value head: the fragments of two 64 x 64 triangles as the
+// matrix units take them, and a float4 of scalars for each token.
+struct DeltaWork {
+  void* tri;       // (slots, HV, 2, 6, parts, 64) 16-byte fragments
+  float* dec;      // (slots, HV, 64, 4)
+  float* gam;      // (slots, HV): the decay over the chunk
+  float* trans;    // (part slots, HV, DKP, DKP) transitions of the parts, or null
+  float* carry;    // (part slots, HV, DK, DV): end states of the parts from zero, then their initial states
+};
+
+struct DeltaBwd {
+  const float* s0;   // (slots, HV, DK, DV): initial states of the chunks
+  const float* vt;   // (T, HV, DV): d_t
+  const void* d_o;
+  const float* dh1;  // or null
+  float* dh0;        // or null
+  float* x;          // (T, HV, DV): dv / beta
+  float* dend;       // (slots, HV, DK, DV): gradients of the chunks' final states
+  void* dq;
+  void* dk;
+  void* dv;
+  float* dg;
+  void* dbeta;
+  int32_t o_vec;     // rows of d_o and dv are accessed 16 bytes at a time
+};
+
+// 16-byte fragments of one triangle of a chunk slot and value head
+constexpr int kTriFrags = 6;                   // of 16 rows and 32 columns that are not all zero
+constexpr int kTriParts = 3;
+constexpr int64_t kTriBytes = int64_t{2} * kTriFrags * kTriParts * 64 * 16;
+
+inline int delta_dkp(int dk) { return dk <= 32 ? 32 : (dk <= 64 ? 64 : 128); }
+
+hipError_t launch_delta_prep(const DeltaGeom& g, const DeltaIn& in, const DeltaWork& w, bool backward, int dtype,
+                             hipStream_t s);
+hipError_t launch_delta_fwd(const DeltaGeom& g, const DeltaIn& in, const DeltaWork& w, const float* h0, float* h1,
+                            void* o, float* s0, float* vt, int dtype, hipStream_t s);
+hipError_t launch_delta_bwd(const DeltaGeom& g, const DeltaIn& in, const DeltaWork& w, const DeltaBwd& b, int dtype,
+                            hipStream_t s);
+hipError_t launch_delta_step(const DeltaGeom& g, const DeltaIn& in, float* states, void* o, int dtype, hipStream_t s);
+
+}  // namespace mvm

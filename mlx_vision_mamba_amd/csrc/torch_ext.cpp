@@ -18,6 +18,7 @@
 #include "mvm_norm.h"
 #include "mvm_scan.h"
 #include "torch_host.h"
+#include "torch_delta.h"
 #include "torch_seq.h"
 
 namespace {
@@ -1006,4 +1007,7 @@ PYBIND11_MODULE(_native, m) {
   m.def("seq_conv", &seq_conv);
   m.def("seq_conv_prefill", &seq_conv_prefill);
   m.def("seq_conv_step", &seq_conv_step);
+  m.def("delta", &delta);
+  m.def("delta_prefill", &delta_prefill);
+  m.def("delta_step", &delta_step);
 }
