@@ -33,6 +33,7 @@ from .delta import (  # noqa: F401
     gated_delta_rule_prefill,
     gated_delta_rule_step,
 )
+from .norm import group_norm  # noqa: F401
 
 from .mamba_block import (  # noqa: F401
     BidirectionalMambaBlock,
@@ -70,6 +71,7 @@ __all__ = [
     "gated_delta_rule_packed",
     "gated_delta_rule_prefill",
     "gated_delta_rule_step",
+    "group_norm",
     "SCAN_MODES",
     "get_scan_fn",
 ]

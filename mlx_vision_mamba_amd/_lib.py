@@ -130,6 +130,15 @@ class DeltaDesc(ctypes.Structure):
     ]
 
 
+class GroupNormDesc(ctypes.Structure):
+    """Mirror of ``mvm_group_norm_desc`` (include/mvm_group_norm.h)."""
+
+    _fields_ = [
+        ("batch", _i64), ("positions", _i64), ("channels", _i64), ("groups", _i64), ("x_stride", _i64),
+        ("z_stride", _i64), ("eps", ctypes.c_float), ("dtype", _i32), ("silu", _i32), ("reserved", _i32),
+    ]
+
+
 class AdamwTensor(ctypes.Structure):
     """Mirror of ``mvm_adamw_tensor`` (include/mvm_optim.h)."""
 
@@ -212,6 +221,14 @@ DELTA_SIGNATURES = {
     "mvm_delta_step": (ctypes.c_int, [ctypes.POINTER(DeltaDesc)] + [_vp] * 8),
 }
 
+# symbol -> (restype, argtypes) of include/mvm_group_norm.h
+GROUP_NORM_SIGNATURES = {
+    "mvm_group_norm_validate": (ctypes.c_int, [ctypes.POINTER(GroupNormDesc)]),
+    "mvm_group_norm_workspace_bytes": (_i64, [ctypes.POINTER(GroupNormDesc), ctypes.c_int]),
+    "mvm_group_norm_fwd": (ctypes.c_int, [ctypes.POINTER(GroupNormDesc)] + [_vp] * 7 + [ctypes.c_size_t, _vp]),
+    "mvm_group_norm_bwd": (ctypes.c_int, [ctypes.POINTER(GroupNormDesc)] + [_vp] * 11 + [ctypes.c_size_t, _vp]),
+}
+
 _lib = None
 
 
@@ -232,7 +249,8 @@ def lib():
                 f"{LIB_PATH} is missing: build it with `python -m mlx_vision_mamba_amd.build` "
                 "(the HIP extension is required; there is no CPU fallback)")
         handle = ctypes.CDLL(LIB_PATH)
-        for name, (res, args) in {**SIGNATURES, **GEMM_SIGNATURES, **SEQ_SIGNATURES, **DELTA_SIGNATURES}.items():
+        for name, (res, args) in {**SIGNATURES, **GEMM_SIGNATURES, **SEQ_SIGNATURES, **DELTA_SIGNATURES,
+                                  **GROUP_NORM_SIGNATURES}.items():
             fn = getattr(handle, name)
             fn.restype = res
             fn.argtypes = args

@@ -26,7 +26,7 @@ INCLUDE = os.path.join(ROOT, "include")
 LIB = os.path.join(PKG, "libmvm_scan.so")
 SOURCES = ["capi.hip", "scan_fwd.hip", "scan_bwd.hip", "conv.hip", "layernorm.hip", "gemm.hip", "optim.hip",
            "seq_capi.hip", "seq_scan.hip", "seq_scan_bwd.hip", "seq_conv.hip",
-           "delta_capi.hip", "delta_prep.hip", "delta_fwd.hip", "delta_bwd.hip", "delta_step.hip"]
+           "delta_capi.hip", "delta_prep.hip", "delta_fwd.hip", "delta_bwd.hip", "delta_step.hip", "group_norm.hip"]
 NATIVE = os.path.join(PKG, "_native.so")
 ARCH = "gfx950"
 

@@ -1,0 +1,765 @@
+// Group norm with an activation, channels last (include/mvm_group_norm.h): C
+// ABI and kernels.  Memory-bound.
+//
+// Rows (one position a sample: the heads of a mixer): a power of two of lanes
+// takes a group, all its values in registers, so that x is read once: mean,
+// then variance from the registers.  A wave keeps its groups and walks rows; the
+// backward sums the channels' gradients in registers on the way and leaves one
+// partial row a workgroup.
+//
+// Maps: the values of a group do not fit, so x is read twice, the second time
+// from the last-level cache where it fits there.  One pass leaves every
+// channel's mean and sum of squared differences over a run of positions, a
+// small one joins them to the groups' statistics, one forms y.  Sums are taken
+// around a value of the run itself, and joined as mean and squares (Chan, Golub
+// and LeVeque, "Algorithms for computing the sample variance", 1983): a mean
+// far from zero costs no digits.  The backward has the same three passes, of the
+// sums of dn and dn xh.
+#include <algorithm>
+
+#include "mvm_group_norm.h"
+#include "mvm_scan.h"
+#include "seq_common.h"
+#include "status.h"
+
+namespace mvm {
+namespace {
+
+struct GnGeom {
+  int64_t N, P;
+  int32_t C, G, Cg;
+  int64_t xs, zs;
+  float eps;
+};
+struct GnPtr {
+  const void* x;
+  const float* w;
+  const float* b;
+  const void* z;
+};
+
+__device__ __forceinline__ float silu_grad(float v, float s) { return s * fmaf(v, 1.f - s, 1.f); }
+
+// One value: y and, backward, dn and dz, from n = xh w + b
+template <bool SILU, bool GATE>
+__device__ __forceinline__ float gn_out(float n, float z) {
+  float y = SILU ? n * sigmoid_f(n) : n;
+  if (GATE) y *= z * sigmoid_f(z);
+  return y;
+}
+template <bool SILU, bool GATE>
+__device__ __forceinline__ float gn_grad(float n, float z, float dy, float& dz) {
+  const float sn = SILU ? sigmoid_f(n) : 0.f;
+  if (GATE) {
+    const float sz = sigmoid_f(z);
+    dz = dy * (SILU ? n * sn : n) * silu_grad(z, sz);
+    dy *= z * sz;
+  }
+  return SILU ? dy * silu_grad(n, sn) : dy;
+}
+
+// ------------------------------------------------------------------- rows
+
+// Lanes of a group, groups of a wave, column of value i of lane l
+struct GnLanes {
+  int32_t log2;        // of the lanes of a group
+  int32_t per_wave;
+  uint32_t blocks;     // waves abreast over a row's groups
+};
+
+template <int V>
+__device__ __forceinline__ float group_sum(float v, int log2) {
+  for (int o = 0; o < log2; ++o) v += __shfl_xor(v, 1 << o);
+  return v;
+}
+
+template <typename T, int V, int PER, bool SILU, bool GATE>
+__global__ void __launch_bounds__(256)
+gn_rows_fwd_kernel(GnGeom g, GnPtr p, GnLanes ln, T* __restrict__ y, float2* __restrict__ stats) {
+  const int lane = threadIdx.x & 63, l = lane & ((1 << ln.log2) - 1);
+  const uint32_t wave = blockIdx.x * 4 + (threadIdx.x >> 6), rows = gridDim.x * 4 / ln.blocks;
+  const uint32_t gb = wave % ln.blocks;
+  const int grp = static_cast<int>(gb) * ln.per_wave + (lane >> ln.log2);
+  const bool on = grp < g.G && (lane >> ln.log2) < ln.per_wave;
+  const int c0 = (on ? grp : 0) * g.Cg;
+  const float inv = 1.f / static_cast<float>(g.Cg);
+  for (int64_t n = wave / ln.blocks; n < g.N; n += rows) {
+    float v[PER][V];
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int c = (l + (i << ln.log2)) * V;
+      const bool ok = on && c < g.Cg;
+      const Pack<T, V> x = load_pack<T, V>(static_cast<const T*>(p.x) + n * g.xs + c0 + (ok ? c : 0));
+#pragma unroll
+      for (int j = 0; j < V; ++j) s += v[i][j] = ok ? to_f32(x.v[j]) : 0.f;
+    }
+    const float mean = group_sum<V>(s, ln.log2) * inv;
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        v[i][j] -= mean;
+        s = (l + (i << ln.log2)) * V < g.Cg ? fmaf(v[i][j], v[i][j], s) : s;
+      }
+    const float rstd = 1.f / sqrtf(group_sum<V>(s, ln.log2) * inv + g.eps);
+    if (on && l == 0 && stats != nullptr) stats[n * g.G + grp] = make_float2(mean, rstd);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int c = (l + (i << ln.log2)) * V;
+      if (on && c < g.Cg) {
+        Pack<T, V> z{}, out;
+        if (GATE) z = load_pack<T, V>(static_cast<const T*>(p.z) + n * g.zs + c0 + c);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float w = p.w != nullptr ? p.w[c0 + c + j] : 1.f, b = p.b != nullptr ? p.b[c0 + c + j] : 0.f;
+          out.v[j] = from_f32<T>(gn_out<SILU, GATE>(fmaf(v[i][j] * rstd, w, b), GATE ? to_f32(z.v[j]) : 0.f));
+        }
+        store_pack(y + n * g.C + c0 + c, out);
+      }
+    }
+  }
+}
+
+template <typename T, int V, int PER, bool SILU, bool GATE>
+__global__ void __launch_bounds__(256)
+gn_rows_bwd_kernel(GnGeom g, GnPtr p, GnLanes ln, const float2* __restrict__ stats, const T* __restrict__ dy,
+                   T* __restrict__ dx, T* __restrict__ dz, float* __restrict__ part) {
+  const int lane = threadIdx.x & 63, l = lane & ((1 << ln.log2) - 1);
+  const uint32_t gb = blockIdx.x % ln.blocks, rb = blockIdx.x / ln.blocks, rows = gridDim.x / ln.blocks * 4;
+  const int grp = static_cast<int>(gb) * ln.per_wave + (lane >> ln.log2);
+  const bool on = grp < g.G && (lane >> ln.log2) < ln.per_wave;
+  const int c0 = (on ? grp : 0) * g.Cg;
+  const float inv = 1.f / static_cast<float>(g.Cg);
+  // (weights of 32 values a lane do not fit in the registers beside the rest: read for every row)
+  constexpr bool kKeep = PER * V < 32;
+  float w[PER][V], b[PER][V], dw[PER][V], db[PER][V];
+  const auto weights = [&](int i) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int c = (l + (i << ln.log2)) * V + j;
+      const bool ok = on && c < g.Cg;
+      w[i][j] = p.w != nullptr ? p.w[c0 + (ok ? c : 0)] : 1.f;
+      b[i][j] = p.b != nullptr ? p.b[c0 + (ok ? c : 0)] : 0.f;
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (kKeep) weights(i);
+#pragma unroll
+    for (int j = 0; j < V; ++j) dw[i][j] = db[i][j] = 0.f;
+  }
+  for (int64_t n = rb * 4 + (threadIdx.x >> 6); n < g.N; n += rows) {
+    const float2 st = stats[n * g.G + (on ? grp : 0)];
+    float h[PER][V], xh[PER][V];
+    Pack<T, V> gz[PER];
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int c = (l + (i << ln.log2)) * V;
+      const bool ok = on && c < g.Cg;
+      const int64_t at = c0 + (ok ? c : 0);
+      if (!kKeep) weights(i);
+      const Pack<T, V> x = load_pack<T, V>(static_cast<const T*>(p.x) + n * g.xs + at);
+      const Pack<T, V> d = load_pack<T, V>(dy + n * g.C + at);
+      Pack<T, V> z{};
+      if (GATE) z = load_pack<T, V>(static_cast<const T*>(p.z) + n * g.zs + at);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        xh[i][j] = (to_f32(x.v[j]) - st.x) * st.y;
+        float dzv = 0.f;
+        const float dn = gn_grad<SILU, GATE>(fmaf(xh[i][j], w[i][j], b[i][j]), GATE ? to_f32(z.v[j]) : 0.f,
+                                             to_f32(d.v[j]), dzv);
+        if (GATE) gz[i].v[j] = from_f32<T>(dzv);
+        h[i][j] = ok ? dn * w[i][j] : 0.f;
+        xh[i][j] = ok ? xh[i][j] : 0.f;
+        if (ok) {
+          dw[i][j] = fmaf(dn, xh[i][j], dw[i][j]);
+          db[i][j] += dn;
+        }
+        s1 += h[i][j];
+        s2 = fmaf(h[i][j], xh[i][j], s2);
+      }
+    }
+    s1 = group_sum<V>(s1, ln.log2) * inv;
+    s2 = group_sum<V>(s2, ln.log2) * inv;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int c = (l + (i << ln.log2)) * V;
+      if (on && c < g.Cg) {
+        Pack<T, V> out;
+#pragma unroll
+        for (int j = 0; j < V; ++j) out.v[j] = from_f32<T>(st.y * (h[i][j] - s1 - xh[i][j] * s2));
+        store_pack(dx + n * g.C + c0 + c, out);
+        if (GATE) store_pack(dz + n * g.C + c0 + c, gz[i]);
+      }
+    }
+  }
+  if (part == nullptr) return;
+  // the workgroup's four waves in order
+  __shared__ float sum[2][PER][V][64];
+  for (int q = 0; q < 4; ++q) {
+    if (static_cast<int>(threadIdx.x >> 6) == q)
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          sum[0][i][j][lane] = (q ? sum[0][i][j][lane] : 0.f) + dw[i][j];
+          sum[1][i][j][lane] = (q ? sum[1][i][j][lane] : 0.f) + db[i][j];
+        }
+    __syncthreads();
+  }
+  float* out = part + static_cast<int64_t>(rb) * 2 * g.C;
+  if (threadIdx.x < 64 && on)
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const int c = (l + (i << ln.log2)) * V + j;
+        if (c < g.Cg) {
+          out[c0 + c] = sum[0][i][j][lane];
+          out[g.C + c0 + c] = sum[1][i][j][lane];
+        }
+      }
+}
+
+// dweight | dbias: sums over the partial rows
+__global__ void __launch_bounds__(1024)
+gn_reduce_kernel(const float* part, int64_t nparts, int32_t C, float* dw, float* db) {
+  sum_columns(part, nparts, 2 * static_cast<int64_t>(C), [&](int64_t c, float v) {
+    if (c < C) {
+      if (dw != nullptr) dw[c] = v;
+    } else if (db != nullptr) {
+      db[c - C] = v;
+    }
+  });
+}
+
+// ------------------------------------------------------------------- maps
+
+// A workgroup takes a run of positions of one sample and 256 V / RI columns, RI positions side by side
+struct GnRun {
+  int32_t log2;      // of the threads that lie along a row
+  uint32_t cblocks;
+  uint32_t runs;     // of a sample
+  int32_t len;       // positions of a run
+};
+struct GnAt {
+  int64_t n;
+  int32_t run, c, ri, RI;
+  int64_t p0, p1;
+};
+template <int V>
+__device__ __forceinline__ GnAt gn_at(const GnGeom& g, const GnRun& r) {
+  GnAt a;
+  const uint32_t b = blockIdx.x, q = b / r.cblocks;
+  a.n = q / r.runs;
+  a.run = static_cast<int32_t>(q - static_cast<uint32_t>(a.n) * r.runs);
+  a.c = static_cast<int32_t>(((b - q * r.cblocks) << r.log2) + (threadIdx.x & ((1 << r.log2) - 1))) * V;
+  a.ri = threadIdx.x >> r.log2;
+  a.RI = 256 >> r.log2;
+  a.p0 = static_cast<int64_t>(a.run) * r.len;
+  a.p1 = a.p0 + r.len < g.P ? a.p0 + r.len : g.P;
+  return a;
+}
+
+// (n, mean, sum of squared differences) of two sets of values as one
+__device__ __forceinline__ void chan(float& n, float& m, float& q, float n2, float m2, float q2) {
+  const float t = n + n2;
+  if (n2 == 0.f) return;
+  const float d = m2 - m, f = n2 / t;
+  q += q2 + d * d * n * f;
+  m = fmaf(d, f, m);
+  n = t;
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(256)
+gn_stats_kernel(GnGeom g, GnPtr p, GnRun r, float2* __restrict__ part) {
+  __shared__ float sN[256], sM[256], sQ[256];
+  const GnAt a = gn_at<V>(g, r);
+  const bool ok = a.c < g.C;
+  float piv[V], s[V], q[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) piv[j] = s[j] = q[j] = 0.f;
+  const T* x = static_cast<const T*>(p.x) + a.n * g.P * g.xs + (ok ? a.c : 0);
+  float cnt = 0.f;
+  for (int64_t t = a.p0 + a.ri; t < a.p1; t += a.RI) {
+    const Pack<T, V> v = load_pack<T, V>(x + t * g.xs);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float f = to_f32(v.v[j]);
+      piv[j] = cnt == 0.f ? f : piv[j];
+      const float d = f - piv[j];
+      s[j] += d;
+      q[j] = fmaf(d, d, q[j]);
+    }
+    cnt += 1.f;
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const float m = cnt > 0.f ? s[j] / cnt : 0.f;
+    __syncthreads();
+    sN[threadIdx.x] = cnt;
+    sM[threadIdx.x] = piv[j] + m;
+    sQ[threadIdx.x] = fmaxf(q[j] - s[j] * m, 0.f);
+    __syncthreads();
+    if (a.ri == 0 && ok && a.c + j < g.C) {
+      float n1 = sN[threadIdx.x], m1 = sM[threadIdx.x], q1 = sQ[threadIdx.x];
+      for (int i = 1; i < a.RI; ++i) {
+        const int o = threadIdx.x + (i << r.log2);
+        chan(n1, m1, q1, sN[o], sM[o], sQ[o]);
+      }
+      part[(a.n * r.runs + a.run) * g.C + a.c + j] = make_float2(m1, q1);
+    }
+  }
+}
+
+// A wave a group and sample: its channels' partial statistics as one
+__global__ void __launch_bounds__(256)
+gn_join_kernel(GnGeom g, GnRun r, const float2* __restrict__ part, float2* __restrict__ stats) {
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (item >= g.N * g.G) return;
+  const int64_t n = item / g.G;
+  const int lane = threadIdx.x & 63, c0 = static_cast<int>(item - n * g.G) * g.Cg;
+  float cn = 0.f, m = 0.f, q = 0.f;
+  const int total = static_cast<int>(r.runs) * g.Cg;
+  for (int i = lane; i < total; i += 64) {
+    const int run = i / g.Cg;
+    const float2 v = part[(n * r.runs + run) * g.C + c0 + (i - run * g.Cg)];
+    const int64_t left = g.P - static_cast<int64_t>(run) * r.len;
+    chan(cn, m, q, static_cast<float>(left < r.len ? left : r.len), v.x, v.y);
+  }
+  for (int o = 1; o < 64; o <<= 1) {
+    const float n2 = __shfl_xor(cn, o), m2 = __shfl_xor(m, o), q2 = __shfl_xor(q, o);
+    // (both lanes of a pair join the lower lane's set with the upper's: equal bits)
+    if (lane & o) {
+      float a = n2, b = m2, c = q2;
+      chan(a, b, c, cn, m, q);
+      cn = a, m = b, q = c;
+    } else {
+      chan(cn, m, q, n2, m2, q2);
+    }
+  }
+  if (lane == 0) stats[item] = make_float2(m, 1.f / sqrtf(q / cn + g.eps));
+}
+
+template <typename T, int V, bool SILU, bool GATE>
+__global__ void __launch_bounds__(256)
+gn_apply_kernel(GnGeom g, GnPtr p, GnRun r, const float2* __restrict__ stats, T* __restrict__ y) {
+  const GnAt a = gn_at<V>(g, r);
+  if (a.c >= g.C) return;
+  float mean[V], sc[V], b[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const float2 st = stats[a.n * g.G + (a.c + j) / g.Cg];
+    mean[j] = st.x;
+    sc[j] = st.y * (p.w != nullptr ? p.w[a.c + j] : 1.f);
+    b[j] = p.b != nullptr ? p.b[a.c + j] : 0.f;
+  }
+  for (int64_t t = a.p0 + a.ri; t < a.p1; t += a.RI) {
+    const int64_t row = a.n * g.P + t;
+    const Pack<T, V> x = load_pack<T, V>(static_cast<const T*>(p.x) + row * g.xs + a.c);
+    Pack<T, V> z{}, out;
+    if (GATE) z = load_pack<T, V>(static_cast<const T*>(p.z) + row * g.zs + a.c);
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      out.v[j] = from_f32<T>(gn_out<SILU, GATE>(fmaf(to_f32(x.v[j]) - mean[j], sc[j], b[j]), GATE ? to_f32(z.v[j]) : 0.f));
+    store_pack(y + row * g.C + a.c, out);
+  }
+}
+
+// Every channel's sums of dn xh and dn over a run: part (sample, run)[2][C]
+template <typename T, int V, bool SILU, bool GATE>
+__global__ void __launch_bounds__(256)
+gn_bwd_sums_kernel(GnGeom g, GnPtr p, GnRun r, const float2* __restrict__ stats, const T* __restrict__ dy,
+                   float* __restrict__ part) {
+  __shared__ float sA[256], sB[256];
+  const GnAt a = gn_at<V>(g, r);
+  const bool ok = a.c < g.C;
+  float mean[V], rs[V], w[V], b[V], s1[V], s2[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int c = ok ? a.c + j : 0;
+    const float2 st = stats[a.n * g.G + c / g.Cg];
+    mean[j] = st.x;
+    rs[j] = st.y;
+    w[j] = p.w != nullptr ? p.w[c] : 1.f;
+    b[j] = p.b != nullptr ? p.b[c] : 0.f;
+    s1[j] = s2[j] = 0.f;
+  }
+  for (int64_t t = a.p0 + a.ri; ok && t < a.p1; t += a.RI) {
+    const int64_t row = a.n * g.P + t;
+    const Pack<T, V> x = load_pack<T, V>(static_cast<const T*>(p.x) + row * g.xs + a.c);
+    const Pack<T, V> d = load_pack<T, V>(dy + row * g.C + a.c);
+    Pack<T, V> z{};
+    if (GATE) z = load_pack<T, V>(static_cast<const T*>(p.z) + row * g.zs + a.c);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float xh = (to_f32(x.v[j]) - mean[j]) * rs[j];
+      float dzv = 0.f;
+      const float dn = gn_grad<SILU, GATE>(fmaf(xh, w[j], b[j]), GATE ? to_f32(z.v[j]) : 0.f, to_f32(d.v[j]), dzv);
+      s1[j] = fmaf(dn, xh, s1[j]);
+      s2[j] += dn;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    __syncthreads();
+    sA[threadIdx.x] = s1[j];
+    sB[threadIdx.x] = s2[j];
+    __syncthreads();
+    if (a.ri == 0 && ok && a.c + j < g.C) {
+      float u = s1[j], v = s2[j];
+      for (int i = 1; i < a.RI; ++i) {
+        u += sA[threadIdx.x + (i << r.log2)];
+        v += sB[threadIdx.x + (i << r.log2)];
+      }
+      float* out = part + (a.n * r.runs + a.run) * 2 * g.C + a.c + j;
+      out[0] = u;
+      out[g.C] = v;
+    }
+  }
+}
+
+// A wave a group and sample: the means of dn w xh and dn w
+__global__ void __launch_bounds__(256)
+gn_bwd_join_kernel(GnGeom g, GnPtr p, GnRun r, const float* __restrict__ part, float2* __restrict__ sums) {
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (item >= g.N * g.G) return;
+  const int64_t n = item / g.G;
+  const int lane = threadIdx.x & 63, c0 = static_cast<int>(item - n * g.G) * g.Cg;
+  double u = 0.0, v = 0.0;
+  const int total = static_cast<int>(r.runs) * g.Cg;
+  for (int i = lane; i < total; i += 64) {
+    const int run = i / g.Cg, c = c0 + (i - run * g.Cg);
+    const float* at = part + (n * r.runs + run) * 2 * g.C + c;
+    const float w = p.w != nullptr ? p.w[c] : 1.f;
+    u += static_cast<double>(at[0]) * w;
+    v += static_cast<double>(at[g.C]) * w;
+  }
+  for (int o = 32; o > 0; o >>= 1) {
+    u += __shfl_xor(u, o);
+    v += __shfl_xor(v, o);
+  }
+  const double m = static_cast<double>(g.P) * g.Cg;
+  if (lane == 0) sums[item] = make_float2(static_cast<float>(u / m), static_cast<float>(v / m));
+}
+
+template <typename T, int V, bool SILU, bool GATE>
+__global__ void __launch_bounds__(256)
+gn_bwd_apply_kernel(GnGeom g, GnPtr p, GnRun r, const float2* __restrict__ stats, const float2* __restrict__ sums,
+                    const T* __restrict__ dy, T* __restrict__ dx, T* __restrict__ dz) {
+  const GnAt a = gn_at<V>(g, r);
+  if (a.c >= g.C) return;
+  float mean[V], rs[V], w[V], b[V], m1[V], m2[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int64_t at = a.n * g.G + (a.c + j) / g.Cg;
+    const float2 st = stats[at], sm = sums[at];
+    mean[j] = st.x;
+    rs[j] = st.y;
+    m1[j] = sm.x;
+    m2[j] = sm.y;
+    w[j] = p.w != nullptr ? p.w[a.c + j] : 1.f;
+    b[j] = p.b != nullptr ? p.b[a.c + j] : 0.f;
+  }
+  for (int64_t t = a.p0 + a.ri; t < a.p1; t += a.RI) {
+    const int64_t row = a.n * g.P + t;
+    const Pack<T, V> x = load_pack<T, V>(static_cast<const T*>(p.x) + row * g.xs + a.c);
+    const Pack<T, V> d = load_pack<T, V>(dy + row * g.C + a.c);
+    Pack<T, V> z{}, ox, oz;
+    if (GATE) z = load_pack<T, V>(static_cast<const T*>(p.z) + row * g.zs + a.c);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float xh = (to_f32(x.v[j]) - mean[j]) * rs[j];
+      float dzv = 0.f;
+      const float dn = gn_grad<SILU, GATE>(fmaf(xh, w[j], b[j]), GATE ? to_f32(z.v[j]) : 0.f, to_f32(d.v[j]), dzv);
+      ox.v[j] = from_f32<T>(rs[j] * (dn * w[j] - m2[j] - xh * m1[j]));
+      if (GATE) oz.v[j] = from_f32<T>(dzv);
+    }
+    store_pack(dx + row * g.C + a.c, ox);
+    if (GATE) store_pack(dz + row * g.C + a.c, oz);
+  }
+}
+
+// ------------------------------------------------------------- host side
+
+constexpr int64_t kMaxRows = int64_t{1} << 31;
+constexpr int64_t kMaxBlocks = (int64_t{1} << 24) - 8;  // of 256 threads, 2^32 a launch
+constexpr int kRowValues = 2048;        // of a group, held in registers by 64 lanes
+constexpr int64_t kPartRows = 512;      // partial rows of the channels' gradients
+constexpr size_t kAlign = 256;
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+size_t align_up(size_t x) { return (x + kAlign - 1) / kAlign * kAlign; }
+int log2_ceil(int64_t n) {
+  int l = 0;
+  while ((int64_t{1} << l) < n) ++l;
+  return l;
+}
+
+int check_fields(const mvm_group_norm_desc* d) {
+  if (d == nullptr) return fail(MVM_ERR_INVALID_ARG, "desc is NULL");
+  if (d->batch < 0 || d->positions < 0)
+    return fail(MVM_ERR_INVALID_ARG, "negative size (batch=%lld positions=%lld)", (long long)d->batch,
+                (long long)d->positions);
+  if (d->channels < 1 || d->channels > MVM_GROUP_NORM_MAX_CHANNELS)
+    return fail(MVM_ERR_UNSUPPORTED, "channels=%lld unsupported (1..%d)", (long long)d->channels,
+                MVM_GROUP_NORM_MAX_CHANNELS);
+  if (d->groups < 1 || d->groups > d->channels || d->channels % d->groups != 0)
+    return fail(MVM_ERR_INVALID_ARG, "groups=%lld must divide channels=%lld", (long long)d->groups,
+                (long long)d->channels);
+  if (d->dtype != MVM_F32 && d->dtype != MVM_BF16) return fail(MVM_ERR_UNSUPPORTED, "dtype=%d unsupported", d->dtype);
+  if (d->reserved != 0) return fail(MVM_ERR_INVALID_ARG, "reserved must be 0");
+  if (d->silu != 0 && d->silu != 1) return fail(MVM_ERR_INVALID_ARG, "silu=%d must be 0 or 1", d->silu);
+  if (!(d->eps >= 0.f)) return fail(MVM_ERR_INVALID_ARG, "eps must be >= 0");
+  if (d->positions > 0 && d->batch > kMaxRows / d->positions)
+    return fail(MVM_ERR_UNSUPPORTED, "batch=%lld * positions=%lld: at most %lld rows", (long long)d->batch,
+                (long long)d->positions, (long long)kMaxRows);
+  for (const int64_t s : {d->x_stride, d->z_stride})
+    if (s < 0 || s > (int64_t{1} << 40))
+      return fail(MVM_ERR_INVALID_ARG, "stride %lld must be in [0, 2^40]", (long long)s);
+  return MVM_OK;
+}
+
+GnGeom geom_of(const mvm_group_norm_desc* d) {
+  return {d->batch, d->positions, static_cast<int32_t>(d->channels), static_cast<int32_t>(d->groups),
+          static_cast<int32_t>(d->channels / d->groups), d->x_stride, d->z_stride, d->eps};
+}
+
+bool by_rows(const GnGeom& g) { return g.P == 1 && g.Cg <= kRowValues; }
+
+// The rows kernels' lanes for accesses of V values
+GnLanes lanes_of(const GnGeom& g, int V) {
+  GnLanes l;
+  l.log2 = std::min(6, log2_ceil(ceil_div(g.Cg, V)));
+  l.per_wave = std::min(64 >> l.log2, g.G);
+  l.blocks = static_cast<uint32_t>(ceil_div(g.G, l.per_wave));
+  return l;
+}
+// workgroups along the rows of the backward
+int64_t row_blocks(const GnGeom& g, const GnLanes& l) {
+  return std::max<int64_t>(1, std::min(ceil_div(g.N, 4), std::max<int64_t>(1, kPartRows * 4 / l.blocks)));
+}
+
+// The maps' runs: enough workgroups to fill the card, of 32 positions at least a thread
+GnRun run_of(const GnGeom& g, int V) {
+  GnRun r;
+  r.log2 = std::min(8, log2_ceil(ceil_div(g.C, V)));
+  r.cblocks = static_cast<uint32_t>(ceil_div(g.C, static_cast<int64_t>(V) << r.log2));
+  const int64_t side = 256 >> r.log2;
+  const int64_t want = std::max<int64_t>(1, ceil_div(2048, std::max<int64_t>(1, g.N * r.cblocks)));
+  int64_t len = std::max(ceil_div(g.P, want), std::min<int64_t>(g.P, 8 * side));
+  len = std::max<int64_t>(1, ceil_div(len, side) * side);
+  // (no more workgroups than a launch takes, however many samples)
+  r.len = static_cast<int32_t>(std::min<int64_t>(len, int64_t{1} << 30));
+  r.runs = static_cast<uint32_t>(std::max<int64_t>(1, ceil_div(g.P, r.len)));
+  return r;
+}
+
+// Everything that a call of either direction would be refused for.
+int check_desc(const mvm_group_norm_desc* d) {
+  const int rc = check_fields(d);
+  if (rc != MVM_OK) return rc;
+  const GnGeom g = geom_of(d);
+  if (by_rows(g) || g.N == 0) return MVM_OK;
+  const GnRun r = run_of(g, 1);
+  if (g.N > kMaxBlocks / (static_cast<int64_t>(r.runs) * r.cblocks) || g.N > kMaxBlocks * 4 / g.G)
+    return fail(MVM_ERR_UNSUPPORTED, "batch=%lld, positions=%lld, channels=%lld are too many for one launch",
+                (long long)d->batch, (long long)d->positions, (long long)d->channels);
+  return MVM_OK;
+}
+
+struct GnWs {
+  size_t part = 0, stats = 0, total = 0;
+};
+GnWs ws_of(const GnGeom& g, bool backward) {
+  GnWs w;
+  // (the lanes and runs for the accesses that the pointers will allow: the larger of the two)
+  const size_t row = static_cast<size_t>(g.C) * 8;
+  for (const int V : {1, 4, 8}) {
+    size_t part = 0;
+    if (by_rows(g))
+      part = backward ? static_cast<size_t>(row_blocks(g, lanes_of(g, V))) * row : 0;
+    else
+      part = static_cast<size_t>(g.N) * run_of(g, V).runs * row;
+    w.part = std::max(w.part, align_up(part));
+  }
+  w.stats = by_rows(g) ? 0 : align_up(static_cast<size_t>(g.N) * g.G * 8);
+  w.total = w.part + w.stats;
+  return w;
+}
+
+int check_ws(const char* what, const void* ws, size_t have, size_t need) {
+  if (need > 0 && (ws == nullptr || have < need))
+    return fail(MVM_ERR_WORKSPACE, "%s: workspace %zu bytes < %zu needed", what, have, need);
+  if (need > 0 && (reinterpret_cast<uintptr_t>(ws) & (kAlign - 1)) != 0)
+    return fail(MVM_ERR_WORKSPACE, "%s: workspace must be %zu-byte aligned", what, kAlign);
+  return MVM_OK;
+}
+
+// 16-byte accesses: every row and, for rows, every group starts on one
+template <typename T>
+bool wide(const GnGeom& g, std::initializer_list<const void*> ptrs, bool gate) {
+  constexpr int V = 16 / sizeof(T);
+  uintptr_t u = 0;
+  for (const void* p : ptrs) u |= reinterpret_cast<uintptr_t>(p);
+  const int64_t unit = by_rows(g) ? g.Cg : g.C;
+  return (u & 15) == 0 && unit % V == 0 && g.xs % V == 0 && (!gate || g.zs % V == 0);
+}
+
+// f(type, values an access, silu, gate)
+template <typename F>
+hipError_t dispatch(const mvm_group_norm_desc* d, bool w32, bool w16, bool gate, F&& f) {
+  const auto flags = [&](auto t, auto v) {
+    using std::false_type;
+    using std::true_type;
+    if (d->silu) return gate ? f(t, v, true_type{}, true_type{}) : f(t, v, true_type{}, false_type{});
+    return gate ? f(t, v, false_type{}, true_type{}) : f(t, v, false_type{}, false_type{});
+  };
+  using One = std::integral_constant<int, 1>;
+  if (d->dtype == MVM_F32) return w32 ? flags(float{}, std::integral_constant<int, 4>{}) : flags(float{}, One{});
+  return w16 ? flags(bf16_t{}, std::integral_constant<int, 8>{}) : flags(bf16_t{}, One{});
+}
+
+// f(std::integral_constant<int, accesses of a lane>)
+template <int V, typename F>
+hipError_t with_per(const GnGeom& g, const GnLanes& l, F&& f) {
+  const int64_t per = ceil_div(g.Cg, static_cast<int64_t>(V) << l.log2);
+  if (per <= 1) return f(std::integral_constant<int, 1>{});
+  if (per <= 2) return f(std::integral_constant<int, 2>{});
+  if (per <= 4) return f(std::integral_constant<int, 4>{});
+  if constexpr (V <= 4) {
+    if (per <= 8) return f(std::integral_constant<int, 8>{});
+  }
+  if constexpr (V == 1) {
+    if (per <= 32) return f(std::integral_constant<int, 32>{});
+  }
+  return hipErrorInvalidValue;  // (kRowValues)
+}
+
+}  // namespace
+}  // namespace mvm
+
+extern "C" {
+
+int mvm_group_norm_validate(const mvm_group_norm_desc* desc) {
+  const int rc = mvm::check_desc(desc);
+  return rc == MVM_OK ? mvm::ok() : rc;
+}
+
+int64_t mvm_group_norm_workspace_bytes(const mvm_group_norm_desc* desc, int which) {
+  const int rc = mvm::check_desc(desc);
+  if (rc != MVM_OK) return rc;
+  if (which != 0 && which != 1) return mvm::fail(MVM_ERR_INVALID_ARG, "which=%d must be 0 or 1", which);
+  return static_cast<int64_t>(mvm::ws_of(mvm::geom_of(desc), which == 1).total);
+}
+
+int mvm_group_norm_fwd(const mvm_group_norm_desc* desc, const void* x, const float* weight, const float* bias,
+                       const void* z, void* y, float* stats, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace mvm;
+  int rc = check_desc(desc);
+  if (rc != MVM_OK) return rc;
+  const GnGeom g = geom_of(desc);
+  if (g.N == 0 || g.P == 0) return ok();
+  if (!x || !y) return fail(MVM_ERR_INVALID_ARG, "mvm_group_norm_fwd: NULL pointer");
+  const GnWs w = ws_of(g, false);
+  if ((rc = check_ws("mvm_group_norm_fwd", workspace, workspace_bytes, w.total)) != MVM_OK) return rc;
+  const GnPtr p{x, weight, bias, z};
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const bool gate = z != nullptr;
+  const hipError_t e = dispatch(desc, wide<float>(g, {x, z, y}, gate), wide<bf16_t>(g, {x, z, y}, gate), gate,
+                                [&](auto t, auto v, auto silu, auto gt) {
+    using T = decltype(t);
+    constexpr int V = decltype(v)::value;
+    constexpr bool SILU = decltype(silu)::value, GATE = decltype(gt)::value;
+    if (by_rows(g)) {
+      const GnLanes l = lanes_of(g, V);
+      // (whole workgroups of waves that have one block of groups each; up to 8 waves a SIMD walk the rows)
+      const int64_t waves = std::min<int64_t>(g.N, std::max<int64_t>(1, 16384 / l.blocks)) * l.blocks;
+      const int64_t unit = static_cast<int64_t>(l.blocks) * 4;
+      const dim3 grid(static_cast<unsigned>(ceil_div(ceil_div(waves, unit) * unit, 4)));
+      return with_per<V>(g, l, [&](auto per) {
+        hipLaunchKernelGGL((gn_rows_fwd_kernel<T, V, decltype(per)::value, SILU, GATE>), grid, dim3(256), 0, s, g, p, l,
+                           static_cast<T*>(y), reinterpret_cast<float2*>(stats));
+        return hipGetLastError();
+      });
+    }
+    const GnRun r = run_of(g, V);
+    const dim3 grid(static_cast<unsigned>(g.N * r.runs * r.cblocks));
+    float2* part = static_cast<float2*>(workspace);
+    float2* st = stats != nullptr ? reinterpret_cast<float2*>(stats)
+                                  : reinterpret_cast<float2*>(static_cast<char*>(workspace) + w.part);
+    hipLaunchKernelGGL((gn_stats_kernel<T, V>), grid, dim3(256), 0, s, g, p, r, part);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(gn_join_kernel, dim3(static_cast<unsigned>(ceil_div(g.N * g.G, 4))), dim3(256), 0, s, g, r, part, st);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    hipLaunchKernelGGL((gn_apply_kernel<T, V, SILU, GATE>), grid, dim3(256), 0, s, g, p, r, st, static_cast<T*>(y));
+    return hipGetLastError();
+  });
+  return hip_status(e, "mvm_group_norm_fwd launch");
+}
+
+int mvm_group_norm_bwd(const mvm_group_norm_desc* desc, const void* x, const float* weight, const float* bias,
+                       const void* z, const float* stats, const void* dy, void* dx, float* dweight, float* dbias,
+                       void* dz, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace mvm;
+  int rc = check_desc(desc);
+  if (rc != MVM_OK) return rc;
+  const GnGeom g = geom_of(desc);
+  const bool some = g.N > 0 && g.P > 0, gate = z != nullptr;
+  if (some && (!x || !stats || !dy || !dx || gate != (dz != nullptr)))
+    return fail(MVM_ERR_INVALID_ARG, "mvm_group_norm_bwd: NULL pointer");
+  const GnWs w = ws_of(g, true);
+  if ((rc = check_ws("mvm_group_norm_bwd", workspace, workspace_bytes, w.total)) != MVM_OK) return rc;
+  const GnPtr p{x, weight, bias, z};
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  float* part = static_cast<float*>(workspace);
+  const float2* st = reinterpret_cast<const float2*>(stats);
+  int64_t nparts = 0;
+  const bool params = dweight != nullptr || dbias != nullptr;
+  hipError_t e = hipSuccess;
+  if (some)
+    e = dispatch(desc, wide<float>(g, {x, z, dy, dx, dz}, gate), wide<bf16_t>(g, {x, z, dy, dx, dz}, gate), gate,
+                 [&](auto t, auto v, auto silu, auto gt) {
+      using T = decltype(t);
+      constexpr int V = decltype(v)::value;
+      constexpr bool SILU = decltype(silu)::value, GATE = decltype(gt)::value;
+      if (by_rows(g)) {
+        const GnLanes l = lanes_of(g, V);
+        nparts = row_blocks(g, l);
+        const dim3 grid(static_cast<unsigned>(nparts * l.blocks));
+        return with_per<V>(g, l, [&](auto per) {
+          hipLaunchKernelGGL((gn_rows_bwd_kernel<T, V, decltype(per)::value, SILU, GATE>), grid, dim3(256), 0, s, g, p,
+                             l, st, static_cast<const T*>(dy), static_cast<T*>(dx), static_cast<T*>(dz),
+                             params ? part : nullptr);
+          return hipGetLastError();
+        });
+      }
+      const GnRun r = run_of(g, V);
+      const dim3 grid(static_cast<unsigned>(g.N * r.runs * r.cblocks));
+      nparts = g.N * r.runs;
+      float2* sums = reinterpret_cast<float2*>(static_cast<char*>(workspace) + w.part);
+      hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V, SILU, GATE>), grid, dim3(256), 0, s, g, p, r, st,
+                         static_cast<const T*>(dy), part);
+      hipError_t e = hipGetLastError();
+      if (e != hipSuccess) return e;
+      hipLaunchKernelGGL(gn_bwd_join_kernel, dim3(static_cast<unsigned>(ceil_div(g.N * g.G, 4))), dim3(256), 0, s, g, p,
+                         r, part, sums);
+      if ((e = hipGetLastError()) != hipSuccess) return e;
+      hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, SILU, GATE>), grid, dim3(256), 0, s, g, p, r, st, sums,
+                         static_cast<const T*>(dy), static_cast<T*>(dx), static_cast<T*>(dz));
+      return hipGetLastError();
+    });
+  if (e == hipSuccess && params) {
+    hipLaunchKernelGGL(gn_reduce_kernel, dim3(static_cast<unsigned>(ceil_div(2 * static_cast<int64_t>(g.C), 64))),
+                       dim3(1024), 0, s, part, nparts, g.C, dweight, dbias);
+    e = hipGetLastError();
+  }
+  return hip_status(e, "mvm_group_norm_bwd launch");
+}
+
+}  // extern "C"

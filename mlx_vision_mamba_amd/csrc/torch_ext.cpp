@@ -19,6 +19,7 @@
 #include "mvm_scan.h"
 #include "torch_host.h"
 #include "torch_delta.h"
+#include "torch_group_norm.h"
 #include "torch_seq.h"
 
 namespace {
@@ -1010,4 +1011,5 @@ PYBIND11_MODULE(_native, m) {
   m.def("delta", &delta);
   m.def("delta_prefill", &delta_prefill);
   m.def("delta_step", &delta_step);
+  m.def("group_norm", &group_norm);
 }
