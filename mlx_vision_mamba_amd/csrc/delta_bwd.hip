@@ -42,7 +42,7 @@ __global__ void __launch_bounds__(256)
 delta_bwd_kernel(BwdArgs a) {
   constexpr int P = kRawParts<T>, KT = DKP / 16, KS = DKP / 32;
   __shared__ __attribute__((aligned(16))) Tile<kC, DKP, P> sK, sQ;
-  __shared__ uint4 sTri[2 * kTriFrags * kTriParts * 64];
+  __shared__ uint4 sTri[StageTri<3>::kCount];
   __shared__ float4 sDec[kC];
   const DeltaGeom& g = a.g;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 15, grp = lane >> 4;
@@ -66,27 +66,46 @@ delta_bwd_kernel(BwdArgs a) {
   const T* kp = static_cast<const T*>(a.in.k) + hk * g.kh;
   const T* qp = static_cast<const T*>(a.in.q) + hk * g.qh;
   const int64_t orow = static_cast<int64_t>(g.HV) * g.DV, ocol = static_cast<int64_t>(h) * g.DV + col;
-  const T* dop = static_cast<const T*>(a.b.d_o) + ocol;
+  const T* dop = static_cast<const T*>(a.b.d_o) + (live ? ocol : 0);
   const int32_t slot0 = cut_div(g.cut, part.start) + part.seq + (part.t0 - part.start) / kC;
-  for (int32_t nth = (part.t1 - part.t0 + kC - 1) / kC - 1; nth >= 0; --nth) {
+  const int32_t chunks = (part.t1 - part.t0 + kC - 1) / kC;
+  StageRows<T, DKP> rK, rQ;
+  StageTri<3> rT;
+  float4 rDec;
+  float rGam;
+  T rO[16];
+  const auto load = [&](int32_t i) {
+    const int32_t t0 = part.t0 + i * kC;
+    const int n = part.t1 - t0 < kC ? part.t1 - t0 : kC;
+    const int64_t at = static_cast<int64_t>(slot0 + i) * g.HV + h;
+    rK.load(kp + t0 * g.ks, g.ks, n, g.DK, g.qk_vec, tid);
+    rQ.load(qp + t0 * g.qs, g.qs, n, g.DK, g.qk_vec, tid);
+    rT.load(reinterpret_cast<const uint4*>(a.w.tri) + at * kTriFragments, tid);
+    rDec = reinterpret_cast<const float4*>(a.w.dec)[at * kC + lane];
+    rGam = a.w.gam[at];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int t = 16 * (i >> 2) + 4 * grp + (i & 3);
+      rO[i] = dop[live ? (t0 + (t < n ? t : 0)) * orow : 0];
+    }
+  };
+  if (chunks > 0) load(chunks - 1);
+  for (int32_t nth = chunks - 1; nth >= 0; --nth) {
     const int32_t t0 = part.t0 + nth * kC;
     const int n = part.t1 - t0 < kC ? part.t1 - t0 : kC;
     const int64_t at = static_cast<int64_t>(slot0 + nth) * g.HV + h;
     __syncthreads();
-    stage_rows<T, DKP>(sK, kp + t0 * g.ks, g.ks, n, g.DK, g.qk_vec, tid, 256);
-    stage_rows<T, DKP>(sQ, qp + t0 * g.qs, g.qs, n, g.DK, g.qk_vec, tid, 256);
-    const uint4* tri = reinterpret_cast<const uint4*>(a.w.tri) + at * (2 * kTriFrags * kTriParts * 64);
-    for (int i = tid; i < 2 * kTriFrags * kTriParts * 64; i += 256) sTri[i] = tri[i];
-    if (tid < kC) sDec[tid] = reinterpret_cast<const float4*>(a.w.dec)[at * kC + tid];
-    const float gam = a.w.gam[at];
+    rK.put(sK, n, g.DK, tid);
+    rQ.put(sQ, n, g.DK, tid);
+    rT.put(sTri, tid);
+    if (wave == 0) sDec[lane] = rDec;
+    const float gam = rGam;
     f32x4 O[4];
 #pragma unroll
     for (int rt = 0; rt < 4; ++rt)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = 16 * rt + 4 * grp + r;
-        O[rt][r] = live && i < n ? to_f32(dop[(t0 + i) * orow]) : 0.f;
-      }
+      for (int r = 0; r < 4; ++r) O[rt][r] = live && 16 * rt + 4 * grp + r < n ? to_f32(rO[4 * rt + r]) : 0.f;
+    if (nth > 0) load(nth - 1);
     {
       float* e = a.b.dend + at * cells + col;
       if (live)
@@ -118,19 +137,13 @@ delta_bwd_kernel(BwdArgs a) {
         sx[rt][r] = -d.w * d.x;
         so[rt][r] = d.z;
       }
-    const auto tri_at = [&](int which, int f) {
-      Frag<3> x;
-#pragma unroll
-      for (int q = 0; q < 3; ++q) x.p[q] = sTri[((which * kTriFrags + f) * kTriParts + q) * 64 + lane];
-      return x;
-    };
     {
       const Frag<P> of[2] = {split_tiles<P>(O[0], O[1]), split_tiles<P>(O[2], O[3])};
 #pragma unroll
       for (int rt = 0; rt < 4; ++rt)
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
-          if (tri_frag<true>(rt, ks) >= 0) D[rt] = mma<3>(tri_at(1, tri_frag<true>(rt, ks)), of[ks], D[rt]);
+          if (tri_frag<true>(rt, ks) >= 0) D[rt] = mma<3>(tri_at<3>(sTri, 1, tri_frag<true>(rt, ks), lane), of[ks], D[rt]);
     }
     {
       const Frag<3> df[2] = {split_tiles<3>(D[0], D[1]), split_tiles<3>(D[2], D[3])};
@@ -138,7 +151,7 @@ delta_bwd_kernel(BwdArgs a) {
       for (int rt = 0; rt < 4; ++rt)
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
-          if (tri_frag<true>(rt, ks) >= 0) X[rt] = mma<3>(tri_at(0, tri_frag<true>(rt, ks)), df[ks], X[rt]);
+          if (tri_frag<true>(rt, ks) >= 0) X[rt] = mma<3>(tri_at<3>(sTri, 0, tri_frag<true>(rt, ks), lane), df[ks], X[rt]);
     }
 #pragma unroll
     for (int rt = 0; rt < 4; ++rt)
@@ -311,8 +324,13 @@ delta_grads_kernel(BwdArgs a) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) se += __shfl_xor(se, o);
     __syncthreads();
-    stage_rows<T, DKP>(sm.k.K, static_cast<const T*>(a.in.k) + c.t0 * g.ks + hk * g.kh, g.ks, n, g.DK, g.qk_vec, tid, 256);
-    stage_rows<T, DKP>(sm.k.Q, static_cast<const T*>(a.in.q) + c.t0 * g.qs + hk * g.qh, g.qs, n, g.DK, g.qk_vec, tid, 256);
+    {
+      StageRows<T, DKP> rK, rQ;
+      rK.load(static_cast<const T*>(a.in.k) + c.t0 * g.ks + hk * g.kh, g.ks, n, g.DK, g.qk_vec, tid);
+      rQ.load(static_cast<const T*>(a.in.q) + c.t0 * g.qs + hk * g.qh, g.qs, n, g.DK, g.qk_vec, tid);
+      rK.put(sm.k.K, n, g.DK, tid);
+      rQ.put(sm.k.Q, n, g.DK, tid);
+    }
     __syncthreads();
     {
       float nk = 0.f, nq = 0.f;

@@ -90,7 +90,7 @@ void set_vec(mvm::DeltaGeom& g, const mvm::DeltaIn& in, int dtype) {
   const auto fits = [&](const void* p, int64_t s, int64_t h) {
     return ((static_cast<int64_t>(reinterpret_cast<uintptr_t>(p)) | s * e | h * e) & 15) == 0;
   };
-  g.qk_vec = fits(in.q, g.qs, g.qh) && fits(in.k, g.ks, g.kh);
+  g.qk_vec = g.DK * e % 16 == 0 && fits(in.q, g.qs, g.qh) && fits(in.k, g.ks, g.kh);
   g.v_vec = fits(in.v, g.vs, g.vh);
 }
 

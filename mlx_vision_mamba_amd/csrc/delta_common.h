@@ -30,6 +30,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
@@ -214,15 +215,82 @@ __device__ __forceinline__ Frag<kRawParts<T>> load8(const T* p, int c, int n, bo
   }
 }
 
-// Rows [t0, t0 + 64) of a head's q or k as parts in LDS, zero from row n on and from column dk on
+// 8 values of a row as they lie in memory
+template <typename T>
+struct Raw8 {
+  uint4 v[std::is_same_v<T, float> ? 2 : 1];
+};
+// The 64 rows of a chunk's q or k, dk values each, on their way from global memory (load) into LDS (put), all
+// loads in flight together; rows from n on and columns from dk on are zero.
 template <typename T, int DKP>
-__device__ __forceinline__ void stage_rows(Tile<kC, DKP, kRawParts<T>>& tile, const T* p, int64_t stride, int n, int dk,
-                                           bool vec, int tid, int nthreads) {
-  constexpr int kPer = DKP / 8;
-  for (int i = tid; i < kC * kPer; i += nthreads) {
-    const int row = i / kPer, c = (i % kPer) * 8;
-    tile.put(row, c, load8<T>(p + (row < n ? row : 0) * stride, c, row < n ? dk : 0, vec));
+struct StageRows {
+  static constexpr int kPer = DKP / 8, kItems = kC * kPer / 256;
+  Raw8<T> r[kItems];
+
+  __device__ __forceinline__ static int row(int i, int tid) { return (tid + 256 * i) / kPer; }
+  __device__ __forceinline__ static int col(int i, int tid) { return (tid + 256 * i) % kPer * 8; }
+
+  __device__ __forceinline__ void load(const T* p, int64_t stride, int n, int dk, bool vec, int tid) {
+    if (vec) {  // (dk is a multiple of a 16-byte access)
+#pragma unroll
+      for (int i = 0; i < kItems; ++i) {
+        const int c = col(i, tid), rw = row(i, tid);
+        const T* at = p + (rw < n ? rw : 0) * stride;
+        constexpr int V = 16 / sizeof(T);
+#pragma unroll
+        for (int j = 0; j < 8 / V; ++j) {
+          const uint4 x = *reinterpret_cast<const uint4*>(at + (c + V * j < dk ? c + V * j : 0));
+          r[i].v[j] = x;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kItems; ++i) {
+        const int c = col(i, tid), rw = row(i, tid);
+        const T* at = p + (rw < n ? rw : 0) * stride;
+        uint32_t w[8 * sizeof(T) / 4];
+#pragma unroll
+        for (int j = 0; j < static_cast<int>(8 * sizeof(T) / 4); ++j) {
+          if constexpr (std::is_same_v<T, float>) {
+            w[j] = __float_as_uint(at[c + j < dk ? c + j : 0]);
+          } else {
+            const uint32_t lo = at[c + 2 * j < dk ? c + 2 * j : 0].bits, hi = at[c + 2 * j + 1 < dk ? c + 2 * j + 1 : 0].bits;
+            w[j] = (c + 2 * j < dk ? lo : 0u) | (c + 2 * j + 1 < dk ? hi << 16 : 0u);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < static_cast<int>(sizeof(T) / 2); ++j)
+          r[i].v[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+      }
+    }
   }
+  // the parts of item i
+  __device__ __forceinline__ Frag<kRawParts<T>> parts(int i, int n, int dk, int tid) const {
+    const bool ok = row(i, tid) < n;
+    const int c = col(i, tid);
+    if constexpr (std::is_same_v<T, float>) {
+      float v[8];
+      const uint32_t* u = reinterpret_cast<const uint32_t*>(r[i].v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = ok && c + j < dk ? __uint_as_float(u[j]) : 0.f;
+      return split8<3>(v);
+    } else {
+      // (columns past dk: whole accesses, or zero already)
+      Frag<1> f;
+      f.p[0] = ok && c < dk ? r[i].v[0] : make_uint4(0u, 0u, 0u, 0u);
+      return f;
+    }
+  }
+  __device__ __forceinline__ void put(Tile<kC, DKP, kRawParts<T>>& tile, int n, int dk, int tid) const {
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) tile.put(row(i, tid), col(i, tid), parts(i, n, dk, tid));
+  }
+};
+
+// One row's operand: 8 values from column c on, zero past dk (or where !ok), as parts
+template <typename T>
+__device__ __forceinline__ Frag<kRawParts<T>> row_frag(const T* p, int c, int dk, bool vec, bool ok) {
+  return load8<T>(p, c, ok ? dk : 0, vec);
 }
 
 // Number of the fragment of 16 rows (tile rt) and 32 columns (ks) of a lower
@@ -231,6 +299,30 @@ template <bool BWD>
 constexpr int tri_frag(int rt, int ks) {
   if (BWD) return rt < 2 ? 2 * rt + ks : (ks == 0 ? -1 : rt + 2);
   return rt < 2 ? (ks == 0 ? rt : -1) : 2 * rt - 2 + ks;
+}
+
+// A chunk's two triangles on their way into LDS: three parts of the first, PP of the second
+template <int PP>
+struct StageTri {
+  static constexpr int kCount = tri_index(1, PP, 0), kItems = (kCount + 255) / 256;
+  u32x4 r[kItems];
+  __device__ __forceinline__ void load(const uint4* tri, int tid) {
+    const u32x4* at = reinterpret_cast<const u32x4*>(tri);
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) r[i] = at[256 * (i + 1) <= kCount || tid + 256 * i < kCount ? tid + 256 * i : 0];
+  }
+  __device__ __forceinline__ void put(uint4* lds, int tid) const {
+#pragma unroll
+    for (int i = 0; i < kItems; ++i)
+      if (256 * (i + 1) <= kCount || tid + 256 * i < kCount) reinterpret_cast<u32x4*>(lds)[tid + 256 * i] = r[i];
+  }
+};
+template <int P>
+__device__ __forceinline__ Frag<P> tri_at(const uint4* lds, int which, int f, int lane) {
+  Frag<P> x;
+#pragma unroll
+  for (int q = 0; q < P; ++q) x.p[q] = lds[tri_index(which, q, f) + lane];
+  return x;
 }
 
 // Sum over the 4 lane groups of the lanes with the same m

@@ -30,7 +30,7 @@ delta_fwd_kernel(FwdArgs a) {
   constexpr int P = kRawParts<T>, KT = DKP / 16, KS = DKP / 32;
   constexpr int ORD = P == 3 ? 3 : 2;  // of what only the outputs see: bfloat16 keeps 8 bits of them
   __shared__ __attribute__((aligned(16))) Tile<kC, DKP, P> sK, sQ;
-  __shared__ uint4 sTri[2 * kTriFrags * kTriParts * 64];
+  __shared__ uint4 sTri[StageTri<ORD>::kCount];
   __shared__ float4 sDec[kC];
   const DeltaGeom& g = a.g;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 15, grp = lane >> 4;
@@ -63,26 +63,47 @@ delta_fwd_kernel(FwdArgs a) {
   }
   const T* kp = static_cast<const T*>(a.in.k) + hk * g.kh;
   const T* qp = static_cast<const T*>(a.in.q) + hk * g.qh;
-  const T* vp = static_cast<const T*>(a.in.v) + h * g.vh + col;
-  int32_t slot = cut_div(g.cut, part.start) + part.seq + (part.t0 - part.start) / kC;
-  for (int32_t t0 = part.t0; t0 < part.t1; t0 += kC, ++slot) {
+  const T* vp = static_cast<const T*>(a.in.v) + h * g.vh + (live ? col : 0);
+  const int32_t slot0 = cut_div(g.cut, part.start) + part.seq + (part.t0 - part.start) / kC;
+  const int32_t chunks = (part.t1 - part.t0 + kC - 1) / kC;
+  // the next chunk's operands, on their way while this one's are at work
+  StageRows<T, DKP> rK, rQ;
+  StageTri<ORD> rT;
+  float4 rDec;
+  float rGam;
+  T rV[16];
+  const auto load = [&](int32_t i) {
+    const int32_t t0 = part.t0 + i * kC;
     const int n = part.t1 - t0 < kC ? part.t1 - t0 : kC;
-    const int64_t at = static_cast<int64_t>(slot) * g.HV + h;
+    const int64_t at = static_cast<int64_t>(slot0 + i) * g.HV + h;
+    rK.load(kp + t0 * g.ks, g.ks, n, g.DK, g.qk_vec, tid);
+    rQ.load(qp + t0 * g.qs, g.qs, n, g.DK, g.qk_vec, tid);
+    rT.load(reinterpret_cast<const uint4*>(a.w.tri) + at * kTriFragments, tid);
+    rDec = reinterpret_cast<const float4*>(a.w.dec)[at * kC + lane];
+    rGam = a.w.gam[at];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int t = 16 * (i >> 2) + 4 * grp + (i & 3);
+      rV[i] = vp[live ? (t0 + (t < n ? t : 0)) * g.vs : 0];
+    }
+  };
+  if (chunks > 0) load(0);
+  for (int32_t nth = 0; nth < chunks; ++nth) {
+    const int32_t t0 = part.t0 + nth * kC;
+    const int n = part.t1 - t0 < kC ? part.t1 - t0 : kC;
+    const int64_t at = static_cast<int64_t>(slot0 + nth) * g.HV + h;
     __syncthreads();
-    stage_rows<T, DKP>(sK, kp + t0 * g.ks, g.ks, n, g.DK, g.qk_vec, tid, 256);
-    stage_rows<T, DKP>(sQ, qp + t0 * g.qs, g.qs, n, g.DK, g.qk_vec, tid, 256);
-    const uint4* tri = reinterpret_cast<const uint4*>(a.w.tri) + at * (2 * kTriFrags * kTriParts * 64);
-    for (int i = tid; i < 2 * kTriFrags * kTriParts * 64; i += 256) sTri[i] = tri[i];
-    if (tid < kC) sDec[tid] = reinterpret_cast<const float4*>(a.w.dec)[at * kC + tid];
-    const float gam = a.w.gam[at];
+    rK.put(sK, n, g.DK, tid);
+    rQ.put(sQ, n, g.DK, tid);
+    rT.put(sTri, tid);
+    if (wave == 0) sDec[lane] = rDec;
+    const float gam = rGam;
     f32x4 V[4];
 #pragma unroll
     for (int rt = 0; rt < 4; ++rt)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = 16 * rt + 4 * grp + r;
-        V[rt][r] = live && i < n ? to_f32(vp[(t0 + i) * g.vs]) : 0.f;
-      }
+      for (int r = 0; r < 4; ++r) V[rt][r] = live && 16 * rt + 4 * grp + r < n ? to_f32(rV[4 * rt + r]) : 0.f;
+    if (nth + 1 < chunks) load(nth + 1);
     if constexpr (SAVE) {
       float* s0 = a.s0 + at * cells + col;
       if (live)
@@ -118,12 +139,6 @@ delta_fwd_kernel(FwdArgs a) {
         O[rt][r] *= d.z;
         up[rt][r] = d.y;
       }
-    const auto tri_at = [&](int which, int f) {
-      Frag<3> x;
-#pragma unroll
-      for (int q = 0; q < 3; ++q) x.p[q] = sTri[((which * kTriFrags + f) * kTriParts + q) * 64 + lane];
-      return x;
-    };
     f32x4 D[4];
     {
       const Frag<3> rf[2] = {split_tiles<3>(R[0], R[1]), split_tiles<3>(R[2], R[3])};
@@ -132,16 +147,16 @@ delta_fwd_kernel(FwdArgs a) {
         D[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
-          if (tri_frag<false>(rt, ks) >= 0) D[rt] = mma<3>(tri_at(0, tri_frag<false>(rt, ks)), rf[ks], D[rt]);
+          if (tri_frag<false>(rt, ks) >= 0) D[rt] = mma<3>(tri_at<3>(sTri, 0, tri_frag<false>(rt, ks), lane), rf[ks], D[rt]);
       }
     }
     {
-      const Frag<3> df[2] = {split_tiles<3>(D[0], D[1]), split_tiles<3>(D[2], D[3])};
+      const Frag<ORD> df[2] = {split_tiles<ORD>(D[0], D[1]), split_tiles<ORD>(D[2], D[3])};
 #pragma unroll
       for (int rt = 0; rt < 4; ++rt) {
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
-          if (tri_frag<false>(rt, ks) >= 0) O[rt] = mma<ORD>(tri_at(1, tri_frag<false>(rt, ks)), df[ks], O[rt]);
+          if (tri_frag<false>(rt, ks) >= 0) O[rt] = mma<ORD>(tri_at<ORD>(sTri, 1, tri_frag<false>(rt, ks), lane), df[ks], O[rt]);
       }
     }
 #pragma unroll

@@ -36,7 +36,7 @@ struct DeltaIn {
 // chunk slot and value head: the fragments of two 64 x 64 triangles as the
 // matrix units take them, and a float4 of scalars for each token.
 struct DeltaWork {
-  void* tri;       // (slots, HV, 2, 6, parts, 64) 16-byte fragments
+  void* tri;       // (slots, HV, 2, parts, 6, 64) 16-byte fragments
   float* dec;      // (slots, HV, 64, 4)
   float* gam;      // (slots, HV): the decay over the chunk
   float* trans;    // (part slots, HV, DKP, DKP) transitions of the parts, or null
@@ -62,7 +62,11 @@ struct DeltaBwd {
 // 16-byte fragments of one triangle of a chunk slot and value head
 constexpr int kTriFrags = 6;                   // of 16 rows and 32 columns that are not all zero
 constexpr int kTriParts = 3;
-constexpr int64_t kTriBytes = int64_t{2} * kTriFrags * kTriParts * 64 * 16;
+constexpr int kTriFragments = 2 * kTriFrags * kTriParts * 64;
+constexpr int64_t kTriBytes = int64_t{kTriFragments} * 16;
+// where lane 0's fragment f of part p of the which-th triangle lies: the leading parts of the second come first,
+// so that a pass that needs no more of them reads one run
+constexpr int tri_index(int which, int p, int f) { return ((which * kTriParts + p) * kTriFrags + f) * 64; }
 
 inline int delta_dkp(int dk) { return dk <= 32 ? 32 : (dk <= 64 ? 64 : 128); }
 

@@ -5,11 +5,15 @@
 // delta_bwd.hip), which take T and P as ready A operands: their bf16 parts in
 // the order in which the lanes load them (the backward pass: of T' and P').
 //
-// A workgroup of four waves takes one chunk and head.  T: the four 16 x 16
-// blocks on the diagonal by substitution, a column a lane (a series in powers
-// of A would cancel: they grow like binomials where keys repeat), those below
-// by products of blocks, T_ij = -T_ii sum_k A_ik T_kj, in the float32 matrix
-// instructions, a block column a wave.
+// A workgroup of four waves takes one chunk and head, a wave 16 rows of both
+// triangles.  A result tile is, as the lanes hold it, an A operand of its
+// transpose: so the forward pass forms K Q' and the inverse of I + A', the
+// backward Q K' and that of I + A, and nothing is transposed.  The inverse M of
+// the triangle (below, its transpose's blocks are meant where it is upper): the
+// four 16 x 16 blocks on the diagonal by substitution, a column a lane (a series
+// in powers of A would cancel: they grow like binomials where keys repeat), the
+// others by products of blocks, M_iw = -M_ii sum_k A_ik M_kw, in the float32
+// matrix instructions, a block column a wave, chained in registers.
 #include "delta_common.h"
 
 namespace mvm {
@@ -28,8 +32,8 @@ template <typename T, int DKP, bool BWD>
 __global__ void __launch_bounds__(256)
 delta_prep_kernel(DeltaGeom g, DeltaIn in, DeltaWork w) {
   constexpr int P = kRawParts<T>;
-  __shared__ __attribute__((aligned(16))) Tile<kC, DKP, P> sK, sQ;
-  __shared__ __attribute__((aligned(16))) float sA[kC][kLda], sT[kC][kLda];
+  // A (forward: transposed), and the inverses of its diagonal blocks
+  __shared__ __attribute__((aligned(16))) float sA[kC][kLda], sD[4][16][20];
   __shared__ double sG[kC];
   __shared__ float sBeta[kC], sRk[kC], sRq[kC];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 15, grp = lane >> 4;
@@ -38,127 +42,121 @@ delta_prep_kernel(DeltaGeom g, DeltaIn in, DeltaWork w) {
   const SeqChunk c = seq_chunk(g.q, static_cast<int32_t>(slot), g.cut, lane);
   if (c.seq >= g.q.S || c.t0 < 0 || c.t1 == c.t0) return;
   const int n = c.t1 - c.t0;
-  stage_rows<T, DKP>(sK, static_cast<const T*>(in.k) + c.t0 * g.ks + hk * g.kh, g.ks, n, g.DK, g.qk_vec, tid, 256);
-  stage_rows<T, DKP>(sQ, static_cast<const T*>(in.q) + c.t0 * g.qs + hk * g.qh, g.qs, n, g.DK, g.qk_vec, tid, 256);
-  const double G = log_decay(g, in.g, c.t0, n, h, lane);
-  const float beta = lane < n ? load_beta<T>(g, in.beta, c.t0 + lane, h) : 0.f;
-  if (wave == 0) {
-    sG[lane] = G;
-    sBeta[lane] = beta;
-  }
-  __syncthreads();
-  {
-    float nk = 0.f, nq = 0.f;
+  const T* kp = static_cast<const T*>(in.k) + c.t0 * g.ks + hk * g.kh;
+  const T* qp = static_cast<const T*>(in.q) + c.t0 * g.qs + hk * g.qh;
+  // Tiles of K K' and of the q . k products, rows jt, columns the wave's: for the forward pass rows are keys up
+  // to the wave's tokens, for the backward queries from them on.
+  f32x4 kk[4], qk[4], qq = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int t = 0; t < DKP / 16; ++t) {
-      const f32x4 a = sK.get4(16 * wave + m, 16 * t + 4 * grp), b = sQ.get4(16 * wave + m, 16 * t + 4 * grp);
+  for (int jt = 0; jt < 4; ++jt) kk[jt] = qk[jt] = qq;
+  const auto need = [&](int jt) { return BWD ? jt >= wave : jt <= wave; };
+  const int own = 16 * wave + m;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) nk = fmaf(a[r], a[r], nk), nq = fmaf(b[r], b[r], nq);
-    }
-    nk = sum_g(nk);
-    nq = sum_g(nq);
-    if (grp == 0) {
-      sRk[16 * wave + m] = g.l2 ? 1.f / sqrtf(nk + kL2Eps) : 1.f;
-      sRq[16 * wave + m] = g.l2 ? 1.f / sqrtf(nq + kL2Eps) : 1.f;
-    }
-  }
-  __syncthreads();
-  const int64_t at = static_cast<int64_t>(slot) * g.HV + h;
-  const double Gc = __shfl(G, 63);
-  if (wave == 0) {
-    const float eG = exp_diff(G), eR = exp_diff(Gc - G);
-    reinterpret_cast<float4*>(w.dec)[at * kC + lane] =
-        make_float4(sRk[lane] * eG, sRk[lane] * eR, g.scale * sRq[lane] * eG, beta);
-    if (lane == 0) w.gam[at] = exp_diff(Gc);
-  }
-  // row tile `wave` of K K' and Q K'
-  f32x4 kk[4], qk[4];
-#pragma unroll
-  for (int ct = 0; ct < 4; ++ct) kk[ct] = qk[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
   for (int ks = 0; ks < DKP / 32; ++ks) {
     const int k0 = 32 * ks + 8 * grp;
-    const Frag<P> a = sK.rows_plain(16 * wave + m, k0), aq = sQ.rows_plain(16 * wave + m, k0);
+    const auto frag = [&](const T* p, int64_t stride, int row) {
+      return row_frag<T>(p + (row < n ? row : 0) * stride, k0, g.DK, g.qk_vec, row < n);
+    };
+    const Frag<P> bk = frag(kp, g.ks, own), bq = frag(qp, g.qs, own);
+    qq = mma<3>(bq, bq, qq);
 #pragma unroll
-    for (int ct = 0; ct < 4; ++ct)
-      if (ct <= wave) {
-        const Frag<P> b = sK.rows_plain(16 * ct + m, k0);
-        kk[ct] = mma<3>(a, b, kk[ct]);
-        qk[ct] = mma<3>(aq, b, qk[ct]);
+    for (int jt = 0; jt < 4; ++jt)
+      if (need(jt)) {
+        const Frag<P> ak = jt == wave ? bk : frag(kp, g.ks, 16 * jt + m);
+        kk[jt] = mma<3>(ak, bk, kk[jt]);
+        if (BWD)
+          qk[jt] = mma<3>(jt == wave ? bq : frag(qp, g.qs, 16 * jt + m), bk, qk[jt]);
+        else
+          qk[jt] = mma<3>(ak, bq, qk[jt]);
       }
   }
-#pragma unroll
-  for (int ct = 0; ct < 4; ++ct) {
-    const int j = 16 * ct + m;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int i = 16 * wave + 4 * grp + r;
-      const float e = j <= i ? exp_diff(sG[i] - sG[j]) * sRk[j] : 0.f;
-      sA[i][j] = j < i ? sBeta[i] * sRk[i] * e * kk[ct][r] : 0.f;
-      qk[ct][r] = j <= i ? g.scale * sRq[i] * e * qk[ct][r] : 0.f;
-    }
+  const double G = log_decay(g, in.g, c.t0, n, h, lane);
+  if (wave == 0) {
+    sG[lane] = G;
+    sBeta[lane] = lane < n ? load_beta<T>(g, in.beta, c.t0 + lane, h) : 0.f;
   }
-  __syncthreads();
-  {  // the diagonal block, column m
-    float t[16];
+  // the squared norms lie on the diagonal tiles' diagonals
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float s = i == m ? 1.f : 0.f;
+  for (int r = 0; r < 4; ++r)
+    if (m == 4 * grp + r) {
+      float nk = 0.f;
 #pragma unroll
-      for (int j = 0; j < i; ++j) s = fmaf(-sA[16 * wave + i][16 * wave + j], t[j], s);
-      t[i] = s;
+      for (int jt = 0; jt < 4; ++jt) nk = jt == wave ? kk[jt][r] : nk;
+      sRk[own] = g.l2 ? 1.f / sqrtf(nk + kL2Eps) : 1.f;
+      sRq[own] = g.l2 ? 1.f / sqrtf(qq[r] + kL2Eps) : 1.f;
     }
-    if (grp == 0)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) sT[16 * wave + i][16 * wave + m] = t[i];
-    for (int ct = wave + 1; ct < 4; ++ct)
-      *reinterpret_cast<float4*>(&sT[16 * wave + m][16 * ct + 4 * grp]) = make_float4(0.f, 0.f, 0.f, 0.f);
-  }
   __syncthreads();
-  {  // block column `wave`
-    f32x4 X[4];
+  const int64_t at = static_cast<int64_t>(slot) * g.HV + h;
+  if (wave == 0) {
+    const double Gc = __shfl(G, 63);
+    const float eG = exp_diff(G), eR = exp_diff(Gc - G);
+    reinterpret_cast<float4*>(w.dec)[at * kC + lane] =
+        make_float4(sRk[lane] * eG, sRk[lane] * eR, g.scale * sRq[lane] * eG, sBeta[lane]);
+    if (lane == 0) w.gam[at] = exp_diff(Gc);
+  }
+  const double Gown = sG[own];
+  const float bown = sBeta[own] * sRk[own], kown = sRk[own], qown = g.scale * sRq[own];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (i == wave)
+  for (int jt = 0; jt < 4; ++jt)
+    if (need(jt)) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) X[i][r] = sT[16 * i + 4 * grp + r][16 * i + m];
-      if (i > wave) {
-        f32x4 s = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int k = 0; k < i; ++k)
-          if (k >= wave) s = mma_f32(*reinterpret_cast<const f32x4*>(&sA[16 * i + m][16 * k + 4 * grp]), X[k], s);
-        const f32x4 z = {0.f, 0.f, 0.f, 0.f};
-        X[i] = -mma_f32(*reinterpret_cast<const f32x4*>(&sT[16 * i + m][16 * i + 4 * grp]), s, z);
+      for (int r = 0; r < 4; ++r) {
+        const int j = 16 * jt + 4 * grp + r;
+        // the later token is the column's forward, the row's backward
+        const bool on = BWD ? j >= own : j <= own;
+        const float e = on ? exp_diff(BWD ? sG[j] - Gown : Gown - sG[j]) : 0.f;
+        sA[j][own] = j == own ? 0.f : e * kk[jt][r] * (BWD ? sBeta[j] * sRk[j] * kown : bown * sRk[j]);
+        qk[jt][r] *= e * (BWD ? g.scale * sRq[j] * kown : qown * sRk[j]);
       }
     }
+  // (a wave's own diagonal block: its own writes)
+  float t[16];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i > wave)
+  for (int x = 0; x < 16; ++x) {
+    const int i = BWD ? x : 15 - x;
+    float s = i == m ? 1.f : 0.f;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) sT[16 * i + 4 * grp + r][16 * wave + m] = X[i][r];
+    for (int y = 0; y < 16; ++y)
+      if (BWD ? y < i : y > i) s = fmaf(-sA[16 * wave + i][16 * wave + y], t[y], s);
+    t[i] = s;
   }
+  if (grp == 0)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sD[wave][i][m] = t[i];
   __syncthreads();
+  f32x4 X[4];
 #pragma unroll
-  for (int ct = 0; ct < 4; ++ct)
+  for (int r = 0; r < 4; ++r) {
+    const float v = grp == 0 ? t[r] : grp == 1 ? t[4 + r] : grp == 2 ? t[8 + r] : t[12 + r];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) sA[16 * wave + 4 * grp + r][16 * ct + m] = qk[ct][r];
-  __syncthreads();
-  uint4* out = reinterpret_cast<uint4*>(w.tri) + at * (2 * kTriFrags * kTriParts * 64);
-  for (int f = wave; f < 2 * kTriFrags; f += 4) {
-    const float(*src)[kLda] = f < kTriFrags ? sT : sA;
-    const int i = f % kTriFrags;
-    const int rt = BWD ? (i < 4 ? i >> 1 : i - 2) : (i < 2 ? i : (i + 2) >> 1);
-    const int ks = BWD ? (i < 4 ? i & 1 : 1) : (i < 2 ? 0 : i & 1);
-    const int row = 16 * rt + m, k0 = 32 * ks + 4 * grp;
-    f32x4 a, b;
+    for (int i = 0; i < 4; ++i) X[i][r] = i == wave ? v : 0.f;
+  }
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      a[r] = BWD ? src[k0 + r][row] : src[row][k0 + r];
-      b[r] = BWD ? src[k0 + 16 + r][row] : src[row][k0 + 16 + r];
+  for (int x = 0; x < 4; ++x) {
+    const int i = BWD ? x : 3 - x;
+    if (BWD ? i > wave : i < wave) {
+      f32x4 s = {0.f, 0.f, 0.f, 0.f};
+      const f32x4 z = s;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (BWD ? k < i && k >= wave : k > i && k <= wave)
+          s = mma_f32(*reinterpret_cast<const f32x4*>(&sA[16 * i + m][16 * k + 4 * grp]), X[k], s);
+      X[i] = -mma_f32(*reinterpret_cast<const f32x4*>(&sD[i][m][4 * grp]), s, z);
     }
-    const Frag<kTriParts> fr = split_tiles<kTriParts>(a, b);
-#pragma unroll
-    for (int p = 0; p < kTriParts; ++p) out[(f * kTriParts + p) * 64 + lane] = fr.p[p];
   }
+  uint4* out = reinterpret_cast<uint4*>(w.tri) + at * kTriFragments + lane;
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks)
+    if (BWD ? 2 * ks + 1 >= wave : 2 * ks <= wave) {
+      const int f = BWD ? (wave < 2 ? 2 * wave + ks : wave + 2) : (wave < 2 ? wave : 2 * wave - 2 + ks);
+      const Frag<kTriParts> a = split_tiles<kTriParts>(X[2 * ks], X[2 * ks + 1]),
+                            b = split_tiles<kTriParts>(qk[2 * ks], qk[2 * ks + 1]);
+#pragma unroll
+      for (int p = 0; p < kTriParts; ++p) {
+        out[tri_index(0, p, f)] = a.p[p];
+        out[tri_index(1, p, f)] = b.p[p];
+      }
+    }
 }
 
 }  // namespace
