@@ -34,10 +34,12 @@ struct BwdArgs {
   DeltaIn in;
   DeltaWork w;
   DeltaBwd b;
-  uint32_t ncb, nslots;
+  uint32_t vcb, ncb, nslots;  // column blocks of the values, and of the launch
 };
 
-template <typename T, int DKP>
+// AGG: a part's gradient of its initial state from zero, and (column blocks
+// from a.vcb on) its transition: what the identity becomes where dO is zero.
+template <typename T, int DKP, bool AGG>
 __global__ void __launch_bounds__(256)
 delta_bwd_kernel(BwdArgs a) {
   constexpr int P = kRawParts<T>, KT = DKP / 16, KS = DKP / 32;
@@ -49,24 +51,29 @@ delta_bwd_kernel(BwdArgs a) {
   const DeltaPos p = delta_pos(a.ncb, a.nslots, static_cast<uint32_t>(g.HV));
   if (!p.ok) return;
   const int h = p.h, hk = h / g.group;
-  const int col = p.cb * kDeltaCols + 16 * wave + m;
-  const bool live = col < g.DV;
+  const bool trans = AGG && p.cb >= static_cast<int32_t>(a.vcb);
+  const int col = (trans ? p.cb - static_cast<int32_t>(a.vcb) : p.cb) * kDeltaCols + 16 * wave + m;
+  const bool live = trans ? col < DKP : col < g.DV;
   const SeqChunk part = seq_chunk(g.q, p.slot, g.part, lane);
-  if (part.t0 < 0 || part.seq >= g.q.S) return;
+  if (part.t0 < 0 || part.seq >= g.q.S || (AGG && part.t0 == part.start)) return;  // (nothing precedes a first part)
   const int64_t cells = static_cast<int64_t>(g.DK) * g.DV;
   const int64_t at_h = (static_cast<int64_t>(part.seq) * g.HV + h) * cells + col;
+  const int64_t at_part = (static_cast<int64_t>(p.slot) * g.HV + h) * cells + col;
   f32x4 E[KT];
+  {
+    const float* src = AGG ? nullptr : a.w.carry != nullptr ? a.w.carry + at_part : a.b.dh1 != nullptr ? a.b.dh1 + at_h : nullptr;
 #pragma unroll
-  for (int t = 0; t < KT; ++t)
+    for (int t = 0; t < KT; ++t)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int d = 16 * t + 4 * grp + r;
-      E[t][r] = a.b.dh1 != nullptr && live && d < g.DK ? a.b.dh1[at_h + static_cast<int64_t>(d) * g.DV] : 0.f;
-    }
+      for (int r = 0; r < 4; ++r) {
+        const int d = 16 * t + 4 * grp + r;
+        E[t][r] = trans ? (d == col ? 1.f : 0.f) : src != nullptr && live && d < g.DK ? src[static_cast<int64_t>(d) * g.DV] : 0.f;
+      }
+  }
   const T* kp = static_cast<const T*>(a.in.k) + hk * g.kh;
   const T* qp = static_cast<const T*>(a.in.q) + hk * g.qh;
   const int64_t orow = static_cast<int64_t>(g.HV) * g.DV, ocol = static_cast<int64_t>(h) * g.DV + col;
-  const T* dop = static_cast<const T*>(a.b.d_o) + (live ? ocol : 0);
+  const T* dop = static_cast<const T*>(a.b.d_o) + (live && !trans ? ocol : 0);
   const int32_t slot0 = cut_div(g.cut, part.start) + part.seq + (part.t0 - part.start) / kC;
   const int32_t chunks = (part.t1 - part.t0 + kC - 1) / kC;
   StageRows<T, DKP> rK, rQ;
@@ -86,7 +93,7 @@ delta_bwd_kernel(BwdArgs a) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int t = 16 * (i >> 2) + 4 * grp + (i & 3);
-      rO[i] = dop[live ? (t0 + (t < n ? t : 0)) * orow : 0];
+      rO[i] = dop[live && !trans ? (t0 + (t < n ? t : 0)) * orow : 0];
     }
   };
   if (chunks > 0) load(chunks - 1);
@@ -104,9 +111,9 @@ delta_bwd_kernel(BwdArgs a) {
 #pragma unroll
     for (int rt = 0; rt < 4; ++rt)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) O[rt][r] = live && 16 * rt + 4 * grp + r < n ? to_f32(rO[4 * rt + r]) : 0.f;
+      for (int r = 0; r < 4; ++r) O[rt][r] = live && !trans && 16 * rt + 4 * grp + r < n ? to_f32(rO[4 * rt + r]) : 0.f;
     if (nth > 0) load(nth - 1);
-    {
+    if constexpr (!AGG) {
       float* e = a.b.dend + at * cells + col;
       if (live)
 #pragma unroll
@@ -158,7 +165,7 @@ delta_bwd_kernel(BwdArgs a) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int i = 16 * rt + 4 * grp + r;
-        if (live && i < n) a.b.x[(t0 + i) * orow + ocol] = X[rt][r];
+        if (!AGG && live && i < n) a.b.x[(t0 + i) * orow + ocol] = X[rt][r];
         X[rt][r] *= sx[rt][r];
         O[rt][r] *= so[rt][r];
       }
@@ -174,13 +181,22 @@ delta_bwd_kernel(BwdArgs a) {
       }
     }
   }
-  if (a.b.dh0 != nullptr && live && part.t0 == part.start) {
+  float* dst = nullptr;
+  int64_t ld = g.DV;
+  int rows = g.DK;
+  if (AGG && trans)
+    dst = a.w.trans + (static_cast<int64_t>(p.slot) * g.HV + h) * (DKP * DKP) + col, ld = DKP, rows = DKP;
+  else if (AGG)
+    dst = a.w.carry + at_part;
+  else if (a.b.dh0 != nullptr && part.t0 == part.start)
+    dst = a.b.dh0 + at_h;
+  if (dst != nullptr && live) {
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int d = 16 * t + 4 * grp + r;
-        if (d < g.DK) a.b.dh0[at_h + static_cast<int64_t>(d) * g.DV] = E[t][r];
+        if (d < rows) dst[d * ld] = E[t][r];
       }
   }
 }
@@ -477,16 +493,24 @@ delta_grads_kernel(BwdArgs a) {
 
 hipError_t launch_delta_bwd(const DeltaGeom& g, const DeltaIn& in, const DeltaWork& w, const DeltaBwd& b, int dtype,
                             hipStream_t s) {
-  BwdArgs a{g, in, w, b, static_cast<uint32_t>((g.DV + kDeltaCols - 1) / kDeltaCols),
-            static_cast<uint32_t>(chunk_slots(g.q, g.part))};
-  const dim3 grid(static_cast<unsigned>(delta_blocks(a.ncb, a.nslots, g.HV)));
+  const uint32_t vcb = delta_col_blocks(g.DV);
+  BwdArgs a{g, in, w, b, vcb, vcb, static_cast<uint32_t>(chunk_slots(g.q, g.part))};
   hipError_t e = launch_delta_prep(g, in, w, true, dtype, s);
   if (e != hipSuccess) return e;
   return delta_dispatch(dtype, g.DK, [&](auto t, auto dkp) {
     using T = decltype(t);
     constexpr int DKP = decltype(dkp)::value;
-    hipLaunchKernelGGL((delta_bwd_kernel<T, DKP>), grid, dim3(256), 0, s, a);
-    hipError_t e = hipGetLastError();
+    hipError_t e;
+    if (g.parts > 1) {
+      a.ncb = vcb + delta_col_blocks(DKP);
+      hipLaunchKernelGGL((delta_bwd_kernel<T, DKP, true>),
+                         dim3(static_cast<unsigned>(delta_blocks(a.ncb, a.nslots, g.HV))), dim3(256), 0, s, a);
+      if ((e = hipGetLastError()) != hipSuccess || (e = launch_delta_carry<true>(g, w, b.dh1, s)) != hipSuccess) return e;
+      a.ncb = vcb;
+    }
+    hipLaunchKernelGGL((delta_bwd_kernel<T, DKP, false>),
+                       dim3(static_cast<unsigned>(delta_blocks(a.ncb, a.nslots, g.HV))), dim3(256), 0, s, a);
+    e = hipGetLastError();
     if (e != hipSuccess || g.q.T == 0) return e;
     hipLaunchKernelGGL((delta_grads_kernel<T, DKP>), dim3(static_cast<unsigned>(chunk_slots(g.q, g.cut) * g.HK)),
                        dim3(256), 0, s, a);

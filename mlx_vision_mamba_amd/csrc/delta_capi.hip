@@ -50,8 +50,13 @@ void pick_parts(const mvm_delta_desc* d, mvm::DeltaGeom& g) {
   const int64_t T = d->seq.tokens;
   int64_t longest = d->seq.offsets == nullptr ? d->seq.seqlen : T;
   if (d->max_len > 0) longest = std::min(longest, d->max_len);
-  g.parts = 1;
-  g.part = mvm::seq_cut(std::max<int64_t>(mvm::kDeltaChunk, T + 1));
+  int64_t len = d->split_len;
+  if (len == 0) {
+    len = longest;
+  }
+  // Whole sequences: one part whatever max_len says
+  g.parts = len < longest ? static_cast<int32_t>(ceil_div(longest, len)) : 1;
+  g.part = mvm::seq_cut(g.parts > 1 ? len : std::max<int64_t>(mvm::kDeltaChunk, T + 1));
 }
 
 mvm::DeltaGeom geom(const mvm_delta_desc* d) {

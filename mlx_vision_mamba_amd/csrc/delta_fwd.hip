@@ -3,10 +3,15 @@
 //   D  = T R                                   (rows d_t)
 //   O  = scale diag(e^G) Q S + P D
 //   S' = e^Gc S + K' diag(e^(Gc - G)) D        (Gc: G of the last token)
-// with T and P of delta_prep.hip.  The columns of S are independent: a wave
+// (with T and P of delta_prep.hip).  The columns of S are independent: a wave
 // keeps 16 of them in registers, as result tiles whose rows are the keys'
 // index, for the whole sequence, and the four waves of a workgroup share the
 // chunk's A operands in LDS.
+//
+// Where sequences and heads are too few to fill the card, the sequences are cut
+// into parts (delta_capi.hip decides): one pass leaves every part's end state
+// from zero and its transition M (S' = M S + e), a second one joins them, and
+// the main pass starts each part from its own state.
 #include "delta_common.h"
 
 namespace mvm {
@@ -21,28 +26,34 @@ struct FwdArgs {
   void* o;
   float* s0;
   float* vt;
-  uint32_t ncb, nslots;
+  uint32_t vcb, ncb, nslots;  // column blocks of the values, and of the launch
 };
 
-template <typename T, int DKP, bool SAVE>
+// AGG: a part's end state from zero, and (column blocks from a.vcb on) its
+// transition: what the identity becomes where V is zero.
+template <typename T, int DKP, bool SAVE, bool AGG>
 __global__ void __launch_bounds__(256)
 delta_fwd_kernel(FwdArgs a) {
   constexpr int P = kRawParts<T>, KT = DKP / 16, KS = DKP / 32;
   constexpr int ORD = P == 3 ? 3 : 2;  // of what only the outputs see: bfloat16 keeps 8 bits of them
-  __shared__ __attribute__((aligned(16))) Tile<kC, DKP, P> sK, sQ;
-  __shared__ uint4 sTri[StageTri<ORD>::kCount];
+  constexpr int PP = AGG ? 0 : ORD;
+  __shared__ __attribute__((aligned(16))) Tile<kC, DKP, P> sK;
+  __shared__ __attribute__((aligned(16))) Tile<AGG ? 1 : kC, DKP, P> sQ;
+  __shared__ uint4 sTri[StageTri<PP>::kCount];
   __shared__ float4 sDec[kC];
   const DeltaGeom& g = a.g;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 15, grp = lane >> 4;
   const DeltaPos p = delta_pos(a.ncb, a.nslots, static_cast<uint32_t>(g.HV));
   if (!p.ok) return;
   const int h = p.h, hk = h / g.group;
-  const int col = p.cb * kDeltaCols + 16 * wave + m;
-  const bool live = col < g.DV;
+  const bool trans = AGG && p.cb >= static_cast<int32_t>(a.vcb);
+  const int col = (trans ? p.cb - static_cast<int32_t>(a.vcb) : p.cb) * kDeltaCols + 16 * wave + m;
+  const bool live = trans ? col < DKP : col < g.DV;
   T* o = static_cast<T*>(a.o) + static_cast<int64_t>(h) * g.DV + col;
   const int64_t orow = static_cast<int64_t>(g.HV) * g.DV;
   const SeqChunk part = seq_chunk(g.q, p.slot, g.part, lane);
   if (part.t0 < 0) return;
+  if (AGG && (part.seq >= g.q.S || part.t1 == part.end)) return;  // (nothing follows a last part)
   if (part.seq >= g.q.S) {  // rows of no sequence
     if (live)
       for (int32_t t = part.t0 + 4 * 0 + grp; t < part.t1; t += 4) o[t * orow] = from_f32<T>(0.f);
@@ -50,25 +61,30 @@ delta_fwd_kernel(FwdArgs a) {
   }
   const int32_t row = seq_slot(g.q, part.seq);
   const int64_t cells = static_cast<int64_t>(g.DK) * g.DV, at_h = static_cast<int64_t>(h) * cells + col;
+  const int64_t at_part = (static_cast<int64_t>(p.slot) * g.HV + h) * cells + col;
   f32x4 S[KT];
   {
-    const float* src = a.h0 != nullptr && row >= 0 && !seq_fresh(g.q, part.seq) ? a.h0 + row * (g.HV * cells) + at_h : nullptr;
+    const float* src = nullptr;
+    if (!AGG && a.w.carry != nullptr)
+      src = a.w.carry + at_part;
+    else if (!AGG && a.h0 != nullptr && row >= 0 && !seq_fresh(g.q, part.seq))
+      src = a.h0 + row * (g.HV * cells) + at_h;
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int d = 16 * t + 4 * grp + r;
-        S[t][r] = src != nullptr && live && d < g.DK ? src[static_cast<int64_t>(d) * g.DV] : 0.f;
+        S[t][r] = trans ? (d == col ? 1.f : 0.f) : src != nullptr && live && d < g.DK ? src[static_cast<int64_t>(d) * g.DV] : 0.f;
       }
   }
   const T* kp = static_cast<const T*>(a.in.k) + hk * g.kh;
   const T* qp = static_cast<const T*>(a.in.q) + hk * g.qh;
-  const T* vp = static_cast<const T*>(a.in.v) + h * g.vh + (live ? col : 0);
+  const T* vp = static_cast<const T*>(a.in.v) + h * g.vh + (live && !trans ? col : 0);
   const int32_t slot0 = cut_div(g.cut, part.start) + part.seq + (part.t0 - part.start) / kC;
   const int32_t chunks = (part.t1 - part.t0 + kC - 1) / kC;
   // the next chunk's operands, on their way while this one's are at work
   StageRows<T, DKP> rK, rQ;
-  StageTri<ORD> rT;
+  StageTri<PP> rT;
   float4 rDec;
   float rGam;
   T rV[16];
@@ -77,14 +93,14 @@ delta_fwd_kernel(FwdArgs a) {
     const int n = part.t1 - t0 < kC ? part.t1 - t0 : kC;
     const int64_t at = static_cast<int64_t>(slot0 + i) * g.HV + h;
     rK.load(kp + t0 * g.ks, g.ks, n, g.DK, g.qk_vec, tid);
-    rQ.load(qp + t0 * g.qs, g.qs, n, g.DK, g.qk_vec, tid);
+    if constexpr (!AGG) rQ.load(qp + t0 * g.qs, g.qs, n, g.DK, g.qk_vec, tid);
     rT.load(reinterpret_cast<const uint4*>(a.w.tri) + at * kTriFragments, tid);
     rDec = reinterpret_cast<const float4*>(a.w.dec)[at * kC + lane];
     rGam = a.w.gam[at];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int t = 16 * (i >> 2) + 4 * grp + (i & 3);
-      rV[i] = vp[live ? (t0 + (t < n ? t : 0)) * g.vs : 0];
+      rV[i] = vp[live && !trans ? (t0 + (t < n ? t : 0)) * g.vs : 0];
     }
   };
   if (chunks > 0) load(0);
@@ -94,7 +110,7 @@ delta_fwd_kernel(FwdArgs a) {
     const int64_t at = static_cast<int64_t>(slot0 + nth) * g.HV + h;
     __syncthreads();
     rK.put(sK, n, g.DK, tid);
-    rQ.put(sQ, n, g.DK, tid);
+    if constexpr (!AGG) rQ.put(sQ, n, g.DK, tid);
     rT.put(sTri, tid);
     if (wave == 0) sDec[lane] = rDec;
     const float gam = rGam;
@@ -102,7 +118,7 @@ delta_fwd_kernel(FwdArgs a) {
 #pragma unroll
     for (int rt = 0; rt < 4; ++rt)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) V[rt][r] = live && 16 * rt + 4 * grp + r < n ? to_f32(rV[4 * rt + r]) : 0.f;
+      for (int r = 0; r < 4; ++r) V[rt][r] = live && !trans && 16 * rt + 4 * grp + r < n ? to_f32(rV[4 * rt + r]) : 0.f;
     if (nth + 1 < chunks) load(nth + 1);
     if constexpr (SAVE) {
       float* s0 = a.s0 + at * cells + col;
@@ -126,7 +142,7 @@ delta_fwd_kernel(FwdArgs a) {
 #pragma unroll
       for (int rt = 0; rt < 4; ++rt) {
         R[rt] = mma<3>(sK.rows(16 * rt + m, k0), sf, R[rt]);
-        O[rt] = mma<ORD>(sQ.rows(16 * rt + m, k0), sf, O[rt]);
+        if constexpr (!AGG) O[rt] = mma<ORD>(sQ.rows(16 * rt + m, k0), sf, O[rt]);
       }
     }
     float up[4][4];
@@ -150,7 +166,7 @@ delta_fwd_kernel(FwdArgs a) {
           if (tri_frag<false>(rt, ks) >= 0) D[rt] = mma<3>(tri_at<3>(sTri, 0, tri_frag<false>(rt, ks), lane), rf[ks], D[rt]);
       }
     }
-    {
+    if constexpr (!AGG) {
       const Frag<ORD> df[2] = {split_tiles<ORD>(D[0], D[1]), split_tiles<ORD>(D[2], D[3])};
 #pragma unroll
       for (int rt = 0; rt < 4; ++rt) {
@@ -164,7 +180,7 @@ delta_fwd_kernel(FwdArgs a) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int i = 16 * rt + 4 * grp + r;
-        if (live && i < n) {
+        if (!AGG && live && i < n) {
           o[(t0 + i) * orow] = from_f32<T>(O[rt][r]);
           if constexpr (SAVE) a.vt[(t0 + i) * orow + static_cast<int64_t>(h) * g.DV + col] = D[rt][r];
         }
@@ -178,34 +194,131 @@ delta_fwd_kernel(FwdArgs a) {
       for (int ks = 0; ks < 2; ++ks) S[t] = mma<3>(sK.cols(16 * t, 32 * ks + 4 * grp, m), uf[ks], S[t]);
     }
   }
-  if (a.h1 != nullptr && row >= 0 && live && part.t1 == part.end) {
-    float* dst = a.h1 + row * (g.HV * cells) + at_h;
+  float* dst = nullptr;
+  int64_t ld = g.DV;
+  int rows = g.DK;
+  if (AGG && trans)
+    dst = a.w.trans + (static_cast<int64_t>(p.slot) * g.HV + h) * (DKP * DKP) + col, ld = DKP, rows = DKP;
+  else if (AGG)
+    dst = a.w.carry + at_part;
+  else if (a.h1 != nullptr && row >= 0 && part.t1 == part.end)
+    dst = a.h1 + row * (g.HV * cells) + at_h;
+  if (dst != nullptr && live) {
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int d = 16 * t + 4 * grp + r;
-        if (d < g.DK) dst[static_cast<int64_t>(d) * g.DV] = S[t][r];
+        if (d < rows) dst[d * ld] = S[t][r];
       }
+  }
+}
+
+// Joins the parts of a sequence: carry holds each part's end state from zero (REV: the gradient of its initial
+// state) and gets its initial state (of its final one), S' = M S + e with the parts' transitions M.
+template <int DKP, bool REV>
+__global__ void __launch_bounds__(256)
+delta_carry_kernel(DeltaGeom g, DeltaWork w, const float* __restrict__ enter, uint32_t ncb) {
+  constexpr int KT = DKP / 16, KS = DKP / 32;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, grp = lane >> 4;
+  const uint32_t item = blockIdx.x / ncb;
+  const int32_t seq = static_cast<int32_t>(item / static_cast<uint32_t>(g.HV));
+  const int h = static_cast<int>(item - static_cast<uint32_t>(seq) * g.HV);
+  const int col = static_cast<int>(blockIdx.x - item * ncb) * kDeltaCols + 16 * wave + m;
+  const bool live = col < g.DV;
+  const int32_t start = seq_off_u(g.q, seq), next = seq_off_u(g.q, seq + 1), end = next < start ? start : next;
+  const int32_t slot0 = cut_div(g.part, start) + seq, parts = end > start ? cut_div(g.part, end - start - 1) + 1 : 1;
+  const int32_t row = REV ? seq : seq_slot(g.q, seq);
+  const int64_t cells = static_cast<int64_t>(g.DK) * g.DV, step = g.HV * cells;
+  f32x4 S[KT];
+  {
+    const bool any = enter != nullptr && row >= 0 && (REV || !seq_fresh(g.q, seq));
+    const float* src = enter + (any ? row * step + h * cells : 0) + (live ? col : 0);
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int d = 16 * t + 4 * grp + r;
+        S[t][r] = any && live && d < g.DK ? src[static_cast<int64_t>(d) * g.DV] : 0.f;
+      }
+  }
+  for (int32_t i = 0; i < parts; ++i) {
+    const int64_t at = static_cast<int64_t>(slot0 + (REV ? parts - 1 - i : i)) * g.HV + h;
+    float* c = w.carry + at * cells + (live ? col : 0);
+    const bool last = i + 1 == parts;
+    f32x4 E[KT];
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int d = 16 * t + 4 * grp + r;
+        E[t][r] = !last && live && d < g.DK ? c[static_cast<int64_t>(d) * g.DV] : 0.f;
+      }
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int d = 16 * t + 4 * grp + r;
+        if (live && d < g.DK) c[static_cast<int64_t>(d) * g.DV] = S[t][r];
+      }
+    if (last) break;
+    const float* M = w.trans + at * (DKP * DKP);
+    Frag<3> sf[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) sf[ks] = split_tiles<3>(S[2 * ks], S[2 * ks + 1]);
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const float* at_m = M + (16 * t + m) * DKP + 32 * ks + 4 * grp;
+        E[t] = mma<3>(split_tiles<3>(*reinterpret_cast<const f32x4*>(at_m), *reinterpret_cast<const f32x4*>(at_m + 16)),
+                      sf[ks], E[t]);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < KT; ++t) S[t] = E[t];
   }
 }
 
 }  // namespace
 
+template <bool REV>
+hipError_t launch_delta_carry(const DeltaGeom& g, const DeltaWork& w, const float* enter, hipStream_t s) {
+  if (g.q.S == 0) return hipSuccess;
+  const uint32_t ncb = delta_col_blocks(g.DV);
+  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(g.q.S) * g.HV * ncb));
+  switch (delta_dkp(g.DK)) {
+    case 32: hipLaunchKernelGGL((delta_carry_kernel<32, REV>), grid, dim3(256), 0, s, g, w, enter, ncb); break;
+    case 64: hipLaunchKernelGGL((delta_carry_kernel<64, REV>), grid, dim3(256), 0, s, g, w, enter, ncb); break;
+    default: hipLaunchKernelGGL((delta_carry_kernel<128, REV>), grid, dim3(256), 0, s, g, w, enter, ncb); break;
+  }
+  return hipGetLastError();
+}
+template hipError_t launch_delta_carry<false>(const DeltaGeom&, const DeltaWork&, const float*, hipStream_t);
+template hipError_t launch_delta_carry<true>(const DeltaGeom&, const DeltaWork&, const float*, hipStream_t);
+
 hipError_t launch_delta_fwd(const DeltaGeom& g, const DeltaIn& in, const DeltaWork& w, const float* h0, float* h1,
                             void* o, float* s0, float* vt, int dtype, hipStream_t s) {
-  FwdArgs a{g, in, w, h0, h1, o, s0, vt, static_cast<uint32_t>((g.DV + kDeltaCols - 1) / kDeltaCols),
-            static_cast<uint32_t>(chunk_slots(g.q, g.part))};
-  const dim3 grid(static_cast<unsigned>(delta_blocks(a.ncb, a.nslots, g.HV)));
+  const uint32_t vcb = delta_col_blocks(g.DV);
+  FwdArgs a{g, in, w, h0, h1, o, s0, vt, vcb, vcb, static_cast<uint32_t>(chunk_slots(g.q, g.part))};
   hipError_t e = launch_delta_prep(g, in, w, false, dtype, s);
   if (e != hipSuccess) return e;
   return delta_dispatch(dtype, g.DK, [&](auto t, auto dkp) {
     using T = decltype(t);
     constexpr int DKP = decltype(dkp)::value;
+    if (g.parts > 1) {
+      a.ncb = vcb + delta_col_blocks(DKP);
+      hipLaunchKernelGGL((delta_fwd_kernel<T, DKP, false, true>),
+                         dim3(static_cast<unsigned>(delta_blocks(a.ncb, a.nslots, g.HV))), dim3(256), 0, s, a);
+      hipError_t e = hipGetLastError();
+      if (e != hipSuccess || (e = launch_delta_carry<false>(g, w, h0, s)) != hipSuccess) return e;
+      a.ncb = vcb;
+    }
+    const dim3 grid(static_cast<unsigned>(delta_blocks(a.ncb, a.nslots, g.HV)));
     if (s0 != nullptr)
-      hipLaunchKernelGGL((delta_fwd_kernel<T, DKP, true>), grid, dim3(256), 0, s, a);
+      hipLaunchKernelGGL((delta_fwd_kernel<T, DKP, true, false>), grid, dim3(256), 0, s, a);
     else
-      hipLaunchKernelGGL((delta_fwd_kernel<T, DKP, false>), grid, dim3(256), 0, s, a);
+      hipLaunchKernelGGL((delta_fwd_kernel<T, DKP, false, false>), grid, dim3(256), 0, s, a);
     return hipGetLastError();
   });
 }

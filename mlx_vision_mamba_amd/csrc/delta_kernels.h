@@ -70,6 +70,11 @@ constexpr int tri_index(int which, int p, int f) { return ((which * kTriParts + 
 
 inline int delta_dkp(int dk) { return dk <= 32 ? 32 : (dk <= 64 ? 64 : 128); }
 
+inline uint32_t delta_col_blocks(int cols) { return static_cast<uint32_t>((cols + kDeltaCols - 1) / kDeltaCols); }
+
+// joins the parts, from the initial states (REV: from the gradients of the final ones)
+template <bool REV>
+hipError_t launch_delta_carry(const DeltaGeom& g, const DeltaWork& w, const float* enter, hipStream_t s);
 hipError_t launch_delta_prep(const DeltaGeom& g, const DeltaIn& in, const DeltaWork& w, bool backward, int dtype,
                              hipStream_t s);
 hipError_t launch_delta_fwd(const DeltaGeom& g, const DeltaIn& in, const DeltaWork& w, const float* h0, float* h1,

@@ -82,6 +82,34 @@ def test_packed_shared_keys(cuda, dtype, HK, HV):
     _compare(*_run(cuda, [66, 9], *ins))
 
 
+@pytest.mark.parametrize("split", [64, 128, 192, 6400])
+@pytest.mark.parametrize("DK,DV", [(32, 32), (60, 70), (128, 128)])
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_packed_splits(cuda, dtype, DK, DV, split):
+    """Every split of the time axis gives the same function; the lengths end inside chunks and parts."""
+    lens = [300, 0, 64, 129, 1]
+    ins = _inputs(lens, 1, 2, DK, DV, TYPES[dtype], 30, extra=200)
+    _compare(*_run(cuda, lens, *ins, split_len=split))
+    _compare(*_run(cuda, lens, *ins, split_len=split, use_init=False, max_len=70))
+
+
+def test_prefill_in_parts(cuda):
+    """A cache that is read and written by sequences in several parts."""
+    lens = [200, 70, 0, 130]
+    a, init, do, df = _inputs(lens, 2, 2, 32, 32, torch.bfloat16, 31)
+    states = init.to(cuda)
+    slots, fresh = [2, -1, 0, 3], [False, False, False, True]
+    o = mvm.gated_delta_rule_prefill(*_on(cuda, a), states, _off(lens), slots=slots, qk_l2norm=True, split_len=64,
+                                     fresh=torch.tensor(fresh, device=cuda))
+    start = torch.stack([torch.zeros_like(init[0]) if s < 0 or f else init[s] for s, f in zip(slots, fresh)])
+    want, factor = ref.reference(_off(lens), **a, qk_l2norm=True, initial=start)
+    ref.check("o", o, want["o"], factor)
+    for i, s in enumerate(slots):
+        if s >= 0:
+            ref.check("final", states[s], tuple(x[i] for x in want["final"]), factor)
+    assert torch.equal(states[1].cpu(), init[1])
+
+
 @pytest.mark.parametrize("options", [dict(l2=False), dict(use_init=False), dict(scale=0.7), dict(max_len=3), dict(max_len=10 ** 6)])
 def test_packed_options(cuda, options):
     ins = _inputs([40, 90], 2, 2, 32, 48, torch.float32, 4, l2=options.get("l2", True))
