@@ -39,64 +39,64 @@ struct BwdArgs {
 
 // AGG: a part's gradient of its initial state from zero, and (column blocks
 // from a.vcb on) its transition: what the identity becomes where dO is zero.
-template <typename T, int DKP, bool AGG>
-__global__ void __launch_bounds__(256)
+template <typename T, int DKP, int NW, bool VEC, bool AGG>
+__global__ void __launch_bounds__(64 * NW)
 delta_bwd_kernel(BwdArgs a) {
-  constexpr int P = kRawParts<T>, KT = DKP / 16, KS = DKP / 32;
+  constexpr int P = kRawParts<T>, KT = DKP / 16, KS = DKP / 32, NT = 64 * NW;
   __shared__ __attribute__((aligned(16))) Tile<kC, DKP, P> sK, sQ;
-  __shared__ uint4 sTri[StageTri<3>::kCount];
-  __shared__ float4 sDec[kC];
+  __shared__ uint4 sTri[StageTri<3, NT>::kCount];
+  __shared__ __attribute__((aligned(16))) float sDec[4][kC];
   const DeltaGeom& g = a.g;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 15, grp = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), m = lane & 15, grp = lane >> 4;
   const DeltaPos p = delta_pos(a.ncb, a.nslots, static_cast<uint32_t>(g.HV));
   if (!p.ok) return;
   const int h = p.h, hk = h / g.group;
   const bool trans = AGG && p.cb >= static_cast<int32_t>(a.vcb);
-  const int col = (trans ? p.cb - static_cast<int32_t>(a.vcb) : p.cb) * kDeltaCols + 16 * wave + m;
+  const int col0 = ((trans ? p.cb - static_cast<int32_t>(a.vcb) : p.cb) * NW + wave) * 16, col = col0 + m;
   const bool live = trans ? col < DKP : col < g.DV;
+  const int at_col = col0 < g.DV ? col0 : 0;  // (waves without columns address the first)
   const SeqChunk part = seq_chunk(g.q, p.slot, g.part, lane);
   if (part.t0 < 0 || part.seq >= g.q.S || (AGG && part.t0 == part.start)) return;  // (nothing precedes a first part)
   const int64_t cells = static_cast<int64_t>(g.DK) * g.DV;
-  const int64_t at_h = (static_cast<int64_t>(part.seq) * g.HV + h) * cells + col;
-  const int64_t at_part = (static_cast<int64_t>(p.slot) * g.HV + h) * cells + col;
+  const int64_t at_h = (static_cast<int64_t>(part.seq) * g.HV + h) * cells + at_col;
+  const int64_t at_part = (static_cast<int64_t>(p.slot) * g.HV + h) * cells + at_col;
   f32x4 E[KT];
-  {
-    const float* src = AGG ? nullptr : a.w.carry != nullptr ? a.w.carry + at_part : a.b.dh1 != nullptr ? a.b.dh1 + at_h : nullptr;
+  if (trans) {
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int d = 16 * t + 4 * grp + r;
-        E[t][r] = trans ? (d == col ? 1.f : 0.f) : src != nullptr && live && d < g.DK ? src[static_cast<int64_t>(d) * g.DV] : 0.f;
-      }
+      for (int r = 0; r < 4; ++r) E[t][r] = 16 * t + 4 * grp + r == col ? 1.f : 0.f;
+  } else {
+    const float* src = AGG ? nullptr : a.w.carry != nullptr ? a.w.carry + at_part : a.b.dh1 != nullptr ? a.b.dh1 + at_h : nullptr;
+    load_state<KT>(E, src, g.DV, src != nullptr ? g.DK : 0, m, grp, live);
   }
   const T* kp = static_cast<const T*>(a.in.k) + hk * g.kh;
   const T* qp = static_cast<const T*>(a.in.q) + hk * g.qh;
-  const int64_t orow = static_cast<int64_t>(g.HV) * g.DV, ocol = static_cast<int64_t>(h) * g.DV + col;
-  const T* dop = static_cast<const T*>(a.b.d_o) + (live && !trans ? ocol : 0);
+  const int64_t orow = static_cast<int64_t>(g.HV) * g.DV, ocol = static_cast<int64_t>(h) * g.DV + at_col;
+  const T* dop = static_cast<const T*>(a.b.d_o) + ocol;
+  const bool vlive = live && !trans;
   const int32_t slot0 = cut_div(g.cut, part.start) + part.seq + (part.t0 - part.start) / kC;
   const int32_t chunks = (part.t1 - part.t0 + kC - 1) / kC;
-  StageRows<T, DKP> rK, rQ;
-  StageTri<3> rT;
-  float4 rDec;
+  StageRows<T, DKP, NT> rK, rQ;
+  StageTri<3, NT> rT;
+  float rDec;
   float rGam;
-  T rO[16];
+  Cols<T> rO;
   const auto load = [&](int32_t i) {
     const int32_t t0 = part.t0 + i * kC;
     const int n = part.t1 - t0 < kC ? part.t1 - t0 : kC;
     const int64_t at = static_cast<int64_t>(slot0 + i) * g.HV + h;
-    rK.load(kp + t0 * g.ks, g.ks, n, g.DK, g.qk_vec, tid);
-    rQ.load(qp + t0 * g.qs, g.qs, n, g.DK, g.qk_vec, tid);
+    rK.template load<VEC>(kp + t0 * g.ks, g.ks, n, g.DK, tid);
+    rQ.template load<VEC>(qp + t0 * g.qs, g.qs, n, g.DK, tid);
     rT.load(reinterpret_cast<const uint4*>(a.w.tri) + at * kTriFragments, tid);
-    rDec = reinterpret_cast<const float4*>(a.w.dec)[at * kC + lane];
+    if (tid < 4 * kC) rDec = a.w.dec[at * (4 * kC) + tid];
     rGam = a.w.gam[at];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int t = 16 * (i >> 2) + 4 * grp + (i & 3);
-      rO[i] = dop[live && !trans ? (t0 + (t < n ? t : 0)) * orow : 0];
-    }
   };
-  if (chunks > 0) load(chunks - 1);
+  const auto load_o = [&](int32_t i) {
+    const int32_t t0 = part.t0 + i * kC;
+    rO.load(dop + t0 * orow, orow, m, grp, part.t1 - t0 < kC ? part.t1 - t0 : kC, vlive);
+  };
+  if (chunks > 0) load(chunks - 1), load_o(chunks - 1);
   for (int32_t nth = chunks - 1; nth >= 0; --nth) {
     const int32_t t0 = part.t0 + nth * kC;
     const int n = part.t1 - t0 < kC ? part.t1 - t0 : kC;
@@ -105,100 +105,109 @@ delta_bwd_kernel(BwdArgs a) {
     rK.put(sK, n, g.DK, tid);
     rQ.put(sQ, n, g.DK, tid);
     rT.put(sTri, tid);
-    if (wave == 0) sDec[lane] = rDec;
+    if (tid < 4 * kC) sDec[0][tid] = rDec;
     const float gam = rGam;
-    f32x4 O[4];
-#pragma unroll
-    for (int rt = 0; rt < 4; ++rt)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) O[rt][r] = live && !trans && 16 * rt + 4 * grp + r < n ? to_f32(rO[4 * rt + r]) : 0.f;
     if (nth > 0) load(nth - 1);
-    if constexpr (!AGG) {
-      float* e = a.b.dend + at * cells + col;
-      if (live)
-#pragma unroll
-        for (int t = 0; t < KT; ++t)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int d = 16 * t + 4 * grp + r;
-            if (d < g.DK) e[static_cast<int64_t>(d) * g.DV] = E[t][r];
-          }
-    }
+    if constexpr (!AGG) store_state<KT>(a.b.dend + at * cells + at_col, g.DV, g.DK, E, m, grp, live);
     __syncthreads();
-    f32x4 D[4], X[4];
+    f32x4 D[4], X[4], O[4];
 #pragma unroll
     for (int rt = 0; rt < 4; ++rt) D[rt] = X[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    Frag<P> fk[2][4];
+    const auto rows = [&](int ks) {
+#pragma unroll
+      for (int rt = 0; rt < 4; ++rt) fk[ks & 1][rt] = sK.rows(16 * rt + m, 32 * ks + 4 * grp);
+    };
+    Frag<3> ft[2][2];
+    const auto tri = [&](int which, int rt) {
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+        if (tri_frag<true>(rt, ks) >= 0) ft[rt & 1][ks] = tri_at<3>(sTri, which, tri_frag<true>(rt, ks), lane);
+    };
+    f32x4 up[4];
+    rows(0);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
+      if (ks + 1 < KS)
+        rows(ks + 1);
+      else
+#pragma unroll
+        for (int rt = 0; rt < 4; ++rt) up[rt] = dec_at(sDec, kDecUp, rt, grp);
       const Frag<3> ef = split_tiles<3>(E[2 * ks], E[2 * ks + 1]);
 #pragma unroll
-      for (int rt = 0; rt < 4; ++rt) D[rt] = mma<3>(sK.rows(16 * rt + m, 32 * ks + 4 * grp), ef, D[rt]);
+      for (int rt = 0; rt < 4; ++rt) D[rt] = mma<3>(fk[ks & 1][rt], ef, D[rt]);
+      phase();
     }
-    float sx[4][4], so[4][4];
+    tri(1, 0);
+    tri(1, 1);
 #pragma unroll
-    for (int rt = 0; rt < 4; ++rt)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float4 d = sDec[16 * rt + 4 * grp + r];
-        D[rt][r] *= d.y;
-        sx[rt][r] = -d.w * d.x;
-        so[rt][r] = d.z;
-      }
+    for (int rt = 0; rt < 4; ++rt) {
+      O[rt] = rO.tile(rt, grp, n, vlive);
+      D[rt] *= up[rt];
+    }
+    if (nth > 0) load_o(nth - 1);
     {
       const Frag<P> of[2] = {split_tiles<P>(O[0], O[1]), split_tiles<P>(O[2], O[3])};
+      phase();
 #pragma unroll
-      for (int rt = 0; rt < 4; ++rt)
+      for (int rt = 0; rt < 4; ++rt) {
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
-          if (tri_frag<true>(rt, ks) >= 0) D[rt] = mma<3>(tri_at<3>(sTri, 1, tri_frag<true>(rt, ks), lane), of[ks], D[rt]);
+          if (tri_frag<true>(rt, ks) >= 0) D[rt] = mma<3>(ft[rt & 1][ks], of[ks], D[rt]);
+        phase();
+        tri(rt < 2 ? 1 : 0, rt < 2 ? rt + 2 : rt - 2);
+      }
     }
+    f32x4 dx[4], dout[4];
     {
       const Frag<3> df[2] = {split_tiles<3>(D[0], D[1]), split_tiles<3>(D[2], D[3])};
 #pragma unroll
-      for (int rt = 0; rt < 4; ++rt)
+      for (int rt = 0; rt < 4; ++rt) {
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
-          if (tri_frag<true>(rt, ks) >= 0) X[rt] = mma<3>(tri_at<3>(sTri, 0, tri_frag<true>(rt, ks), lane), df[ks], X[rt]);
-    }
-#pragma unroll
-    for (int rt = 0; rt < 4; ++rt)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = 16 * rt + 4 * grp + r;
-        if (!AGG && live && i < n) a.b.x[(t0 + i) * orow + ocol] = X[rt][r];
-        X[rt][r] *= sx[rt][r];
-        O[rt][r] *= so[rt][r];
+          if (tri_frag<true>(rt, ks) >= 0) X[rt] = mma<3>(ft[rt & 1][ks], df[ks], X[rt]);
+        phase();
+        if (rt < 2) tri(0, rt + 2);
+        dx[rt] = dec_at(sDec, kDecBetaKey, rt, grp);
+        dout[rt] = dec_at(sDec, kDecOut, rt, grp);
       }
+    }
+    if constexpr (!AGG) store_cols<float>(a.b.x + t0 * orow + ocol, orow, X, m, grp, n, live);
+    Frag<P> fc[2][2], fd[2][2];
+    const auto keys = [&](int t) {
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        fc[t & 1][ks] = sK.cols(16 * t, 32 * ks + 4 * grp, m);
+        fd[t & 1][ks] = sQ.cols(16 * t, 32 * ks + 4 * grp, m);
+      }
+    };
+    keys(0);
+#pragma unroll
+    for (int rt = 0; rt < 4; ++rt) {
+      X[rt] *= -dx[rt];
+      O[rt] *= dout[rt];
+    }
     const Frag<3> xf[2] = {split_tiles<3>(X[0], X[1]), split_tiles<3>(X[2], X[3])};
     const Frag<3> of[2] = {split_tiles<3>(O[0], O[1]), split_tiles<3>(O[2], O[3])};
+    phase();
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
+      if (t + 1 < KT) keys(t + 1);
       E[t] *= gam;
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
-        E[t] = mma<3>(sK.cols(16 * t, 32 * ks + 4 * grp, m), xf[ks], E[t]);
-        E[t] = mma<3>(sQ.cols(16 * t, 32 * ks + 4 * grp, m), of[ks], E[t]);
+        E[t] = mma<3>(fc[t & 1][ks], xf[ks], E[t]);
+        E[t] = mma<3>(fd[t & 1][ks], of[ks], E[t]);
       }
+      phase();
     }
   }
-  float* dst = nullptr;
-  int64_t ld = g.DV;
-  int rows = g.DK;
   if (AGG && trans)
-    dst = a.w.trans + (static_cast<int64_t>(p.slot) * g.HV + h) * (DKP * DKP) + col, ld = DKP, rows = DKP;
+    store_state<KT>(a.w.trans + (static_cast<int64_t>(p.slot) * g.HV + h) * (DKP * DKP) + col0, DKP, DKP, E, m, grp, live);
   else if (AGG)
-    dst = a.w.carry + at_part;
+    store_state<KT>(a.w.carry + at_part, g.DV, g.DK, E, m, grp, live);
   else if (a.b.dh0 != nullptr && part.t0 == part.start)
-    dst = a.b.dh0 + at_h;
-  if (dst != nullptr && live) {
-#pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int d = 16 * t + 4 * grp + r;
-        if (d < rows) dst[d * ld] = E[t][r];
-      }
-  }
+    store_state<KT>(a.b.dh0 + at_h, g.DV, g.DK, E, m, grp, live);
 }
 
 // Zeros in the gradients of the rows that belong to no sequence.
@@ -224,7 +233,7 @@ __device__ void zero_rows(const BwdArgs& a, int32_t t0, int32_t t1, int hk, int 
   }
 }
 
-template <typename T, int DKP>
+template <typename T, int DKP, bool VEC>
 __global__ void __launch_bounds__(256)
 delta_grads_kernel(BwdArgs a) {
   constexpr int P = kRawParts<T>, KT = DKP / 16;
@@ -341,9 +350,9 @@ delta_grads_kernel(BwdArgs a) {
     for (int o = 32; o > 0; o >>= 1) se += __shfl_xor(se, o);
     __syncthreads();
     {
-      StageRows<T, DKP> rK, rQ;
-      rK.load(static_cast<const T*>(a.in.k) + c.t0 * g.ks + hk * g.kh, g.ks, n, g.DK, g.qk_vec, tid);
-      rQ.load(static_cast<const T*>(a.in.q) + c.t0 * g.qs + hk * g.qh, g.qs, n, g.DK, g.qk_vec, tid);
+      StageRows<T, DKP, 256> rK, rQ;
+      rK.template load<VEC>(static_cast<const T*>(a.in.k) + c.t0 * g.ks + hk * g.kh, g.ks, n, g.DK, tid);
+      rQ.template load<VEC>(static_cast<const T*>(a.in.q) + c.t0 * g.qs + hk * g.qh, g.qs, n, g.DK, tid);
       rK.put(sm.k.K, n, g.DK, tid);
       rQ.put(sm.k.Q, n, g.DK, tid);
     }
@@ -493,28 +502,36 @@ delta_grads_kernel(BwdArgs a) {
 
 hipError_t launch_delta_bwd(const DeltaGeom& g, const DeltaIn& in, const DeltaWork& w, const DeltaBwd& b, int dtype,
                             hipStream_t s) {
-  const uint32_t vcb = delta_col_blocks(g.DV);
+  // (rows that are read value by value: more registers, so four waves)
+  const int nw = g.qk_vec ? delta_waves(g.DV) : 4;
+  const uint32_t vcb = delta_col_blocks(g.DV, nw);
   BwdArgs a{g, in, w, b, vcb, vcb, static_cast<uint32_t>(chunk_slots(g.q, g.part))};
   hipError_t e = launch_delta_prep(g, in, w, true, dtype, s);
   if (e != hipSuccess) return e;
-  return delta_dispatch(dtype, g.DK, [&](auto t, auto dkp) {
+  const auto run = [&](auto t, auto dkp, auto waves, auto vec) {
     using T = decltype(t);
-    constexpr int DKP = decltype(dkp)::value;
+    constexpr int DKP = decltype(dkp)::value, NW = decltype(waves)::value;
+    constexpr bool VEC = decltype(vec)::value;
     hipError_t e;
     if (g.parts > 1) {
-      a.ncb = vcb + delta_col_blocks(DKP);
-      hipLaunchKernelGGL((delta_bwd_kernel<T, DKP, true>),
-                         dim3(static_cast<unsigned>(delta_blocks(a.ncb, a.nslots, g.HV))), dim3(256), 0, s, a);
+      a.ncb = vcb + delta_col_blocks(DKP, NW);
+      hipLaunchKernelGGL((delta_bwd_kernel<T, DKP, NW, VEC, true>),
+                         dim3(static_cast<unsigned>(delta_blocks(a.ncb, a.nslots, g.HV))), dim3(64 * NW), 0, s, a);
       if ((e = hipGetLastError()) != hipSuccess || (e = launch_delta_carry<true>(g, w, b.dh1, s)) != hipSuccess) return e;
       a.ncb = vcb;
     }
-    hipLaunchKernelGGL((delta_bwd_kernel<T, DKP, false>),
-                       dim3(static_cast<unsigned>(delta_blocks(a.ncb, a.nslots, g.HV))), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((delta_bwd_kernel<T, DKP, NW, VEC, false>),
+                       dim3(static_cast<unsigned>(delta_blocks(a.ncb, a.nslots, g.HV))), dim3(64 * NW), 0, s, a);
     e = hipGetLastError();
     if (e != hipSuccess || g.q.T == 0) return e;
-    hipLaunchKernelGGL((delta_grads_kernel<T, DKP>), dim3(static_cast<unsigned>(chunk_slots(g.q, g.cut) * g.HK)),
+    hipLaunchKernelGGL((delta_grads_kernel<T, DKP, VEC>), dim3(static_cast<unsigned>(chunk_slots(g.q, g.cut) * g.HK)),
                        dim3(256), 0, s, a);
     return hipGetLastError();
+  };
+  return delta_dispatch(dtype, g.DK, [&](auto t, auto dkp) {
+    using Four = std::integral_constant<int, 4>;
+    if (!g.qk_vec) return run(t, dkp, Four{}, std::false_type{});
+    return nw == 8 ? run(t, dkp, std::integral_constant<int, 8>{}, std::true_type{}) : run(t, dkp, Four{}, std::true_type{});
   });
 }
 

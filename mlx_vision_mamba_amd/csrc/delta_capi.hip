@@ -126,6 +126,9 @@ int check_delta(const mvm_delta_desc* d) {
       (rc = check_stride("v_stride", d->v_stride)) || (rc = check_stride("v_stride_head", d->v_stride_head)) ||
       (rc = check_stride("g_stride", d->g_stride)) || (rc = check_stride("beta_stride", d->beta_stride)))
     return rc;
+  if (d->v_stride > mvm::kDeltaMaxStride || d->value_heads * d->dv > mvm::kDeltaMaxStride)
+    return fail(MVM_ERR_UNSUPPORTED, "v_stride=%lld and value_heads * dv: at most %lld", (long long)d->v_stride,
+                (long long)mvm::kDeltaMaxStride);
   // the largest launch: a chunk of every part, head and block of 16 columns
   const int64_t slots = d->seq.tokens / mvm::kDeltaChunk + d->seq.nseq + 1;
   if (slots > kMaxBlocks / (d->value_heads + 8) / ceil_div(std::max(d->dk, d->dv), 16))

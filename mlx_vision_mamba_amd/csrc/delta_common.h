@@ -91,21 +91,25 @@ __device__ __forceinline__ f32x4 mma(const Frag<PA>& a, const Frag<PB>& b, f32x4
   return c;
 }
 
-// A tile of ROWS rows of LD values (LD a multiple of 8, not of 64: rows start in different banks) in
-// LDS, one plane for each part
+// A tile of ROWS rows of COLS values in LDS, one plane for each part.  Rows lie 16 values past a multiple of 64
+// banks apart or an odd multiple of 16 values, and in every other eight of them the 16-byte words of a pair trade
+// places: then neither 16 lanes' rows, nor the 8 rows by 16 columns of a transposing read, share a bank.
 template <int ROWS, int COLS, int P>
 struct Tile {
-  static constexpr int LD = COLS + 8;
+  static constexpr int LD = COLS + 16;
   static constexpr int kPlane = ROWS * LD;
   uint16_t v[P * kPlane];
+
+  __device__ __forceinline__ static int at(int row, int col) { return row * LD + (col ^ (row & 8)); }
 
   // row `row`, summed index k0 .. k0 + 31 in the chained order (k0 includes 4g)
   __device__ __forceinline__ Frag<P> rows(int row, int k0) const {
     Frag<P> f;
+    const uint16_t* at0 = v + at(row, k0);
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-      const uint2 a = *reinterpret_cast<const uint2*>(v + p * kPlane + row * LD + k0);
-      const uint2 b = *reinterpret_cast<const uint2*>(v + p * kPlane + row * LD + k0 + 16);
+      const uint2 a = *reinterpret_cast<const uint2*>(at0 + p * kPlane);
+      const uint2 b = *reinterpret_cast<const uint2*>(at0 + p * kPlane + 16);
       f.p[p] = make_uint4(a.x, a.y, b.x, b.y);
     }
     return f;
@@ -114,7 +118,7 @@ struct Tile {
   __device__ __forceinline__ Frag<P> rows_plain(int row, int k0) const {
     Frag<P> f;
 #pragma unroll
-    for (int p = 0; p < P; ++p) f.p[p] = *reinterpret_cast<const uint4*>(v + p * kPlane + row * LD + k0);
+    for (int p = 0; p < P; ++p) f.p[p] = *reinterpret_cast<const uint4*>(v + p * kPlane + at(row, k0));
     return f;
   }
   // column c0 + m of the tile, summed index rows r0 .. r0 + 31 in the chained order (r0 includes 4g).  The
@@ -122,25 +126,26 @@ struct Tile {
   // i / 4, i / 4 + 4, + 8, + 12.
   __device__ __forceinline__ Frag<P> cols(int c0, int r0, int m) const {
     Frag<P> f;
+    const uint16_t* at0 = v + at(r0 + (m >> 2), c0 + 4 * (m & 3));
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-      const uint16_t* at = v + p * kPlane + (r0 + (m >> 2)) * LD + c0 + 4 * (m & 3);
-      const uint2 a = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at));
-      const uint2 b = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 16 * LD)));
+      const uint16_t* x = at0 + p * kPlane;
+      const uint2 a = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)x));
+      const uint2 b = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(x + 16 * LD)));
       f.p[p] = make_uint4(a.x, a.y, b.x, b.y);
     }
     return f;
   }
   __device__ __forceinline__ void put(int row, int col, const Frag<P>& f) {
 #pragma unroll
-    for (int p = 0; p < P; ++p) *reinterpret_cast<uint4*>(v + p * kPlane + row * LD + col) = f.p[p];
+    for (int p = 0; p < P; ++p) *reinterpret_cast<uint4*>(v + p * kPlane + at(row, col)) = f.p[p];
   }
   // values col .. col + 3 of a row (col a multiple of 4)
   __device__ __forceinline__ f32x4 get4(int row, int col) const {
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int p = P - 1; p >= 0; --p) {
-      const uint2 a = *reinterpret_cast<const uint2*>(v + p * kPlane + row * LD + col);
+      const uint2 a = *reinterpret_cast<const uint2*>(v + p * kPlane + at(row, col));
       s[0] += __uint_as_float(a.x << 16);
       s[1] += __uint_as_float(a.x & 0xffff0000u);
       s[2] += __uint_as_float(a.y << 16);
@@ -222,16 +227,18 @@ struct Raw8 {
 };
 // The 64 rows of a chunk's q or k, dk values each, on their way from global memory (load) into LDS (put), all
 // loads in flight together; rows from n on and columns from dk on are zero.
-template <typename T, int DKP>
+template <typename T, int DKP, int NT>
 struct StageRows {
-  static constexpr int kPer = DKP / 8, kItems = kC * kPer / 256;
+  static constexpr int kPer = DKP / 8, kItems = (kC * kPer + NT - 1) / NT;
   Raw8<T> r[kItems];
 
-  __device__ __forceinline__ static int row(int i, int tid) { return (tid + 256 * i) / kPer; }
-  __device__ __forceinline__ static int col(int i, int tid) { return (tid + 256 * i) % kPer * 8; }
+  // (threads past the last item take part in the loads)
+  __device__ __forceinline__ static int row(int i, int tid) { return (tid + NT * i) / kPer % kC; }
+  __device__ __forceinline__ static int col(int i, int tid) { return (tid + NT * i) % kPer * 8; }
 
-  __device__ __forceinline__ void load(const T* p, int64_t stride, int n, int dk, bool vec, int tid) {
-    if (vec) {  // (dk is a multiple of a 16-byte access)
+  template <bool VEC>
+  __device__ __forceinline__ void load(const T* p, int64_t stride, int n, int dk, int tid) {
+    if constexpr (VEC) {  // (dk is a multiple of a 16-byte access)
 #pragma unroll
       for (int i = 0; i < kItems; ++i) {
         const int c = col(i, tid), rw = row(i, tid);
@@ -283,9 +290,87 @@ struct StageRows {
   }
   __device__ __forceinline__ void put(Tile<kC, DKP, kRawParts<T>>& tile, int n, int dk, int tid) const {
 #pragma unroll
-    for (int i = 0; i < kItems; ++i) tile.put(row(i, tid), col(i, tid), parts(i, n, dk, tid));
+    for (int i = 0; i < kItems; ++i)
+      if (NT * (i + 1) <= kC * kPer || tid + NT * i < kC * kPer) tile.put(row(i, tid), col(i, tid), parts(i, n, dk, tid));
   }
 };
+
+// One column a lane of a chunk's n rows, as result tiles hold them (element 4 rt + r: row 16 rt + 4g + r).  `at` is
+// the wave's first column in the chunk's first row, `stride` the rows' (at most kDeltaMaxStride: a scalar base for
+// each row, and one 32-bit offset a lane).  Lanes past the last row read an earlier one.
+template <typename T>
+__device__ __forceinline__ uint32_t lane_offset(int64_t stride, int m, int grp) {
+  return (4u * grp * static_cast<uint32_t>(stride) + m) * static_cast<uint32_t>(sizeof(T));
+}
+template <typename T>
+struct Cols {
+  T r[16];
+  __device__ __forceinline__ void load(const T* at, int64_t stride, int m, int grp, int n, bool live) {
+    const uint32_t off = live ? lane_offset<T>(stride, m, grp) : 0u;
+    if (n == kC) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        r[i] = *reinterpret_cast<const T*>(reinterpret_cast<const char*>(at) + off);
+        at += (i & 3) == 3 ? 13 * stride : stride;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int u = 16 * (i >> 2) + (i & 3);
+        r[i] = *reinterpret_cast<const T*>(reinterpret_cast<const char*>(at + (u < n ? u : 0) * stride) +
+                                           (u + 4 * grp < n ? off : 0u));
+      }
+    }
+  }
+  __device__ __forceinline__ f32x4 tile(int rt, int grp, int n, bool live) const {
+    f32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = live && 16 * rt + 4 * grp + i < n ? to_f32(r[4 * rt + i]) : 0.f;
+    return v;
+  }
+};
+template <typename T>
+__device__ __forceinline__ void store_cols(T* at, int64_t stride, const f32x4 (&v)[4], int m, int grp, int n, bool live) {
+  if (!live) return;
+  const uint32_t off = lane_offset<T>(stride, m, grp);
+  if (n == kC) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      *reinterpret_cast<T*>(reinterpret_cast<char*>(at) + off) = from_f32<T>(v[i >> 2][i & 3]);
+      at += (i & 3) == 3 ? 13 * stride : stride;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int u = 16 * (i >> 2) + (i & 3);
+      if (u + 4 * grp < n)
+        *reinterpret_cast<T*>(reinterpret_cast<char*>(at + u * stride) + off) = from_f32<T>(v[i >> 2][i & 3]);
+    }
+  }
+}
+// The rows dk of a state's 16 columns: `at` is the wave's first column of row 0.  Rows are `ld` values apart.
+template <int KT>
+__device__ __forceinline__ void load_state(f32x4 (&S)[KT], const float* at, int ld, int rows, int m, int grp, bool live) {
+  const uint32_t off = live ? (4u * grp * static_cast<uint32_t>(ld) + m) * 4u : 0u;
+#pragma unroll
+  for (int t = 0; t < KT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const bool ok = live && 16 * t + 4 * grp + r < rows;
+      S[t][r] = ok ? *reinterpret_cast<const float*>(reinterpret_cast<const char*>(at + (16 * t + r) * ld) + off) : 0.f;
+    }
+}
+template <int KT>
+__device__ __forceinline__ void store_state(float* at, int ld, int rows, const f32x4 (&S)[KT], int m, int grp, bool live) {
+  if (!live) return;
+  const uint32_t off = (4u * grp * static_cast<uint32_t>(ld) + m) * 4u;
+#pragma unroll
+  for (int t = 0; t < KT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (rows == 16 * KT || 16 * t + 4 * grp + r < rows)
+        *reinterpret_cast<float*>(reinterpret_cast<char*>(at + (16 * t + r) * ld) + off) = S[t][r];
+}
 
 // One row's operand: 8 values from column c on, zero past dk (or where !ok), as parts
 template <typename T>
@@ -302,19 +387,19 @@ constexpr int tri_frag(int rt, int ks) {
 }
 
 // A chunk's two triangles on their way into LDS: three parts of the first, PP of the second
-template <int PP>
+template <int PP, int NT>
 struct StageTri {
-  static constexpr int kCount = tri_index(1, PP, 0), kItems = (kCount + 255) / 256;
+  static constexpr int kCount = tri_index(1, PP, 0), kItems = (kCount + NT - 1) / NT;
   u32x4 r[kItems];
   __device__ __forceinline__ void load(const uint4* tri, int tid) {
     const u32x4* at = reinterpret_cast<const u32x4*>(tri);
 #pragma unroll
-    for (int i = 0; i < kItems; ++i) r[i] = at[256 * (i + 1) <= kCount || tid + 256 * i < kCount ? tid + 256 * i : 0];
+    for (int i = 0; i < kItems; ++i) r[i] = at[NT * (i + 1) <= kCount || tid + NT * i < kCount ? tid + NT * i : 0];
   }
   __device__ __forceinline__ void put(uint4* lds, int tid) const {
 #pragma unroll
     for (int i = 0; i < kItems; ++i)
-      if (256 * (i + 1) <= kCount || tid + 256 * i < kCount) reinterpret_cast<u32x4*>(lds)[tid + 256 * i] = r[i];
+      if (NT * (i + 1) <= kCount || tid + NT * i < kCount) reinterpret_cast<u32x4*>(lds)[tid + NT * i] = r[i];
   }
 };
 template <int P>
@@ -367,6 +452,19 @@ __device__ __forceinline__ DeltaPos delta_pos(uint32_t ncb, uint32_t nslots, uin
   return {static_cast<int32_t>(slot), static_cast<int32_t>(item - slot * heads), static_cast<int32_t>(in / 8), slot < nslots};
 }
 inline int64_t delta_blocks(int64_t ncb, int64_t nslots, int64_t heads) { return (nslots * heads + 7) / 8 * 8 * ncb; }
+
+// The tokens' scalars of a chunk, as delta_prep.hip leaves them: four rows of 64
+enum DecRow { kDecKey, kDecUp, kDecOut, kDecBetaKey };
+__device__ __forceinline__ f32x4 dec_at(const float (*dec)[kC], DecRow which, int rt, int grp) {
+  return *reinterpret_cast<const f32x4*>(&dec[which][16 * rt + 4 * grp]);
+}
+
+// Waves of a workgroup of the passes along time, 16 state columns each: eight share a chunk's operands where there
+// are columns for them
+// Instructions stay on their side: without it the reads of all operands are moved to the front, and their
+// registers spill.  Each phase reads the next one's operands.
+__device__ __forceinline__ void phase() { __builtin_amdgcn_sched_barrier(0); }
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6)); }
 
 // f(type of the activations, std::integral_constant<int, padded dk>)
 template <typename F>

@@ -31,79 +31,79 @@ struct FwdArgs {
 
 // AGG: a part's end state from zero, and (column blocks from a.vcb on) its
 // transition: what the identity becomes where V is zero.
-template <typename T, int DKP, bool SAVE, bool AGG>
-__global__ void __launch_bounds__(256)
+template <typename T, int DKP, int NW, bool VEC, bool SAVE, bool AGG>
+__global__ void __launch_bounds__(64 * NW)
 delta_fwd_kernel(FwdArgs a) {
-  constexpr int P = kRawParts<T>, KT = DKP / 16, KS = DKP / 32;
+  constexpr int P = kRawParts<T>, KT = DKP / 16, KS = DKP / 32, NT = 64 * NW;
   constexpr int ORD = P == 3 ? 3 : 2;  // of what only the outputs see: bfloat16 keeps 8 bits of them
   constexpr int PP = AGG ? 0 : ORD;
   __shared__ __attribute__((aligned(16))) Tile<kC, DKP, P> sK;
   __shared__ __attribute__((aligned(16))) Tile<AGG ? 1 : kC, DKP, P> sQ;
-  __shared__ uint4 sTri[StageTri<PP>::kCount];
-  __shared__ float4 sDec[kC];
+  __shared__ uint4 sTri[StageTri<PP, NT>::kCount];
+  __shared__ __attribute__((aligned(16))) float sDec[4][kC];
   const DeltaGeom& g = a.g;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 15, grp = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), m = lane & 15, grp = lane >> 4;
   const DeltaPos p = delta_pos(a.ncb, a.nslots, static_cast<uint32_t>(g.HV));
   if (!p.ok) return;
   const int h = p.h, hk = h / g.group;
   const bool trans = AGG && p.cb >= static_cast<int32_t>(a.vcb);
-  const int col = (trans ? p.cb - static_cast<int32_t>(a.vcb) : p.cb) * kDeltaCols + 16 * wave + m;
+  const int col0 = ((trans ? p.cb - static_cast<int32_t>(a.vcb) : p.cb) * NW + wave) * 16, col = col0 + m;
   const bool live = trans ? col < DKP : col < g.DV;
-  T* o = static_cast<T*>(a.o) + static_cast<int64_t>(h) * g.DV + col;
-  const int64_t orow = static_cast<int64_t>(g.HV) * g.DV;
+  const int at_col = col0 < g.DV ? col0 : 0;  // (waves without columns address the first)
   const SeqChunk part = seq_chunk(g.q, p.slot, g.part, lane);
   if (part.t0 < 0) return;
   if (AGG && (part.seq >= g.q.S || part.t1 == part.end)) return;  // (nothing follows a last part)
+  const int64_t orow = static_cast<int64_t>(g.HV) * g.DV, ocol = static_cast<int64_t>(h) * g.DV + at_col;
+  T* o = static_cast<T*>(a.o) + ocol;
   if (part.seq >= g.q.S) {  // rows of no sequence
     if (live)
-      for (int32_t t = part.t0 + 4 * 0 + grp; t < part.t1; t += 4) o[t * orow] = from_f32<T>(0.f);
+      for (int32_t t = part.t0 + grp; t < part.t1; t += 4) o[t * orow + m] = from_f32<T>(0.f);
     return;
   }
   const int32_t row = seq_slot(g.q, part.seq);
-  const int64_t cells = static_cast<int64_t>(g.DK) * g.DV, at_h = static_cast<int64_t>(h) * cells + col;
-  const int64_t at_part = (static_cast<int64_t>(p.slot) * g.HV + h) * cells + col;
+  const int64_t cells = static_cast<int64_t>(g.DK) * g.DV, at_h = static_cast<int64_t>(h) * cells + at_col;
+  const int64_t at_part = (static_cast<int64_t>(p.slot) * g.HV + h) * cells + at_col;
   f32x4 S[KT];
-  {
+  if (trans) {
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) S[t][r] = 16 * t + 4 * grp + r == col ? 1.f : 0.f;
+  } else {
     const float* src = nullptr;
     if (!AGG && a.w.carry != nullptr)
       src = a.w.carry + at_part;
     else if (!AGG && a.h0 != nullptr && row >= 0 && !seq_fresh(g.q, part.seq))
       src = a.h0 + row * (g.HV * cells) + at_h;
-#pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int d = 16 * t + 4 * grp + r;
-        S[t][r] = trans ? (d == col ? 1.f : 0.f) : src != nullptr && live && d < g.DK ? src[static_cast<int64_t>(d) * g.DV] : 0.f;
-      }
+    load_state<KT>(S, src, g.DV, src != nullptr ? g.DK : 0, m, grp, live);
   }
   const T* kp = static_cast<const T*>(a.in.k) + hk * g.kh;
   const T* qp = static_cast<const T*>(a.in.q) + hk * g.qh;
-  const T* vp = static_cast<const T*>(a.in.v) + h * g.vh + (live && !trans ? col : 0);
+  const T* vp = static_cast<const T*>(a.in.v) + h * g.vh + at_col;
+  const bool vlive = live && !trans;
   const int32_t slot0 = cut_div(g.cut, part.start) + part.seq + (part.t0 - part.start) / kC;
   const int32_t chunks = (part.t1 - part.t0 + kC - 1) / kC;
   // the next chunk's operands, on their way while this one's are at work
-  StageRows<T, DKP> rK, rQ;
-  StageTri<PP> rT;
-  float4 rDec;
+  StageRows<T, DKP, NT> rK, rQ;
+  StageTri<PP, NT> rT;
+  float rDec;
   float rGam;
-  T rV[16];
+  Cols<T> rV;
   const auto load = [&](int32_t i) {
     const int32_t t0 = part.t0 + i * kC;
     const int n = part.t1 - t0 < kC ? part.t1 - t0 : kC;
     const int64_t at = static_cast<int64_t>(slot0 + i) * g.HV + h;
-    rK.load(kp + t0 * g.ks, g.ks, n, g.DK, g.qk_vec, tid);
-    if constexpr (!AGG) rQ.load(qp + t0 * g.qs, g.qs, n, g.DK, g.qk_vec, tid);
+    rK.template load<VEC>(kp + t0 * g.ks, g.ks, n, g.DK, tid);
+    if constexpr (!AGG) rQ.template load<VEC>(qp + t0 * g.qs, g.qs, n, g.DK, tid);
     rT.load(reinterpret_cast<const uint4*>(a.w.tri) + at * kTriFragments, tid);
-    rDec = reinterpret_cast<const float4*>(a.w.dec)[at * kC + lane];
+    if (tid < 3 * kC) rDec = a.w.dec[at * (4 * kC) + tid];
     rGam = a.w.gam[at];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int t = 16 * (i >> 2) + 4 * grp + (i & 3);
-      rV[i] = vp[live && !trans ? (t0 + (t < n ? t : 0)) * g.vs : 0];
-    }
   };
-  if (chunks > 0) load(0);
+  const auto load_v = [&](int32_t i) {
+    const int32_t t0 = part.t0 + i * kC;
+    rV.load(vp + t0 * g.vs, g.vs, m, grp, part.t1 - t0 < kC ? part.t1 - t0 : kC, vlive);
+  };
+  if (chunks > 0) load(0), load_v(0);
   for (int32_t nth = 0; nth < chunks; ++nth) {
     const int32_t t0 = part.t0 + nth * kC;
     const int n = part.t1 - t0 < kC ? part.t1 - t0 : kC;
@@ -112,106 +112,111 @@ delta_fwd_kernel(FwdArgs a) {
     rK.put(sK, n, g.DK, tid);
     if constexpr (!AGG) rQ.put(sQ, n, g.DK, tid);
     rT.put(sTri, tid);
-    if (wave == 0) sDec[lane] = rDec;
+    if (tid < 3 * kC) sDec[0][tid] = rDec;
     const float gam = rGam;
-    f32x4 V[4];
-#pragma unroll
-    for (int rt = 0; rt < 4; ++rt)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) V[rt][r] = live && !trans && 16 * rt + 4 * grp + r < n ? to_f32(rV[4 * rt + r]) : 0.f;
     if (nth + 1 < chunks) load(nth + 1);
-    if constexpr (SAVE) {
-      float* s0 = a.s0 + at * cells + col;
-      if (live)
-#pragma unroll
-        for (int t = 0; t < KT; ++t)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int d = 16 * t + 4 * grp + r;
-            if (d < g.DK) s0[static_cast<int64_t>(d) * g.DV] = S[t][r];
-          }
-    }
+    if constexpr (SAVE) store_state<KT>(a.s0 + at * cells + at_col, g.DV, g.DK, S, m, grp, live);
     __syncthreads();
-    f32x4 R[4], O[4];
+    f32x4 R[4], O[4], D[4];
 #pragma unroll
-    for (int rt = 0; rt < 4; ++rt) R[rt] = O[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int rt = 0; rt < 4; ++rt) R[rt] = O[rt] = D[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    Frag<P> fk[2][4], fq[2][AGG ? 1 : 4];
+    const auto rows = [&](int ks) {
+#pragma unroll
+      for (int rt = 0; rt < 4; ++rt) {
+        fk[ks & 1][rt] = sK.rows(16 * rt + m, 32 * ks + 4 * grp);
+        if constexpr (!AGG) fq[ks & 1][rt] = sQ.rows(16 * rt + m, 32 * ks + 4 * grp);
+      }
+    };
+    Frag<3> ft[2][2];
+    const auto tri = [&](int rt) {
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+        if (tri_frag<false>(rt, ks) >= 0) ft[rt & 1][ks] = tri_at<3>(sTri, 0, tri_frag<false>(rt, ks), lane);
+    };
+    f32x4 dk[4];
+    rows(0);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
+      if (ks + 1 < KS)
+        rows(ks + 1);
+      else
+#pragma unroll
+        for (int rt = 0; rt < 4; ++rt) dk[rt] = dec_at(sDec, kDecKey, rt, grp);
       const Frag<3> sf = split_tiles<3>(S[2 * ks], S[2 * ks + 1]);
-      const int k0 = 32 * ks + 4 * grp;
 #pragma unroll
       for (int rt = 0; rt < 4; ++rt) {
-        R[rt] = mma<3>(sK.rows(16 * rt + m, k0), sf, R[rt]);
-        if constexpr (!AGG) O[rt] = mma<ORD>(sQ.rows(16 * rt + m, k0), sf, O[rt]);
+        R[rt] = mma<3>(fk[ks & 1][rt], sf, R[rt]);
+        if constexpr (!AGG) O[rt] = mma<ORD>(fq[ks & 1][rt], sf, O[rt]);
       }
+      phase();
     }
-    float up[4][4];
+    tri(0);
+    tri(1);
 #pragma unroll
-    for (int rt = 0; rt < 4; ++rt)
+    for (int rt = 0; rt < 4; ++rt) R[rt] = rV.tile(rt, grp, n, vlive) - dk[rt] * R[rt];
+    if (nth + 1 < chunks) load_v(nth + 1);
+    const Frag<3> rf[2] = {split_tiles<3>(R[0], R[1]), split_tiles<3>(R[2], R[3])};
+    phase();
+    Frag<ORD> fp[2][2];
+    const auto tri_p = [&](int rt) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float4 d = sDec[16 * rt + 4 * grp + r];
-        R[rt][r] = d.w * fmaf(-d.x, R[rt][r], V[rt][r]);
-        O[rt][r] *= d.z;
-        up[rt][r] = d.y;
+      for (int ks = 0; ks < 2; ++ks)
+        if (tri_frag<false>(rt, ks) >= 0) fp[rt & 1][ks] = tri_at<ORD>(sTri, 1, tri_frag<false>(rt, ks), lane);
+    };
+    f32x4 up[4], dout[4];
+#pragma unroll
+    for (int rt = 0; rt < 4; ++rt) {
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+        if (tri_frag<false>(rt, ks) >= 0) D[rt] = mma<3>(ft[rt & 1][ks], rf[ks], D[rt]);
+      phase();
+      if (rt < 2) tri(rt + 2);
+      if constexpr (!AGG) {
+        if (rt >= 2) tri_p(rt - 2);
+        dout[rt] = dec_at(sDec, kDecOut, rt, grp);
       }
-    f32x4 D[4];
-    {
-      const Frag<3> rf[2] = {split_tiles<3>(R[0], R[1]), split_tiles<3>(R[2], R[3])};
-#pragma unroll
-      for (int rt = 0; rt < 4; ++rt) {
-        D[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-          if (tri_frag<false>(rt, ks) >= 0) D[rt] = mma<3>(tri_at<3>(sTri, 0, tri_frag<false>(rt, ks), lane), rf[ks], D[rt]);
-      }
+      up[rt] = dec_at(sDec, kDecUp, rt, grp);
     }
     if constexpr (!AGG) {
       const Frag<ORD> df[2] = {split_tiles<ORD>(D[0], D[1]), split_tiles<ORD>(D[2], D[3])};
 #pragma unroll
       for (int rt = 0; rt < 4; ++rt) {
+        O[rt] *= dout[rt];
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
-          if (tri_frag<false>(rt, ks) >= 0) O[rt] = mma<ORD>(tri_at<ORD>(sTri, 1, tri_frag<false>(rt, ks), lane), df[ks], O[rt]);
+          if (tri_frag<false>(rt, ks) >= 0) O[rt] = mma<ORD>(fp[rt & 1][ks], df[ks], O[rt]);
+        phase();
+        if (rt < 2) tri_p(rt + 2);
       }
+      store_cols<T>(o + t0 * orow, orow, O, m, grp, n, live);
+      if constexpr (SAVE) store_cols<float>(a.vt + t0 * orow + ocol, orow, D, m, grp, n, live);
     }
+    Frag<P> fc[2][2];
+    const auto keys = [&](int t) {
 #pragma unroll
-    for (int rt = 0; rt < 4; ++rt)
+      for (int ks = 0; ks < 2; ++ks) fc[t & 1][ks] = sK.cols(16 * t, 32 * ks + 4 * grp, m);
+    };
+    keys(0);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = 16 * rt + 4 * grp + r;
-        if (!AGG && live && i < n) {
-          o[(t0 + i) * orow] = from_f32<T>(O[rt][r]);
-          if constexpr (SAVE) a.vt[(t0 + i) * orow + static_cast<int64_t>(h) * g.DV + col] = D[rt][r];
-        }
-        D[rt][r] *= up[rt][r];
-      }
+    for (int rt = 0; rt < 4; ++rt) D[rt] *= up[rt];
     const Frag<3> uf[2] = {split_tiles<3>(D[0], D[1]), split_tiles<3>(D[2], D[3])};
+    phase();
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
+      if (t + 1 < KT) keys(t + 1);
       S[t] *= gam;
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) S[t] = mma<3>(sK.cols(16 * t, 32 * ks + 4 * grp, m), uf[ks], S[t]);
+      for (int ks = 0; ks < 2; ++ks) S[t] = mma<3>(fc[t & 1][ks], uf[ks], S[t]);
+      if (t % 2) phase();
     }
   }
-  float* dst = nullptr;
-  int64_t ld = g.DV;
-  int rows = g.DK;
   if (AGG && trans)
-    dst = a.w.trans + (static_cast<int64_t>(p.slot) * g.HV + h) * (DKP * DKP) + col, ld = DKP, rows = DKP;
+    store_state<KT>(a.w.trans + (static_cast<int64_t>(p.slot) * g.HV + h) * (DKP * DKP) + col0, DKP, DKP, S, m, grp, live);
   else if (AGG)
-    dst = a.w.carry + at_part;
+    store_state<KT>(a.w.carry + at_part, g.DV, g.DK, S, m, grp, live);
   else if (a.h1 != nullptr && row >= 0 && part.t1 == part.end)
-    dst = a.h1 + row * (g.HV * cells) + at_h;
-  if (dst != nullptr && live) {
-#pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int d = 16 * t + 4 * grp + r;
-        if (d < rows) dst[d * ld] = S[t][r];
-      }
-  }
+    store_state<KT>(a.h1 + row * (g.HV * cells) + at_h, g.DV, g.DK, S, m, grp, live);
 }
 
 // Joins the parts of a sequence: carry holds each part's end state from zero (REV: the gradient of its initial
@@ -224,7 +229,7 @@ delta_carry_kernel(DeltaGeom g, DeltaWork w, const float* __restrict__ enter, ui
   const uint32_t item = blockIdx.x / ncb;
   const int32_t seq = static_cast<int32_t>(item / static_cast<uint32_t>(g.HV));
   const int h = static_cast<int>(item - static_cast<uint32_t>(seq) * g.HV);
-  const int col = static_cast<int>(blockIdx.x - item * ncb) * kDeltaCols + 16 * wave + m;
+  const int col = static_cast<int>(blockIdx.x - item * ncb) * 64 + 16 * wave + m;
   const bool live = col < g.DV;
   const int32_t start = seq_off_u(g.q, seq), next = seq_off_u(g.q, seq + 1), end = next < start ? start : next;
   const int32_t slot0 = cut_div(g.part, start) + seq, parts = end > start ? cut_div(g.part, end - start - 1) + 1 : 1;
@@ -285,7 +290,7 @@ delta_carry_kernel(DeltaGeom g, DeltaWork w, const float* __restrict__ enter, ui
 template <bool REV>
 hipError_t launch_delta_carry(const DeltaGeom& g, const DeltaWork& w, const float* enter, hipStream_t s) {
   if (g.q.S == 0) return hipSuccess;
-  const uint32_t ncb = delta_col_blocks(g.DV);
+  const uint32_t ncb = delta_col_blocks(g.DV, 4);
   const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(g.q.S) * g.HV * ncb));
   switch (delta_dkp(g.DK)) {
     case 32: hipLaunchKernelGGL((delta_carry_kernel<32, REV>), grid, dim3(256), 0, s, g, w, enter, ncb); break;
@@ -299,27 +304,35 @@ template hipError_t launch_delta_carry<true>(const DeltaGeom&, const DeltaWork&,
 
 hipError_t launch_delta_fwd(const DeltaGeom& g, const DeltaIn& in, const DeltaWork& w, const float* h0, float* h1,
                             void* o, float* s0, float* vt, int dtype, hipStream_t s) {
-  const uint32_t vcb = delta_col_blocks(g.DV);
+  // (rows that are read value by value: more registers, so four waves)
+  const int nw = g.qk_vec ? delta_waves(g.DV) : 4;
+  const uint32_t vcb = delta_col_blocks(g.DV, nw);
   FwdArgs a{g, in, w, h0, h1, o, s0, vt, vcb, vcb, static_cast<uint32_t>(chunk_slots(g.q, g.part))};
   hipError_t e = launch_delta_prep(g, in, w, false, dtype, s);
   if (e != hipSuccess) return e;
-  return delta_dispatch(dtype, g.DK, [&](auto t, auto dkp) {
+  const auto run = [&](auto t, auto dkp, auto waves, auto vec) {
     using T = decltype(t);
-    constexpr int DKP = decltype(dkp)::value;
+    constexpr int DKP = decltype(dkp)::value, NW = decltype(waves)::value;
+    constexpr bool VEC = decltype(vec)::value;
     if (g.parts > 1) {
-      a.ncb = vcb + delta_col_blocks(DKP);
-      hipLaunchKernelGGL((delta_fwd_kernel<T, DKP, false, true>),
-                         dim3(static_cast<unsigned>(delta_blocks(a.ncb, a.nslots, g.HV))), dim3(256), 0, s, a);
+      a.ncb = vcb + delta_col_blocks(DKP, NW);
+      hipLaunchKernelGGL((delta_fwd_kernel<T, DKP, NW, VEC, false, true>),
+                         dim3(static_cast<unsigned>(delta_blocks(a.ncb, a.nslots, g.HV))), dim3(64 * NW), 0, s, a);
       hipError_t e = hipGetLastError();
       if (e != hipSuccess || (e = launch_delta_carry<false>(g, w, h0, s)) != hipSuccess) return e;
       a.ncb = vcb;
     }
     const dim3 grid(static_cast<unsigned>(delta_blocks(a.ncb, a.nslots, g.HV)));
     if (s0 != nullptr)
-      hipLaunchKernelGGL((delta_fwd_kernel<T, DKP, true, false>), grid, dim3(256), 0, s, a);
+      hipLaunchKernelGGL((delta_fwd_kernel<T, DKP, NW, VEC, true, false>), grid, dim3(64 * NW), 0, s, a);
     else
-      hipLaunchKernelGGL((delta_fwd_kernel<T, DKP, false, false>), grid, dim3(256), 0, s, a);
+      hipLaunchKernelGGL((delta_fwd_kernel<T, DKP, NW, VEC, false, false>), grid, dim3(64 * NW), 0, s, a);
     return hipGetLastError();
+  };
+  return delta_dispatch(dtype, g.DK, [&](auto t, auto dkp) {
+    using Four = std::integral_constant<int, 4>;
+    if (!g.qk_vec) return run(t, dkp, Four{}, std::false_type{});
+    return nw == 8 ? run(t, dkp, std::integral_constant<int, 8>{}, std::true_type{}) : run(t, dkp, Four{}, std::true_type{});
   });
 }
 

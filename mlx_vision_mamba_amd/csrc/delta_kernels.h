@@ -8,7 +8,13 @@
 namespace mvm {
 
 constexpr int kDeltaChunk = 64;   // tokens of a chunk
-constexpr int kDeltaCols = 64;    // state columns of a workgroup: 16 a wave
+constexpr int64_t kDeltaMaxStride = 1 << 25;  // of v's and o's rows: 12 of them and a row are within 2^31 bytes
+// Waves of a workgroup of the passes along time, 16 columns of the state each: eight share a chunk's operands
+// where the state has columns for them.
+inline int delta_waves(int dv) { return dv > 64 ? 8 : 4; }
+inline uint32_t delta_col_blocks(int cols, int waves) {
+  return static_cast<uint32_t>((cols + 16 * waves - 1) / (16 * waves));
+}
 
 struct DeltaGeom {
   SeqGeom q;
@@ -34,10 +40,10 @@ struct DeltaIn {
 
 // What the chunks' own products leave for the passes along time, for every
 // chunk slot and value head: the fragments of two 64 x 64 triangles as the
-// matrix units take them, and a float4 of scalars for each token.
+// matrix units take them, and four scalars for each token.
 struct DeltaWork {
   void* tri;       // (slots, HV, 2, parts, 6, 64) 16-byte fragments
-  float* dec;      // (slots, HV, 64, 4)
+  float* dec;      // (slots, HV, 4, 64)
   float* gam;      // (slots, HV): the decay over the chunk
   float* trans;    // (part slots, HV, DKP, DKP) transitions of the parts, or null
   float* carry;    // (part slots, HV, DK, DV): end states of the parts from zero, then their initial states
@@ -69,8 +75,6 @@ constexpr int64_t kTriBytes = int64_t{kTriFragments} * 16;
 constexpr int tri_index(int which, int p, int f) { return ((which * kTriParts + p) * kTriFrags + f) * 64; }
 
 inline int delta_dkp(int dk) { return dk <= 32 ? 32 : (dk <= 64 ? 64 : 128); }
-
-inline uint32_t delta_col_blocks(int cols) { return static_cast<uint32_t>((cols + kDeltaCols - 1) / kDeltaCols); }
 
 // joins the parts, from the initial states (REV: from the gradients of the final ones)
 template <bool REV>

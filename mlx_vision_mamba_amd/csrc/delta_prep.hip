@@ -3,7 +3,8 @@
 //   P_ij = scale (q_i . k_j) exp(G_i - G_j), i >= j     (G: log decays summed)
 // and the tokens' scalars, for the passes along time (delta_fwd.hip,
 // delta_bwd.hip), which take T and P as ready A operands: their bf16 parts in
-// the order in which the lanes load them (the backward pass: of T' and P').
+// the order in which the lanes load them (forward T diag(beta), backward T' and
+// P').
 //
 // A workgroup of four waves takes one chunk and head, a wave 16 rows of both
 // triangles.  A result tile is, as the lanes hold it, an A operand of its
@@ -90,8 +91,11 @@ delta_prep_kernel(DeltaGeom g, DeltaIn in, DeltaWork w) {
   if (wave == 0) {
     const double Gc = __shfl(G, 63);
     const float eG = exp_diff(G), eR = exp_diff(Gc - G);
-    reinterpret_cast<float4*>(w.dec)[at * kC + lane] =
-        make_float4(sRk[lane] * eG, sRk[lane] * eR, g.scale * sRq[lane] * eG, sBeta[lane]);
+    float* dec = w.dec + at * (4 * kC) + lane;
+    dec[kDecKey * kC] = sRk[lane] * eG;
+    dec[kDecUp * kC] = sRk[lane] * eR;
+    dec[kDecOut * kC] = g.scale * sRq[lane] * eG;
+    dec[kDecBetaKey * kC] = sBeta[lane] * sRk[lane] * eG;
     if (lane == 0) w.gam[at] = exp_diff(Gc);
   }
   const double Gown = sG[own];
@@ -144,6 +148,11 @@ delta_prep_kernel(DeltaGeom g, DeltaIn in, DeltaWork w) {
       X[i] = -mma_f32(*reinterpret_cast<const f32x4*>(&sD[i][m][4 * grp]), s, z);
     }
   }
+  if (!BWD)  // T diag(beta): the summed index is the row here
+#pragma unroll
+    for (int jt = 0; jt < 4; ++jt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) X[jt][r] *= sBeta[16 * jt + 4 * grp + r];
   uint4* out = reinterpret_cast<uint4*>(w.tri) + at * kTriFragments + lane;
 #pragma unroll
   for (int ks = 0; ks < 2; ++ks)
