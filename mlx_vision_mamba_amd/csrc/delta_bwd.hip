@@ -34,6 +34,7 @@ struct BwdArgs {
   DeltaIn in;
   DeltaWork w;
   DeltaBwd b;
+  int64_t col_tiles;
   uint32_t vcb, ncb, nslots;  // column blocks of the values, and of the launch
 };
 
@@ -44,6 +45,8 @@ __global__ void __launch_bounds__(64 * NW)
 delta_bwd_kernel(BwdArgs a) {
   constexpr int P = kRawParts<T>, KT = DKP / 16, KS = DKP / 32, NT = 64 * NW;
   __shared__ __attribute__((aligned(16))) Tile<kC, DKP, P> sK, sQ;
+  constexpr bool OLDS = P == 1;  // (as V in the forward)
+  __shared__ __attribute__((aligned(16))) Tile<OLDS ? kC : 1, 16 * NW, 1> sO;
   __shared__ uint4 sTri[StageTri<3, NT>::kCount];
   __shared__ __attribute__((aligned(16))) float sDec[4][kC];
   const DeltaGeom& g = a.g;
@@ -72,8 +75,9 @@ delta_bwd_kernel(BwdArgs a) {
   }
   const T* kp = static_cast<const T*>(a.in.k) + hk * g.kh;
   const T* qp = static_cast<const T*>(a.in.q) + hk * g.qh;
-  const int64_t orow = static_cast<int64_t>(g.HV) * g.DV, ocol = static_cast<int64_t>(h) * g.DV + at_col;
-  const T* dop = static_cast<const T*>(a.b.d_o) + ocol;
+  const int64_t orow = static_cast<int64_t>(g.HV) * g.DV;
+  const int vcol0 = trans ? 0 : p.cb * NW * 16;
+  const T* dop = static_cast<const T*>(a.b.d_o) + static_cast<int64_t>(h) * g.DV + (OLDS ? vcol0 : at_col);
   const bool vlive = live && !trans;
   const int32_t slot0 = cut_div(g.cut, part.start) + part.seq + (part.t0 - part.start) / kC;
   const int32_t chunks = (part.t1 - part.t0 + kC - 1) / kC;
@@ -82,6 +86,7 @@ delta_bwd_kernel(BwdArgs a) {
   float rDec;
   float rGam;
   Cols<T> rO;
+  StageRows<T, 16 * NW, NT> rOt;
   const auto load = [&](int32_t i) {
     const int32_t t0 = part.t0 + i * kC;
     const int n = part.t1 - t0 < kC ? part.t1 - t0 : kC;
@@ -89,6 +94,7 @@ delta_bwd_kernel(BwdArgs a) {
     rK.template load<VEC>(kp + t0 * g.ks, g.ks, n, g.DK, tid);
     rQ.template load<VEC>(qp + t0 * g.qs, g.qs, n, g.DK, tid);
     rT.load(reinterpret_cast<const uint4*>(a.w.tri) + at * kTriFragments, tid);
+    if constexpr (OLDS) rOt.template load<VEC>(dop + t0 * orow, orow, n, trans ? 0 : g.DV - vcol0, tid);
     if (tid < 4 * kC) rDec = a.w.dec[at * (4 * kC) + tid];
     rGam = a.w.gam[at];
   };
@@ -96,7 +102,10 @@ delta_bwd_kernel(BwdArgs a) {
     const int32_t t0 = part.t0 + i * kC;
     rO.load(dop + t0 * orow, orow, m, grp, part.t1 - t0 < kC ? part.t1 - t0 : kC, vlive);
   };
-  if (chunks > 0) load(chunks - 1), load_o(chunks - 1);
+  if (chunks > 0) {
+    load(chunks - 1);
+    if constexpr (!OLDS) load_o(chunks - 1);
+  }
   for (int32_t nth = chunks - 1; nth >= 0; --nth) {
     const int32_t t0 = part.t0 + nth * kC;
     const int n = part.t1 - t0 < kC ? part.t1 - t0 : kC;
@@ -104,11 +113,14 @@ delta_bwd_kernel(BwdArgs a) {
     __syncthreads();
     rK.put(sK, n, g.DK, tid);
     rQ.put(sQ, n, g.DK, tid);
+    if constexpr (OLDS) rOt.put(sO, n, trans ? 0 : g.DV - vcol0, tid);
     rT.put(sTri, tid);
     if (tid < 4 * kC) sDec[0][tid] = rDec;
     const float gam = rGam;
     if (nth > 0) load(nth - 1);
-    if constexpr (!AGG) store_state<KT>(a.b.dend + at * cells + at_col, g.DV, g.DK, E, m, grp, live);
+    const int64_t at_tile = (at * a.col_tiles + col0 / 16) * 256;
+    if constexpr (!AGG)
+      if (col0 < g.DV) store_tiles<KT>(a.b.dend + at_tile * KT, E, lane);
     __syncthreads();
     f32x4 D[4], X[4], O[4];
 #pragma unroll
@@ -116,13 +128,7 @@ delta_bwd_kernel(BwdArgs a) {
     Frag<P> fk[2][4];
     const auto rows = [&](int ks) {
 #pragma unroll
-      for (int rt = 0; rt < 4; ++rt) fk[ks & 1][rt] = sK.rows(16 * rt + m, 32 * ks + 4 * grp);
-    };
-    Frag<3> ft[2][2];
-    const auto tri = [&](int which, int rt) {
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
-        if (tri_frag<true>(rt, ks) >= 0) ft[rt & 1][ks] = tri_at<3>(sTri, which, tri_frag<true>(rt, ks), lane);
+      for (int rt = 0; rt < 4; ++rt) fk[ks & 1][rt] = sK.rows(16 * rt + m, ks, grp);
     };
     f32x4 up[4];
     rows(0);
@@ -134,54 +140,54 @@ delta_bwd_kernel(BwdArgs a) {
 #pragma unroll
         for (int rt = 0; rt < 4; ++rt) up[rt] = dec_at(sDec, kDecUp, rt, grp);
       const Frag<3> ef = split_tiles<3>(E[2 * ks], E[2 * ks + 1]);
-#pragma unroll
-      for (int rt = 0; rt < 4; ++rt) D[rt] = mma<3>(fk[ks & 1][rt], ef, D[rt]);
+      mma_n<3>(fk[ks & 1], ef, D);
       phase();
     }
-    tri(1, 0);
-    tri(1, 1);
+    Frag<3> f1[4], f0[2];
+    tri_tiles<true, 0>(f1, sTri, 1, 1, lane);
 #pragma unroll
     for (int rt = 0; rt < 4; ++rt) {
-      O[rt] = rO.tile(rt, grp, n, vlive);
+      if constexpr (OLDS)
+        O[rt] = sO.col4(16 * wave, 16 * rt + 4 * grp, m);
+      else
+        O[rt] = rO.tile(rt, grp, n, vlive);
       D[rt] *= up[rt];
     }
-    if (nth > 0) load_o(nth - 1);
+    if constexpr (!OLDS)
+      if (nth > 0) load_o(nth - 1);
     {
       const Frag<P> of[2] = {split_tiles<P>(O[0], O[1]), split_tiles<P>(O[2], O[3])};
       phase();
-#pragma unroll
-      for (int rt = 0; rt < 4; ++rt) {
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-          if (tri_frag<true>(rt, ks) >= 0) D[rt] = mma<3>(ft[rt & 1][ks], of[ks], D[rt]);
-        phase();
-        tri(rt < 2 ? 1 : 0, rt < 2 ? rt + 2 : rt - 2);
-      }
+      tri_tiles<true, 0>(f0, sTri, 1, 0, lane);
+      mma_n<3>(f1, of[1], D);
+      phase();
+      tri_tiles<true, 0>(f1, sTri, 0, 1, lane);
+      mma_n<3>(f0, of[0], D);
+      phase();
     }
     f32x4 dx[4], dout[4];
     {
       const Frag<3> df[2] = {split_tiles<3>(D[0], D[1]), split_tiles<3>(D[2], D[3])};
+      tri_tiles<true, 0>(f0, sTri, 0, 0, lane);
+      mma_n<3>(f1, df[1], X);
+      phase();
 #pragma unroll
       for (int rt = 0; rt < 4; ++rt) {
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-          if (tri_frag<true>(rt, ks) >= 0) X[rt] = mma<3>(ft[rt & 1][ks], df[ks], X[rt]);
-        phase();
-        if (rt < 2) tri(0, rt + 2);
         dx[rt] = dec_at(sDec, kDecBetaKey, rt, grp);
         dout[rt] = dec_at(sDec, kDecOut, rt, grp);
       }
+      mma_n<3>(f0, df[0], X);
     }
-    if constexpr (!AGG) store_cols<float>(a.b.x + t0 * orow + ocol, orow, X, m, grp, n, live);
-    Frag<P> fc[2][2], fd[2][2];
-    const auto keys = [&](int t) {
+    constexpr int KG = KT < 4 ? KT : 4;  // row tiles of the state at a time
+    Frag<P> fc[2][KG];
+    const auto keys = [&](int i) {  // K's and Q's columns, of the chunk's first and second half, in turn
+      const int t0 = i / 4 * KG, ks = i / 2 % 2;
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        fc[t & 1][ks] = sK.cols(16 * t, 32 * ks + 4 * grp, m);
-        fd[t & 1][ks] = sQ.cols(16 * t, 32 * ks + 4 * grp, m);
-      }
+      for (int j = 0; j < KG; ++j) fc[i & 1][j] = (i % 2 ? sQ : sK).cols(16 * (t0 + j), 32 * ks + 4 * grp, m);
     };
     keys(0);
+    if constexpr (!AGG)
+      if (col0 < g.DV) store_tiles<4>(a.b.x + at_tile * 4, X, lane);
 #pragma unroll
     for (int rt = 0; rt < 4; ++rt) {
       X[rt] *= -dx[rt];
@@ -189,16 +195,13 @@ delta_bwd_kernel(BwdArgs a) {
     }
     const Frag<3> xf[2] = {split_tiles<3>(X[0], X[1]), split_tiles<3>(X[2], X[3])};
     const Frag<3> of[2] = {split_tiles<3>(O[0], O[1]), split_tiles<3>(O[2], O[3])};
+#pragma unroll
+    for (int t = 0; t < KT; ++t) E[t] *= gam;
     phase();
 #pragma unroll
-    for (int t = 0; t < KT; ++t) {
-      if (t + 1 < KT) keys(t + 1);
-      E[t] *= gam;
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        E[t] = mma<3>(fc[t & 1][ks], xf[ks], E[t]);
-        E[t] = mma<3>(fd[t & 1][ks], of[ks], E[t]);
-      }
+    for (int i = 0; i < 4 * (KT / KG); ++i) {
+      if (i + 1 < 4 * (KT / KG)) keys(i + 1);
+      mma_n<3>(fc[i & 1], i % 2 ? of[i / 2 % 2] : xf[i / 2 % 2], E + i / 4 * KG);
       phase();
     }
   }
@@ -212,17 +215,17 @@ delta_bwd_kernel(BwdArgs a) {
 
 // Zeros in the gradients of the rows that belong to no sequence.
 template <typename T>
-__device__ void zero_rows(const BwdArgs& a, int32_t t0, int32_t t1, int hk, int tid) {
+__device__ void zero_rows(const BwdArgs& a, int32_t t0, int32_t t1, int hk, int tid, int nt) {
   const DeltaGeom& g = a.g;
   for (int32_t t = t0; t < t1; ++t) {
-    for (int c = tid; c < g.DK; c += 256) {
+    for (int c = tid; c < g.DK; c += nt) {
       const int64_t i = (static_cast<int64_t>(t) * g.HK + hk) * g.DK + c;
       static_cast<T*>(a.b.dq)[i] = from_f32<T>(0.f);
       static_cast<T*>(a.b.dk)[i] = from_f32<T>(0.f);
     }
-    for (int c = tid; c < g.group * g.DV; c += 256)
+    for (int c = tid; c < g.group * g.DV; c += nt)
       static_cast<T*>(a.b.dv)[(static_cast<int64_t>(t) * g.HV + hk * g.group) * g.DV + c] = from_f32<T>(0.f);
-    for (int c = tid; c < g.group; c += 256) {
+    for (int c = tid; c < g.group; c += nt) {
       const int64_t i = static_cast<int64_t>(t) * g.HV + hk * g.group + c;
       a.b.dg[i] = 0.f;
       if (g.beta_f32)
@@ -233,39 +236,53 @@ __device__ void zero_rows(const BwdArgs& a, int32_t t0, int32_t t1, int hk, int 
   }
 }
 
-template <typename T, int DKP, bool VEC>
-__global__ void __launch_bounds__(256)
+// Eight waves a chunk and key head: a wave has 16 tokens and half of the keys' columns; the small triangles of its
+// tokens are formed by both waves.  GROUPED: more than one value head a key head.
+template <typename T, int DKP, bool VEC, bool GROUPED>
+__global__ void __launch_bounds__(512)
 delta_grads_kernel(BwdArgs a) {
-  constexpr int P = kRawParts<T>, KT = DKP / 16;
-  struct Rows {  // 32 columns of the values' side
-    Tile<kC, 32, 3> X, D;
+  constexpr int P = kRawParts<T>, KT = DKP / 16, KH = KT / 2, NT = 512;
+  struct Rows {  // 32 columns of the values' side, rows the columns; dO: rows the tokens
+    Tile<32, kC, 3> X, D;
+    Tile<32, DKP, 3> S, E;
     Tile<kC, 32, P> O;
-    Tile<DKP, 32, 3> S, E;
   };
   struct Keys {
     Tile<kC, DKP, P> K, Q;
   };
   __shared__ __attribute__((aligned(16))) union { Rows r; Keys k; } sm;
-  __shared__ double sG[kC], sDG[kC];
-  __shared__ float sBeta[kC], sRk[kC], sRq[kC], sXv[kC], sSum[4][2];
+  __shared__ double sG[kC];
+  __shared__ float sBeta[kC], sRk[kC], sRq[kC], sSe[8];
+  __shared__ float4 sDot[2][kC];
   const DeltaGeom& g = a.g;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 15, grp = lane >> 4;
+  int tid = threadIdx.x, lane = tid & 63, m = lane & 15, grp = lane >> 4;
+  const int wave = wave_id(), tw = wave & 3, half = wave >> 2, d0 = half * KH * 16;  // token tile, first key column
   const uint32_t slot = blockIdx.x / static_cast<uint32_t>(g.HK);
   const int hk = static_cast<int>(blockIdx.x - slot * static_cast<uint32_t>(g.HK));
   const SeqChunk c = seq_chunk(g.q, static_cast<int32_t>(slot), g.cut, lane);
   if (c.t0 < 0 || c.t1 == c.t0) return;
-  if (c.seq >= g.q.S) return zero_rows<T>(a, c.t0, c.t1, hk, tid);
+  if (c.seq >= g.q.S) return zero_rows<T>(a, c.t0, c.t1, hk, tid, NT);
   const int n = c.t1 - c.t0;
-  const int64_t orow = static_cast<int64_t>(g.HV) * g.DV, cells = static_cast<int64_t>(g.DK) * g.DV;
-  const bool vec4 = g.DV % 4 == 0;
+  const int64_t orow = static_cast<int64_t>(g.HV) * g.DV;
   const f32x4 z4 = {0.f, 0.f, 0.f, 0.f};
-  const int ti = 16 * wave + m;  // this lane's token
-  f32x4 sumQ[KT], sumK[KT];
+  int ti = 16 * tw + m;  // this lane's token
+  bool mine = ti < n;
+  int64_t row_t = c.t0 + (mine ? ti : 0);
+  f32x4 sumQ[GROUPED ? KH : 1], sumK[GROUPED ? KH : 1];
 #pragma unroll
-  for (int t = 0; t < KT; ++t) sumQ[t] = sumK[t] = z4;
-  for (int hg = 0; hg < g.group; ++hg) {
+  for (int t = 0; t < (GROUPED ? KH : 1); ++t) sumQ[t] = sumK[t] = z4;
+  f32x4 accQ[KH], accU[KH], accK[KH];
+  float rk = 1.f, rq = 1.f;
+  for (int hg = 0; hg < (GROUPED ? g.group : 1); ++hg) {
     const int h = hk * g.group + hg;
     const int64_t at = static_cast<int64_t>(slot) * g.HV + h;
+    if constexpr (GROUPED) {  // addresses are formed anew: kept over the heads, they would spill
+      asm volatile("" : "+v"(tid));
+      lane = tid & 63, m = lane & 15, grp = lane >> 4;
+      ti = 16 * tw + m;
+      mine = ti < n;
+      row_t = c.t0 + (mine ? ti : 0);
+    }
     __syncthreads();
     const double G = log_decay(g, a.in.g, c.t0, n, h, lane);
     if (wave == 0) {
@@ -273,89 +290,131 @@ delta_grads_kernel(BwdArgs a) {
       sBeta[lane] = lane < n ? load_beta<T>(g, a.in.beta, c.t0 + lane, h) : 0.f;
     }
     const double Gc = __shfl(G, 63);
-    f32x4 accQ[KT], accU[KT], accK[KT];
 #pragma unroll
-    for (int t = 0; t < KT; ++t) accQ[t] = accU[t] = accK[t] = z4;
+    for (int t = 0; t < KH; ++t) accQ[t] = accU[t] = accK[t] = z4;
     // rows j of a tile, column the lane's token i: D_j . dO_i and D_j . X_i for j <= i, X_j . D_i and dO_j . D_i
     // for j >= i
     f32x4 DO[4], DX[4], XD[4], OD[4];
 #pragma unroll
     for (int jt = 0; jt < 4; ++jt) DO[jt] = DX[jt] = XD[jt] = OD[jt] = z4;
     float xv = 0.f, se = 0.f;
-    const int row = tid >> 2, cc = (tid & 3) * 8;
-    const bool in_row = row < n;
-    const int64_t vat = (c.t0 + (in_row ? row : 0)) * orow + static_cast<int64_t>(h) * g.DV;
-    const float brow = in_row ? load_beta<T>(g, a.in.beta, c.t0 + row, h) : 0.f;
-    const T* vrow = static_cast<const T*>(a.in.v) + (c.t0 + static_cast<int64_t>(in_row ? row : 0)) * g.vs + h * g.vh;
+    const float btok = mine ? load_beta<T>(g, a.in.beta, row_t, h) : 0.f;
+    const T* vrow = static_cast<const T*>(a.in.v) + row_t * g.vs + h * g.vh;
+    T* dvrow = static_cast<T*>(a.b.dv) + row_t * orow + static_cast<int64_t>(h) * g.DV;
+    const T* dorow = static_cast<const T*>(a.b.d_o) + static_cast<int64_t>(c.t0) * orow + static_cast<int64_t>(h) * g.DV;
+    // the next block's operands, on their way while this one's are at work
+    constexpr int kState = (2 * KT * 64 + NT - 1) / NT;  // 16-byte pieces of two column tiles of a state
+    f32x4 rX, rD, rS[kState], rE[kState], rV[2];
+    StageRows<T, 32, NT> rO;
+    StageRows<T, DKP, NT> rK, rQ;
+    const auto load = [&](int kb) {
+      const int64_t ct = at * a.col_tiles + kb / 16;
+      const bool two = kb + 16 < g.DV;  // (the second column tile exists)
+      const int64_t x = (ct + (two ? tid >> 8 : 0)) * (4 * 256) + (tid & 255) * 4;
+      rX = *reinterpret_cast<const f32x4*>(a.b.x + x);
+      rD = *reinterpret_cast<const f32x4*>(a.b.vt + x);
+#pragma unroll
+      for (int i = 0; i < kState; ++i) {
+        const int j = (tid + NT * i) % (2 * KT * 64);
+        const int64_t y = (ct + (two ? j / (64 * KT) : 0)) * (KT * 256) + j % (64 * KT) * 4;
+        rS[i] = *reinterpret_cast<const f32x4*>(a.b.s0 + y);
+        rE[i] = *reinterpret_cast<const f32x4*>(a.b.dend + y);
+      }
+      rO.template load<VEC>(dorow + kb, orow, n, g.DV - kb, tid);
+      if (half == 0)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) rV[i] = load4(vrow, kb + 16 * i + 4 * grp, mine ? g.DV : 0, VEC);
+    };
+    load(0);
     for (int kb = 0; kb < g.DV; kb += 32) {
+      const bool two = kb + 16 < g.DV;
       __syncthreads();
       {
-        const int lim = in_row ? g.DV : 0;
-        float x[8], v[8];
-        load8f(x, a.b.x + vat, kb + cc, lim, vec4);
-        load8f(v, vrow, kb + cc, lim, g.v_vec);
-        sm.r.X.put(row, cc, split8<3>(x));
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          xv = fmaf(x[i], v[i], xv);
-          x[i] *= brow;
-        }
-        store8(static_cast<T*>(a.b.dv) + vat, kb + cc, lim, a.b.o_vec, x);
-        load8f(v, a.b.vt + vat, kb + cc, lim, vec4);
-        sm.r.D.put(row, cc, split8<3>(v));
-        sm.r.O.put(row, cc, load8(static_cast<const T*>(a.b.d_o) + vat, kb + cc, lim, a.b.o_vec));
+        const bool on = tid < 256 || two;
+        const int t = tid >> 6 & 3;
+        sm.r.X.put4(16 * (tid >> 8) + m, 16 * t + 4 * grp, on ? rX : z4);
+        sm.r.D.put4(16 * (tid >> 8) + m, 16 * t + 4 * grp, on ? rD : z4);
       }
 #pragma unroll
-      for (int i = 0; i < DKP / 64 + (DKP < 64); ++i) {
-        const int d = row + 64 * i;
-        if (DKP < 64 && d >= DKP) break;
-        const int lim = d < g.DK ? g.DV : 0;
-        const int64_t sat = at * cells + static_cast<int64_t>(d < g.DK ? d : 0) * g.DV;
-        float s[8], e[8];
-        load8f(s, a.b.s0 + sat, kb + cc, lim, vec4);
-        load8f(e, a.b.dend + sat, kb + cc, lim, vec4);
+      for (int i = 0; i < kState; ++i) {
+        const int j = tid + NT * i, ct = j / (64 * KT), t = j / 64 % KT;
+        if (j < 2 * KT * 64) {
+          const f32x4 s = ct == 0 || two ? rS[i] : z4, e = ct == 0 || two ? rE[i] : z4;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) se = fmaf(s[j], e[j], se);
-        sm.r.S.put(d, cc, split8<3>(s));
-        sm.r.E.put(d, cc, split8<3>(e));
+          for (int r = 0; r < 4; ++r) se = fmaf(s[r], e[r], se);
+          sm.r.S.put4(16 * ct + m, 16 * t + 4 * grp, s);
+          sm.r.E.put4(16 * ct + m, 16 * t + 4 * grp, e);
+        }
+        phase();
+      }
+      rO.put(sm.r.O, n, g.DV - kb, tid);
+      const f32x4 v0 = rV[0], v1 = rV[1];
+      if (kb + 32 < g.DV) {
+        load(kb + 32);
+      } else {
+        rK.template load<VEC>(static_cast<const T*>(a.in.k) + c.t0 * g.ks + hk * g.kh, g.ks, n, g.DK, tid);
+        rQ.template load<VEC>(static_cast<const T*>(a.in.q) + c.t0 * g.qs + hk * g.qh, g.qs, n, g.DK, tid);
       }
       __syncthreads();
-      const int k0 = 8 * grp;
-      const Frag<3> bX = sm.r.X.rows_plain(ti, k0), bD = sm.r.D.rows_plain(ti, k0);
-      const Frag<P> bO = sm.r.O.rows_plain(ti, k0);
+      const int k0 = 4 * grp;
+      const Frag<3> bX = sm.r.X.cols(16 * tw, k0, m), bD = sm.r.D.cols(16 * tw, k0, m);
+      const Frag<P> bO = sm.r.O.rows(ti, 0, grp);
+      if (half == 0) {  // dv, and X . v
+        f32x4 x0 = z4, x1 = z4;
+#pragma unroll
+        for (int p = 2; p >= 0; --p) {
+          x0 += f32x4{__uint_as_float(bX.p[p].x << 16), __uint_as_float(bX.p[p].x & 0xffff0000u),
+                      __uint_as_float(bX.p[p].y << 16), __uint_as_float(bX.p[p].y & 0xffff0000u)};
+          x1 += f32x4{__uint_as_float(bX.p[p].z << 16), __uint_as_float(bX.p[p].z & 0xffff0000u),
+                      __uint_as_float(bX.p[p].w << 16), __uint_as_float(bX.p[p].w & 0xffff0000u)};
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) xv = fmaf(x0[r], v0[r], fmaf(x1[r], v1[r], xv));
+        if (mine) {
+          Quad<T> q;
+          q.set(x0 * btok);
+          q.store(dvrow, kb + 4 * grp, g.DV, VEC);
+          q.set(x1 * btok);
+          q.store(dvrow, kb + 16 + 4 * grp, g.DV, VEC);
+        }
+      }
+      phase();
 #pragma unroll
       for (int jt = 0; jt < 4; ++jt) {
-        if (jt <= wave) {
-          const Frag<3> f = sm.r.D.rows_plain(16 * jt + m, k0);
+        if (jt <= tw) {
+          const Frag<3> f = sm.r.D.cols(16 * jt, k0, m);
           DO[jt] = mma<3>(f, bO, DO[jt]);
           DX[jt] = mma<3>(f, bX, DX[jt]);
         }
-        if (jt >= wave) {
-          XD[jt] = mma<3>(sm.r.X.rows_plain(16 * jt + m, k0), bD, XD[jt]);
-          OD[jt] = mma<3>(sm.r.O.rows_plain(16 * jt + m, k0), bD, OD[jt]);
+        if (jt >= tw) {
+          XD[jt] = mma<3>(sm.r.X.cols(16 * jt, k0, m), bD, XD[jt]);
+          OD[jt] = mma<3>(sm.r.O.rows(16 * jt + m, 0, grp), bD, OD[jt]);
         }
+        phase();
       }
+      phase();
+      constexpr int TG = KH < 2 ? KH : 2;
 #pragma unroll
-      for (int t = 0; t < KT; ++t) {
-        const Frag<3> f = sm.r.S.rows_plain(16 * t + m, k0);
-        accQ[t] = mma<3>(f, bO, accQ[t]);
-        accU[t] = mma<3>(f, bX, accU[t]);
-        accK[t] = mma<3>(sm.r.E.rows_plain(16 * t + m, k0), bD, accK[t]);
+      for (int t = 0; t < KH; t += TG) {
+        Frag<3> f[TG], e[TG];
+#pragma unroll
+        for (int i = 0; i < TG; ++i) {
+          f[i] = sm.r.S.cols(d0 + 16 * (t + i), k0, m);
+          e[i] = sm.r.E.cols(d0 + 16 * (t + i), k0, m);
+        }
+        mma_n<3>(f, bO, accQ + t);
+        mma_n<3>(f, bX, accU + t);
+        mma_n<3>(e, bD, accK + t);
+        phase();
       }
     }
-    xv += __shfl_xor(xv, 1);
-    xv += __shfl_xor(xv, 2);
-    if ((tid & 3) == 0) sXv[row] = xv;
+    xv = sum_g(xv);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) se += __shfl_xor(se, o);
     __syncthreads();
-    {
-      StageRows<T, DKP, 256> rK, rQ;
-      rK.template load<VEC>(static_cast<const T*>(a.in.k) + c.t0 * g.ks + hk * g.kh, g.ks, n, g.DK, tid);
-      rQ.template load<VEC>(static_cast<const T*>(a.in.q) + c.t0 * g.qs + hk * g.qh, g.qs, n, g.DK, tid);
-      rK.put(sm.k.K, n, g.DK, tid);
-      rQ.put(sm.k.Q, n, g.DK, tid);
-    }
+    rK.put(sm.k.K, n, g.DK, tid);
+    rQ.put(sm.k.Q, n, g.DK, tid);
+    if (lane == 0) sSe[wave] = se;
     __syncthreads();
     {
       float nk = 0.f, nq = 0.f;
@@ -364,26 +423,30 @@ delta_grads_kernel(BwdArgs a) {
         const f32x4 x = sm.k.K.get4(ti, 16 * t + 4 * grp), y = sm.k.Q.get4(ti, 16 * t + 4 * grp);
 #pragma unroll
         for (int r = 0; r < 4; ++r) nk = fmaf(x[r], x[r], nk), nq = fmaf(y[r], y[r], nq);
+        phase();
       }
       nk = sum_g(nk);
       nq = sum_g(nq);
-      if (grp == 0) {
-        sRk[ti] = g.l2 ? 1.f / sqrtf(nk + kL2Eps) : 1.f;
-        sRq[ti] = g.l2 ? 1.f / sqrtf(nq + kL2Eps) : 1.f;
+      rk = g.l2 ? 1.f / sqrtf(nk + kL2Eps) : 1.f;
+      rq = g.l2 ? 1.f / sqrtf(nq + kL2Eps) : 1.f;
+      if (grp == 0 && half == 0) {
+        sRk[ti] = rk;
+        sRq[ti] = rq;
       }
     }
     __syncthreads();
     const double Gi = sG[ti];
-    const float eG = exp_diff(Gi), eR = exp_diff(Gc - Gi), bi = sBeta[ti], rk = sRk[ti], rq = sRq[ti];
+    const float eG = exp_diff(Gi), eR = exp_diff(Gc - Gi), bi = sBeta[ti];
     float kh = 0.f;
 #pragma unroll
-    for (int t = 0; t < KT; ++t) {
+    for (int t = 0; t < KH; ++t) {
       accQ[t] *= g.scale * eG;
       accU[t] *= -eG;
       accK[t] *= eR;
-      const f32x4 x = sm.k.K.get4(ti, 16 * t + 4 * grp);
+      const f32x4 x = sm.k.K.get4(ti, d0 + 16 * t + 4 * grp);
 #pragma unroll
       for (int r = 0; r < 4; ++r) kh = fmaf(accK[t][r], x[r], kh);
+      phase();
     }
 #pragma unroll
     for (int jt = 0; jt < 4; ++jt)
@@ -396,32 +459,36 @@ delta_grads_kernel(BwdArgs a) {
         DX[jt][r] *= j < ti ? -sRk[j] * lo : 0.f;
         XD[jt][r] *= j > ti ? -sBeta[j] * sRk[j] * hi : 0.f;
         OD[jt][r] *= j >= ti ? g.scale * sRq[j] * hi : 0.f;
+        if (r % 2) phase();
       }
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       const int j0 = 32 * ks + 4 * grp;
-      if (2 * ks <= wave) {
+      if (2 * ks <= tw) {
         const Frag<3> f1 = split_tiles<3>(DO[2 * ks], DO[2 * ks + 1]), f2 = split_tiles<3>(DX[2 * ks], DX[2 * ks + 1]);
+        Frag<P> k[KH];
 #pragma unroll
-        for (int t = 0; t < KT; ++t) {
-          const Frag<P> k = sm.k.K.cols(16 * t, j0, m);
-          accQ[t] = mma<3>(k, f1, accQ[t]);
-          accU[t] = mma<3>(k, f2, accU[t]);
-        }
+        for (int t = 0; t < KH; ++t) k[t] = sm.k.K.cols(d0 + 16 * t, j0, m);
+        mma_n<3>(k, f1, accQ);
+        mma_n<3>(k, f2, accU);
       }
-      if (2 * ks + 1 >= wave) {
+      phase();
+      if (2 * ks + 1 >= tw) {
         const Frag<3> f1 = split_tiles<3>(XD[2 * ks], XD[2 * ks + 1]), f2 = split_tiles<3>(OD[2 * ks], OD[2 * ks + 1]);
+        Frag<P> k[KH];
 #pragma unroll
-        for (int t = 0; t < KT; ++t) {
-          accK[t] = mma<3>(sm.k.K.cols(16 * t, j0, m), f1, accK[t]);
-          accK[t] = mma<3>(sm.k.Q.cols(16 * t, j0, m), f2, accK[t]);
-        }
+        for (int t = 0; t < KH; ++t) k[t] = sm.k.K.cols(d0 + 16 * t, j0, m);
+        mma_n<3>(k, f1, accK);
+#pragma unroll
+        for (int t = 0; t < KH; ++t) k[t] = sm.k.Q.cols(d0 + 16 * t, j0, m);
+        mma_n<3>(k, f2, accK);
       }
+      phase();
     }
     float ku = 0.f, qd = 0.f, kd = 0.f;
 #pragma unroll
-    for (int t = 0; t < KT; ++t) {
-      const f32x4 x = sm.k.K.get4(ti, 16 * t + 4 * grp), y = sm.k.Q.get4(ti, 16 * t + 4 * grp);
+    for (int t = 0; t < KH; ++t) {
+      const f32x4 x = sm.k.K.get4(ti, d0 + 16 * t + 4 * grp), y = sm.k.Q.get4(ti, d0 + 16 * t + 4 * grp);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         ku = fmaf(accU[t][r], x[r], ku);
@@ -429,72 +496,86 @@ delta_grads_kernel(BwdArgs a) {
         kd = fmaf(accK[t][r], x[r], kd);
         qd = fmaf(accQ[t][r], y[r], qd);
       }
-      sumQ[t] += accQ[t];
-      sumK[t] += accK[t];
+      if constexpr (GROUPED) {
+        sumQ[t] += accQ[t];
+        sumK[t] += accK[t];
+      }
+      phase();
     }
     ku = sum_g(ku) * rk;
     kd = sum_g(kd) * rk;
     qd = sum_g(qd) * rq;
     kh = sum_g(kh) * rk;
-    if (grp == 0) {
-      sDG[ti] = static_cast<double>(qd) - kd + 2.f * bi * ku;
-      if (ti < n) {
-        const float db = sXv[ti] + ku;
-        const int64_t i = (c.t0 + static_cast<int64_t>(ti)) * g.HV + h;
-        if (g.beta_f32)
-          static_cast<float*>(a.b.dbeta)[i] = db;
-        else
-          static_cast<T*>(a.b.dbeta)[i] = from_f32<T>(db);
-      }
-    }
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) kh += __shfl_xor(kh, o);
-    if (lane == 0) {
-      sSum[wave][0] = se;
-      sSum[wave][1] = kh;
-    }
+    if (grp == 0) sDot[half][ti] = make_float4(ku, kd, qd, kh);
     __syncthreads();
-    if (wave == 0) {
-      double s = sDG[63 - lane];
+    if (wave == 0) {  // lane = token, the last one first
+      const int t = 63 - lane;
+      const float4 x = sDot[0][t], y = sDot[1][t];
+      double s = static_cast<double>(x.z + y.z) - (x.y + y.y) + 2.f * sBeta[t] * (x.x + y.x), all = x.w + y.w;
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
         const double v = __shfl_up(s, o);
         if (lane >= o) s += v;
       }
-      const double all = static_cast<double>(exp_diff(Gc)) * ((sSum[0][0] + sSum[1][0]) + (sSum[2][0] + sSum[3][0])) +
-                         ((sSum[0][1] + sSum[1][1]) + (sSum[2][1] + sSum[3][1]));
-      if (63 - lane < n) a.b.dg[(c.t0 + 63 - lane) * static_cast<int64_t>(g.HV) + h] = static_cast<float>(s + all);
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) all += __shfl_xor(all, o);
+      double sums = 0.0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sums += sSe[i];
+      all += static_cast<double>(exp_diff(Gc)) * sums;
+      if (t < n) a.b.dg[(c.t0 + static_cast<int64_t>(t)) * g.HV + h] = static_cast<float>(s + all);
+    }
+    if (half == 0 && grp == 0 && mine) {
+      const float db = xv + ku + sDot[1][ti].x;
+      const int64_t i = row_t * g.HV + h;
+      if (g.beta_f32)
+        static_cast<float*>(a.b.dbeta)[i] = db;
+      else
+        static_cast<T*>(a.b.dbeta)[i] = from_f32<T>(db);
     }
   }
   // (the keys of the last head are still in LDS)
+  const auto gq = [&](int t) -> const f32x4& {
+    if constexpr (GROUPED) return sumQ[t];
+    else return accQ[t];
+  };
+  const auto gk = [&](int t) -> const f32x4& {
+    if constexpr (GROUPED) return sumK[t];
+    else return accK[t];
+  };
   float qd = 0.f, kd = 0.f;
-  const float rk = sRk[ti], rq = sRq[ti];
   if (g.l2) {
+    if constexpr (GROUPED) {
 #pragma unroll
-    for (int t = 0; t < KT; ++t) {
-      const f32x4 x = sm.k.K.get4(ti, 16 * t + 4 * grp), y = sm.k.Q.get4(ti, 16 * t + 4 * grp);
+      for (int t = 0; t < KH; ++t) {
+        const f32x4 x = sm.k.K.get4(ti, d0 + 16 * t + 4 * grp), y = sm.k.Q.get4(ti, d0 + 16 * t + 4 * grp);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        kd = fmaf(sumK[t][r], x[r], kd);
-        qd = fmaf(sumQ[t][r], y[r], qd);
+        for (int r = 0; r < 4; ++r) {
+          kd = fmaf(gk(t)[r], x[r], kd);
+          qd = fmaf(gq(t)[r], y[r], qd);
+        }
       }
+      kd = sum_g(kd) * rk;
+      qd = sum_g(qd) * rq;
+      __syncthreads();
+      if (grp == 0) sDot[half][ti] = make_float4(0.f, kd, qd, 0.f);
+      __syncthreads();
     }
-    kd = sum_g(kd) * rk * rk;
-    qd = sum_g(qd) * rq * rq;
+    const float4 x = sDot[0][ti], y = sDot[1][ti];
+    kd = (x.y + y.y) * rk;
+    qd = (x.z + y.z) * rq;
   }
-  if (ti >= n) return;
-  const int64_t out = ((c.t0 + static_cast<int64_t>(ti)) * g.HK + hk) * g.DK;
+  if (!mine) return;
+  const int64_t out = (row_t * g.HK + hk) * g.DK;
 #pragma unroll
-  for (int t = 0; t < KT; ++t) {
-    const f32x4 x = sm.k.K.get4(ti, 16 * t + 4 * grp), y = sm.k.Q.get4(ti, 16 * t + 4 * grp);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int d = 16 * t + 4 * grp + r;
-      if (d < g.DK) {
-        static_cast<T*>(a.b.dk)[out + d] = from_f32<T>(rk * fmaf(-kd, x[r], sumK[t][r]));
-        static_cast<T*>(a.b.dq)[out + d] = from_f32<T>(rq * fmaf(-qd, y[r], sumQ[t][r]));
-      }
-    }
+  for (int t = 0; t < KH; ++t) {
+    const int d = d0 + 16 * t + 4 * grp;
+    const f32x4 x = sm.k.K.get4(ti, d), y = sm.k.Q.get4(ti, d);
+    Quad<T> q;
+    q.set((gk(t) - x * kd) * rk);
+    q.store(static_cast<T*>(a.b.dk) + out, d, g.DK, VEC);
+    q.set((gq(t) - y * qd) * rq);
+    q.store(static_cast<T*>(a.b.dq) + out, d, g.DK, VEC);
   }
 }
 
@@ -503,9 +584,9 @@ delta_grads_kernel(BwdArgs a) {
 hipError_t launch_delta_bwd(const DeltaGeom& g, const DeltaIn& in, const DeltaWork& w, const DeltaBwd& b, int dtype,
                             hipStream_t s) {
   // (rows that are read value by value: more registers, so four waves)
-  const int nw = g.qk_vec ? delta_waves(g.DV) : 4;
+  const int nw = g.vec ? delta_waves(g.DV) : 4;
   const uint32_t vcb = delta_col_blocks(g.DV, nw);
-  BwdArgs a{g, in, w, b, vcb, vcb, static_cast<uint32_t>(chunk_slots(g.q, g.part))};
+  BwdArgs a{g, in, w, b, delta_col_tiles(g), vcb, vcb, static_cast<uint32_t>(chunk_slots(g.q, g.part))};
   hipError_t e = launch_delta_prep(g, in, w, true, dtype, s);
   if (e != hipSuccess) return e;
   const auto run = [&](auto t, auto dkp, auto waves, auto vec) {
@@ -524,13 +605,16 @@ hipError_t launch_delta_bwd(const DeltaGeom& g, const DeltaIn& in, const DeltaWo
                        dim3(static_cast<unsigned>(delta_blocks(a.ncb, a.nslots, g.HV))), dim3(64 * NW), 0, s, a);
     e = hipGetLastError();
     if (e != hipSuccess || g.q.T == 0) return e;
-    hipLaunchKernelGGL((delta_grads_kernel<T, DKP, VEC>), dim3(static_cast<unsigned>(chunk_slots(g.q, g.cut) * g.HK)),
-                       dim3(256), 0, s, a);
+    const dim3 grid(static_cast<unsigned>(chunk_slots(g.q, g.cut) * g.HK));
+    if (g.group > 1)
+      hipLaunchKernelGGL((delta_grads_kernel<T, DKP, VEC, true>), grid, dim3(512), 0, s, a);
+    else
+      hipLaunchKernelGGL((delta_grads_kernel<T, DKP, VEC, false>), grid, dim3(512), 0, s, a);
     return hipGetLastError();
   };
   return delta_dispatch(dtype, g.DK, [&](auto t, auto dkp) {
     using Four = std::integral_constant<int, 4>;
-    if (!g.qk_vec) return run(t, dkp, Four{}, std::false_type{});
+    if (!g.vec) return run(t, dkp, Four{}, std::false_type{});
     return nw == 8 ? run(t, dkp, std::integral_constant<int, 8>{}, std::true_type{}) : run(t, dkp, Four{}, std::true_type{});
   });
 }

@@ -1,6 +1,7 @@
 // C ABI of the gated delta rule (include/mvm_delta.h): validation, the split of
 // the time axis, and of the caller's workspace.
 #include <algorithm>
+#include <initializer_list>
 
 #include "delta_kernels.h"
 #include "mvm_delta.h"
@@ -89,14 +90,16 @@ mvm::DeltaGeom geom(const mvm_delta_desc* d) {
   return g;
 }
 
-// Which rows can be read 16 bytes at a time.
-void set_vec(mvm::DeltaGeom& g, const mvm::DeltaIn& in, int dtype) {
+// Which rows are accessed 16 bytes at a time.
+bool fits(const void* p, int64_t row, int64_t head) {
+  return ((static_cast<int64_t>(reinterpret_cast<uintptr_t>(p)) | row | head) & 15) == 0;
+}
+bool wide(const mvm::DeltaGeom& g, const mvm::DeltaIn& in, int dtype, std::initializer_list<const void*> outs) {
   const int64_t e = dtype == MVM_F32 ? 4 : 2;
-  const auto fits = [&](const void* p, int64_t s, int64_t h) {
-    return ((static_cast<int64_t>(reinterpret_cast<uintptr_t>(p)) | s * e | h * e) & 15) == 0;
-  };
-  g.qk_vec = g.DK * e % 16 == 0 && fits(in.q, g.qs, g.qh) && fits(in.k, g.ks, g.kh);
-  g.v_vec = fits(in.v, g.vs, g.vh);
+  bool ok = g.DK * e % 16 == 0 && fits(in.q, g.qs * e, g.qh * e) && fits(in.k, g.ks * e, g.kh * e) &&
+            fits(in.v, g.vs * e, g.vh * e);
+  for (const void* p : outs) ok = ok && fits(p, g.DV * e, 0);
+  return ok;
 }
 
 int check_delta(const mvm_delta_desc* d) {
@@ -141,9 +144,8 @@ struct Ckpt {
   int64_t s0, vt;
 };
 Ckpt ckpt_of(const mvm::DeltaGeom& g) {
-  const int64_t cells = static_cast<int64_t>(g.HV) * g.DK * g.DV;
-  // (the rows start on 16 bytes)
-  return {(mvm::chunk_slots(g.q, g.cut) * cells + 3) / 4 * 4, static_cast<int64_t>(g.q.T) * g.HV * g.DV};
+  const int64_t tiles = mvm::chunk_slots(g.q, g.cut) * g.HV * mvm::delta_col_tiles(g) * 256;
+  return {tiles * (mvm::delta_dkp(g.DK) / 16), tiles * 4};
 }
 
 struct Ws {
@@ -161,8 +163,9 @@ Ws ws_of(const mvm::DeltaGeom& g, bool backward) {
     w.carry = align_up(parts * g.DK * g.DV * 4);
   }
   if (backward) {
-    w.x = align_up(static_cast<size_t>(g.q.T) * g.HV * g.DV * 4);
-    w.dend = align_up(items * g.DK * g.DV * 4);
+    const Ckpt c = ckpt_of(g);
+    w.x = align_up(static_cast<size_t>(c.vt) * 4);
+    w.dend = align_up(static_cast<size_t>(c.s0) * 4);
   }
   w.total = w.tri + w.dec + w.gam + w.trans + w.carry + w.x + w.dend;
   return w;
@@ -227,7 +230,7 @@ int mvm_delta_fwd(const mvm_delta_desc* desc, const void* q, const void* k, cons
   if ((rc = check_ckpt("mvm_delta_fwd", ckpt)) != MVM_OK) return rc;
   const Ws w = ws_of(gm, false);
   if ((rc = check_ws("mvm_delta_fwd", workspace, workspace_bytes, w.total)) != MVM_OK) return rc;
-  set_vec(gm, in, desc->dtype);
+  gm.vec = wide(gm, in, desc->dtype, {o});
   Take take{static_cast<char*>(workspace)};
   mvm::DeltaWork b{};
   b.tri = take(w.tri);
@@ -255,7 +258,7 @@ int mvm_delta_bwd(const mvm_delta_desc* desc, const void* q, const void* k, cons
   if ((rc = check_ckpt("mvm_delta_bwd", ckpt)) != MVM_OK) return rc;
   const Ws w = ws_of(gm, true);
   if ((rc = check_ws("mvm_delta_bwd", workspace, workspace_bytes, w.total)) != MVM_OK) return rc;
-  set_vec(gm, in, desc->dtype);
+  gm.vec = wide(gm, in, desc->dtype, {d_o, dv}) && fits(dq, 0, 0) && fits(dk, 0, 0);
   Take take{static_cast<char*>(workspace)};
   mvm::DeltaWork b{};
   b.tri = take(w.tri);
@@ -269,8 +272,6 @@ int mvm_delta_bwd(const mvm_delta_desc* desc, const void* q, const void* k, cons
   r.d_o = d_o; r.dh1 = dh1; r.dh0 = dh0;
   r.x = take(w.x);
   r.dend = take(w.dend);
-  r.o_vec = ((static_cast<uintptr_t>(gm.DV) * (desc->dtype == MVM_F32 ? 4 : 2) | reinterpret_cast<uintptr_t>(d_o) |
-              reinterpret_cast<uintptr_t>(dv)) & 15) == 0;
   r.dq = dq; r.dk = dk; r.dv = dv; r.dg = dg; r.dbeta = dbeta;
   return hip_status(mvm::launch_delta_bwd(gm, in, b, r, desc->dtype, static_cast<hipStream_t>(stream)),
                     "mvm_delta_bwd launch");

@@ -31,6 +31,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
@@ -91,6 +92,36 @@ __device__ __forceinline__ f32x4 mma(const Frag<PA>& a, const Frag<PB>& b, f32x4
   return c;
 }
 
+// The same for N tiles with operands of their own and one B: the products of one part after the other, so that
+// neighbours in the instruction stream do not wait for each other's sums
+template <int ORD, int PA, int PB, int N>
+__device__ __forceinline__ void mma_n(const Frag<PA> (&a)[N], const Frag<PB>& b, f32x4* c) {
+#pragma unroll
+  for (int o = ORD - 1; o >= 0; --o)
+#pragma unroll
+    for (int i = 0; i < PA; ++i)
+      if (o - i >= 0 && o - i < PB)
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+          c[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a[n].p[i]),
+                                                         __builtin_bit_cast(bf16x8, b.p[o - i]), c[n], 0, 0, 0);
+}
+
+// The same for one A and B operands of their own: a result tile's operand of the chain is, as it is, the A operand
+// of its transpose
+template <int ORD, int PA, int PB, int N>
+__device__ __forceinline__ void mma_t(const Frag<PA>& a, const Frag<PB> (&b)[N], f32x4* c) {
+#pragma unroll
+  for (int o = ORD - 1; o >= 0; --o)
+#pragma unroll
+    for (int i = 0; i < PA; ++i)
+      if (o - i >= 0 && o - i < PB)
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+          c[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a.p[i]),
+                                                         __builtin_bit_cast(bf16x8, b[n].p[o - i]), c[n], 0, 0, 0);
+}
+
 // A tile of ROWS rows of COLS values in LDS, one plane for each part.  Rows lie 16 values past a multiple of 64
 // banks apart or an odd multiple of 16 values, and in every other eight of them the 16-byte words of a pair trade
 // places: then neither 16 lanes' rows, nor the 8 rows by 16 columns of a transposing read, share a bank.
@@ -102,10 +133,11 @@ struct Tile {
 
   __device__ __forceinline__ static int at(int row, int col) { return row * LD + (col ^ (row & 8)); }
 
-  // row `row`, summed index k0 .. k0 + 31 in the chained order (k0 includes 4g)
-  __device__ __forceinline__ Frag<P> rows(int row, int k0) const {
+  // (columns c0, a multiple of 16, and offsets below it apart: an address register and constants)
+  // row `row`, summed index 32 ks .. 32 ks + 31 in the chained order
+  __device__ __forceinline__ Frag<P> rows(int row, int ks, int grp) const {
     Frag<P> f;
-    const uint16_t* at0 = v + at(row, k0);
+    const uint16_t* at0 = v + row * LD + ((4 * grp) ^ (row & 8)) + 32 * ks;
 #pragma unroll
     for (int p = 0; p < P; ++p) {
       const uint2 a = *reinterpret_cast<const uint2*>(at0 + p * kPlane);
@@ -126,7 +158,8 @@ struct Tile {
   // i / 4, i / 4 + 4, + 8, + 12.
   __device__ __forceinline__ Frag<P> cols(int c0, int r0, int m) const {
     Frag<P> f;
-    const uint16_t* at0 = v + at(r0 + (m >> 2), c0 + 4 * (m & 3));
+    const int row = r0 + (m >> 2);
+    const uint16_t* at0 = v + row * LD + ((4 * (m & 3)) ^ (row & 8)) + c0;
 #pragma unroll
     for (int p = 0; p < P; ++p) {
       const uint16_t* x = at0 + p * kPlane;
@@ -135,6 +168,28 @@ struct Tile {
       f.p[p] = make_uint4(a.x, a.y, b.x, b.y);
     }
     return f;
+  }
+  // rows r0 .. r0 + 3 of column c0 + m (r0 includes 4g), as a result tile holds them
+  __device__ __forceinline__ f32x4 col4(int c0, int r0, int m) const {
+    static_assert(P == 1, "one part");
+    const int row = r0 + (m >> 2);
+    const uint16_t* at0 = v + row * LD + ((4 * (m & 3)) ^ (row & 8)) + c0;
+    const uint2 a = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at0));
+    return {__uint_as_float(a.x << 16), __uint_as_float(a.x & 0xffff0000u), __uint_as_float(a.y << 16),
+            __uint_as_float(a.y & 0xffff0000u)};
+  }
+  // four values of a row
+  __device__ __forceinline__ void put4(int row, int col, const f32x4& x) {
+    float a = x[0], b = x[1], c = x[2], d = x[3];
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const uint2 w = make_uint2(pack_bf16(a, b), pack_bf16(c, d));
+      *reinterpret_cast<uint2*>(v + p * kPlane + at(row, col)) = w;
+      a -= __uint_as_float(w.x << 16);
+      b -= __uint_as_float(w.x & 0xffff0000u);
+      c -= __uint_as_float(w.y << 16);
+      d -= __uint_as_float(w.y & 0xffff0000u);
+    }
   }
   __device__ __forceinline__ void put(int row, int col, const Frag<P>& f) {
 #pragma unroll
@@ -179,24 +234,6 @@ __device__ __forceinline__ void load8f(float (&v)[8], const T* p, int c, int n, 
 template <int P>
 __device__ __forceinline__ Frag<P> split8(const float (&v)[8]) {
   return split8<P>(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]);
-}
-template <typename T>
-__device__ __forceinline__ void store8(T* p, int c, int n, bool vec, const float (&v)[8]) {
-  if (vec && c + 8 <= n) {
-    Pack<T, 8> x;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x.v[i] = from_f32<T>(v[i]);
-    if constexpr (std::is_same_v<T, float>) {
-      reinterpret_cast<float4*>(p + c)[0] = make_float4(v[0], v[1], v[2], v[3]);
-      reinterpret_cast<float4*>(p + c)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-      *reinterpret_cast<Pack<T, 8>*>(p + c) = x;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (c + i < n) p[c + i] = from_f32<T>(v[i]);
-  }
 }
 // the same as the parts of an operand: bfloat16 as it is
 template <typename T>
@@ -329,25 +366,61 @@ struct Cols {
     return v;
   }
 };
+// Four values of a row in their type
 template <typename T>
-__device__ __forceinline__ void store_cols(T* at, int64_t stride, const f32x4 (&v)[4], int m, int grp, int n, bool live) {
-  if (!live) return;
-  const uint32_t off = lane_offset<T>(stride, m, grp);
-  if (n == kC) {
+struct Quad {
+  uint32_t w[sizeof(T)];
+  __device__ __forceinline__ void set(const f32x4& v) {
+    if constexpr (std::is_same_v<T, float>) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      *reinterpret_cast<T*>(reinterpret_cast<char*>(at) + off) = from_f32<T>(v[i >> 2][i & 3]);
-      at += (i & 3) == 3 ? 13 * stride : stride;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int u = 16 * (i >> 2) + (i & 3);
-      if (u + 4 * grp < n)
-        *reinterpret_cast<T*>(reinterpret_cast<char*>(at + u * stride) + off) = from_f32<T>(v[i >> 2][i & 3]);
+      for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(v[i]);
+    } else {
+      w[0] = pack_bf16(v[0], v[1]);
+      w[1] = pack_bf16(v[2], v[3]);
     }
   }
+  // values c .. c + 3 of a row of n
+  __device__ __forceinline__ void store(T* p, int c, int n, bool vec) const {
+    if (vec) {  // (n is a multiple of 4)
+      if (c < n) {
+        if constexpr (std::is_same_v<T, float>)
+          *reinterpret_cast<u32x4*>(p + c) = u32x4{w[0], w[1], w[2], w[3]};
+        else
+          *reinterpret_cast<u32x2*>(p + c) = u32x2{w[0], w[1]};
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c + i < n) {
+          if constexpr (std::is_same_v<T, float>)
+            p[c + i] = __uint_as_float(w[i]);
+          else
+            p[c + i] = T{static_cast<uint16_t>(i & 1 ? w[i / 2] >> 16 : w[i / 2])};
+        }
+    }
+  }
+};
+template <typename T>
+__device__ __forceinline__ f32x4 load4(const T* p, int c, int n, bool vec) {
+  f32x4 v;
+  if (vec) {
+    const T* at = p + (c < n ? c : 0);
+    if constexpr (std::is_same_v<T, float>) {
+      v = *reinterpret_cast<const f32x4*>(at);
+    } else {
+      const u32x2 a = *reinterpret_cast<const u32x2*>(at);
+      v = {__uint_as_float(a[0] << 16), __uint_as_float(a[0] & 0xffff0000u), __uint_as_float(a[1] << 16),
+           __uint_as_float(a[1] & 0xffff0000u)};
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = c < n ? v[i] : 0.f;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = c + i < n ? to_f32(p[c + i]) : 0.f;
+  }
+  return v;
 }
+
 // The rows dk of a state's 16 columns: `at` is the wave's first column of row 0.  Rows are `ld` values apart.
 template <int KT>
 __device__ __forceinline__ void load_state(f32x4 (&S)[KT], const float* at, int ld, int rows, int m, int grp, bool live) {
@@ -386,6 +459,13 @@ constexpr int tri_frag(int rt, int ks) {
   return rt < 2 ? (ks == 0 ? rt : -1) : 2 * rt - 2 + ks;
 }
 
+// Result tiles in memory as the lanes hold them, 16 bytes a lane: N tiles of one column block
+template <int N>
+__device__ __forceinline__ void store_tiles(float* at, const f32x4 (&v)[N], int lane) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) reinterpret_cast<f32x4*>(at)[64 * i + lane] = v[i];
+}
+
 // A chunk's two triangles on their way into LDS: three parts of the first, PP of the second
 template <int PP, int NT>
 struct StageTri {
@@ -402,14 +482,14 @@ struct StageTri {
       if (NT * (i + 1) <= kCount || tid + NT * i < kCount) reinterpret_cast<u32x4*>(lds)[tid + NT * i] = r[i];
   }
 };
-template <int P>
-__device__ __forceinline__ Frag<P> tri_at(const uint4* lds, int which, int f, int lane) {
-  Frag<P> x;
+// the fragments of row tiles RT0 .. RT0 + N - 1, columns 32 ks .. 32 ks + 31
+template <bool BWD, int RT0, int N, int P>
+__device__ __forceinline__ void tri_tiles(Frag<P> (&f)[N], const uint4* lds, int which, int ks, int lane) {
 #pragma unroll
-  for (int q = 0; q < P; ++q) x.p[q] = lds[tri_index(which, q, f) + lane];
-  return x;
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int q = 0; q < P; ++q) f[i].p[q] = lds[tri_index(which, q, tri_frag<BWD>(RT0 + i, ks)) + lane];
 }
-
 // Sum over the 4 lane groups of the lanes with the same m
 __device__ __forceinline__ float sum_g(float x) {
   x += __shfl_xor(x, 16);

@@ -1,7 +1,8 @@
 // The gated delta rule along time, by chunks of 64 tokens:
 //   R  = diag(beta) (V - diag(e^G) K S)
 //   D  = T R                                   (rows d_t)
-//   O  = scale diag(e^G) Q S + P D
+//   O  = scale diag(e^G) Q S + P D             (formed as O', whose lanes hold
+//                                               four columns of a token)
 //   S' = e^Gc S + K' diag(e^(Gc - G)) D        (Gc: G of the last token)
 // (with T and P of delta_prep.hip).  The columns of S are independent: a wave
 // keeps 16 of them in registers, as result tiles whose rows are the keys'
@@ -26,6 +27,7 @@ struct FwdArgs {
   void* o;
   float* s0;
   float* vt;
+  int64_t col_tiles;
   uint32_t vcb, ncb, nslots;  // column blocks of the values, and of the launch
 };
 
@@ -39,6 +41,9 @@ delta_fwd_kernel(FwdArgs a) {
   constexpr int PP = AGG ? 0 : ORD;
   __shared__ __attribute__((aligned(16))) Tile<kC, DKP, P> sK;
   __shared__ __attribute__((aligned(16))) Tile<AGG ? 1 : kC, DKP, P> sQ;
+  // float32 values go straight to the registers: with them the tiles would not fit
+  constexpr bool VLDS = P == 1;
+  __shared__ __attribute__((aligned(16))) Tile<VLDS ? kC : 1, 16 * NW, 1> sV;
   __shared__ uint4 sTri[StageTri<PP, NT>::kCount];
   __shared__ __attribute__((aligned(16))) float sDec[4][kC];
   const DeltaGeom& g = a.g;
@@ -54,10 +59,10 @@ delta_fwd_kernel(FwdArgs a) {
   if (part.t0 < 0) return;
   if (AGG && (part.seq >= g.q.S || part.t1 == part.end)) return;  // (nothing follows a last part)
   const int64_t orow = static_cast<int64_t>(g.HV) * g.DV, ocol = static_cast<int64_t>(h) * g.DV + at_col;
-  T* o = static_cast<T*>(a.o) + ocol;
+  const bool wlive = live && !trans;
   if (part.seq >= g.q.S) {  // rows of no sequence
     if (live)
-      for (int32_t t = part.t0 + grp; t < part.t1; t += 4) o[t * orow + m] = from_f32<T>(0.f);
+      for (int32_t t = part.t0 + grp; t < part.t1; t += 4) static_cast<T*>(a.o)[t * orow + ocol + m] = from_f32<T>(0.f);
     return;
   }
   const int32_t row = seq_slot(g.q, part.seq);
@@ -79,8 +84,8 @@ delta_fwd_kernel(FwdArgs a) {
   }
   const T* kp = static_cast<const T*>(a.in.k) + hk * g.kh;
   const T* qp = static_cast<const T*>(a.in.q) + hk * g.qh;
-  const T* vp = static_cast<const T*>(a.in.v) + h * g.vh + at_col;
-  const bool vlive = live && !trans;
+  const int vcol0 = trans ? 0 : p.cb * NW * 16;  // the workgroup's columns of v
+  const T* vp = static_cast<const T*>(a.in.v) + h * g.vh + (VLDS ? vcol0 : at_col);
   const int32_t slot0 = cut_div(g.cut, part.start) + part.seq + (part.t0 - part.start) / kC;
   const int32_t chunks = (part.t1 - part.t0 + kC - 1) / kC;
   // the next chunk's operands, on their way while this one's are at work
@@ -89,6 +94,7 @@ delta_fwd_kernel(FwdArgs a) {
   float rDec;
   float rGam;
   Cols<T> rV;
+  StageRows<T, 16 * NW, NT> rVt;
   const auto load = [&](int32_t i) {
     const int32_t t0 = part.t0 + i * kC;
     const int n = part.t1 - t0 < kC ? part.t1 - t0 : kC;
@@ -96,14 +102,25 @@ delta_fwd_kernel(FwdArgs a) {
     rK.template load<VEC>(kp + t0 * g.ks, g.ks, n, g.DK, tid);
     if constexpr (!AGG) rQ.template load<VEC>(qp + t0 * g.qs, g.qs, n, g.DK, tid);
     rT.load(reinterpret_cast<const uint4*>(a.w.tri) + at * kTriFragments, tid);
+    if constexpr (VLDS) rVt.template load<VEC>(vp + t0 * g.vs, g.vs, n, trans ? 0 : g.DV - vcol0, tid);
     if (tid < 3 * kC) rDec = a.w.dec[at * (4 * kC) + tid];
     rGam = a.w.gam[at];
   };
   const auto load_v = [&](int32_t i) {
     const int32_t t0 = part.t0 + i * kC;
-    rV.load(vp + t0 * g.vs, g.vs, m, grp, part.t1 - t0 < kC ? part.t1 - t0 : kC, vlive);
+    rV.load(vp + t0 * g.vs, g.vs, m, grp, part.t1 - t0 < kC ? part.t1 - t0 : kC, wlive);
   };
-  if (chunks > 0) load(0), load_v(0);
+  Quad<T> out[4];
+  const auto store = [&](int32_t t0, int n) {
+#pragma unroll
+    for (int rt = 0; rt < 4; ++rt)
+      if (16 * rt + m < n)
+        out[rt].store(static_cast<T*>(a.o) + (t0 + 16 * rt + m) * orow + static_cast<int64_t>(h) * g.DV, col0 + 4 * grp, g.DV, VEC);
+  };
+  if (chunks > 0) {
+    load(0);
+    if constexpr (!VLDS) load_v(0);
+  }
   for (int32_t nth = 0; nth < chunks; ++nth) {
     const int32_t t0 = part.t0 + nth * kC;
     const int n = part.t1 - t0 < kC ? part.t1 - t0 : kC;
@@ -111,11 +128,18 @@ delta_fwd_kernel(FwdArgs a) {
     __syncthreads();
     rK.put(sK, n, g.DK, tid);
     if constexpr (!AGG) rQ.put(sQ, n, g.DK, tid);
+    if constexpr (VLDS) rVt.put(sV, n, trans ? 0 : g.DV - vcol0, tid);
     rT.put(sTri, tid);
     if (tid < 3 * kC) sDec[0][tid] = rDec;
     const float gam = rGam;
+    // The last chunk's outputs go out here: the wait for the loads above is one for all earlier memory accesses,
+    // and stores right before it would be waited for.
+    if constexpr (!AGG)
+      if (nth > 0) store(t0 - kC, kC);
     if (nth + 1 < chunks) load(nth + 1);
-    if constexpr (SAVE) store_state<KT>(a.s0 + at * cells + at_col, g.DV, g.DK, S, m, grp, live);
+    const int64_t at_tile = (at * a.col_tiles + col0 / 16) * 256;
+    if constexpr (SAVE)
+      if (col0 < g.DV) store_tiles<KT>(a.s0 + at_tile * KT, S, lane);
     __syncthreads();
     f32x4 R[4], O[4], D[4];
 #pragma unroll
@@ -124,15 +148,9 @@ delta_fwd_kernel(FwdArgs a) {
     const auto rows = [&](int ks) {
 #pragma unroll
       for (int rt = 0; rt < 4; ++rt) {
-        fk[ks & 1][rt] = sK.rows(16 * rt + m, 32 * ks + 4 * grp);
-        if constexpr (!AGG) fq[ks & 1][rt] = sQ.rows(16 * rt + m, 32 * ks + 4 * grp);
+        fk[ks & 1][rt] = sK.rows(16 * rt + m, ks, grp);
+        if constexpr (!AGG) fq[ks & 1][rt] = sQ.rows(16 * rt + m, ks, grp);
       }
-    };
-    Frag<3> ft[2][2];
-    const auto tri = [&](int rt) {
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
-        if (tri_frag<false>(rt, ks) >= 0) ft[rt & 1][ks] = tri_at<3>(sTri, 0, tri_frag<false>(rt, ks), lane);
     };
     f32x4 dk[4];
     rows(0);
@@ -144,73 +162,81 @@ delta_fwd_kernel(FwdArgs a) {
 #pragma unroll
         for (int rt = 0; rt < 4; ++rt) dk[rt] = dec_at(sDec, kDecKey, rt, grp);
       const Frag<3> sf = split_tiles<3>(S[2 * ks], S[2 * ks + 1]);
-#pragma unroll
-      for (int rt = 0; rt < 4; ++rt) {
-        R[rt] = mma<3>(fk[ks & 1][rt], sf, R[rt]);
-        if constexpr (!AGG) O[rt] = mma<ORD>(fq[ks & 1][rt], sf, O[rt]);
-      }
+      mma_n<3>(fk[ks & 1], sf, R);
+      if constexpr (!AGG) mma_t<ORD>(sf, fq[ks & 1], O);
       phase();
     }
-    tri(0);
-    tri(1);
-#pragma unroll
-    for (int rt = 0; rt < 4; ++rt) R[rt] = rV.tile(rt, grp, n, vlive) - dk[rt] * R[rt];
-    if (nth + 1 < chunks) load_v(nth + 1);
-    const Frag<3> rf[2] = {split_tiles<3>(R[0], R[1]), split_tiles<3>(R[2], R[3])};
-    phase();
-    Frag<ORD> fp[2][2];
-    const auto tri_p = [&](int rt) {
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
-        if (tri_frag<false>(rt, ks) >= 0) fp[rt & 1][ks] = tri_at<ORD>(sTri, 1, tri_frag<false>(rt, ks), lane);
-    };
-    f32x4 up[4], dout[4];
+    Frag<3> t0f[4], t1f[2];
+    tri_tiles<false, 0>(t0f, sTri, 0, 0, lane);
 #pragma unroll
     for (int rt = 0; rt < 4; ++rt) {
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
-        if (tri_frag<false>(rt, ks) >= 0) D[rt] = mma<3>(ft[rt & 1][ks], rf[ks], D[rt]);
-      phase();
-      if (rt < 2) tri(rt + 2);
-      if constexpr (!AGG) {
-        if (rt >= 2) tri_p(rt - 2);
-        dout[rt] = dec_at(sDec, kDecOut, rt, grp);
-      }
-      up[rt] = dec_at(sDec, kDecUp, rt, grp);
+      f32x4 V;
+      if constexpr (VLDS)
+        V = sV.col4(16 * wave, 16 * rt + 4 * grp, m);
+      else
+        V = rV.tile(rt, grp, n, wlive);
+      R[rt] = V - dk[rt] * R[rt];
     }
+    if constexpr (!VLDS)
+      if (nth + 1 < chunks) load_v(nth + 1);
+    const Frag<3> rf[2] = {split_tiles<3>(R[0], R[1]), split_tiles<3>(R[2], R[3])};
+    phase();
+    tri_tiles<false, 2>(t1f, sTri, 0, 1, lane);
+    mma_n<3>(t0f, rf[0], D);
+    phase();
+    Frag<ORD> p0f[4], p1f[2];
+    float dout[4];  // (the outputs' tiles have the token in the column)
+    if constexpr (!AGG) {
+      tri_tiles<false, 0>(p0f, sTri, 1, 0, lane);
+#pragma unroll
+      for (int rt = 0; rt < 4; ++rt) dout[rt] = sDec[kDecOut][16 * rt + m];
+    }
+    mma_n<3>(t1f, rf[1], D + 2);
+    phase();
+    if constexpr (SAVE)
+      if (col0 < g.DV) store_tiles<4>(a.vt + at_tile * 4, D, lane);
+    f32x4 up[4];
+#pragma unroll
+    for (int rt = 0; rt < 4; ++rt) up[rt] = dec_at(sDec, kDecUp, rt, grp);
     if constexpr (!AGG) {
       const Frag<ORD> df[2] = {split_tiles<ORD>(D[0], D[1]), split_tiles<ORD>(D[2], D[3])};
 #pragma unroll
-      for (int rt = 0; rt < 4; ++rt) {
-        O[rt] *= dout[rt];
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-          if (tri_frag<false>(rt, ks) >= 0) O[rt] = mma<ORD>(fp[rt & 1][ks], df[ks], O[rt]);
-        phase();
-        if (rt < 2) tri_p(rt + 2);
-      }
-      store_cols<T>(o + t0 * orow, orow, O, m, grp, n, live);
-      if constexpr (SAVE) store_cols<float>(a.vt + t0 * orow + ocol, orow, D, m, grp, n, live);
+      for (int rt = 0; rt < 4; ++rt) O[rt] *= dout[rt];
+      tri_tiles<false, 2>(p1f, sTri, 1, 1, lane);
+      mma_t<ORD>(df[0], p0f, O);
+      phase();
+      mma_t<ORD>(df[1], p1f, O + 2);
     }
-    Frag<P> fc[2][2];
-    const auto keys = [&](int t) {
+    constexpr int KG = KT < 4 ? KT : 4;  // row tiles of the state at a time
+    Frag<P> fc[2][KG];
+    const auto keys = [&](int t0, int ks) {
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) fc[t & 1][ks] = sK.cols(16 * t, 32 * ks + 4 * grp, m);
+      for (int i = 0; i < KG; ++i) fc[ks][i] = sK.cols(16 * (t0 + i), 32 * ks + 4 * grp, m);
     };
-    keys(0);
+    keys(0, 0);
 #pragma unroll
     for (int rt = 0; rt < 4; ++rt) D[rt] *= up[rt];
     const Frag<3> uf[2] = {split_tiles<3>(D[0], D[1]), split_tiles<3>(D[2], D[3])};
+#pragma unroll
+    for (int t = 0; t < KT; ++t) S[t] *= gam;
     phase();
 #pragma unroll
-    for (int t = 0; t < KT; ++t) {
-      if (t + 1 < KT) keys(t + 1);
-      S[t] *= gam;
+    for (int t = 0; t < KT; t += KG)
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) S[t] = mma<3>(fc[t & 1][ks], uf[ks], S[t]);
-      if (t % 2) phase();
-    }
+      for (int ks = 0; ks < 2; ++ks) {
+        if (ks == 0)
+          keys(t, 1);
+        else if (t + KG < KT)
+          keys(t + KG, 0);
+        mma_n<3>(fc[ks], uf[ks], S + t);
+        phase();
+      }
+    if constexpr (!AGG)
+#pragma unroll
+      for (int rt = 0; rt < 4; ++rt) out[rt].set(O[rt]);
   }
+  if constexpr (!AGG)
+    if (chunks > 0) store(part.t0 + (chunks - 1) * kC, part.t1 - part.t0 - (chunks - 1) * kC);
   if (AGG && trans)
     store_state<KT>(a.w.trans + (static_cast<int64_t>(p.slot) * g.HV + h) * (DKP * DKP) + col0, DKP, DKP, S, m, grp, live);
   else if (AGG)
@@ -305,9 +331,9 @@ template hipError_t launch_delta_carry<true>(const DeltaGeom&, const DeltaWork&,
 hipError_t launch_delta_fwd(const DeltaGeom& g, const DeltaIn& in, const DeltaWork& w, const float* h0, float* h1,
                             void* o, float* s0, float* vt, int dtype, hipStream_t s) {
   // (rows that are read value by value: more registers, so four waves)
-  const int nw = g.qk_vec ? delta_waves(g.DV) : 4;
+  const int nw = g.vec ? delta_waves(g.DV) : 4;
   const uint32_t vcb = delta_col_blocks(g.DV, nw);
-  FwdArgs a{g, in, w, h0, h1, o, s0, vt, vcb, vcb, static_cast<uint32_t>(chunk_slots(g.q, g.part))};
+  FwdArgs a{g, in, w, h0, h1, o, s0, vt, delta_col_tiles(g), vcb, vcb, static_cast<uint32_t>(chunk_slots(g.q, g.part))};
   hipError_t e = launch_delta_prep(g, in, w, false, dtype, s);
   if (e != hipSuccess) return e;
   const auto run = [&](auto t, auto dkp, auto waves, auto vec) {
@@ -331,7 +357,7 @@ hipError_t launch_delta_fwd(const DeltaGeom& g, const DeltaIn& in, const DeltaWo
   };
   return delta_dispatch(dtype, g.DK, [&](auto t, auto dkp) {
     using Four = std::integral_constant<int, 4>;
-    if (!g.qk_vec) return run(t, dkp, Four{}, std::false_type{});
+    if (!g.vec) return run(t, dkp, Four{}, std::false_type{});
     return nw == 8 ? run(t, dkp, std::integral_constant<int, 8>{}, std::true_type{}) : run(t, dkp, Four{}, std::true_type{});
   });
 }

@@ -24,7 +24,7 @@ struct DeltaGeom {
   float scale;
   int32_t l2;
   int32_t beta_f32;               // beta is float32, else of the activations' type
-  int32_t qk_vec, v_vec;          // rows of q and k, of v are read 16 bytes at a time
+  int32_t vec;                    // rows of q, k, v, o (and of the gradients) are accessed 16 bytes at a time
   SeqCut cut;                     // chunks
   SeqCut part;                    // parts of the time axis, whole chunks
   int32_t parts;                  // 1: a sequence is one part
@@ -38,6 +38,10 @@ struct DeltaIn {
   const void* beta;
 };
 
+// States and rows that one pass leaves for another lie as the matrix units' result tiles, 16 x 16 values (256
+// floats, 16 bytes a lane) each, the 16 columns' tiles one after the other.
+inline int64_t delta_col_tiles(const DeltaGeom& g) { return (g.DV + 15) / 16; }
+
 // What the chunks' own products leave for the passes along time, for every
 // chunk slot and value head: the fragments of two 64 x 64 triangles as the
 // matrix units take them, and four scalars for each token.
@@ -50,19 +54,18 @@ struct DeltaWork {
 };
 
 struct DeltaBwd {
-  const float* s0;   // (slots, HV, DK, DV): initial states of the chunks
-  const float* vt;   // (T, HV, DV): d_t
+  const float* s0;   // (slots, HV, column tiles, DKP / 16 tiles): initial states of the chunks
+  const float* vt;   // (slots, HV, column tiles, 4 tiles): d_t
   const void* d_o;
   const float* dh1;  // or null
   float* dh0;        // or null
-  float* x;          // (T, HV, DV): dv / beta
-  float* dend;       // (slots, HV, DK, DV): gradients of the chunks' final states
+  float* x;          // as vt: dv / beta
+  float* dend;       // as s0: gradients of the chunks' final states
   void* dq;
   void* dk;
   void* dv;
   float* dg;
   void* dbeta;
-  int32_t o_vec;     // rows of d_o and dv are accessed 16 bytes at a time
 };
 
 // 16-byte fragments of one triangle of a chunk slot and value head

@@ -56,7 +56,7 @@ delta_prep_kernel(DeltaGeom g, DeltaIn in, DeltaWork w) {
   for (int ks = 0; ks < DKP / 32; ++ks) {
     const int k0 = 32 * ks + 8 * grp;
     const auto frag = [&](const T* p, int64_t stride, int row) {
-      return row_frag<T>(p + (row < n ? row : 0) * stride, k0, g.DK, g.qk_vec, row < n);
+      return row_frag<T>(p + (row < n ? row : 0) * stride, k0, g.DK, g.vec, row < n);
     };
     const Frag<P> bk = frag(kp, g.ks, own), bq = frag(qp, g.qs, own);
     qq = mma<3>(bq, bq, qq);
