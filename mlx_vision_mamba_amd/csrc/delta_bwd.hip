@@ -87,23 +87,32 @@ delta_bwd_kernel(BwdArgs a) {
   float rGam;
   Cols<T> rO;
   StageRows<T, 16 * NW, NT> rOt;
-  const auto load = [&](int32_t i) {
+  // (a few at a time, as in the forward)
+  constexpr int kLoads = 8;
+  const auto load = [&](int32_t i, int which) {
     const int32_t t0 = part.t0 + i * kC;
     const int n = part.t1 - t0 < kC ? part.t1 - t0 : kC;
     const int64_t at = static_cast<int64_t>(slot0 + i) * g.HV + h;
-    rK.template load<VEC>(kp + t0 * g.ks, g.ks, n, g.DK, tid);
-    rQ.template load<VEC>(qp + t0 * g.qs, g.qs, n, g.DK, tid);
-    rT.load(reinterpret_cast<const uint4*>(a.w.tri) + at * kTriFragments, tid);
-    if constexpr (OLDS) rOt.template load<VEC>(dop + t0 * orow, orow, n, trans ? 0 : g.DV - vcol0, tid);
-    if (tid < 4 * kC) rDec = a.w.dec[at * (4 * kC) + tid];
-    rGam = a.w.gam[at];
+    switch (which) {
+      case 0: rK.template load<VEC>(kp + t0 * g.ks, g.ks, n, g.DK, tid); break;
+      case 1: rQ.template load<VEC>(qp + t0 * g.qs, g.qs, n, g.DK, tid); break;
+      case 2:
+        if constexpr (OLDS) rOt.template load<VEC>(dop + t0 * orow, orow, n, trans ? 0 : g.DV - vcol0, tid);
+        break;
+      case 3:
+        if (tid < 4 * kC) rDec = a.w.dec[at * (4 * kC) + tid];
+        rGam = a.w.gam[at];
+        break;
+      default: rT.load(reinterpret_cast<const uint4*>(a.w.tri) + at * kTriFragments, tid, which - 4, which - 3); break;
+    }
   };
   const auto load_o = [&](int32_t i) {
     const int32_t t0 = part.t0 + i * kC;
     rO.load(dop + t0 * orow, orow, m, grp, part.t1 - t0 < kC ? part.t1 - t0 : kC, vlive);
   };
   if (chunks > 0) {
-    load(chunks - 1);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) load(chunks - 1, i);
     if constexpr (!OLDS) load_o(chunks - 1);
   }
   for (int32_t nth = chunks - 1; nth >= 0; --nth) {
@@ -117,7 +126,7 @@ delta_bwd_kernel(BwdArgs a) {
     rT.put(sTri, tid);
     if (tid < 4 * kC) sDec[0][tid] = rDec;
     const float gam = rGam;
-    if (nth > 0) load(nth - 1);
+    const int32_t ahead = nth > 0 ? nth - 1 : 0;
     const int64_t at_tile = (at * a.col_tiles + col0 / 16) * 256;
     if constexpr (!AGG)
       if (col0 < g.DV) store_tiles<KT>(a.b.dend + at_tile * KT, E, lane);
@@ -141,6 +150,8 @@ delta_bwd_kernel(BwdArgs a) {
         for (int rt = 0; rt < 4; ++rt) up[rt] = dec_at(sDec, kDecUp, rt, grp);
       const Frag<3> ef = split_tiles<3>(E[2 * ks], E[2 * ks + 1]);
       mma_n<3>(fk[ks & 1], ef, D);
+#pragma unroll
+      for (int i = 4 * ks / KS; i < 4 * (ks + 1) / KS; ++i) load(ahead, i);
       phase();
     }
     Frag<3> f1[4], f0[2];
@@ -153,8 +164,7 @@ delta_bwd_kernel(BwdArgs a) {
         O[rt] = rO.tile(rt, grp, n, vlive);
       D[rt] *= up[rt];
     }
-    if constexpr (!OLDS)
-      if (nth > 0) load_o(nth - 1);
+    if constexpr (!OLDS) load_o(ahead);
     {
       const Frag<P> of[2] = {split_tiles<P>(O[0], O[1]), split_tiles<P>(O[2], O[3])};
       phase();
@@ -163,6 +173,7 @@ delta_bwd_kernel(BwdArgs a) {
       phase();
       tri_tiles<true, 0>(f1, sTri, 0, 1, lane);
       mma_n<3>(f0, of[0], D);
+      load(ahead, 4);
       phase();
     }
     f32x4 dx[4], dout[4];
@@ -170,6 +181,7 @@ delta_bwd_kernel(BwdArgs a) {
       const Frag<3> df[2] = {split_tiles<3>(D[0], D[1]), split_tiles<3>(D[2], D[3])};
       tri_tiles<true, 0>(f0, sTri, 0, 0, lane);
       mma_n<3>(f1, df[1], X);
+      load(ahead, 5);
       phase();
 #pragma unroll
       for (int rt = 0; rt < 4; ++rt) {
@@ -197,6 +209,8 @@ delta_bwd_kernel(BwdArgs a) {
     const Frag<3> of[2] = {split_tiles<3>(O[0], O[1]), split_tiles<3>(O[2], O[3])};
 #pragma unroll
     for (int t = 0; t < KT; ++t) E[t] *= gam;
+    load(ahead, 6);
+    load(ahead, 7);
     phase();
 #pragma unroll
     for (int i = 0; i < 4 * (KT / KG); ++i) {

@@ -471,10 +471,12 @@ template <int PP, int NT>
 struct StageTri {
   static constexpr int kCount = tri_index(1, PP, 0), kItems = (kCount + NT - 1) / NT;
   u32x4 r[kItems];
-  __device__ __forceinline__ void load(const uint4* tri, int tid) {
+  // (the items from a to b of 4)
+  __device__ __forceinline__ void load(const uint4* tri, int tid, int a = 0, int b = 4) {
     const u32x4* at = reinterpret_cast<const u32x4*>(tri);
 #pragma unroll
-    for (int i = 0; i < kItems; ++i) r[i] = at[NT * (i + 1) <= kCount || tid + NT * i < kCount ? tid + NT * i : 0];
+    for (int i = 0; i < kItems; ++i)
+      if (i >= kItems * a / 4 && i < kItems * b / 4) r[i] = at[NT * (i + 1) <= kCount || tid + NT * i < kCount ? tid + NT * i : 0];
   }
   __device__ __forceinline__ void put(uint4* lds, int tid) const {
 #pragma unroll

@@ -95,16 +95,27 @@ delta_fwd_kernel(FwdArgs a) {
   float rGam;
   Cols<T> rV;
   StageRows<T, 16 * NW, NT> rVt;
-  const auto load = [&](int32_t i) {
+  // Loads of chunk i, a few at a time between the phases of the products: all at once they hold up the wave that
+  // issues them, and all waves at the next barrier, for as long as the memory pipeline takes them.
+  constexpr int kLoads = 8;
+  const auto load = [&](int32_t i, int which) {
     const int32_t t0 = part.t0 + i * kC;
     const int n = part.t1 - t0 < kC ? part.t1 - t0 : kC;
     const int64_t at = static_cast<int64_t>(slot0 + i) * g.HV + h;
-    rK.template load<VEC>(kp + t0 * g.ks, g.ks, n, g.DK, tid);
-    if constexpr (!AGG) rQ.template load<VEC>(qp + t0 * g.qs, g.qs, n, g.DK, tid);
-    rT.load(reinterpret_cast<const uint4*>(a.w.tri) + at * kTriFragments, tid);
-    if constexpr (VLDS) rVt.template load<VEC>(vp + t0 * g.vs, g.vs, n, trans ? 0 : g.DV - vcol0, tid);
-    if (tid < 3 * kC) rDec = a.w.dec[at * (4 * kC) + tid];
-    rGam = a.w.gam[at];
+    switch (which) {
+      case 0: rK.template load<VEC>(kp + t0 * g.ks, g.ks, n, g.DK, tid); break;
+      case 1:
+        if constexpr (!AGG) rQ.template load<VEC>(qp + t0 * g.qs, g.qs, n, g.DK, tid);
+        break;
+      case 2:
+        if constexpr (VLDS) rVt.template load<VEC>(vp + t0 * g.vs, g.vs, n, trans ? 0 : g.DV - vcol0, tid);
+        break;
+      case 3:
+        if (tid < 3 * kC) rDec = a.w.dec[at * (4 * kC) + tid];
+        rGam = a.w.gam[at];
+        break;
+      default: rT.load(reinterpret_cast<const uint4*>(a.w.tri) + at * kTriFragments, tid, which - 4, which - 3); break;
+    }
   };
   const auto load_v = [&](int32_t i) {
     const int32_t t0 = part.t0 + i * kC;
@@ -118,7 +129,8 @@ delta_fwd_kernel(FwdArgs a) {
         out[rt].store(static_cast<T*>(a.o) + (t0 + 16 * rt + m) * orow + static_cast<int64_t>(h) * g.DV, col0 + 4 * grp, g.DV, VEC);
   };
   if (chunks > 0) {
-    load(0);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) load(0, i);
     if constexpr (!VLDS) load_v(0);
   }
   for (int32_t nth = 0; nth < chunks; ++nth) {
@@ -136,7 +148,8 @@ delta_fwd_kernel(FwdArgs a) {
     // and stores right before it would be waited for.
     if constexpr (!AGG)
       if (nth > 0) store(t0 - kC, kC);
-    if (nth + 1 < chunks) load(nth + 1);
+    // (past the last chunk: the last one again, so that no branch parts the phases)
+    const int32_t ahead = nth + 1 < chunks ? nth + 1 : nth;
     const int64_t at_tile = (at * a.col_tiles + col0 / 16) * 256;
     if constexpr (SAVE)
       if (col0 < g.DV) store_tiles<KT>(a.s0 + at_tile * KT, S, lane);
@@ -164,6 +177,8 @@ delta_fwd_kernel(FwdArgs a) {
       const Frag<3> sf = split_tiles<3>(S[2 * ks], S[2 * ks + 1]);
       mma_n<3>(fk[ks & 1], sf, R);
       if constexpr (!AGG) mma_t<ORD>(sf, fq[ks & 1], O);
+#pragma unroll
+      for (int i = 4 * ks / KS; i < 4 * (ks + 1) / KS; ++i) load(ahead, i);
       phase();
     }
     Frag<3> t0f[4], t1f[2];
@@ -177,12 +192,12 @@ delta_fwd_kernel(FwdArgs a) {
         V = rV.tile(rt, grp, n, wlive);
       R[rt] = V - dk[rt] * R[rt];
     }
-    if constexpr (!VLDS)
-      if (nth + 1 < chunks) load_v(nth + 1);
+    if constexpr (!VLDS) load_v(ahead);
     const Frag<3> rf[2] = {split_tiles<3>(R[0], R[1]), split_tiles<3>(R[2], R[3])};
     phase();
     tri_tiles<false, 2>(t1f, sTri, 0, 1, lane);
     mma_n<3>(t0f, rf[0], D);
+    load(ahead, 4);
     phase();
     Frag<ORD> p0f[4], p1f[2];
     float dout[4];  // (the outputs' tiles have the token in the column)
@@ -192,6 +207,7 @@ delta_fwd_kernel(FwdArgs a) {
       for (int rt = 0; rt < 4; ++rt) dout[rt] = sDec[kDecOut][16 * rt + m];
     }
     mma_n<3>(t1f, rf[1], D + 2);
+    load(ahead, 5);
     phase();
     if constexpr (SAVE)
       if (col0 < g.DV) store_tiles<4>(a.vt + at_tile * 4, D, lane);
@@ -219,6 +235,8 @@ delta_fwd_kernel(FwdArgs a) {
     const Frag<3> uf[2] = {split_tiles<3>(D[0], D[1]), split_tiles<3>(D[2], D[3])};
 #pragma unroll
     for (int t = 0; t < KT; ++t) S[t] *= gam;
+    load(ahead, 6);
+    load(ahead, 7);
     phase();
 #pragma unroll
     for (int t = 0; t < KT; t += KG)
