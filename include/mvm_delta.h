@@ -65,7 +65,7 @@ typedef struct mvm_delta_desc {
 int mvm_delta_validate(const mvm_delta_desc* desc);
 
 /* float32 elements of the checkpoints that a forward leaves for a backward:
- * each chunk's initial state, and the rows d_t. */
+ * each chunk's initial state, the rows d_t, the chunk's triangles and decays. */
 int64_t mvm_delta_ckpt_elems(const mvm_delta_desc* desc);
 
 /* Workspace bytes: which = 0 forward, 1 backward.  The workspace must be

@@ -62,16 +62,21 @@ delta_bwd_kernel(BwdArgs a) {
   if (part.t0 < 0 || part.seq >= g.q.S || (AGG && part.t0 == part.start)) return;  // (nothing precedes a first part)
   const int64_t cells = static_cast<int64_t>(g.DK) * g.DV;
   const int64_t at_h = (static_cast<int64_t>(part.seq) * g.HV + h) * cells + at_col;
-  const int64_t at_part = (static_cast<int64_t>(p.slot) * g.HV + h) * cells + at_col;
+  const int64_t at_part = ((static_cast<int64_t>(p.slot) * g.HV + h) * a.col_tiles + col0 / 16) * (KT * 256);
+  const bool tiles = !trans && col0 < g.DV;
   f32x4 E[KT];
   if (trans) {
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) E[t][r] = 16 * t + 4 * grp + r == col ? 1.f : 0.f;
+  } else if (!AGG && a.w.carry != nullptr) {
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+      E[t] = tiles ? reinterpret_cast<const f32x4*>(a.w.carry + at_part)[64 * t + lane] : f32x4{0.f, 0.f, 0.f, 0.f};
   } else {
-    const float* src = AGG ? nullptr : a.w.carry != nullptr ? a.w.carry + at_part : a.b.dh1 != nullptr ? a.b.dh1 + at_h : nullptr;
-    load_state<KT>(E, src, g.DV, src != nullptr ? g.DK : 0, m, grp, live);
+    const int32_t on = !AGG && a.b.dh1 != nullptr;
+    load_state<KT>(E, a.b.dh1 + on * at_h, g.DV, on * g.DK, m, grp, live);
   }
   const T* kp = static_cast<const T*>(a.in.k) + hk * g.kh;
   const T* qp = static_cast<const T*>(a.in.q) + hk * g.qh;
@@ -155,7 +160,7 @@ delta_bwd_kernel(BwdArgs a) {
       phase();
     }
     Frag<3> f1[4], f0[2];
-    tri_tiles<true, 0>(f1, sTri, 1, 1, lane);
+    tri_tiles_t<0>(f1, sTri, 1, 1, m, grp);
 #pragma unroll
     for (int rt = 0; rt < 4; ++rt) {
       if constexpr (OLDS)
@@ -168,10 +173,10 @@ delta_bwd_kernel(BwdArgs a) {
     {
       const Frag<P> of[2] = {split_tiles<P>(O[0], O[1]), split_tiles<P>(O[2], O[3])};
       phase();
-      tri_tiles<true, 0>(f0, sTri, 1, 0, lane);
+      tri_tiles_t<0>(f0, sTri, 1, 0, m, grp);
       mma_n<3>(f1, of[1], D);
       phase();
-      tri_tiles<true, 0>(f1, sTri, 0, 1, lane);
+      tri_tiles_t<0>(f1, sTri, 0, 1, m, grp);
       mma_n<3>(f0, of[0], D);
       load(ahead, 4);
       phase();
@@ -179,13 +184,13 @@ delta_bwd_kernel(BwdArgs a) {
     f32x4 dx[4], dout[4];
     {
       const Frag<3> df[2] = {split_tiles<3>(D[0], D[1]), split_tiles<3>(D[2], D[3])};
-      tri_tiles<true, 0>(f0, sTri, 0, 0, lane);
+      tri_tiles_t<0>(f0, sTri, 0, 0, m, grp);
       mma_n<3>(f1, df[1], X);
       load(ahead, 5);
       phase();
 #pragma unroll
       for (int rt = 0; rt < 4; ++rt) {
-        dx[rt] = dec_at(sDec, kDecBetaKey, rt, grp);
+        dx[rt] = dec_at(sDec, kDecBeta, rt, grp) * dec_at(sDec, kDecKey, rt, grp);
         dout[rt] = dec_at(sDec, kDecOut, rt, grp);
       }
       mma_n<3>(f0, df[0], X);
@@ -219,10 +224,11 @@ delta_bwd_kernel(BwdArgs a) {
       phase();
     }
   }
-  if (AGG && trans)
-    store_state<KT>(a.w.trans + (static_cast<int64_t>(p.slot) * g.HV + h) * (DKP * DKP) + col0, DKP, DKP, E, m, grp, live);
-  else if (AGG)
-    store_state<KT>(a.w.carry + at_part, g.DV, g.DK, E, m, grp, live);
+  if (AGG && trans) {
+    if (col0 < DKP) store_tiles<KT>(a.w.trans + ((static_cast<int64_t>(p.slot) * g.HV + h) * KT + col0 / 16) * (KT * 256), E, lane);
+  } else if (AGG) {
+    if (tiles) store_tiles<KT>(a.w.carry + at_part, E, lane);
+  }
   else if (a.b.dh0 != nullptr && part.t0 == part.start)
     store_state<KT>(a.b.dh0 + at_h, g.DV, g.DK, E, m, grp, live);
 }
@@ -601,8 +607,6 @@ hipError_t launch_delta_bwd(const DeltaGeom& g, const DeltaIn& in, const DeltaWo
   const int nw = g.vec ? delta_waves(g.DV) : 4;
   const uint32_t vcb = delta_col_blocks(g.DV, nw);
   BwdArgs a{g, in, w, b, delta_col_tiles(g), vcb, vcb, static_cast<uint32_t>(chunk_slots(g.q, g.part))};
-  hipError_t e = launch_delta_prep(g, in, w, true, dtype, s);
-  if (e != hipSuccess) return e;
   const auto run = [&](auto t, auto dkp, auto waves, auto vec) {
     using T = decltype(t);
     constexpr int DKP = decltype(dkp)::value, NW = decltype(waves)::value;

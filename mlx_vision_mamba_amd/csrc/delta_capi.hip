@@ -46,14 +46,36 @@ int check_stride(const char* name, int64_t stride) {
   return MVM_OK;
 }
 
-// The parts of the time axis.
+// The parts of the time axis.  Whole sequences leave compute units idle where
+// there are few of them and heads; parts cost a pass for their ends and
+// transitions, of twice the columns, and their joining, one after the other.  The
+// cheapest cut by a model in units of a main pass's chunk (5.5-7 us, 128 x 128
+// heads of bfloat16): a workgroup a compute unit, so passes take whole rounds of
+// them; a chunk of the parts' pass takes 0.7, a part's joining 0.2 to 0.75.
+// Measured on MI355X with 12 such heads, us forward whole / in parts: one
+// sequence of 32768 tokens 2986 / 640, of 8192 750 / 330; 6 of 2730 314 / 343; 16
+// of 512 95 / 177.
+constexpr int64_t kUnits = 256;
+
 void pick_parts(const mvm_delta_desc* d, mvm::DeltaGeom& g) {
-  const int64_t T = d->seq.tokens;
+  const int64_t T = d->seq.tokens, S = std::max<int64_t>(1, d->seq.nseq);
   int64_t longest = d->seq.offsets == nullptr ? d->seq.seqlen : T;
   if (d->max_len > 0) longest = std::min(longest, d->max_len);
   int64_t len = d->split_len;
   if (len == 0) {
+    const int waves = mvm::delta_waves(g.DV), dkp = mvm::delta_dkp(g.DK);
+    const int64_t vcb = mvm::delta_col_blocks(g.DV, waves), tcb = mvm::delta_col_blocks(dkp, waves);
+    const int64_t C = mvm::kDeltaChunk, chunks = ceil_div(longest, C);
+    const double join = dkp == 128 ? 0.75 : (dkp == 64 ? 0.3 : 0.2);
+    // a tenth in favour of whole sequences: less memory, fewer launches
+    double best = 0.9 * std::max<int64_t>(chunks, ceil_div((T / C + S / 2) * g.HV * vcb, kUnits));
     len = longest;
+    for (int64_t n = 2; n <= std::min<int64_t>(chunks, 128); ++n) {
+      const int64_t lc = ceil_div(chunks, n), parts = T / (lc * C) + (S + 1) / 2;
+      const double cost = static_cast<double>(lc) * ceil_div(parts * g.HV * vcb, kUnits) +
+                          0.7 * lc * ceil_div(std::max<int64_t>(1, parts - S) * g.HV * (vcb + tcb), kUnits) + join * n + 2;
+      if (cost < best) best = cost, len = lc * C;
+    }
   }
   // Whole sequences: one part whatever max_len says
   g.parts = len < longest ? static_cast<int32_t>(ceil_div(longest, len)) : 1;
@@ -140,12 +162,21 @@ int check_delta(const mvm_delta_desc* d) {
   return MVM_OK;
 }
 
+// What a training forward leaves: the chunks' initial states, the rows d_t, and (DeltaWork) their triangles and scalars.
 struct Ckpt {
-  int64_t s0, vt;
+  size_t s0, vt, tri, dec, gam, total;
 };
 Ckpt ckpt_of(const mvm::DeltaGeom& g) {
-  const int64_t tiles = mvm::chunk_slots(g.q, g.cut) * g.HV * mvm::delta_col_tiles(g) * 256;
-  return {tiles * (mvm::delta_dkp(g.DK) / 16), tiles * 4};
+  const size_t items = static_cast<size_t>(mvm::chunk_slots(g.q, g.cut)) * g.HV;
+  const size_t tiles = items * static_cast<size_t>(mvm::delta_col_tiles(g)) * 256 * 4;
+  Ckpt c;
+  c.s0 = align_up(tiles * (mvm::delta_dkp(g.DK) / 16));
+  c.vt = align_up(tiles * 4);
+  c.tri = align_up(items * mvm::kTriBytes);
+  c.dec = align_up(items * mvm::kDeltaChunk * 16);
+  c.gam = align_up(items * 4);
+  c.total = c.s0 + c.vt + c.tri + c.dec + c.gam;
+  return c;
 }
 
 struct Ws {
@@ -153,19 +184,19 @@ struct Ws {
 };
 Ws ws_of(const mvm::DeltaGeom& g, bool backward) {
   Ws w;
-  const size_t items = static_cast<size_t>(mvm::chunk_slots(g.q, g.cut)) * g.HV;
-  w.tri = align_up(items * mvm::kTriBytes);
-  w.dec = align_up(items * mvm::kDeltaChunk * 16);
-  w.gam = align_up(items * 4);
+  const Ckpt c = ckpt_of(g);
+  if (backward) {
+    w.x = c.vt;
+    w.dend = c.s0;
+  } else {
+    w.tri = c.tri;
+    w.dec = c.dec;
+    w.gam = c.gam;
+  }
   if (g.parts > 1) {
     const size_t parts = static_cast<size_t>(mvm::chunk_slots(g.q, g.part)) * g.HV, dkp = mvm::delta_dkp(g.DK);
     w.trans = align_up(parts * dkp * dkp * 4);
-    w.carry = align_up(parts * g.DK * g.DV * 4);
-  }
-  if (backward) {
-    const Ckpt c = ckpt_of(g);
-    w.x = align_up(static_cast<size_t>(c.vt) * 4);
-    w.dend = align_up(static_cast<size_t>(c.s0) * 4);
+    w.carry = align_up(parts * static_cast<size_t>(mvm::delta_col_tiles(g)) * 16 * dkp * 4);
   }
   w.total = w.tri + w.dec + w.gam + w.trans + w.carry + w.x + w.dend;
   return w;
@@ -179,6 +210,16 @@ struct Take {
     return p;
   }
 };
+
+void take_ckpt(const mvm::DeltaGeom& g, const float* ckpt, float*& s0, float*& vt, mvm::DeltaWork& w) {
+  const Ckpt c = ckpt_of(g);
+  Take take{reinterpret_cast<char*>(const_cast<float*>(ckpt))};
+  s0 = take(c.s0);
+  vt = take(c.vt);
+  w.tri = take(c.tri);
+  w.dec = take(c.dec);
+  w.gam = take(c.gam);
+}
 
 int check_ws(const char* what, const void* ws, size_t have, size_t need) {
   if (need > 0 && (ws == nullptr || have < need))
@@ -207,8 +248,7 @@ int mvm_delta_validate(const mvm_delta_desc* desc) {
 int64_t mvm_delta_ckpt_elems(const mvm_delta_desc* desc) {
   const int rc = check_delta(desc);
   if (rc != MVM_OK) return rc;
-  const Ckpt c = ckpt_of(geom(desc));
-  return c.s0 + c.vt;
+  return static_cast<int64_t>(ckpt_of(geom(desc)).total / sizeof(float));
 }
 
 int64_t mvm_delta_workspace_bytes(const mvm_delta_desc* desc, int which) {
@@ -238,8 +278,9 @@ int mvm_delta_fwd(const mvm_delta_desc* desc, const void* q, const void* k, cons
   b.gam = take(w.gam);
   b.trans = take(w.trans);
   b.carry = take(w.carry);
-  float* vt = ckpt != nullptr ? ckpt + ckpt_of(gm).s0 : nullptr;
-  return hip_status(mvm::launch_delta_fwd(gm, in, b, h0, h1, o, ckpt, vt, desc->dtype, static_cast<hipStream_t>(stream)),
+  float *s0 = nullptr, *vt = nullptr;
+  if (ckpt != nullptr) take_ckpt(gm, ckpt, s0, vt, b);
+  return hip_status(mvm::launch_delta_fwd(gm, in, b, h0, h1, o, s0, vt, desc->dtype, static_cast<hipStream_t>(stream)),
                     "mvm_delta_fwd launch");
 }
 
@@ -261,14 +302,13 @@ int mvm_delta_bwd(const mvm_delta_desc* desc, const void* q, const void* k, cons
   gm.vec = wide(gm, in, desc->dtype, {d_o, dv}) && fits(dq, 0, 0) && fits(dk, 0, 0);
   Take take{static_cast<char*>(workspace)};
   mvm::DeltaWork b{};
-  b.tri = take(w.tri);
-  b.dec = take(w.dec);
-  b.gam = take(w.gam);
   b.trans = take(w.trans);
   b.carry = take(w.carry);
   mvm::DeltaBwd r{};
-  r.s0 = ckpt;
-  r.vt = ckpt != nullptr ? ckpt + ckpt_of(gm).s0 : nullptr;
+  float *s0 = nullptr, *vt = nullptr;
+  if (ckpt != nullptr) take_ckpt(gm, ckpt, s0, vt, b);
+  r.s0 = s0;
+  r.vt = vt;
   r.d_o = d_o; r.dh1 = dh1; r.dh0 = dh0;
   r.x = take(w.x);
   r.dend = take(w.dend);

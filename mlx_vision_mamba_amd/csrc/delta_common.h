@@ -421,6 +421,13 @@ __device__ __forceinline__ f32x4 load4(const T* p, int c, int n, bool vec) {
   return v;
 }
 
+// 1 where sequence i starts from the state in row `row` of `states`, else 0.  (A scalar that selects by a product:
+// with conditions, of which one comes from a vector load, this toolchain lost a value on one of their paths.)
+__device__ __forceinline__ int32_t seq_starts(const SeqGeom& g, int32_t i, int32_t row, const float* states) {
+  const int32_t fresh = g.fresh != nullptr ? g.fresh[i] : 0;
+  return (states != nullptr) & (row >= 0) & (__builtin_amdgcn_readfirstlane(fresh) == 0);
+}
+
 // The rows dk of a state's 16 columns: `at` is the wave's first column of row 0.  Rows are `ld` values apart.
 template <int KT>
 __device__ __forceinline__ void load_state(f32x4 (&S)[KT], const float* at, int ld, int rows, int m, int grp, bool live) {
@@ -451,13 +458,11 @@ __device__ __forceinline__ Frag<kRawParts<T>> row_frag(const T* p, int c, int dk
   return load8<T>(p, c, ok ? dk : 0, vec);
 }
 
-// Number of the fragment of 16 rows (tile rt) and 32 columns (ks) of a lower
-// (BWD: upper) triangle of 64 x 64, or -1 where all of it is zero.
-template <bool BWD>
-constexpr int tri_frag(int rt, int ks) {
-  if (BWD) return rt < 2 ? 2 * rt + ks : (ks == 0 ? -1 : rt + 2);
-  return rt < 2 ? (ks == 0 ? rt : -1) : 2 * rt - 2 + ks;
-}
+// Number of the fragment of 16 rows (tile rt) and 32 columns (ks) of a lower triangle of 64 x 64, or -1 where all of
+// it is zero.  Within a fragment the four lanes of a row lie together: so neither a row's readers nor those of a
+// column share a bank.
+constexpr int tri_frag(int rt, int ks) { return rt < 2 ? (ks == 0 ? rt : -1) : 2 * rt - 2 + ks; }
+__device__ __forceinline__ int tri_lane(int m, int grp) { return 4 * m + grp; }
 
 // Result tiles in memory as the lanes hold them, 16 bytes a lane: N tiles of one column block
 template <int N>
@@ -484,14 +489,33 @@ struct StageTri {
       if (NT * (i + 1) <= kCount || tid + NT * i < kCount) reinterpret_cast<u32x4*>(lds)[tid + NT * i] = r[i];
   }
 };
-// the fragments of row tiles RT0 .. RT0 + N - 1, columns 32 ks .. 32 ks + 31
-template <bool BWD, int RT0, int N, int P>
-__device__ __forceinline__ void tri_tiles(Frag<P> (&f)[N], const uint4* lds, int which, int ks, int lane) {
+// A triangle's operands for row tiles RT0 .. RT0 + N - 1, summed index 32 ks .. 32 ks + 31
+template <int RT0, int N, int P>
+__device__ __forceinline__ void tri_tiles(Frag<P> (&f)[N], const uint4* lds, int which, int ks, int m, int grp) {
 #pragma unroll
   for (int i = 0; i < N; ++i)
 #pragma unroll
-    for (int q = 0; q < P; ++q) f[i].p[q] = lds[tri_index(which, q, tri_frag<BWD>(RT0 + i, ks)) + lane];
+    for (int q = 0; q < P; ++q) f[i].p[q] = lds[tri_index(which, q, tri_frag(RT0 + i, ks)) + tri_lane(m, grp)];
 }
+// the same of its transpose, whose summed index are the triangle's rows
+template <int RT0, int N, int P>
+__device__ __forceinline__ void tri_tiles_t(Frag<P> (&f)[N], const uint4* lds, int which, int ks, int m, int grp) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int jt = RT0 + i;
+#pragma unroll
+    for (int q = 0; q < P; ++q) {
+      // 4 columns of row 32 ks (+ 16) + 4g + m / 4
+      const uint2* at = reinterpret_cast<const uint2*>(lds + tri_lane(4 * grp + (m >> 2), m & 3)) + (jt & 1);
+      const uint2 a = __builtin_bit_cast(
+          uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 2 * tri_index(which, q, tri_frag(2 * ks, jt / 2)))));
+      const uint2 b = __builtin_bit_cast(
+          uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 2 * tri_index(which, q, tri_frag(2 * ks + 1, jt / 2)))));
+      f[i].p[q] = make_uint4(a.x, a.y, b.x, b.y);
+    }
+  }
+}
+
 // Sum over the 4 lane groups of the lanes with the same m
 __device__ __forceinline__ float sum_g(float x) {
   x += __shfl_xor(x, 16);
@@ -536,7 +560,7 @@ __device__ __forceinline__ DeltaPos delta_pos(uint32_t ncb, uint32_t nslots, uin
 inline int64_t delta_blocks(int64_t ncb, int64_t nslots, int64_t heads) { return (nslots * heads + 7) / 8 * 8 * ncb; }
 
 // The tokens' scalars of a chunk, as delta_prep.hip leaves them: four rows of 64
-enum DecRow { kDecKey, kDecUp, kDecOut, kDecBetaKey };
+enum DecRow { kDecKey, kDecUp, kDecOut, kDecBeta };
 __device__ __forceinline__ f32x4 dec_at(const float (*dec)[kC], DecRow which, int rt, int grp) {
   return *reinterpret_cast<const f32x4*>(&dec[which][16 * rt + 4 * grp]);
 }

@@ -67,20 +67,21 @@ delta_fwd_kernel(FwdArgs a) {
   }
   const int32_t row = seq_slot(g.q, part.seq);
   const int64_t cells = static_cast<int64_t>(g.DK) * g.DV, at_h = static_cast<int64_t>(h) * cells + at_col;
-  const int64_t at_part = (static_cast<int64_t>(p.slot) * g.HV + h) * cells + at_col;
+  const int64_t at_part = ((static_cast<int64_t>(p.slot) * g.HV + h) * a.col_tiles + col0 / 16) * (KT * 256);
+  const bool tiles = !trans && col0 < g.DV;  // (this wave's column tile exists)
   f32x4 S[KT];
   if (trans) {
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) S[t][r] = 16 * t + 4 * grp + r == col ? 1.f : 0.f;
+  } else if (!AGG && a.w.carry != nullptr) {
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+      S[t] = tiles ? reinterpret_cast<const f32x4*>(a.w.carry + at_part)[64 * t + lane] : f32x4{0.f, 0.f, 0.f, 0.f};
   } else {
-    const float* src = nullptr;
-    if (!AGG && a.w.carry != nullptr)
-      src = a.w.carry + at_part;
-    else if (!AGG && a.h0 != nullptr && row >= 0 && !seq_fresh(g.q, part.seq))
-      src = a.h0 + row * (g.HV * cells) + at_h;
-    load_state<KT>(S, src, g.DV, src != nullptr ? g.DK : 0, m, grp, live);
+    const int32_t on = AGG ? 0 : seq_starts(g.q, part.seq, row, a.h0);
+    load_state<KT>(S, a.h0 + on * (row * (g.HV * cells) + at_h), g.DV, on * g.DK, m, grp, live);
   }
   const T* kp = static_cast<const T*>(a.in.k) + hk * g.kh;
   const T* qp = static_cast<const T*>(a.in.q) + hk * g.qh;
@@ -111,7 +112,7 @@ delta_fwd_kernel(FwdArgs a) {
         if constexpr (VLDS) rVt.template load<VEC>(vp + t0 * g.vs, g.vs, n, trans ? 0 : g.DV - vcol0, tid);
         break;
       case 3:
-        if (tid < 3 * kC) rDec = a.w.dec[at * (4 * kC) + tid];
+        if (tid < 4 * kC) rDec = a.w.dec[at * (4 * kC) + tid];
         rGam = a.w.gam[at];
         break;
       default: rT.load(reinterpret_cast<const uint4*>(a.w.tri) + at * kTriFragments, tid, which - 4, which - 3); break;
@@ -142,7 +143,7 @@ delta_fwd_kernel(FwdArgs a) {
     if constexpr (!AGG) rQ.put(sQ, n, g.DK, tid);
     if constexpr (VLDS) rVt.put(sV, n, trans ? 0 : g.DV - vcol0, tid);
     rT.put(sTri, tid);
-    if (tid < 3 * kC) sDec[0][tid] = rDec;
+    if (tid < 4 * kC) sDec[0][tid] = rDec;
     const float gam = rGam;
     // The last chunk's outputs go out here: the wait for the loads above is one for all earlier memory accesses,
     // and stores right before it would be waited for.
@@ -165,7 +166,7 @@ delta_fwd_kernel(FwdArgs a) {
         if constexpr (!AGG) fq[ks & 1][rt] = sQ.rows(16 * rt + m, ks, grp);
       }
     };
-    f32x4 dk[4];
+    f32x4 dk[4], beta[4];
     rows(0);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
@@ -173,7 +174,10 @@ delta_fwd_kernel(FwdArgs a) {
         rows(ks + 1);
       else
 #pragma unroll
-        for (int rt = 0; rt < 4; ++rt) dk[rt] = dec_at(sDec, kDecKey, rt, grp);
+        for (int rt = 0; rt < 4; ++rt) {
+          dk[rt] = dec_at(sDec, kDecKey, rt, grp);
+          beta[rt] = dec_at(sDec, kDecBeta, rt, grp);
+        }
       const Frag<3> sf = split_tiles<3>(S[2 * ks], S[2 * ks + 1]);
       mma_n<3>(fk[ks & 1], sf, R);
       if constexpr (!AGG) mma_t<ORD>(sf, fq[ks & 1], O);
@@ -182,7 +186,7 @@ delta_fwd_kernel(FwdArgs a) {
       phase();
     }
     Frag<3> t0f[4], t1f[2];
-    tri_tiles<false, 0>(t0f, sTri, 0, 0, lane);
+    tri_tiles<0>(t0f, sTri, 0, 0, m, grp);
 #pragma unroll
     for (int rt = 0; rt < 4; ++rt) {
       f32x4 V;
@@ -190,19 +194,19 @@ delta_fwd_kernel(FwdArgs a) {
         V = sV.col4(16 * wave, 16 * rt + 4 * grp, m);
       else
         V = rV.tile(rt, grp, n, wlive);
-      R[rt] = V - dk[rt] * R[rt];
+      R[rt] = beta[rt] * (V - dk[rt] * R[rt]);
     }
     if constexpr (!VLDS) load_v(ahead);
     const Frag<3> rf[2] = {split_tiles<3>(R[0], R[1]), split_tiles<3>(R[2], R[3])};
     phase();
-    tri_tiles<false, 2>(t1f, sTri, 0, 1, lane);
+    tri_tiles<2>(t1f, sTri, 0, 1, m, grp);
     mma_n<3>(t0f, rf[0], D);
     load(ahead, 4);
     phase();
     Frag<ORD> p0f[4], p1f[2];
     float dout[4];  // (the outputs' tiles have the token in the column)
     if constexpr (!AGG) {
-      tri_tiles<false, 0>(p0f, sTri, 1, 0, lane);
+      tri_tiles<0>(p0f, sTri, 1, 0, m, grp);
 #pragma unroll
       for (int rt = 0; rt < 4; ++rt) dout[rt] = sDec[kDecOut][16 * rt + m];
     }
@@ -218,7 +222,7 @@ delta_fwd_kernel(FwdArgs a) {
       const Frag<ORD> df[2] = {split_tiles<ORD>(D[0], D[1]), split_tiles<ORD>(D[2], D[3])};
 #pragma unroll
       for (int rt = 0; rt < 4; ++rt) O[rt] *= dout[rt];
-      tri_tiles<false, 2>(p1f, sTri, 1, 1, lane);
+      tri_tiles<2>(p1f, sTri, 1, 1, m, grp);
       mma_t<ORD>(df[0], p0f, O);
       phase();
       mma_t<ORD>(df[1], p1f, O + 2);
@@ -255,75 +259,77 @@ delta_fwd_kernel(FwdArgs a) {
   }
   if constexpr (!AGG)
     if (chunks > 0) store(part.t0 + (chunks - 1) * kC, part.t1 - part.t0 - (chunks - 1) * kC);
-  if (AGG && trans)
-    store_state<KT>(a.w.trans + (static_cast<int64_t>(p.slot) * g.HV + h) * (DKP * DKP) + col0, DKP, DKP, S, m, grp, live);
-  else if (AGG)
-    store_state<KT>(a.w.carry + at_part, g.DV, g.DK, S, m, grp, live);
+  if (AGG && trans) {
+    if (col0 < DKP) store_tiles<KT>(a.w.trans + ((static_cast<int64_t>(p.slot) * g.HV + h) * KT + col0 / 16) * (KT * 256), S, lane);
+  } else if (AGG) {
+    if (tiles) store_tiles<KT>(a.w.carry + at_part, S, lane);
+  }
   else if (a.h1 != nullptr && row >= 0 && part.t1 == part.end)
     store_state<KT>(a.h1 + row * (g.HV * cells) + at_h, g.DV, g.DK, S, m, grp, live);
 }
 
 // Joins the parts of a sequence: carry holds each part's end state from zero (REV: the gradient of its initial
-// state) and gets its initial state (of its final one), S' = M S + e with the parts' transitions M.
+// state) and gets its initial state (of its final one), S' = M S + e with the parts' transitions M.  The parts come
+// one after the other: four waves have 16 columns of S each, share M in LDS, and load the next part's while they
+// work.  (Every wave loading and splitting M for itself took 13.5 us a part, this 2.6: 128 x 128.)
 template <int DKP, bool REV>
 __global__ void __launch_bounds__(256)
-delta_carry_kernel(DeltaGeom g, DeltaWork w, const float* __restrict__ enter, uint32_t ncb) {
-  constexpr int KT = DKP / 16, KS = DKP / 32;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, grp = lane >> 4;
+delta_carry_kernel(DeltaGeom g, DeltaWork w, const float* __restrict__ enter, uint32_t ncb, int64_t col_tiles) {
+  constexpr int KT = DKP / 16, KS = DKP / 32, kItems = KT * KT * 64 / 256;
+  __shared__ __attribute__((aligned(16))) Tile<DKP, DKP, 3> sM;  // rows: M's columns
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), m = lane & 15, grp = lane >> 4;
   const uint32_t item = blockIdx.x / ncb;
   const int32_t seq = static_cast<int32_t>(item / static_cast<uint32_t>(g.HV));
   const int h = static_cast<int>(item - static_cast<uint32_t>(seq) * g.HV);
-  const int col = static_cast<int>(blockIdx.x - item * ncb) * 64 + 16 * wave + m;
-  const bool live = col < g.DV;
+  const int col0 = static_cast<int>(blockIdx.x - item * ncb) * 64 + 16 * wave;
+  const bool tiles = col0 < g.DV, live = col0 + m < g.DV;
   const int32_t start = seq_off_u(g.q, seq), next = seq_off_u(g.q, seq + 1), end = next < start ? start : next;
   const int32_t slot0 = cut_div(g.part, start) + seq, parts = end > start ? cut_div(g.part, end - start - 1) + 1 : 1;
   const int32_t row = REV ? seq : seq_slot(g.q, seq);
-  const int64_t cells = static_cast<int64_t>(g.DK) * g.DV, step = g.HV * cells;
-  f32x4 S[KT];
+  const int64_t cells = static_cast<int64_t>(g.DK) * g.DV;
+  f32x4 S[KT], E[KT], rM[kItems];
   {
-    const bool any = enter != nullptr && row >= 0 && (REV || !seq_fresh(g.q, seq));
-    const float* src = enter + (any ? row * step + h * cells : 0) + (live ? col : 0);
-#pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int d = 16 * t + 4 * grp + r;
-        S[t][r] = any && live && d < g.DK ? src[static_cast<int64_t>(d) * g.DV] : 0.f;
-      }
+    const int32_t on = REV ? enter != nullptr : seq_starts(g.q, seq, row, enter);
+    load_state<KT>(S, enter + on * ((row * static_cast<int64_t>(g.HV) + h) * cells + (tiles ? col0 : 0)), g.DV,
+                   on * g.DK, m, grp, live);
   }
+  const auto at_part = [&](int32_t i) { return static_cast<int64_t>(slot0 + (REV ? parts - 1 - i : i)) * g.HV + h; };
+  const auto load = [&](int32_t i) {
+    const f32x4* M = reinterpret_cast<const f32x4*>(w.trans + at_part(i) * (KT * KT * 256));
+#pragma unroll
+    for (int j = 0; j < kItems; ++j) rM[j] = M[tid + 256 * j];
+  };
+  if (parts > 1) load(0);
   for (int32_t i = 0; i < parts; ++i) {
-    const int64_t at = static_cast<int64_t>(slot0 + (REV ? parts - 1 - i : i)) * g.HV + h;
-    float* c = w.carry + at * cells + (live ? col : 0);
+    f32x4* c = reinterpret_cast<f32x4*>(w.carry + (at_part(i) * col_tiles + col0 / 16) * (KT * 256)) + lane;
     const bool last = i + 1 == parts;
-    f32x4 E[KT];
 #pragma unroll
-    for (int t = 0; t < KT; ++t)
+    for (int t = 0; t < KT; ++t) E[t] = tiles && !last ? c[64 * t] : f32x4{0.f, 0.f, 0.f, 0.f};
+    if (tiles)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int d = 16 * t + 4 * grp + r;
-        E[t][r] = !last && live && d < g.DK ? c[static_cast<int64_t>(d) * g.DV] : 0.f;
-      }
-#pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int d = 16 * t + 4 * grp + r;
-        if (live && d < g.DK) c[static_cast<int64_t>(d) * g.DV] = S[t][r];
-      }
+      for (int t = 0; t < KT; ++t) c[64 * t] = S[t];
     if (last) break;
-    const float* M = w.trans + at * (DKP * DKP);
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kItems; ++j) {
+      const int x = (tid + 256 * j) / 64;  // column tile x / KT, row tile x % KT
+      sM.put4(16 * (x / KT) + m, 16 * (x % KT) + 4 * grp, rM[j]);
+    }
+    if (i + 2 < parts) load(i + 1);
+    __syncthreads();
+    constexpr int KG = KT < 4 ? KT : 4;
     Frag<3> sf[KS];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) sf[ks] = split_tiles<3>(S[2 * ks], S[2 * ks + 1]);
 #pragma unroll
-    for (int t = 0; t < KT; ++t) {
+    for (int t = 0; t < KT; t += KG)
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        const float* at_m = M + (16 * t + m) * DKP + 32 * ks + 4 * grp;
-        E[t] = mma<3>(split_tiles<3>(*reinterpret_cast<const f32x4*>(at_m), *reinterpret_cast<const f32x4*>(at_m + 16)),
-                      sf[ks], E[t]);
+        Frag<3> f[KG];
+#pragma unroll
+        for (int j = 0; j < KG; ++j) f[j] = sM.cols(16 * (t + j), 32 * ks + 4 * grp, m);
+        mma_n<3>(f, sf[ks], E + t);
       }
-    }
 #pragma unroll
     for (int t = 0; t < KT; ++t) S[t] = E[t];
   }
@@ -337,9 +343,9 @@ hipError_t launch_delta_carry(const DeltaGeom& g, const DeltaWork& w, const floa
   const uint32_t ncb = delta_col_blocks(g.DV, 4);
   const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(g.q.S) * g.HV * ncb));
   switch (delta_dkp(g.DK)) {
-    case 32: hipLaunchKernelGGL((delta_carry_kernel<32, REV>), grid, dim3(256), 0, s, g, w, enter, ncb); break;
-    case 64: hipLaunchKernelGGL((delta_carry_kernel<64, REV>), grid, dim3(256), 0, s, g, w, enter, ncb); break;
-    default: hipLaunchKernelGGL((delta_carry_kernel<128, REV>), grid, dim3(256), 0, s, g, w, enter, ncb); break;
+    case 32: hipLaunchKernelGGL((delta_carry_kernel<32, REV>), grid, dim3(256), 0, s, g, w, enter, ncb, delta_col_tiles(g)); break;
+    case 64: hipLaunchKernelGGL((delta_carry_kernel<64, REV>), grid, dim3(256), 0, s, g, w, enter, ncb, delta_col_tiles(g)); break;
+    default: hipLaunchKernelGGL((delta_carry_kernel<128, REV>), grid, dim3(256), 0, s, g, w, enter, ncb, delta_col_tiles(g)); break;
   }
   return hipGetLastError();
 }
@@ -352,7 +358,7 @@ hipError_t launch_delta_fwd(const DeltaGeom& g, const DeltaIn& in, const DeltaWo
   const int nw = g.vec ? delta_waves(g.DV) : 4;
   const uint32_t vcb = delta_col_blocks(g.DV, nw);
   FwdArgs a{g, in, w, h0, h1, o, s0, vt, delta_col_tiles(g), vcb, vcb, static_cast<uint32_t>(chunk_slots(g.q, g.part))};
-  hipError_t e = launch_delta_prep(g, in, w, false, dtype, s);
+  hipError_t e = launch_delta_prep(g, in, w, dtype, s);
   if (e != hipSuccess) return e;
   const auto run = [&](auto t, auto dkp, auto waves, auto vec) {
     using T = decltype(t);

@@ -44,13 +44,15 @@ inline int64_t delta_col_tiles(const DeltaGeom& g) { return (g.DV + 15) / 16; }
 
 // What the chunks' own products leave for the passes along time, for every
 // chunk slot and value head: the fragments of two 64 x 64 triangles as the
-// matrix units take them, and four scalars for each token.
+// matrix units take them, and four scalars for each token.  A training forward
+// leaves all of it to the backward.
 struct DeltaWork {
   void* tri;       // (slots, HV, 2, parts, 6, 64) 16-byte fragments
   float* dec;      // (slots, HV, 4, 64)
   float* gam;      // (slots, HV): the decay over the chunk
-  float* trans;    // (part slots, HV, DKP, DKP) transitions of the parts, or null
-  float* carry;    // (part slots, HV, DK, DV): end states of the parts from zero, then their initial states
+  float* trans;    // (part slots, HV, DKP / 16, DKP / 16 tiles) transitions of the parts, or null
+  float* carry;    // (part slots, HV, column tiles, DKP / 16 tiles): end states of the parts from zero, then their
+                   // initial states
 };
 
 struct DeltaBwd {
@@ -82,8 +84,7 @@ inline int delta_dkp(int dk) { return dk <= 32 ? 32 : (dk <= 64 ? 64 : 128); }
 // joins the parts, from the initial states (REV: from the gradients of the final ones)
 template <bool REV>
 hipError_t launch_delta_carry(const DeltaGeom& g, const DeltaWork& w, const float* enter, hipStream_t s);
-hipError_t launch_delta_prep(const DeltaGeom& g, const DeltaIn& in, const DeltaWork& w, bool backward, int dtype,
-                             hipStream_t s);
+hipError_t launch_delta_prep(const DeltaGeom& g, const DeltaIn& in, const DeltaWork& w, int dtype, hipStream_t s);
 hipError_t launch_delta_fwd(const DeltaGeom& g, const DeltaIn& in, const DeltaWork& w, const float* h0, float* h1,
                             void* o, float* s0, float* vt, int dtype, hipStream_t s);
 hipError_t launch_delta_bwd(const DeltaGeom& g, const DeltaIn& in, const DeltaWork& w, const DeltaBwd& b, int dtype,

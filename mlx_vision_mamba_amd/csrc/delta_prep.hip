@@ -3,18 +3,16 @@
 //   P_ij = scale (q_i . k_j) exp(G_i - G_j), i >= j     (G: log decays summed)
 // and the tokens' scalars, for the passes along time (delta_fwd.hip,
 // delta_bwd.hip), which take T and P as ready A operands: their bf16 parts in
-// the order in which the lanes load them (forward T diag(beta), backward T' and
-// P').
+// the order in which the lanes load them.
 //
 // A workgroup of four waves takes one chunk and head, a wave 16 rows of both
 // triangles.  A result tile is, as the lanes hold it, an A operand of its
-// transpose: so the forward pass forms K Q' and the inverse of I + A', the
-// backward Q K' and that of I + A, and nothing is transposed.  The inverse M of
-// the triangle (below, its transpose's blocks are meant where it is upper): the
-// four 16 x 16 blocks on the diagonal by substitution, a column a lane (a series
-// in powers of A would cancel: they grow like binomials where keys repeat), the
-// others by products of blocks, M_iw = -M_ii sum_k A_ik M_kw, in the float32
-// matrix instructions, a block column a wave, chained in registers.
+// transpose: so K Q' and the inverse of I + A' are formed, and nothing is
+// transposed.  The inverse: the four 16 x 16 blocks on the diagonal by
+// substitution, a column a lane (a series in powers of A would cancel: they grow
+// like binomials where keys repeat), the others by products of blocks, with M =
+// T': M_iw = -M_ii sum_k A'_ik M_kw, in the float32 matrix instructions, a block
+// column a wave, chained in registers.
 #include "delta_common.h"
 
 namespace mvm {
@@ -29,11 +27,11 @@ __device__ __forceinline__ f32x4 mma_f32(const f32x4& a, const f32x4& b, f32x4 c
   return c;
 }
 
-template <typename T, int DKP, bool BWD>
+template <typename T, int DKP>
 __global__ void __launch_bounds__(256)
 delta_prep_kernel(DeltaGeom g, DeltaIn in, DeltaWork w) {
   constexpr int P = kRawParts<T>;
-  // A (forward: transposed), and the inverses of its diagonal blocks
+  // A', and the inverses of its diagonal blocks
   __shared__ __attribute__((aligned(16))) float sA[kC][kLda], sD[4][16][20];
   __shared__ double sG[kC];
   __shared__ float sBeta[kC], sRk[kC], sRq[kC];
@@ -45,12 +43,10 @@ delta_prep_kernel(DeltaGeom g, DeltaIn in, DeltaWork w) {
   const int n = c.t1 - c.t0;
   const T* kp = static_cast<const T*>(in.k) + c.t0 * g.ks + hk * g.kh;
   const T* qp = static_cast<const T*>(in.q) + c.t0 * g.qs + hk * g.qh;
-  // Tiles of K K' and of the q . k products, rows jt, columns the wave's: for the forward pass rows are keys up
-  // to the wave's tokens, for the backward queries from them on.
+  // Tiles of K K' and K Q': rows jt, the keys up to the wave's tokens, which are the columns.
   f32x4 kk[4], qk[4], qq = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int jt = 0; jt < 4; ++jt) kk[jt] = qk[jt] = qq;
-  const auto need = [&](int jt) { return BWD ? jt >= wave : jt <= wave; };
   const int own = 16 * wave + m;
 #pragma unroll
   for (int ks = 0; ks < DKP / 32; ++ks) {
@@ -62,13 +58,10 @@ delta_prep_kernel(DeltaGeom g, DeltaIn in, DeltaWork w) {
     qq = mma<3>(bq, bq, qq);
 #pragma unroll
     for (int jt = 0; jt < 4; ++jt)
-      if (need(jt)) {
+      if (jt <= wave) {
         const Frag<P> ak = jt == wave ? bk : frag(kp, g.ks, 16 * jt + m);
         kk[jt] = mma<3>(ak, bk, kk[jt]);
-        if (BWD)
-          qk[jt] = mma<3>(jt == wave ? bq : frag(qp, g.qs, 16 * jt + m), bk, qk[jt]);
-        else
-          qk[jt] = mma<3>(ak, bq, qk[jt]);
+        qk[jt] = mma<3>(ak, bq, qk[jt]);
       }
   }
   const double G = log_decay(g, in.g, c.t0, n, h, lane);
@@ -95,33 +88,31 @@ delta_prep_kernel(DeltaGeom g, DeltaIn in, DeltaWork w) {
     dec[kDecKey * kC] = sRk[lane] * eG;
     dec[kDecUp * kC] = sRk[lane] * eR;
     dec[kDecOut * kC] = g.scale * sRq[lane] * eG;
-    dec[kDecBetaKey * kC] = sBeta[lane] * sRk[lane] * eG;
+    dec[kDecBeta * kC] = sBeta[lane];
     if (lane == 0) w.gam[at] = exp_diff(Gc);
   }
   const double Gown = sG[own];
-  const float bown = sBeta[own] * sRk[own], kown = sRk[own], qown = g.scale * sRq[own];
+  const float bown = sBeta[own] * sRk[own], qown = g.scale * sRq[own];
 #pragma unroll
   for (int jt = 0; jt < 4; ++jt)
-    if (need(jt)) {
+    if (jt <= wave) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int j = 16 * jt + 4 * grp + r;
-        // the later token is the column's forward, the row's backward
-        const bool on = BWD ? j >= own : j <= own;
-        const float e = on ? exp_diff(BWD ? sG[j] - Gown : Gown - sG[j]) : 0.f;
-        sA[j][own] = j == own ? 0.f : e * kk[jt][r] * (BWD ? sBeta[j] * sRk[j] * kown : bown * sRk[j]);
-        qk[jt][r] *= e * (BWD ? g.scale * sRq[j] * kown : qown * sRk[j]);
+        const float e = j <= own ? exp_diff(Gown - sG[j]) * sRk[j] : 0.f;
+        sA[j][own] = j < own ? e * kk[jt][r] * bown : 0.f;
+        qk[jt][r] *= e * qown;
       }
     }
   // (a wave's own diagonal block: its own writes)
   float t[16];
 #pragma unroll
   for (int x = 0; x < 16; ++x) {
-    const int i = BWD ? x : 15 - x;
+    const int i = 15 - x;
     float s = i == m ? 1.f : 0.f;
 #pragma unroll
     for (int y = 0; y < 16; ++y)
-      if (BWD ? y < i : y > i) s = fmaf(-sA[16 * wave + i][16 * wave + y], t[y], s);
+      if (y > i) s = fmaf(-sA[16 * wave + i][16 * wave + y], t[y], s);
     t[i] = s;
   }
   if (grp == 0)
@@ -137,27 +128,22 @@ delta_prep_kernel(DeltaGeom g, DeltaIn in, DeltaWork w) {
   }
 #pragma unroll
   for (int x = 0; x < 4; ++x) {
-    const int i = BWD ? x : 3 - x;
-    if (BWD ? i > wave : i < wave) {
+    const int i = 3 - x;
+    if (i < wave) {
       f32x4 s = {0.f, 0.f, 0.f, 0.f};
       const f32x4 z = s;
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        if (BWD ? k < i && k >= wave : k > i && k <= wave)
+        if (k > i && k <= wave)
           s = mma_f32(*reinterpret_cast<const f32x4*>(&sA[16 * i + m][16 * k + 4 * grp]), X[k], s);
       X[i] = -mma_f32(*reinterpret_cast<const f32x4*>(&sD[i][m][4 * grp]), s, z);
     }
   }
-  if (!BWD)  // T diag(beta): the summed index is the row here
-#pragma unroll
-    for (int jt = 0; jt < 4; ++jt)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) X[jt][r] *= sBeta[16 * jt + 4 * grp + r];
-  uint4* out = reinterpret_cast<uint4*>(w.tri) + at * kTriFragments + lane;
+  uint4* out = reinterpret_cast<uint4*>(w.tri) + at * kTriFragments + tri_lane(m, grp);
 #pragma unroll
   for (int ks = 0; ks < 2; ++ks)
-    if (BWD ? 2 * ks + 1 >= wave : 2 * ks <= wave) {
-      const int f = BWD ? (wave < 2 ? 2 * wave + ks : wave + 2) : (wave < 2 ? wave : 2 * wave - 2 + ks);
+    if (2 * ks <= wave) {
+      const int f = wave < 2 ? wave : 2 * wave - 2 + ks;
       const Frag<kTriParts> a = split_tiles<kTriParts>(X[2 * ks], X[2 * ks + 1]),
                             b = split_tiles<kTriParts>(qk[2 * ks], qk[2 * ks + 1]);
 #pragma unroll
@@ -170,17 +156,11 @@ delta_prep_kernel(DeltaGeom g, DeltaIn in, DeltaWork w) {
 
 }  // namespace
 
-hipError_t launch_delta_prep(const DeltaGeom& g, const DeltaIn& in, const DeltaWork& w, bool backward, int dtype,
-                             hipStream_t s) {
+hipError_t launch_delta_prep(const DeltaGeom& g, const DeltaIn& in, const DeltaWork& w, int dtype, hipStream_t s) {
   if (g.q.T == 0) return hipSuccess;
   const dim3 grid(static_cast<unsigned>(chunk_slots(g.q, g.cut) * g.HV));
   return delta_dispatch(dtype, g.DK, [&](auto t, auto dkp) {
-    using T = decltype(t);
-    constexpr int DKP = decltype(dkp)::value;
-    if (backward)
-      hipLaunchKernelGGL((delta_prep_kernel<T, DKP, true>), grid, dim3(256), 0, s, g, in, w);
-    else
-      hipLaunchKernelGGL((delta_prep_kernel<T, DKP, false>), grid, dim3(256), 0, s, g, in, w);
+    hipLaunchKernelGGL((delta_prep_kernel<decltype(t), decltype(dkp)::value>), grid, dim3(256), 0, s, g, in, w);
     return hipGetLastError();
   });
 }

@@ -43,7 +43,7 @@ delta_step_kernel(DeltaGeom g, DeltaIn in, uint32_t ncb, float* __restrict__ sta
   const T* qp = static_cast<const T*>(in.q) + i * g.qs + hk * g.qh;
   const T* vp = static_cast<const T*>(in.v) + i * g.vs + h * g.vh;
   float* sp = states + (static_cast<int64_t>(row) * g.HV + h) * g.DK * static_cast<int64_t>(g.DV);
-  const bool zero = seq_fresh(g.q, i), in_c = c0 < g.DV;  // (DV is a multiple of V)
+  const bool zero = __builtin_amdgcn_readfirstlane(seq_fresh(g.q, i) ? 1 : 0) != 0, in_c = c0 < g.DV;  // (DV is a multiple of V)
   Pack<float, V> S[RP];
   float kd[RP], qd[RP];
 #pragma unroll
