@@ -271,8 +271,9 @@ delta_grads_kernel(BwdArgs a) {
     Tile<kC, DKP, P> K, Q;
   };
   __shared__ __attribute__((aligned(16))) union { Rows r; Keys k; } sm;
-  __shared__ double sG[kC];
-  __shared__ float sBeta[kC], sRk[kC], sRq[kC], sSe[8];
+  __shared__ __attribute__((aligned(16))) double sG[kC];
+  __shared__ __attribute__((aligned(16))) float sBeta[kC], sRk[kC], sRq[kC];
+  __shared__ float sSe[8];
   __shared__ float4 sDot[2][kC];
   const DeltaGeom& g = a.g;
   int tid = threadIdx.x, lane = tid & 63, m = lane & 15, grp = lane >> 4;
@@ -327,25 +328,29 @@ delta_grads_kernel(BwdArgs a) {
     f32x4 rX, rD, rS[kState], rE[kState], rV[2];
     StageRows<T, 32, NT> rO;
     StageRows<T, DKP, NT> rK, rQ;
-    const auto load = [&](int kb) {
+    const auto load = [&](int kb, int which) {
       const int64_t ct = at * a.col_tiles + kb / 16;
       const bool two = kb + 16 < g.DV;  // (the second column tile exists)
-      const int64_t x = (ct + (two ? tid >> 8 : 0)) * (4 * 256) + (tid & 255) * 4;
-      rX = *reinterpret_cast<const f32x4*>(a.b.x + x);
-      rD = *reinterpret_cast<const f32x4*>(a.b.vt + x);
+      if (which == 0) {
+        const int64_t x = (ct + (two ? tid >> 8 : 0)) * (4 * 256) + (tid & 255) * 4;
+        rX = *reinterpret_cast<const f32x4*>(a.b.x + x);
+        rD = *reinterpret_cast<const f32x4*>(a.b.vt + x);
+      } else if (which == 1 || which == 2) {
 #pragma unroll
-      for (int i = 0; i < kState; ++i) {
-        const int j = (tid + NT * i) % (2 * KT * 64);
-        const int64_t y = (ct + (two ? j / (64 * KT) : 0)) * (KT * 256) + j % (64 * KT) * 4;
-        rS[i] = *reinterpret_cast<const f32x4*>(a.b.s0 + y);
-        rE[i] = *reinterpret_cast<const f32x4*>(a.b.dend + y);
+        for (int i = 0; i < kState; ++i) {
+          const int j = (tid + NT * i) % (2 * KT * 64);
+          const int64_t y = (ct + (two ? j / (64 * KT) : 0)) * (KT * 256) + j % (64 * KT) * 4;
+          (which == 1 ? rS : rE)[i] = *reinterpret_cast<const f32x4*>((which == 1 ? a.b.s0 : a.b.dend) + y);
+        }
+      } else {
+        rO.template load<VEC>(dorow + kb, orow, n, g.DV - kb, tid);
+        if (half == 0)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) rV[i] = load4(vrow, kb + 16 * i + 4 * grp, mine ? g.DV : 0, VEC);
       }
-      rO.template load<VEC>(dorow + kb, orow, n, g.DV - kb, tid);
-      if (half == 0)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) rV[i] = load4(vrow, kb + 16 * i + 4 * grp, mine ? g.DV : 0, VEC);
     };
-    load(0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) load(0, i);
     for (int kb = 0; kb < g.DV; kb += 32) {
       const bool two = kb + 16 < g.DV;
       __syncthreads();
@@ -369,13 +374,9 @@ delta_grads_kernel(BwdArgs a) {
       }
       rO.put(sm.r.O, n, g.DV - kb, tid);
       const f32x4 v0 = rV[0], v1 = rV[1];
-      if (kb + 32 < g.DV) {
-        load(kb + 32);
-      } else {
-        rK.template load<VEC>(static_cast<const T*>(a.in.k) + c.t0 * g.ks + hk * g.kh, g.ks, n, g.DK, tid);
-        rQ.template load<VEC>(static_cast<const T*>(a.in.q) + c.t0 * g.qs + hk * g.qh, g.qs, n, g.DK, tid);
-      }
       __syncthreads();
+      // (a few loads between the phases: more at once hold up the wave that issues them; in the last block, q and k)
+      const bool more = kb + 32 < g.DV;
       const int k0 = 4 * grp;
       const Frag<3> bX = sm.r.X.cols(16 * tw, k0, m), bD = sm.r.D.cols(16 * tw, k0, m);
       const Frag<P> bO = sm.r.O.rows(ti, 0, grp);
@@ -409,6 +410,13 @@ delta_grads_kernel(BwdArgs a) {
         if (jt >= tw) {
           XD[jt] = mma<3>(sm.r.X.cols(16 * jt, k0, m), bD, XD[jt]);
           OD[jt] = mma<3>(sm.r.O.rows(16 * jt + m, 0, grp), bD, OD[jt]);
+        }
+        if (more) {
+          load(kb + 32, jt);
+        } else if (jt == 0) {
+          rK.template load<VEC>(static_cast<const T*>(a.in.k) + c.t0 * g.ks + hk * g.kh, g.ks, n, g.DK, tid);
+        } else if (jt == 2) {
+          rQ.template load<VEC>(static_cast<const T*>(a.in.q) + c.t0 * g.qs + hk * g.qh, g.qs, n, g.DK, tid);
         }
         phase();
       }
@@ -469,18 +477,22 @@ delta_grads_kernel(BwdArgs a) {
       phase();
     }
 #pragma unroll
-    for (int jt = 0; jt < 4; ++jt)
+    for (int jt = 0; jt < 4; ++jt) {
+      const int j0 = 16 * jt + 4 * grp;
+      const f32x4 rkj = *reinterpret_cast<const f32x4*>(&sRk[j0]), rqj = *reinterpret_cast<const f32x4*>(&sRq[j0]),
+                  bj = *reinterpret_cast<const f32x4*>(&sBeta[j0]);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int j = 16 * jt + 4 * grp + r;
-        const double Gj = sG[j];
-        const float lo = j <= ti ? exp_diff(Gi - Gj) : 0.f, hi = j >= ti ? exp_diff(Gj - Gi) : 0.f;
-        DO[jt][r] *= j <= ti ? g.scale * sRk[j] * lo : 0.f;
-        DX[jt][r] *= j < ti ? -sRk[j] * lo : 0.f;
-        XD[jt][r] *= j > ti ? -sBeta[j] * sRk[j] * hi : 0.f;
-        OD[jt][r] *= j >= ti ? g.scale * sRq[j] * hi : 0.f;
-        if (r % 2) phase();
+        const int j = j0 + r;
+        const float e = exp_diff(-fabs(Gi - sG[j]));  // from the earlier of the two to the later
+        const float lo = j <= ti ? e : 0.f, hi = j >= ti ? e : 0.f;
+        DO[jt][r] *= g.scale * rkj[r] * lo;
+        DX[jt][r] *= j < ti ? -rkj[r] * e : 0.f;
+        XD[jt][r] *= j > ti ? -bj[r] * rkj[r] * e : 0.f;
+        OD[jt][r] *= g.scale * rqj[r] * hi;
       }
+      phase();
+    }
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       const int j0 = 32 * ks + 4 * grp;
@@ -532,13 +544,8 @@ delta_grads_kernel(BwdArgs a) {
       const int t = 63 - lane;
       const float4 x = sDot[0][t], y = sDot[1][t];
       double s = static_cast<double>(x.z + y.z) - (x.y + y.y) + 2.f * sBeta[t] * (x.x + y.x), all = x.w + y.w;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const double v = __shfl_up(s, o);
-        if (lane >= o) s += v;
-      }
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) all += __shfl_xor(all, o);
+      s = wave_scan(s);
+      all = __shfl(wave_scan(all), 63);
       double sums = 0.0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) sums += sSe[i];

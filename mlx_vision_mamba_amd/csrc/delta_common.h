@@ -523,6 +523,24 @@ __device__ __forceinline__ float sum_g(float x) {
   return x;
 }
 
+// Inclusive sums over a wave's lanes: within rows of 16 by shifts, then the rows' last lanes into the rows behind
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_part(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(u), CTRL, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(u >> 32), CTRL, ROWS, 0xf, false);
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+__device__ __forceinline__ double wave_scan(double x) {
+  x += dpp_part<0x111, 0xf>(x);
+  x += dpp_part<0x112, 0xf>(x);
+  x += dpp_part<0x114, 0xf>(x);
+  x += dpp_part<0x118, 0xf>(x);
+  x += dpp_part<0x142, 0xa>(x);
+  x += dpp_part<0x143, 0xc>(x);
+  return x;
+}
+
 // Lane = token of a chunk of n: the log decay summed from the chunk's start up to it, in 64 bits: the decay between
 // two tokens is the exponential of a difference, which 32 bits would leave with the rounding of the sums.
 __device__ __forceinline__ double log_decay(const DeltaGeom& g, const float* gp, int t0, int n, int h, int lane) {
@@ -531,12 +549,7 @@ __device__ __forceinline__ double log_decay(const DeltaGeom& g, const float* gp,
     const float x = gp[(t0 + static_cast<int64_t>(lane)) * g.gs + h];
     s = x < kMinLogDecay ? kMinLogDecay : x;  // (NaN stays)
   }
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double v = __shfl_up(s, o);
-    if (lane >= o) s += v;
-  }
-  return s;
+  return wave_scan(s);
 }
 __device__ __forceinline__ float exp_diff(double x) { return fast_exp2(static_cast<float>(x * 1.4426950408889634)); }
 
