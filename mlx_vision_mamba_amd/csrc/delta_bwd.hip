@@ -313,11 +313,11 @@ delta_grads_kernel(BwdArgs a) {
     const double Gc = __shfl(G, 63);
 #pragma unroll
     for (int t = 0; t < KH; ++t) accQ[t] = accU[t] = accK[t] = z4;
-    // rows j of a tile, column the lane's token i: D_j . dO_i and D_j . X_i for j <= i, X_j . D_i and dO_j . D_i
-    // for j >= i
-    f32x4 DO[4], DX[4], XD[4], OD[4];
+    // Rows j of a tile, column the lane's token i: D_j . dO_i and D_j . X_i for tiles up to the wave's own, dO_j .
+    // D_i and X_j . D_i behind it; of its own tile both.
+    f32x4 UO[4], UX[4], ownO = z4, ownX = z4;
 #pragma unroll
-    for (int jt = 0; jt < 4; ++jt) DO[jt] = DX[jt] = XD[jt] = OD[jt] = z4;
+    for (int jt = 0; jt < 4; ++jt) UO[jt] = UX[jt] = z4;
     float xv = 0.f, se = 0.f;
     const float btok = mine ? load_beta<T>(g, a.in.beta, row_t, h) : 0.f;
     const T* vrow = static_cast<const T*>(a.in.v) + row_t * g.vs + h * g.vh;
@@ -351,7 +351,9 @@ delta_grads_kernel(BwdArgs a) {
     };
 #pragma unroll
     for (int i = 0; i < 4; ++i) load(0, i);
-    for (int kb = 0; kb < g.DV; kb += 32) {
+    // (the last block apart: its registers are others)
+    const auto block = [&](int kb, auto last_block) {
+      constexpr bool more = !decltype(last_block)::value;
       const bool two = kb + 16 < g.DV;
       __syncthreads();
       {
@@ -376,7 +378,6 @@ delta_grads_kernel(BwdArgs a) {
       const f32x4 v0 = rV[0], v1 = rV[1];
       __syncthreads();
       // (a few loads between the phases: more at once hold up the wave that issues them; in the last block, q and k)
-      const bool more = kb + 32 < g.DV;
       const int k0 = 4 * grp;
       const Frag<3> bX = sm.r.X.cols(16 * tw, k0, m), bD = sm.r.D.cols(16 * tw, k0, m);
       const Frag<P> bO = sm.r.O.rows(ti, 0, grp);
@@ -393,9 +394,11 @@ delta_grads_kernel(BwdArgs a) {
         for (int r = 0; r < 4; ++r) xv = fmaf(x0[r], v0[r], fmaf(x1[r], v1[r], xv));
         if (mine) {
           Quad<T> q;
-          q.set(x0 * btok);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x0[r] *= btok, x1[r] *= btok;
+          q.set(x0);
           q.store(dvrow, kb + 4 * grp, g.DV, VEC);
-          q.set(x1 * btok);
+          q.set(x1);
           q.store(dvrow, kb + 16 + 4 * grp, g.DV, VEC);
         }
       }
@@ -404,14 +407,21 @@ delta_grads_kernel(BwdArgs a) {
       for (int jt = 0; jt < 4; ++jt) {
         if (jt <= tw) {
           const Frag<3> f = sm.r.D.cols(16 * jt, k0, m);
-          DO[jt] = mma<3>(f, bO, DO[jt]);
-          DX[jt] = mma<3>(f, bX, DX[jt]);
+          UO[jt] = mma<3>(f, bO, UO[jt]);
+          UX[jt] = mma<3>(f, bX, UX[jt]);
         }
         if (jt >= tw) {
-          XD[jt] = mma<3>(sm.r.X.cols(16 * jt, k0, m), bD, XD[jt]);
-          OD[jt] = mma<3>(sm.r.O.rows(16 * jt + m, 0, grp), bD, OD[jt]);
+          const Frag<3> fx = sm.r.X.cols(16 * jt, k0, m);
+          const Frag<P> fo = sm.r.O.rows(16 * jt + m, 0, grp);
+          if (jt == tw) {
+            ownX = mma<3>(fx, bD, ownX);
+            ownO = mma<3>(fo, bD, ownO);
+          } else {
+            UX[jt] = mma<3>(fx, bD, UX[jt]);
+            UO[jt] = mma<3>(fo, bD, UO[jt]);
+          }
         }
-        if (more) {
+        if constexpr (more) {
           load(kb + 32, jt);
         } else if (jt == 0) {
           rK.template load<VEC>(static_cast<const T*>(a.in.k) + c.t0 * g.ks + hk * g.kh, g.ks, n, g.DK, tid);
@@ -435,7 +445,10 @@ delta_grads_kernel(BwdArgs a) {
         mma_n<3>(e, bD, accK + t);
         phase();
       }
-    }
+    };
+    int kb = 0;
+    for (; kb + 32 < g.DV; kb += 32) block(kb, std::false_type{});
+    block(kb, std::true_type{});
     xv = sum_g(xv);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) se += __shfl_xor(se, o);
@@ -477,27 +490,28 @@ delta_grads_kernel(BwdArgs a) {
       phase();
     }
 #pragma unroll
-    for (int jt = 0; jt < 4; ++jt) {
-      const int j0 = 16 * jt + 4 * grp;
-      const f32x4 rkj = *reinterpret_cast<const f32x4*>(&sRk[j0]), rqj = *reinterpret_cast<const f32x4*>(&sRq[j0]),
-                  bj = *reinterpret_cast<const f32x4*>(&sBeta[j0]);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int j = j0 + r;
-        const float e = exp_diff(-fabs(Gi - sG[j]));  // from the earlier of the two to the later
-        const float lo = j <= ti ? e : 0.f, hi = j >= ti ? e : 0.f;
-        DO[jt][r] *= g.scale * rkj[r] * lo;
-        DX[jt][r] *= j < ti ? -rkj[r] * e : 0.f;
-        XD[jt][r] *= j > ti ? -bj[r] * rkj[r] * e : 0.f;
-        OD[jt][r] *= g.scale * rqj[r] * hi;
-      }
-      phase();
-    }
-#pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
+      f32x4 DO[2], DX[2], XD[2], OD[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int jt = 2 * ks + i, j0 = 16 * jt + 4 * grp;
+        const f32x4 rkj = *reinterpret_cast<const f32x4*>(&sRk[j0]), rqj = *reinterpret_cast<const f32x4*>(&sRq[j0]),
+                    bj = *reinterpret_cast<const f32x4*>(&sBeta[j0]);
+        const f32x4 uo = jt == tw ? ownO : UO[jt], ux = jt == tw ? ownX : UX[jt];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int j = j0 + r;
+          const float e = exp_diff(-fabs(Gi - sG[j]));  // from the earlier of the two to the later
+          DO[i][r] = j <= ti ? g.scale * rkj[r] * e * UO[jt][r] : 0.f;
+          DX[i][r] = j < ti ? -rkj[r] * e * UX[jt][r] : 0.f;
+          XD[i][r] = j > ti ? -bj[r] * rkj[r] * e * ux[r] : 0.f;
+          OD[i][r] = j >= ti ? g.scale * rqj[r] * e * uo[r] : 0.f;
+        }
+        phase();
+      }
       const int j0 = 32 * ks + 4 * grp;
       if (2 * ks <= tw) {
-        const Frag<3> f1 = split_tiles<3>(DO[2 * ks], DO[2 * ks + 1]), f2 = split_tiles<3>(DX[2 * ks], DX[2 * ks + 1]);
+        const Frag<3> f1 = split_tiles<3>(DO[0], DO[1]), f2 = split_tiles<3>(DX[0], DX[1]);
         Frag<P> k[KH];
 #pragma unroll
         for (int t = 0; t < KH; ++t) k[t] = sm.k.K.cols(d0 + 16 * t, j0, m);
@@ -506,7 +520,7 @@ delta_grads_kernel(BwdArgs a) {
       }
       phase();
       if (2 * ks + 1 >= tw) {
-        const Frag<3> f1 = split_tiles<3>(XD[2 * ks], XD[2 * ks + 1]), f2 = split_tiles<3>(OD[2 * ks], OD[2 * ks + 1]);
+        const Frag<3> f1 = split_tiles<3>(XD[0], XD[1]), f2 = split_tiles<3>(OD[0], OD[1]);
         Frag<P> k[KH];
 #pragma unroll
         for (int t = 0; t < KH; ++t) k[t] = sm.k.K.cols(d0 + 16 * t, j0, m);
