@@ -501,7 +501,7 @@ delta_grads_kernel(BwdArgs a) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int j = j0 + r;
-          const float e = exp_diff(-fabs(Gi - sG[j]));  // from the earlier of the two to the later
+          const float e = exp_diff(j <= ti ? Gi - sG[j] : sG[j] - Gi);  // from the earlier of the two to the later
           DO[i][r] = j <= ti ? g.scale * rkj[r] * e * UO[jt][r] : 0.f;
           DX[i][r] = j < ti ? -rkj[r] * e * UX[jt][r] : 0.f;
           XD[i][r] = j > ti ? -bj[r] * rkj[r] * e * ux[r] : 0.f;

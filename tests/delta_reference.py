@@ -12,7 +12,8 @@ and as many again behind them for the gradients.  Errors of the inverse T and of
 what it is applied to grow by at most the 2-norm of |T|, KAPPA below, formed
 from the inputs.  Along a sequence errors do not grow: for |k| <= 1 and 0 <=
 beta <= 1 every step a (I - beta k k^T) is a contraction, and errors of the
-chunks add up as the root of their number.  So
+chunks add up as the root of their number; a gate above 0 grows them by as much
+as the magnitudes below.  So
 
     |got - ref| <= LAMBDA sqrt(192) 2^-24 STAGES KAPPA sqrt(chunks) mag + half a step of the type
 
@@ -59,7 +60,8 @@ def kappa(off, k, g, beta, qk_l2norm):
         for t in range(off[i], off[i + 1], CHUNK):
             s = slice(t, min(t + CHUNK, off[i + 1]))
             G = g[s].clamp(min=-1e4).cumsum(0).t()
-            A = torch.einsum("ihk,jhk->hij", k[s], k[s]) * (G[:, :, None] - G[:, None, :]).clamp(max=0).exp()
+            D = torch.tril(G[:, :, None] - G[:, None, :], -1)  # (gates above 0 grow)
+            A = torch.einsum("ihk,jhk->hij", k[s], k[s]) * D.exp()
             A = torch.tril(A * beta[s].t()[:, :, None], -1)
             T = torch.linalg.inv(torch.eye(A.shape[-1], dtype=A.dtype) + A)
             worst = max(worst, float(torch.linalg.matrix_norm(T.abs(), 2).max()))

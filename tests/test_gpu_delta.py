@@ -142,6 +142,17 @@ def test_decays_from_none_to_all(cuda):
         assert torch.equal(got[n], again[n]), n
 
 
+@pytest.mark.parametrize("DK", [32, 100])
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_gates_that_grow(cuda, dtype, DK):
+    """g above 0 as well as below: pairs of tokens whose state grew between them."""
+    a, init, do, df = _inputs([70, 131], 1, 2, DK, 32, TYPES[dtype], 14)
+    a["g"] = 0.1 * torch.randn(a["g"].shape, generator=torch.Generator().manual_seed(15))
+    a["g"][20:30] = 0.2
+    _compare(*_run(cuda, [70, 131], a, init, do, df))
+    _compare(*_run(cuda, [70, 131], a, init, do, df, split_len=64))
+
+
 def test_batch_form_and_strides(cuda):
     """(B, L, ...) without offsets; operands that are columns of one wide projection."""
     Bn, L, HK, HV, DK, DV = 3, 21, 2, 4, 16, 24
