@@ -73,6 +73,21 @@ __device__ __forceinline__ float group_sum(float v, int log2) {
   return v;
 }
 
+// A lane's weights: kept over the rows, unless 32 values would not fit in the registers beside the rest
+template <int V, int PER>
+struct RowWeights {
+  static constexpr bool kKeep = PER * V < 32;
+  float w[PER][V], b[PER][V];
+  __device__ __forceinline__ void load(const GnGeom& g, const GnPtr& p, const GnLanes& ln, int i, int l, int c0, bool on) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int c = (l + (i << ln.log2)) * V + j, at = c0 + (on && c < g.Cg ? c : 0);
+      w[i][j] = p.w != nullptr ? p.w[at] : 1.f;
+      b[i][j] = p.b != nullptr ? p.b[at] : 0.f;
+    }
+  }
+};
+
 template <typename T, int V, int PER, bool SILU, bool GATE>
 __global__ void __launch_bounds__(256)
 gn_rows_fwd_kernel(GnGeom g, GnPtr p, GnLanes ln, T* __restrict__ y, float2* __restrict__ stats) {
@@ -83,16 +98,25 @@ gn_rows_fwd_kernel(GnGeom g, GnPtr p, GnLanes ln, T* __restrict__ y, float2* __r
   const bool on = grp < g.G && (lane >> ln.log2) < ln.per_wave;
   const int c0 = (on ? grp : 0) * g.Cg;
   const float inv = 1.f / static_cast<float>(g.Cg);
+  RowWeights<V, PER> wt;
+  if constexpr (wt.kKeep)
+#pragma unroll
+    for (int i = 0; i < PER; ++i) wt.load(g, p, ln, i, l, c0, on);
   for (int64_t n = wave / ln.blocks; n < g.N; n += rows) {
     float v[PER][V];
+    Pack<T, V> x[PER], z[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int c = (l + (i << ln.log2)) * V, at = c0 + (on && c < g.Cg ? c : 0);
+      x[i] = load_pack<T, V>(static_cast<const T*>(p.x) + n * g.xs + at);
+      if (GATE) z[i] = load_pack<T, V>(static_cast<const T*>(p.z) + n * g.zs + at);
+    }
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int c = (l + (i << ln.log2)) * V;
-      const bool ok = on && c < g.Cg;
-      const Pack<T, V> x = load_pack<T, V>(static_cast<const T*>(p.x) + n * g.xs + c0 + (ok ? c : 0));
+      const bool ok = on && (l + (i << ln.log2)) * V < g.Cg;
 #pragma unroll
-      for (int j = 0; j < V; ++j) s += v[i][j] = ok ? to_f32(x.v[j]) : 0.f;
+      for (int j = 0; j < V; ++j) s += v[i][j] = ok ? to_f32(x[i].v[j]) : 0.f;
     }
     const float mean = group_sum<V>(s, ln.log2) * inv;
     s = 0.f;
@@ -108,14 +132,12 @@ gn_rows_fwd_kernel(GnGeom g, GnPtr p, GnLanes ln, T* __restrict__ y, float2* __r
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int c = (l + (i << ln.log2)) * V;
+      if constexpr (!wt.kKeep) wt.load(g, p, ln, i, l, c0, on);
       if (on && c < g.Cg) {
-        Pack<T, V> z{}, out;
-        if (GATE) z = load_pack<T, V>(static_cast<const T*>(p.z) + n * g.zs + c0 + c);
+        Pack<T, V> out;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float w = p.w != nullptr ? p.w[c0 + c + j] : 1.f, b = p.b != nullptr ? p.b[c0 + c + j] : 0.f;
-          out.v[j] = from_f32<T>(gn_out<SILU, GATE>(fmaf(v[i][j] * rstd, w, b), GATE ? to_f32(z.v[j]) : 0.f));
-        }
+        for (int j = 0; j < V; ++j)
+          out.v[j] = from_f32<T>(gn_out<SILU, GATE>(fmaf(v[i][j] * rstd, wt.w[i][j], wt.b[i][j]), GATE ? to_f32(z[i].v[j]) : 0.f));
         store_pack(y + n * g.C + c0 + c, out);
       }
     }
@@ -132,21 +154,11 @@ gn_rows_bwd_kernel(GnGeom g, GnPtr p, GnLanes ln, const float2* __restrict__ sta
   const bool on = grp < g.G && (lane >> ln.log2) < ln.per_wave;
   const int c0 = (on ? grp : 0) * g.Cg;
   const float inv = 1.f / static_cast<float>(g.Cg);
-  // (weights of 32 values a lane do not fit in the registers beside the rest: read for every row)
-  constexpr bool kKeep = PER * V < 32;
-  float w[PER][V], b[PER][V], dw[PER][V], db[PER][V];
-  const auto weights = [&](int i) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int c = (l + (i << ln.log2)) * V + j;
-      const bool ok = on && c < g.Cg;
-      w[i][j] = p.w != nullptr ? p.w[c0 + (ok ? c : 0)] : 1.f;
-      b[i][j] = p.b != nullptr ? p.b[c0 + (ok ? c : 0)] : 0.f;
-    }
-  };
+  RowWeights<V, PER> wt;
+  float dw[PER][V], db[PER][V];
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    if (kKeep) weights(i);
+    if constexpr (wt.kKeep) wt.load(g, p, ln, i, l, c0, on);
 #pragma unroll
     for (int j = 0; j < V; ++j) dw[i][j] = db[i][j] = 0.f;
   }
@@ -160,7 +172,7 @@ gn_rows_bwd_kernel(GnGeom g, GnPtr p, GnLanes ln, const float2* __restrict__ sta
       const int c = (l + (i << ln.log2)) * V;
       const bool ok = on && c < g.Cg;
       const int64_t at = c0 + (ok ? c : 0);
-      if (!kKeep) weights(i);
+      if constexpr (!wt.kKeep) wt.load(g, p, ln, i, l, c0, on);
       const Pack<T, V> x = load_pack<T, V>(static_cast<const T*>(p.x) + n * g.xs + at);
       const Pack<T, V> d = load_pack<T, V>(dy + n * g.C + at);
       Pack<T, V> z{};
@@ -169,10 +181,10 @@ gn_rows_bwd_kernel(GnGeom g, GnPtr p, GnLanes ln, const float2* __restrict__ sta
       for (int j = 0; j < V; ++j) {
         xh[i][j] = (to_f32(x.v[j]) - st.x) * st.y;
         float dzv = 0.f;
-        const float dn = gn_grad<SILU, GATE>(fmaf(xh[i][j], w[i][j], b[i][j]), GATE ? to_f32(z.v[j]) : 0.f,
+        const float dn = gn_grad<SILU, GATE>(fmaf(xh[i][j], wt.w[i][j], wt.b[i][j]), GATE ? to_f32(z.v[j]) : 0.f,
                                              to_f32(d.v[j]), dzv);
         if (GATE) gz[i].v[j] = from_f32<T>(dzv);
-        h[i][j] = ok ? dn * w[i][j] : 0.f;
+        h[i][j] = ok ? dn * wt.w[i][j] : 0.f;
         xh[i][j] = ok ? xh[i][j] : 0.f;
         if (ok) {
           dw[i][j] = fmaf(dn, xh[i][j], dw[i][j]);
@@ -238,6 +250,8 @@ gn_reduce_kernel(const float* part, int64_t nparts, int32_t C, float* dw, float*
 
 // ------------------------------------------------------------------- maps
 
+constexpr int kAhead = 4;  // rows of a thread whose loads are in flight together
+
 // A workgroup takes a run of positions of one sample and 256 V / RI columns, RI positions side by side
 struct GnRun {
   int32_t log2;      // of the threads that lie along a row
@@ -285,17 +299,23 @@ gn_stats_kernel(GnGeom g, GnPtr p, GnRun r, float2* __restrict__ part) {
   for (int j = 0; j < V; ++j) piv[j] = s[j] = q[j] = 0.f;
   const T* x = static_cast<const T*>(p.x) + a.n * g.P * g.xs + (ok ? a.c : 0);
   float cnt = 0.f;
-  for (int64_t t = a.p0 + a.ri; t < a.p1; t += a.RI) {
-    const Pack<T, V> v = load_pack<T, V>(x + t * g.xs);
+  for (int64_t t = a.p0 + a.ri; t < a.p1; t += kAhead * a.RI) {
+    Pack<T, V> v[kAhead];
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float f = to_f32(v.v[j]);
-      piv[j] = cnt == 0.f ? f : piv[j];
-      const float d = f - piv[j];
-      s[j] += d;
-      q[j] = fmaf(d, d, q[j]);
+    for (int i = 0; i < kAhead; ++i) v[i] = load_pack<T, V>(x + (t + i * a.RI < a.p1 ? t + i * a.RI : t) * g.xs);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const bool in = t + i * a.RI < a.p1;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float f = to_f32(v[i].v[j]);
+        piv[j] = cnt == 0.f ? f : piv[j];
+        const float d = in ? f - piv[j] : 0.f;
+        s[j] += d;
+        q[j] = fmaf(d, d, q[j]);
+      }
+      cnt += in ? 1.f : 0.f;
     }
-    cnt += 1.f;
   }
 #pragma unroll
   for (int j = 0; j < V; ++j) {
@@ -323,26 +343,38 @@ gn_join_kernel(GnGeom g, GnRun r, const float2* __restrict__ part, float2* __res
   if (item >= g.N * g.G) return;
   const int64_t n = item / g.G;
   const int lane = threadIdx.x & 63, c0 = static_cast<int>(item - n * g.G) * g.Cg;
-  float cn = 0.f, m = 0.f, q = 0.f;
   const int total = static_cast<int>(r.runs) * g.Cg;
-  for (int i = lane; i < total; i += 64) {
-    const int run = i / g.Cg;
-    const float2 v = part[(n * r.runs + run) * g.C + c0 + (i - run * g.Cg)];
-    const int64_t left = g.P - static_cast<int64_t>(run) * r.len;
-    chan(cn, m, q, static_cast<float>(left < r.len ? left : r.len), v.x, v.y);
-  }
-  for (int o = 1; o < 64; o <<= 1) {
-    const float n2 = __shfl_xor(cn, o), m2 = __shfl_xor(m, o), q2 = __shfl_xor(q, o);
-    // (both lanes of a pair join the lower lane's set with the upper's: equal bits)
-    if (lane & o) {
-      float a = n2, b = m2, c = q2;
-      chan(a, b, c, cn, m, q);
-      cn = a, m = b, q = c;
-    } else {
-      chan(cn, m, q, n2, m2, q2);
+  // the mean of the means, then the squares around it
+  const auto each = [&](auto f) {
+    for (int i = lane; i < total; i += 256) {
+      float2 v[4];
+      float cnt[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int k = i + 64 * j < total ? i + 64 * j : i, run = k / g.Cg;
+        v[j] = part[(n * r.runs + run) * g.C + c0 + (k - run * g.Cg)];
+        const int64_t left = g.P - static_cast<int64_t>(run) * r.len;
+        cnt[j] = i + 64 * j < total ? static_cast<float>(left < r.len ? left : r.len) : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f(v[j], cnt[j]);
     }
-  }
-  if (lane == 0) stats[item] = make_float2(m, 1.f / sqrtf(q / cn + g.eps));
+  };
+  const auto sum = [](double x) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
+    return x;
+  };
+  const double count = static_cast<double>(g.P) * g.Cg;
+  double m = 0.0, q = 0.0;
+  each([&](float2 v, float cnt) { m += static_cast<double>(v.x) * cnt; });
+  m = sum(m) / count;
+  each([&](float2 v, float cnt) {
+    const double d = v.x - m;
+    q += cnt > 0.f ? v.y + d * d * cnt : 0.0;
+  });
+  q = sum(q) / count;
+  if (lane == 0) stats[item] = make_float2(static_cast<float>(m), static_cast<float>(1.0 / sqrt(q + g.eps)));
 }
 
 template <typename T, int V, bool SILU, bool GATE>
@@ -358,15 +390,23 @@ gn_apply_kernel(GnGeom g, GnPtr p, GnRun r, const float2* __restrict__ stats, T*
     sc[j] = st.y * (p.w != nullptr ? p.w[a.c + j] : 1.f);
     b[j] = p.b != nullptr ? p.b[a.c + j] : 0.f;
   }
-  for (int64_t t = a.p0 + a.ri; t < a.p1; t += a.RI) {
-    const int64_t row = a.n * g.P + t;
-    const Pack<T, V> x = load_pack<T, V>(static_cast<const T*>(p.x) + row * g.xs + a.c);
-    Pack<T, V> z{}, out;
-    if (GATE) z = load_pack<T, V>(static_cast<const T*>(p.z) + row * g.zs + a.c);
+  for (int64_t t0 = a.p0 + a.ri; t0 < a.p1; t0 += kAhead * a.RI) {
+    Pack<T, V> x[kAhead], z[kAhead];
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-      out.v[j] = from_f32<T>(gn_out<SILU, GATE>(fmaf(to_f32(x.v[j]) - mean[j], sc[j], b[j]), GATE ? to_f32(z.v[j]) : 0.f));
-    store_pack(y + row * g.C + a.c, out);
+    for (int i = 0; i < kAhead; ++i) {
+      const int64_t row = a.n * g.P + (t0 + i * a.RI < a.p1 ? t0 + i * a.RI : t0);
+      x[i] = load_pack<T, V>(static_cast<const T*>(p.x) + row * g.xs + a.c);
+      if (GATE) z[i] = load_pack<T, V>(static_cast<const T*>(p.z) + row * g.zs + a.c);
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (t0 + i * a.RI < a.p1) {
+        Pack<T, V> out;
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          out.v[j] = from_f32<T>(gn_out<SILU, GATE>(fmaf(to_f32(x[i].v[j]) - mean[j], sc[j], b[j]), GATE ? to_f32(z[i].v[j]) : 0.f));
+        store_pack(y + (a.n * g.P + t0 + i * a.RI) * g.C + a.c, out);
+      }
   }
 }
 
@@ -389,20 +429,26 @@ gn_bwd_sums_kernel(GnGeom g, GnPtr p, GnRun r, const float2* __restrict__ stats,
     b[j] = p.b != nullptr ? p.b[c] : 0.f;
     s1[j] = s2[j] = 0.f;
   }
-  for (int64_t t = a.p0 + a.ri; ok && t < a.p1; t += a.RI) {
-    const int64_t row = a.n * g.P + t;
-    const Pack<T, V> x = load_pack<T, V>(static_cast<const T*>(p.x) + row * g.xs + a.c);
-    const Pack<T, V> d = load_pack<T, V>(dy + row * g.C + a.c);
-    Pack<T, V> z{};
-    if (GATE) z = load_pack<T, V>(static_cast<const T*>(p.z) + row * g.zs + a.c);
+  for (int64_t t0 = a.p0 + a.ri; ok && t0 < a.p1; t0 += 2 * a.RI) {
+    Pack<T, V> x[2], d[2], z[2];
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float xh = (to_f32(x.v[j]) - mean[j]) * rs[j];
-      float dzv = 0.f;
-      const float dn = gn_grad<SILU, GATE>(fmaf(xh, w[j], b[j]), GATE ? to_f32(z.v[j]) : 0.f, to_f32(d.v[j]), dzv);
-      s1[j] = fmaf(dn, xh, s1[j]);
-      s2[j] += dn;
+    for (int i = 0; i < 2; ++i) {
+      const int64_t row = a.n * g.P + (t0 + i * a.RI < a.p1 ? t0 + i * a.RI : t0);
+      x[i] = load_pack<T, V>(static_cast<const T*>(p.x) + row * g.xs + a.c);
+      d[i] = load_pack<T, V>(dy + row * g.C + a.c);
+      if (GATE) z[i] = load_pack<T, V>(static_cast<const T*>(p.z) + row * g.zs + a.c);
     }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (t0 + i * a.RI < a.p1)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float xh = (to_f32(x[i].v[j]) - mean[j]) * rs[j];
+          float dzv = 0.f;
+          const float dn = gn_grad<SILU, GATE>(fmaf(xh, w[j], b[j]), GATE ? to_f32(z[i].v[j]) : 0.f, to_f32(d[i].v[j]), dzv);
+          s1[j] = fmaf(dn, xh, s1[j]);
+          s2[j] += dn;
+        }
   }
 #pragma unroll
   for (int j = 0; j < V; ++j) {
