@@ -11,7 +11,7 @@
 // from the last-level cache where it fits there.  One pass leaves every
 // channel's mean and sum of squared differences over a run of positions, a
 // small one joins them to the groups' statistics, one forms y.  Sums are taken
-// around a value of the run itself, and joined as mean and squares (Chan, Golub
+// around a mean of the run itself, and joined as mean and squares (Chan, Golub
 // and LeVeque, "Algorithms for computing the sample variance", 1983): a mean
 // far from zero costs no digits.  The backward has the same three passes, of the
 // sums of dn and dn xh.
@@ -250,6 +250,198 @@ gn_reduce_kernel(const float* part, int64_t nparts, int32_t C, float* dw, float*
 
 // ------------------------------------------------------------------- maps
 
+// ------------------------------------------------------------------- reductions of a workgroup
+
+// The sums over a workgroup's rows of each of its columns, (1 << log2) lanes of V columns a row: every
+// thread gets its own columns' sums.  A wave's rows by lane exchanges, the waves' through LDS.
+template <int V>
+__device__ __forceinline__ void column_sums(float (&s)[V], int log2, float (*lds)[64][V]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int o = 32; o >= (1 << log2); o >>= 1)
+#pragma unroll
+    for (int j = 0; j < V; ++j) s[j] += __shfl_xor(s[j], o);
+  const int abreast = log2 > 6 ? 1 << (log2 - 6) : 1;  // waves along a row
+  if (abreast == 4) return;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < V; ++j) lds[wave][lane][j] = s[j];
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < V; ++j) s[j] = 0.f;
+  for (int w = wave & (abreast - 1); w < 4; w += abreast)
+#pragma unroll
+    for (int j = 0; j < V; ++j) s[j] += lds[w][lane][j];
+}
+
+__device__ __forceinline__ float2 workgroup_sum(float a, float b, float2* lds) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    a += __shfl_xor(a, o);
+    b += __shfl_xor(b, o);
+  }
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = make_float2(a, b);
+  __syncthreads();
+  return make_float2((lds[0].x + lds[1].x) + (lds[2].x + lds[3].x), (lds[0].y + lds[1].y) + (lds[2].y + lds[3].y));
+}
+
+// ------------------------------------------------------------------- tiles
+
+// A workgroup holds a sample's whole group in registers: PER rows a thread, V columns each, (1 << log2) lanes a row
+struct TileAt {
+  int64_t n;
+  int grp, c, RI, ri;
+  bool ok;
+};
+template <int V>
+__device__ __forceinline__ TileAt tile_at(const GnGeom& g, int log2) {
+  TileAt a;
+  // neighbouring groups, which share cache lines, go to one of the 8 L2s
+  const uint32_t per = gridDim.x / 8, b = blockIdx.x < per * 8 ? blockIdx.x % 8 * per + blockIdx.x / 8 : blockIdx.x;
+  a.n = b / g.G;
+  a.grp = static_cast<int>(b - static_cast<uint32_t>(a.n) * g.G);
+  const int l = (threadIdx.x & ((1 << log2) - 1)) * V;
+  a.ok = l < g.Cg;
+  a.c = a.grp * g.Cg + (a.ok ? l : 0);
+  a.ri = threadIdx.x >> log2;
+  a.RI = 256 >> log2;
+  return a;
+}
+
+template <typename T, int V, int PER, bool SILU, bool GATE>
+__global__ void __launch_bounds__(256)
+gn_tile_fwd_kernel(GnGeom g, GnPtr p, int log2, T* __restrict__ y, float2* __restrict__ stats) {
+  __shared__ float2 lds[4];
+  const TileAt a = tile_at<V>(g, log2);
+  const int P = static_cast<int>(g.P);
+  const T* xp = static_cast<const T*>(p.x) + a.n * g.P * g.xs + a.c;
+  const T* zp = static_cast<const T*>(p.z) + a.n * g.P * g.zs + a.c;
+  Pack<T, V> x[PER], z[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int t = a.ri + i * a.RI, at = t < P ? t : 0;
+    x[i] = load_pack<T, V>(xp + at * g.xs);
+    if (GATE) z[i] = load_pack<T, V>(zp + at * g.zs);
+  }
+  float w[V], b[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    w[j] = p.w != nullptr ? p.w[a.c + j] : 1.f;
+    b[j] = p.b != nullptr ? p.b[a.c + j] : 0.f;
+  }
+  const float inv = 1.f / (static_cast<float>(P) * g.Cg);
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) s += a.ok && a.ri + i * a.RI < P ? to_f32(x[i].v[j]) : 0.f;
+  const float mean = workgroup_sum(s, 0.f, lds).x * inv;
+  s = 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float d = a.ok && a.ri + i * a.RI < P ? to_f32(x[i].v[j]) - mean : 0.f;
+      s = fmaf(d, d, s);
+    }
+  const float rstd = 1.f / sqrtf(workgroup_sum(s, 0.f, lds).x * inv + g.eps);
+  if (threadIdx.x == 0 && stats != nullptr) stats[a.n * g.G + a.grp] = make_float2(mean, rstd);
+  T* yp = y + a.n * g.P * g.C + a.c;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int t = a.ri + i * a.RI;
+    if (a.ok && t < P) {
+      Pack<T, V> out;
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        out.v[j] = from_f32<T>(gn_out<SILU, GATE>(fmaf((to_f32(x[i].v[j]) - mean) * rstd, w[j], b[j]), GATE ? to_f32(z[i].v[j]) : 0.f));
+      store_pack(yp + static_cast<int64_t>(t) * g.C, out);
+    }
+  }
+}
+
+// The two means that dx needs and the channels' sums (part (sample)[2][C]) from the same registers; dn is formed
+// twice, which costs less than the registers that would keep it
+template <typename T, int V, int PER, bool SILU, bool GATE>
+__global__ void __launch_bounds__(256)
+gn_tile_bwd_kernel(GnGeom g, GnPtr p, int log2, const float2* __restrict__ stats, const T* __restrict__ dy,
+                   T* __restrict__ dx, T* __restrict__ dz, float* __restrict__ part) {
+  __shared__ float2 lds[4];
+  __shared__ float sCol[4][64][V];
+  const TileAt a = tile_at<V>(g, log2);
+  const int P = static_cast<int>(g.P);
+  const T* xp = static_cast<const T*>(p.x) + a.n * g.P * g.xs + a.c;
+  const T* zp = static_cast<const T*>(p.z) + a.n * g.P * g.zs + a.c;
+  const int64_t out = a.n * g.P * g.C + a.c;
+  Pack<T, V> x[PER], z[PER], d[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int t = a.ri + i * a.RI, at = t < P ? t : 0;
+    x[i] = load_pack<T, V>(xp + at * g.xs);
+    d[i] = load_pack<T, V>(dy + out + static_cast<int64_t>(at) * g.C);
+    if (GATE) z[i] = load_pack<T, V>(zp + at * g.zs);
+  }
+  const float2 st = stats[a.n * g.G + a.grp];
+  float w[V], b[V], s1[V], s2[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    w[j] = p.w != nullptr ? p.w[a.c + j] : 1.f;
+    b[j] = p.b != nullptr ? p.b[a.c + j] : 0.f;
+    s1[j] = s2[j] = 0.f;
+  }
+  const auto grad = [&](int i, int j, float& xh, float& dzv) {
+    xh = (to_f32(x[i].v[j]) - st.x) * st.y;
+    return gn_grad<SILU, GATE>(fmaf(xh, w[j], b[j]), GATE ? to_f32(z[i].v[j]) : 0.f, to_f32(d[i].v[j]), dzv);
+  };
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      float xh, dzv = 0.f;
+      const float dn = grad(i, j, xh, dzv);
+      if (a.ok && a.ri + i * a.RI < P) {
+        s1[j] = fmaf(dn, xh, s1[j]);
+        s2[j] += dn;
+      }
+    }
+  float u = 0.f, v = 0.f;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    u = fmaf(w[j], s1[j], u);
+    v = fmaf(w[j], s2[j], v);
+  }
+  const float inv = 1.f / (static_cast<float>(P) * g.Cg);
+  const float2 m = workgroup_sum(u, v, lds);
+  const float m1 = m.x * inv, m2 = m.y * inv;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int t = a.ri + i * a.RI;
+    Pack<T, V> ox, oz;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      float xh, dzv = 0.f;
+      const float dn = grad(i, j, xh, dzv);
+      ox.v[j] = from_f32<T>(st.y * (dn * w[j] - m2 - xh * m1));
+      if (GATE) oz.v[j] = from_f32<T>(dzv);
+    }
+    if (a.ok && t < P) {
+      store_pack(dx + out + static_cast<int64_t>(t) * g.C, ox);
+      if (GATE) store_pack(dz + out + static_cast<int64_t>(t) * g.C, oz);
+    }
+  }
+  if (part == nullptr) return;
+  column_sums<V>(s1, log2, sCol);
+  column_sums<V>(s2, log2, sCol);
+  if (a.ri == 0 && a.ok)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      part[a.n * 2 * g.C + a.c + j] = s1[j];
+      part[(a.n * 2 + 1) * g.C + a.c + j] = s2[j];
+    }
+}
+
+// ------------------------------------------------------------------- maps
+
 constexpr int kAhead = 4;  // rows of a thread whose loads are in flight together
 
 // A workgroup takes a run of positions of one sample and 256 V / RI columns, RI positions side by side
@@ -278,103 +470,106 @@ __device__ __forceinline__ GnAt gn_at(const GnGeom& g, const GnRun& r) {
   return a;
 }
 
-// (n, mean, sum of squared differences) of two sets of values as one
-__device__ __forceinline__ void chan(float& n, float& m, float& q, float n2, float m2, float q2) {
-  const float t = n + n2;
-  if (n2 == 0.f) return;
-  const float d = m2 - m, f = n2 / t;
-  q += q2 + d * d * n * f;
-  m = fmaf(d, f, m);
-  n = t;
-}
-
+// Every channel's mean and sum of squared differences over a run.  Sums are taken around the mean of the run's first
+// rows, one for all threads, so that they add up without a division
 template <typename T, int V>
 __global__ void __launch_bounds__(256)
 gn_stats_kernel(GnGeom g, GnPtr p, GnRun r, float2* __restrict__ part) {
-  __shared__ float sN[256], sM[256], sQ[256];
+  __shared__ float lds[4][64][V];
   const GnAt a = gn_at<V>(g, r);
   const bool ok = a.c < g.C;
   float piv[V], s[V], q[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) piv[j] = s[j] = q[j] = 0.f;
   const T* x = static_cast<const T*>(p.x) + a.n * g.P * g.xs + (ok ? a.c : 0);
-  float cnt = 0.f;
-  for (int64_t t = a.p0 + a.ri; t < a.p1; t += kAhead * a.RI) {
+  const int rows = static_cast<int>(a.p1 - a.p0);  // (at least one)
+  for (int t0 = 0; t0 < rows; t0 += kAhead * a.RI) {
     Pack<T, V> v[kAhead];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) v[i] = load_pack<T, V>(x + (t + i * a.RI < a.p1 ? t + i * a.RI : t) * g.xs);
-#pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const bool in = t + i * a.RI < a.p1;
+      const int t = t0 + a.ri + i * a.RI;
+      v[i] = load_pack<T, V>(x + (a.p0 + (t < rows ? t : 0)) * g.xs);
+    }
+    if (t0 == 0) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) piv[j] += a.ri + i * a.RI < rows ? to_f32(v[i].v[j]) : 0.f;
+      column_sums<V>(piv, r.log2, lds);
+      const float inv = 1.f / static_cast<float>(rows < kAhead * a.RI ? rows : kAhead * a.RI);
+#pragma unroll
+      for (int j = 0; j < V; ++j) piv[j] *= inv;
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float f = to_f32(v[i].v[j]);
-        piv[j] = cnt == 0.f ? f : piv[j];
-        const float d = in ? f - piv[j] : 0.f;
+        const float d = t0 + a.ri + i * a.RI < rows ? to_f32(v[i].v[j]) - piv[j] : 0.f;
         s[j] += d;
         q[j] = fmaf(d, d, q[j]);
       }
-      cnt += in ? 1.f : 0.f;
-    }
   }
+  column_sums<V>(s, r.log2, lds);
+  column_sums<V>(q, r.log2, lds);
+  const float inv = 1.f / static_cast<float>(rows);
+  if (a.ri == 0 && ok)
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const float m = cnt > 0.f ? s[j] / cnt : 0.f;
-    __syncthreads();
-    sN[threadIdx.x] = cnt;
-    sM[threadIdx.x] = piv[j] + m;
-    sQ[threadIdx.x] = fmaxf(q[j] - s[j] * m, 0.f);
-    __syncthreads();
-    if (a.ri == 0 && ok && a.c + j < g.C) {
-      float n1 = sN[threadIdx.x], m1 = sM[threadIdx.x], q1 = sQ[threadIdx.x];
-      for (int i = 1; i < a.RI; ++i) {
-        const int o = threadIdx.x + (i << r.log2);
-        chan(n1, m1, q1, sN[o], sM[o], sQ[o]);
-      }
-      part[(a.n * r.runs + a.run) * g.C + a.c + j] = make_float2(m1, q1);
+    for (int j = 0; j < V; ++j) {
+      const float m = s[j] * inv;
+      part[(a.n * r.runs + a.run) * g.C + a.c + j] = make_float2(piv[j] + m, fmaxf(q[j] - s[j] * m, 0.f));
     }
-  }
 }
 
-// A wave a group and sample: its channels' partial statistics as one
+// The sum over a team of W waves of a workgroup of four
+template <int W>
+__device__ __forceinline__ double team_sum(double x, double* lds) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
+  if constexpr (W > 1) {
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
+    __syncthreads();
+    x = (lds[0] + lds[1]) + (lds[2] + lds[3]);
+  }
+  return x;
+}
+
+// W waves a group and sample (one, or the workgroup's four): its channels' partial statistics as one
+template <int W>
 __global__ void __launch_bounds__(256)
 gn_join_kernel(GnGeom g, GnRun r, const float2* __restrict__ part, float2* __restrict__ stats) {
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (item >= g.N * g.G) return;
+  __shared__ double lds[4];
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * (4 / W) + (W == 1 ? threadIdx.x >> 6 : 0);
+  if (item >= g.N * g.G) return;  // (of four waves: all or none)
   const int64_t n = item / g.G;
-  const int lane = threadIdx.x & 63, c0 = static_cast<int>(item - n * g.G) * g.Cg;
-  const int total = static_cast<int>(r.runs) * g.Cg;
+  const int c0 = static_cast<int>(item - n * g.G) * g.Cg, total = static_cast<int>(r.runs) * g.Cg;
   // the mean of the means, then the squares around it
   const auto each = [&](auto f) {
-    for (int i = lane; i < total; i += 256) {
+    for (int i = threadIdx.x & (64 * W - 1); i < total; i += 256 * W) {
       float2 v[4];
       float cnt[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int k = i + 64 * j < total ? i + 64 * j : i, run = k / g.Cg;
+        const int at = i + 64 * W * j, k = at < total ? at : i, run = k / g.Cg;
         v[j] = part[(n * r.runs + run) * g.C + c0 + (k - run * g.Cg)];
         const int64_t left = g.P - static_cast<int64_t>(run) * r.len;
-        cnt[j] = i + 64 * j < total ? static_cast<float>(left < r.len ? left : r.len) : 0.f;
+        cnt[j] = at < total ? static_cast<float>(left < r.len ? left : r.len) : 0.f;
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) f(v[j], cnt[j]);
     }
   };
-  const auto sum = [](double x) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
-    return x;
-  };
   const double count = static_cast<double>(g.P) * g.Cg;
   double m = 0.0, q = 0.0;
   each([&](float2 v, float cnt) { m += static_cast<double>(v.x) * cnt; });
-  m = sum(m) / count;
+  m = team_sum<W>(m, lds) / count;
   each([&](float2 v, float cnt) {
     const double d = v.x - m;
     q += cnt > 0.f ? v.y + d * d * cnt : 0.0;
   });
-  q = sum(q) / count;
-  if (lane == 0) stats[item] = make_float2(static_cast<float>(m), static_cast<float>(1.0 / sqrt(q + g.eps)));
+  q = team_sum<W>(q, lds) / count;
+  if ((threadIdx.x & (64 * W - 1)) == 0)
+    stats[item] = make_float2(static_cast<float>(m), static_cast<float>(1.0 / sqrt(q + g.eps)));
 }
 
 template <typename T, int V, bool SILU, bool GATE>
@@ -415,7 +610,7 @@ template <typename T, int V, bool SILU, bool GATE>
 __global__ void __launch_bounds__(256)
 gn_bwd_sums_kernel(GnGeom g, GnPtr p, GnRun r, const float2* __restrict__ stats, const T* __restrict__ dy,
                    float* __restrict__ part) {
-  __shared__ float sA[256], sB[256];
+  __shared__ float lds[4][64][V];
   const GnAt a = gn_at<V>(g, r);
   const bool ok = a.c < g.C;
   float mean[V], rs[V], w[V], b[V], s1[V], s2[V];
@@ -450,47 +645,40 @@ gn_bwd_sums_kernel(GnGeom g, GnPtr p, GnRun r, const float2* __restrict__ stats,
           s2[j] += dn;
         }
   }
+  column_sums<V>(s1, r.log2, lds);
+  column_sums<V>(s2, r.log2, lds);
+  if (a.ri == 0 && ok) {
+    float* out = part + (a.n * r.runs + a.run) * 2 * g.C + a.c;
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    __syncthreads();
-    sA[threadIdx.x] = s1[j];
-    sB[threadIdx.x] = s2[j];
-    __syncthreads();
-    if (a.ri == 0 && ok && a.c + j < g.C) {
-      float u = s1[j], v = s2[j];
-      for (int i = 1; i < a.RI; ++i) {
-        u += sA[threadIdx.x + (i << r.log2)];
-        v += sB[threadIdx.x + (i << r.log2)];
-      }
-      float* out = part + (a.n * r.runs + a.run) * 2 * g.C + a.c + j;
-      out[0] = u;
-      out[g.C] = v;
+    for (int j = 0; j < V; ++j) {
+      out[j] = s1[j];
+      out[g.C + j] = s2[j];
     }
   }
 }
 
-// A wave a group and sample: the means of dn w xh and dn w
+// W waves a group and sample: the means of dn w xh and dn w
+template <int W>
 __global__ void __launch_bounds__(256)
 gn_bwd_join_kernel(GnGeom g, GnPtr p, GnRun r, const float* __restrict__ part, float2* __restrict__ sums) {
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (item >= g.N * g.G) return;
+  __shared__ double lds[4];
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * (4 / W) + (W == 1 ? threadIdx.x >> 6 : 0);
+  if (item >= g.N * g.G) return;  // (of four waves: all or none)
   const int64_t n = item / g.G;
-  const int lane = threadIdx.x & 63, c0 = static_cast<int>(item - n * g.G) * g.Cg;
+  const int c0 = static_cast<int>(item - n * g.G) * g.Cg, total = static_cast<int>(r.runs) * g.Cg;
   double u = 0.0, v = 0.0;
-  const int total = static_cast<int>(r.runs) * g.Cg;
-  for (int i = lane; i < total; i += 64) {
+#pragma unroll 4
+  for (int i = threadIdx.x & (64 * W - 1); i < total; i += 64 * W) {
     const int run = i / g.Cg, c = c0 + (i - run * g.Cg);
     const float* at = part + (n * r.runs + run) * 2 * g.C + c;
     const float w = p.w != nullptr ? p.w[c] : 1.f;
     u += static_cast<double>(at[0]) * w;
     v += static_cast<double>(at[g.C]) * w;
   }
-  for (int o = 32; o > 0; o >>= 1) {
-    u += __shfl_xor(u, o);
-    v += __shfl_xor(v, o);
-  }
+  u = team_sum<W>(u, lds);
+  v = team_sum<W>(v, lds);
   const double m = static_cast<double>(g.P) * g.Cg;
-  if (lane == 0) sums[item] = make_float2(static_cast<float>(u / m), static_cast<float>(v / m));
+  if ((threadIdx.x & (64 * W - 1)) == 0) sums[item] = make_float2(static_cast<float>(u / m), static_cast<float>(v / m));
 }
 
 template <typename T, int V, bool SILU, bool GATE>
@@ -535,6 +723,7 @@ gn_bwd_apply_kernel(GnGeom g, GnPtr p, GnRun r, const float2* __restrict__ stats
 constexpr int64_t kMaxRows = int64_t{1} << 31;
 constexpr int64_t kMaxBlocks = (int64_t{1} << 24) - 8;  // of 256 threads, 2^32 a launch
 constexpr int kRowValues = 2048;        // of a group, held in registers by 64 lanes
+constexpr int64_t kTileRows = 8;        // of a thread, held in registers
 constexpr int64_t kPartRows = 512;      // partial rows of the channels' gradients
 constexpr size_t kAlign = 256;
 
@@ -588,6 +777,36 @@ GnLanes lanes_of(const GnGeom& g, int V) {
 // workgroups along the rows of the backward
 int64_t row_blocks(const GnGeom& g, const GnLanes& l) {
   return std::max<int64_t>(1, std::min(ceil_div(g.N, 4), std::max<int64_t>(1, kPartRows * 4 / l.blocks)));
+}
+
+// (32 samples of 196 x 384 in 32 groups, gated: 9.4 us forward and 16 backward against 15 and 28 in passes; 256 of them
+// 41 and 129 against 65 and 133)
+// A group in a workgroup's registers, for accesses of V values that groups start on: log2 of the lanes of a row and
+// the rows of a thread, 0 where it does not fit
+struct GnTile {
+  int32_t log2 = 0, per = 0;
+};
+GnTile tile_of(const GnGeom& g, int V) {
+  GnTile t;
+  if (V == 1 || g.Cg % V != 0 || g.Cg > 256 * V || g.N > kMaxBlocks / g.G) return t;
+  t.log2 = log2_ceil(g.Cg / V);
+  const int64_t per = ceil_div(g.P, 256 >> t.log2);
+  if (per <= kTileRows) t.per = per <= 2 ? 2 : per <= 4 ? 4 : 8;
+  return t;
+}
+template <typename F>
+hipError_t with_tile(const GnTile& t, F&& f) {
+  if (t.per == 2) return f(std::integral_constant<int, 2>{});
+  if (t.per == 4) return f(std::integral_constant<int, 4>{});
+  return f(std::integral_constant<int, 8>{});
+}
+
+// Four waves join a group's partial sums where one would take more than four turns of four loads
+bool wide_join(const GnGeom& g, const GnRun& r) {
+  return static_cast<int64_t>(r.runs) * g.Cg > 1024 && g.N <= kMaxBlocks / g.G;
+}
+unsigned join_blocks(const GnGeom& g, const GnRun& r) {
+  return static_cast<unsigned>(wide_join(g, r) ? g.N * g.G : ceil_div(g.N * g.G, 4));
 }
 
 // The maps' runs: enough workgroups to fill the card, of 32 positions at least a thread
@@ -733,6 +952,13 @@ int mvm_group_norm_fwd(const mvm_group_norm_desc* desc, const void* x, const flo
         return hipGetLastError();
       });
     }
+    if constexpr (V > 1)
+      if (const GnTile t = tile_of(g, V); t.per > 0)
+        return with_tile(t, [&](auto per) {
+          hipLaunchKernelGGL((gn_tile_fwd_kernel<T, V, decltype(per)::value, SILU, GATE>), dim3(static_cast<unsigned>(g.N * g.G)),
+                             dim3(256), 0, s, g, p, t.log2, static_cast<T*>(y), reinterpret_cast<float2*>(stats));
+          return hipGetLastError();
+        });
     const GnRun r = run_of(g, V);
     const dim3 grid(static_cast<unsigned>(g.N * r.runs * r.cblocks));
     float2* part = static_cast<float2*>(workspace);
@@ -741,7 +967,8 @@ int mvm_group_norm_fwd(const mvm_group_norm_desc* desc, const void* x, const flo
     hipLaunchKernelGGL((gn_stats_kernel<T, V>), grid, dim3(256), 0, s, g, p, r, part);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(gn_join_kernel, dim3(static_cast<unsigned>(ceil_div(g.N * g.G, 4))), dim3(256), 0, s, g, r, part, st);
+    hipLaunchKernelGGL(wide_join(g, r) ? gn_join_kernel<4> : gn_join_kernel<1>, dim3(join_blocks(g, r)), dim3(256), 0, s, g, r,
+                       part, st);
     if ((e = hipGetLastError()) != hipSuccess) return e;
     hipLaunchKernelGGL((gn_apply_kernel<T, V, SILU, GATE>), grid, dim3(256), 0, s, g, p, r, st, static_cast<T*>(y));
     return hipGetLastError();
@@ -785,6 +1012,18 @@ int mvm_group_norm_bwd(const mvm_group_norm_desc* desc, const void* x, const flo
           return hipGetLastError();
         });
       }
+      if constexpr (V > 1)
+        if (const GnTile t = tile_of(g, V); t.per > 0 && !(g.Cg == V && g.N * g.G > 8192)) {
+          // (many groups of 16 bytes a row would take their lines several times: 1024 samples of 64 x 64 in 16 groups
+          // 58 us against 39 in passes; 8 of 1024 x 256 in 32 groups 14 against 22)
+          nparts = g.N;
+          return with_tile(t, [&](auto per) {
+            hipLaunchKernelGGL((gn_tile_bwd_kernel<T, V, decltype(per)::value, SILU, GATE>),
+                               dim3(static_cast<unsigned>(g.N * g.G)), dim3(256), 0, s, g, p, t.log2, st,
+                               static_cast<const T*>(dy), static_cast<T*>(dx), static_cast<T*>(dz), params ? part : nullptr);
+            return hipGetLastError();
+          });
+        }
       const GnRun r = run_of(g, V);
       const dim3 grid(static_cast<unsigned>(g.N * r.runs * r.cblocks));
       nparts = g.N * r.runs;
@@ -793,8 +1032,8 @@ int mvm_group_norm_bwd(const mvm_group_norm_desc* desc, const void* x, const flo
                          static_cast<const T*>(dy), part);
       hipError_t e = hipGetLastError();
       if (e != hipSuccess) return e;
-      hipLaunchKernelGGL(gn_bwd_join_kernel, dim3(static_cast<unsigned>(ceil_div(g.N * g.G, 4))), dim3(256), 0, s, g, p,
-                         r, part, sums);
+      hipLaunchKernelGGL(wide_join(g, r) ? gn_bwd_join_kernel<4> : gn_bwd_join_kernel<1>, dim3(join_blocks(g, r)), dim3(256), 0,
+                         s, g, p, r, part, sums);
       if ((e = hipGetLastError()) != hipSuccess) return e;
       hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, SILU, GATE>), grid, dim3(256), 0, s, g, p, r, st, sums,
                          static_cast<const T*>(dy), static_cast<T*>(dx), static_cast<T*>(dz));
