@@ -146,6 +146,7 @@ struct DeltaFn : Function<DeltaFn> {
                                {ctx->saved_data["scale"].toDouble(), fl[0] != 0, fl[1], fl[2]});
       a.d.seq = seq_desc(a.seqs, a.seqs.nseq, Tensor(), Tensor());
       c10::OptionalDeviceGuard guard(q.device());
+      check_captured_edges(q, "the gated delta rule");
       const Tensor d_o = go[0].defined() ? go[0].to(v.scalar_type()).contiguous() : at::zeros(v.sizes(), a.v.options());
       const Tensor dh1 = f32(go[1]);
       const auto like = [&](const Tensor& t) { return empty_like_opts(t.sizes(), t, t.scalar_type()); };

@@ -70,6 +70,7 @@ struct GroupNormFn : Function<GroupNormFn> {
     const auto sv = ctx->get_saved_variables();
     const Tensor &x = sv[0], &w = sv[1], &b = sv[2], &z = sv[3];
     c10::OptionalDeviceGuard guard(x.device());
+    check_captured_edges(x, "the group norm");
     const Tensor dy = g[0].to(x.scalar_type()).contiguous();
     Tensor dx = empty_like_opts(x.sizes(), x, x.scalar_type()), dw, db, dz;
     if (w.defined()) dw = empty_like_opts(w.sizes(), x);

@@ -96,6 +96,37 @@ void* stream_of(const Tensor& t) {
   return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream();
 }
 
+bool is_capturing(void* stream) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  // (the null stream is never captured, and not to be asked while another is)
+  return stream != nullptr && hipStreamIsCapturing(static_cast<hipStream_t>(stream), &status) == hipSuccess &&
+         status == hipStreamCaptureStatusActive;
+}
+
+// In a Function's backward: while it is captured into a graph, what takes its gradients must be part of the capture or
+// join it.  A leaf's gradient accumulator, which an eager graph of the same leaf keeps alive, runs on the stream that
+// it was made on; the engine draws that stream into the capture, and waits for it again only where the accumulator
+// runs (backward(), not grad()).  The null stream cannot be drawn into one.  Either ends the process when the capture
+// ends: refused here.
+void check_captured_edges(const Tensor& like, const char* what) {
+  if (!is_capturing(stream_of(like))) return;
+  const auto node = torch::autograd::get_current_node();
+  if (node == nullptr) return;
+  const c10::Stream here = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(like.device().index()).unwrap();
+  const auto* exec = torch::autograd::get_current_graph_task_exec_info();
+  const bool accumulates = exec == nullptr || exec->empty();
+  for (size_t i = 0; i < node->num_outputs(); ++i) {
+    const auto& next = node->next_edge(i).function;
+    if (next == nullptr || !node->task_should_compute_output(i)) continue;
+    const auto s = next->stream();
+    if (!s.has_value() || *s == here || s->device() != here.device()) continue;
+    void* const other = c10::hip::HIPStreamMasqueradingAsCUDA(*s).stream();
+    if (is_capturing(other) || (other != nullptr && accumulates)) continue;
+    throw std::runtime_error(std::string("the backward of ") + what + " is captured into a graph, but an eager graph of "
+                             "its inputs is alive on another stream: delete that graph's outputs before the capture");
+  }
+}
+
 Tensor empty_like_opts(at::IntArrayRef sizes, const Tensor& like, at::ScalarType dt = at::kFloat) {
   return at::empty(sizes, like.options().dtype(dt).requires_grad(false));
 }
