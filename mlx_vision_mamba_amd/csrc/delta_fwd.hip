@@ -271,7 +271,7 @@ delta_fwd_kernel(FwdArgs a) {
 // Joins the parts of a sequence: carry holds each part's end state from zero (REV: the gradient of its initial
 // state) and gets its initial state (of its final one), S' = M S + e with the parts' transitions M.  The parts come
 // one after the other: four waves have 16 columns of S each, share M in LDS, and load the next part's while they
-// work.  (Every wave loading and splitting M for itself took 13.5 us a part, this 2.6: 128 x 128.)
+// work.  (Every wave loading and splitting M for itself took 13.5 us a part, this 5.3: 128 x 128.)
 template <int DKP, bool REV>
 __global__ void __launch_bounds__(256)
 delta_carry_kernel(DeltaGeom g, DeltaWork w, const float* __restrict__ enter, uint32_t ncb, int64_t col_tiles) {

@@ -6,7 +6,9 @@
 //   S' = a S + k d',  d = beta (v - a S^T k),  o = scale (a S^T q + (q . k) d)
 // both sums are over the old state, so it is read once, held in registers and
 // written back.  A workgroup takes a head's columns V CL at a time: CL lanes a
-// row, V columns each, 256 / CL rows side by side.
+// row, V columns each, 256 / CL rows side by side.  512 sequences of 12 heads of
+// 128 x 128 move 812 MB in 190 us, 4.3 TB/s (a large copy: 4.84); loads and stores
+// that pass the caches by took 206.
 #include "delta_common.h"
 
 namespace mvm {
@@ -128,8 +130,13 @@ hipError_t launch_delta_step(const DeltaGeom& g, const DeltaIn& in, float* state
       return hipGetLastError();
     };
     if (!vec) return launch(delta_step_kernel<T, DKP, 32, 1>, 32);
-    return heads * ((g.DV + 127) / 128) >= 512 ? launch(delta_step_kernel<T, DKP, 32, 4>, 128)
-                                               : launch(delta_step_kernel<T, DKP, 8, 4>, 32);
+    // Fewer heads than compute units: more workgroups, of 32 columns (12 heads of 128 x 128 6.2 us, 6.8 by 64 and 9.3 by
+    // 128).  Else 64 (6144 of them 188 us, 194 by 32, 198 by 128, which leaves registers for three waves a SIMD), and
+    // 128 where the state's rows are few and long (1000 heads of 40 x 100: 9.3 us, 13.7 by 64, 19 by 32).
+    if (heads < 256) return launch(delta_step_kernel<T, DKP, 8, 4>, 32);
+    if constexpr (DKP <= 64)
+      if (g.DV > 64) return launch(delta_step_kernel<T, DKP, 32, 4>, 128);
+    return launch(delta_step_kernel<T, DKP, 16, 4>, 64);
   });
 }
 
