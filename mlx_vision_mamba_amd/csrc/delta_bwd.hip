@@ -625,7 +625,7 @@ delta_grads_kernel(BwdArgs a) {
 hipError_t launch_delta_bwd(const DeltaGeom& g, const DeltaIn& in, const DeltaWork& w, const DeltaBwd& b, int dtype,
                             hipStream_t s) {
   // (rows that are read value by value: more registers, so four waves)
-  const int nw = g.vec ? delta_waves(g.DV) : 4;
+  const int nw = g.vec ? g.waves : 4;
   const uint32_t vcb = delta_col_blocks(g.DV, nw);
   BwdArgs a{g, in, w, b, delta_col_tiles(g), vcb, vcb, static_cast<uint32_t>(chunk_slots(g.q, g.part))};
   const auto run = [&](auto t, auto dkp, auto waves, auto vec) {
@@ -654,7 +654,9 @@ hipError_t launch_delta_bwd(const DeltaGeom& g, const DeltaIn& in, const DeltaWo
   return delta_dispatch(dtype, g.DK, [&](auto t, auto dkp) {
     using Four = std::integral_constant<int, 4>;
     if (!g.vec) return run(t, dkp, Four{}, std::false_type{});
-    return nw == 8 ? run(t, dkp, std::integral_constant<int, 8>{}, std::true_type{}) : run(t, dkp, Four{}, std::true_type{});
+    if constexpr (sizeof(t) == 2)
+      if (nw == 8) return run(t, dkp, std::integral_constant<int, 8>{}, std::true_type{});
+    return run(t, dkp, Four{}, std::true_type{});
   });
 }
 

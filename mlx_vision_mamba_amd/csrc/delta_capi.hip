@@ -63,8 +63,8 @@ void pick_parts(const mvm_delta_desc* d, mvm::DeltaGeom& g) {
   if (d->max_len > 0) longest = std::min(longest, d->max_len);
   int64_t len = d->split_len;
   if (len == 0) {
-    const int waves = mvm::delta_waves(g.DV), dkp = mvm::delta_dkp(g.DK);
-    const int64_t vcb = mvm::delta_col_blocks(g.DV, waves), tcb = mvm::delta_col_blocks(dkp, waves);
+    const int dkp = mvm::delta_dkp(g.DK);
+    const int64_t vcb = mvm::delta_col_blocks(g.DV, g.waves), tcb = mvm::delta_col_blocks(dkp, g.waves);
     const int64_t C = mvm::kDeltaChunk, chunks = ceil_div(longest, C);
     const double join = dkp == 128 ? 0.75 : (dkp == 64 ? 0.3 : 0.2);
     // a tenth in favour of whole sequences: less memory, fewer launches
@@ -80,6 +80,15 @@ void pick_parts(const mvm_delta_desc* d, mvm::DeltaGeom& g) {
   // Whole sequences: one part whatever max_len says
   g.parts = len < longest ? static_cast<int32_t>(ceil_div(longest, len)) : 1;
   g.part = mvm::seq_cut(g.parts > 1 ? len : std::max<int64_t>(mvm::kDeltaChunk, T + 1));
+}
+
+// Waves of a workgroup of the passes along time: eight share a chunk's operands where the state has columns for them
+// and the card is full of them (bfloat16, 8191 tokens of 12 heads of 128 x 128: 122 us forward, 134 by four; but 2048
+// tokens of 4 heads 80, and 74 by four, whose chunks take less long).  Float32 operands are three parts, of which
+// eight waves' registers spill (16384 tokens of 12 heads: 568 us forward, 354 by four).
+int pick_waves(const mvm_delta_desc* d, const mvm::DeltaGeom& g) {
+  const int64_t items = (d->seq.tokens / mvm::kDeltaChunk + d->seq.nseq) * g.HV;
+  return d->dtype == MVM_BF16 && g.DV > 64 && items >= 512 ? 8 : 4;
 }
 
 mvm::DeltaGeom geom(const mvm_delta_desc* d) {
@@ -108,6 +117,7 @@ mvm::DeltaGeom geom(const mvm_delta_desc* d) {
   g.l2 = d->qk_l2norm;
   g.beta_f32 = d->beta_dtype == MVM_F32;
   g.cut = mvm::seq_cut(mvm::kDeltaChunk);
+  g.waves = pick_waves(d, g);
   pick_parts(d, g);
   return g;
 }

@@ -355,7 +355,7 @@ template hipError_t launch_delta_carry<true>(const DeltaGeom&, const DeltaWork&,
 hipError_t launch_delta_fwd(const DeltaGeom& g, const DeltaIn& in, const DeltaWork& w, const float* h0, float* h1,
                             void* o, float* s0, float* vt, int dtype, hipStream_t s) {
   // (rows that are read value by value: more registers, so four waves)
-  const int nw = g.vec ? delta_waves(g.DV) : 4;
+  const int nw = g.vec ? g.waves : 4;
   const uint32_t vcb = delta_col_blocks(g.DV, nw);
   FwdArgs a{g, in, w, h0, h1, o, s0, vt, delta_col_tiles(g), vcb, vcb, static_cast<uint32_t>(chunk_slots(g.q, g.part))};
   hipError_t e = launch_delta_prep(g, in, w, dtype, s);
@@ -382,7 +382,9 @@ hipError_t launch_delta_fwd(const DeltaGeom& g, const DeltaIn& in, const DeltaWo
   return delta_dispatch(dtype, g.DK, [&](auto t, auto dkp) {
     using Four = std::integral_constant<int, 4>;
     if (!g.vec) return run(t, dkp, Four{}, std::false_type{});
-    return nw == 8 ? run(t, dkp, std::integral_constant<int, 8>{}, std::true_type{}) : run(t, dkp, Four{}, std::true_type{});
+    if constexpr (sizeof(t) == 2)
+      if (nw == 8) return run(t, dkp, std::integral_constant<int, 8>{}, std::true_type{});
+    return run(t, dkp, Four{}, std::true_type{});
   });
 }
 

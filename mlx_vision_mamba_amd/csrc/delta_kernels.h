@@ -9,9 +9,6 @@ namespace mvm {
 
 constexpr int kDeltaChunk = 64;   // tokens of a chunk
 constexpr int64_t kDeltaMaxStride = 1 << 25;  // of v's and o's rows: 12 of them and a row are within 2^31 bytes
-// Waves of a workgroup of the passes along time, 16 columns of the state each: eight share a chunk's operands
-// where the state has columns for them.
-inline int delta_waves(int dv) { return dv > 64 ? 8 : 4; }
 inline uint32_t delta_col_blocks(int cols, int waves) {
   return static_cast<uint32_t>((cols + 16 * waves - 1) / (16 * waves));
 }
@@ -28,6 +25,7 @@ struct DeltaGeom {
   SeqCut cut;                     // chunks
   SeqCut part;                    // parts of the time axis, whole chunks
   int32_t parts;                  // 1: a sequence is one part
+  int32_t waves;                  // of a workgroup of the passes along time, 16 columns of the state each
 };
 
 struct DeltaIn {

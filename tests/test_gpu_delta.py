@@ -93,6 +93,15 @@ def test_packed_splits(cuda, dtype, DK, DV, split):
     _compare(*_run(cuda, lens, *ins, split_len=split, use_init=False, max_len=70))
 
 
+@pytest.mark.parametrize("split", [0, 64])
+@pytest.mark.parametrize("DK,DV", [(16, 128), (64, 72), (128, 96)])
+def test_packed_many_heads(cuda, DK, DV, split):
+    """Chunks and heads for a full card: bfloat16 takes its wider workgroups."""
+    lens = [70, 0, 64, 5, 129]
+    ins = _inputs(lens, 52, 104, DK, DV, torch.bfloat16, 32, extra=3)
+    _compare(*_run(cuda, lens, *ins, split_len=split))
+
+
 def test_prefill_in_parts(cuda):
     """A cache that is read and written by sequences in several parts."""
     lens = [200, 70, 0, 130]
