@@ -22,6 +22,7 @@
  *   with strides, the last dimension contiguous.  g (tokens, value_heads)
  *   float32, beta the same in beta_dtype: rows with a stride.  o and all
  *   gradients are contiguous.  States: (rows, value_heads, dk, dv) float32.
+ *   Strides are at most 2^29 - 1 values, v_stride and value_heads * dv 2^25.
  *
  * g is taken as at least -10000 (exp of which is 0).  Products run over chunks
  * of 64 tokens: a value that is not finite makes its sequence's outputs

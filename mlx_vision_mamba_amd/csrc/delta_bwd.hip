@@ -7,7 +7,8 @@
 //   X  = T' dD
 //   dS = e^Gc E + Q' diag(e^G) dO' - K' diag(beta e^G) X
 // the same chain of products as the forward's, with a wave keeping 16 columns
-// of E in registers.  It leaves X and every chunk's E.
+// of E in registers.  It leaves X and every chunk's E.  (16384 tokens of 12 heads of
+// 128 x 128 in bfloat16: 137 us, as bound as the forward's.)
 //
 // Then every chunk and key head by itself (delta_grads_kernel), with M_ij =
 // exp(G_i - G_j):
@@ -258,6 +259,8 @@ __device__ void zero_rows(const BwdArgs& a, int32_t t0, int32_t t1, int hk, int 
 
 // Eight waves a chunk and key head: a wave has 16 tokens and half of the keys' columns; the small triangles of its
 // tokens are formed by both waves.  GROUPED: more than one value head a key head.
+// Bound by waits and issue: 16384 tokens of 12 heads of 128 x 128 in bfloat16 take 381 us, MFMA busy 23 %, and two waves
+// a SIMD that wait 45 % of their cycles; K, Q and the triangles fill LDS for one workgroup a compute unit.
 template <typename T, int DKP, bool VEC, bool GROUPED>
 __global__ void __launch_bounds__(512)
 delta_grads_kernel(BwdArgs a) {

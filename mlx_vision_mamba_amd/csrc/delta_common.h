@@ -146,13 +146,6 @@ struct Tile {
     }
     return f;
   }
-  // the same in the plain order (k0 includes 8g)
-  __device__ __forceinline__ Frag<P> rows_plain(int row, int k0) const {
-    Frag<P> f;
-#pragma unroll
-    for (int p = 0; p < P; ++p) f.p[p] = *reinterpret_cast<const uint4*>(v + p * kPlane + at(row, k0));
-    return f;
-  }
   // column c0 + m of the tile, summed index rows r0 .. r0 + 31 in the chained order (r0 includes 4g).  The
   // transposing read hands lane i of 16 the i % 4-th values of the 8-byte words at the addresses of lanes
   // i / 4, i / 4 + 4, + 8, + 12.
@@ -578,8 +571,6 @@ __device__ __forceinline__ f32x4 dec_at(const float (*dec)[kC], DecRow which, in
   return *reinterpret_cast<const f32x4*>(&dec[which][16 * rt + 4 * grp]);
 }
 
-// Waves of a workgroup of the passes along time, 16 state columns each: eight share a chunk's operands where there
-// are columns for them
 // Instructions stay on their side: without it the reads of all operands are moved to the front, and their
 // registers spill.  Each phase reads the next one's operands.
 __device__ __forceinline__ void phase() { __builtin_amdgcn_sched_barrier(0); }

@@ -44,8 +44,9 @@ def gated_delta_rule_packed(q, k, v, g, beta, offsets=None, *, scale=None, qk_l2
     ``selective_scan_packed``; without offsets (B, L, ...), one sequence a batch
     row.  H_v is a multiple of H_k: value head h reads key head h // (H_v / H_k).
     D_k 1..128, D_v 1..512.  q, k, v, o share a type, float32 or bfloat16, and
-    may have any strides but a contiguous last dimension; beta has it too or is
-    float32; g is taken in float32, and as at least -10000.
+    may have any strides (v's rows up to 2^25 values apart) but a contiguous last
+    dimension; beta has it too or is float32; g is taken in float32, and as at
+    least -10000.
 
         S = exp(g_t) S;  d = beta_t (v_t - S^T k_t);  S = S + k_t d^T;  o_t = scale S^T q_t
 

@@ -124,6 +124,25 @@ def test_delta_rows_off_16_bytes(cuda, dtype, shift):
         _compare({"o": o, "final": final, **{"d" + n: g for n, g in zip([*leaves, "initial"], grads)}}, want, factor)
 
 
+@pytest.mark.parametrize("split", [0, 64])
+def test_delta_of_no_tokens(cuda, split):
+    """Sequences without tokens hand their states and gradients through, in both forms."""
+    init = torch.randn(2, 4, 8, 12, generator=torch.Generator().manual_seed(15)).to(cuda).requires_grad_(True)
+    df = torch.randn(2, 4, 8, 12, generator=torch.Generator().manual_seed(16)).to(cuda)
+    for lead, off in (((0,), [0, 0, 0]), ((2, 0), None)):
+        r = lambda *s: torch.zeros(*lead, *s, device=cuda, requires_grad=True)  # noqa: E731
+        leaves = [r(2, 8), r(2, 8), r(4, 12), r(4), r(4)]
+        o, final = mvm.gated_delta_rule_packed(*leaves, off, initial_states=init, split_len=split)
+        assert o.shape == (*lead, 4, 12) and torch.equal(final, init)
+        grads = torch.autograd.grad([o, final], [*leaves, init], [torch.zeros_like(o), df])
+        assert torch.equal(grads[-1], df) and all(g.shape == x.shape for g, x in zip(grads, leaves))
+    states = init.detach().clone()
+    o = mvm.gated_delta_rule_prefill(*[x.detach() for x in leaves], states, fresh=torch.tensor([True, False], device=cuda))
+    assert o.shape == (2, 0, 4, 12) and not states[0].any() and torch.equal(states[1], init[1])
+    o = mvm.gated_delta_rule_step(*[x.detach()[0] for x in leaves], states)
+    assert o.shape == (0, 4, 12)
+
+
 def test_delta_past_32_bits(cuda):
     """More than 2^31 values: the last sequence is what it is by itself, and so are its gradients."""
     HV, D, tail = 12, 128, 200
