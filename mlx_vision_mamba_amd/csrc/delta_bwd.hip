@@ -260,7 +260,7 @@ __device__ void zero_rows(const BwdArgs& a, int32_t t0, int32_t t1, int hk, int 
 // Eight waves a chunk and key head: a wave has 16 tokens and half of the keys' columns; the small triangles of its
 // tokens are formed by both waves.  GROUPED: more than one value head a key head.
 // Bound by waits and issue: 16384 tokens of 12 heads of 128 x 128 in bfloat16 take 381 us, MFMA busy 23 %, and two waves
-// a SIMD that wait 45 % of their cycles; K, Q and the triangles fill LDS for one workgroup a compute unit.
+// a SIMD that wait 45 % of their cycles; their 256 registers leave no room for a second workgroup.
 template <typename T, int DKP, bool VEC, bool GROUPED>
 __global__ void __launch_bounds__(512)
 delta_grads_kernel(BwdArgs a) {

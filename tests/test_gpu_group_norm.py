@@ -63,13 +63,25 @@ def test_maps(cuda, dtype, shape, groups):
     _compare(*_run(cuda, groups, ins, dy))
 
 
+# groups of 256, 128 and 64 lanes, of as many rows as a workgroup's registers hold and of one more; many groups of one
+# access; partial sums for four waves to join
+@pytest.mark.parametrize("shape,groups", [((2, 8, 1024), 1), ((2, 9, 1024), 1), ((3, 16, 512), 1), ((3, 17, 512), 1),
+                                          ((2, 33, 256), 1), ((2, 64, 96), 2), ((2100, 3, 16), 4), ((1, 20000, 32), 2),
+                                          ((9, 1, 2, 2048), 1)])
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_tiles_and_their_borders(cuda, dtype, shape, groups):
+    ins, dy = _inputs(shape, TYPES[dtype], 14)
+    _compare(*_run(cuda, groups, ins, dy, silu=True, gate=True))
+    _compare(*_run(cuda, groups, ins, dy, gate=False))
+
+
 def test_rows_many(cuda):
     """More rows than the waves that walk them."""
     ins, dy = _inputs((9000, 48), torch.bfloat16, 4)
     _compare(*_run(cuda, 3, ins, dy))
 
 
-@pytest.mark.parametrize("shape", [(4, 96), (2, 50, 96)])
+@pytest.mark.parametrize("shape", [(4, 96), (2, 50, 96), (2, 3000, 96)])
 def test_a_mean_far_from_zero(cuda, shape):
     """Means of thousands of standard deviations: what the values' own rounding leaves is kept."""
     ins, dy = _inputs(shape, torch.float32, 5)
@@ -80,7 +92,7 @@ def test_a_mean_far_from_zero(cuda, shape):
     assert float((got["y"].detach().cpu().double() - want["y"].v).norm() / want["y"].v.norm()) < 4096 * 2 ** -22
 
 
-@pytest.mark.parametrize("shape", [(4, 32), (2, 50, 32)])
+@pytest.mark.parametrize("shape", [(4, 32), (2, 50, 32), (2, 5000, 32)])
 def test_constant_groups_and_eps(cuda, shape):
     ins, dy = _inputs(shape, torch.float32, 6)
     ins["x"][..., :8] = 3.0
@@ -88,7 +100,7 @@ def test_constant_groups_and_eps(cuda, shape):
         _compare(*_run(cuda, 4, ins, dy, eps=eps))
 
 
-@pytest.mark.parametrize("shape", [(4, 32), (2, 50, 32)])
+@pytest.mark.parametrize("shape", [(4, 32), (2, 50, 32), (2, 5000, 32)])
 def test_a_value_that_is_not_finite_stays_in_its_group(cuda, shape):
     ins, dy = _inputs(shape, torch.float32, 7)
     clean, _ = _run(cuda, 4, ins, dy)
