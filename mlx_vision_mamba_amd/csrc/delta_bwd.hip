@@ -18,13 +18,16 @@
 //   dq_i    = scale (e^(G_i) S dO_i + sum_{j <= i} M_ij (dO_i . D_j) k_j)
 //   dk_i    = beta_i u_i + e^(Gc - G_i) E D_i - sum_{j > i} M_ji beta_j (X_j . D_i) k_j
 //             + scale sum_{j >= i} M_ji (dO_j . D_i) q_j
-//   dG_i    = q_i . dq_i - k_i . dk_i + 2 beta_i k_i . u_i
-//   dg_t    = sum_{i >= t} dG_i + sum_i e^(Gc - G_i) k_i . E D_i + e^Gc <S, E>
-// where dG collects, for each factor exp(G_i), the gradients' own products, and
-// the last two terms are those of the factor exp(Gc).  All products are formed
-// with the token as the result's column: then the small triangles are B
-// operands as they come out, a token's scalars are a lane's, and a lane holds
-// four consecutive values of dq and dk.
+//   dg_t    = e^Gc <S, E> + sum_{i < t} e^(Gc - G_i) k_i . E D_i
+//             + sum_{i >= t} e^(G_i) (scale q_i . S dO_i - beta_i k_i . S X_i)
+//             + sum_{j < t <= i} M_ij (scale (dO_i . D_j) (q_i . k_j) - beta_i (X_i . D_j) (k_i . k_j))
+// where each product of dg_t has exp(g_t) as a factor, and its sums add, so
+// that a gate that lets little through keeps its gradient's digits.  (The same
+// sums as differences of q . dq, k . dk and k . u hold products without that
+// factor, of which only the rounding is left: 1e-3 of dg at g = -8.)  All
+// products are formed with the token as the result's column: then the small
+// triangles are B operands as they come out, a token's scalars are a lane's,
+// and a lane holds four consecutive values of dq and dk.
 #include "delta_common.h"
 
 namespace mvm {
@@ -257,6 +260,45 @@ __device__ void zero_rows(const BwdArgs& a, int32_t t0, int32_t t1, int hk, int 
   }
 }
 
+// The sum over the 16 lanes of a row
+__device__ __forceinline__ float row_sum(float x) {
+  x += dpp<kRowRor8>(x);
+  x += dpp<kRowRor4>(x);
+  x += dpp<0x122>(x);
+  return x + dpp<0x121>(x);
+}
+
+// x of a pair's even and odd row of 16 lanes, and of a wave's lower and upper half (both results through one 64-bit
+// value, as in scan_common.h)
+struct Halves {
+  float lo, hi;
+};
+__device__ __forceinline__ Halves halves(uint64_t w) {
+  return {__uint_as_float(static_cast<uint32_t>(w)), __uint_as_float(static_cast<uint32_t>(w >> 32))};
+}
+__device__ __forceinline__ Halves rows_of_pair(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return halves(__builtin_bit_cast(uint64_t, __builtin_amdgcn_permlane16_swap(u, u, false, false)));
+}
+__device__ __forceinline__ Halves halves_of_wave(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return halves(__builtin_bit_cast(uint64_t, __builtin_amdgcn_permlane32_swap(u, u, false, false)));
+}
+
+// W: of one token i (the lane's column) and the tile's rows j, zero from j = i on.  Adds to `before`, the sum over the
+// tiles before, and returns for each row's number t the sum of W over j < t, where t <= i, over the tile's tokens.
+__device__ __forceinline__ f32x4 pairs_across(const f32x4& W, float& before, int j0, int ti, int m, int grp) {
+  const float s0 = W[0], s1 = s0 + W[1], s2 = s1 + W[2];
+  const Halves p = rows_of_pair(s2 + W[3]), q = halves_of_wave(p.lo + p.hi);
+  const float b = before + ((grp & 1 ? p.lo : 0.f) + (grp & 2 ? q.lo : 0.f));
+  before += q.lo + q.hi;
+  const f32x4 pre = {b, b + s0, b + s1, b + s2};
+  f32x4 f;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) f[r] = row_sum(j0 + r <= ti ? pre[r] : 0.f);
+  return f;
+}
+
 // Eight waves a chunk and key head: a wave has 16 tokens and half of the keys' columns; the small triangles of its
 // tokens are formed by both waves.  GROUPED: more than one value head a key head.
 // Bound by waits and issue: 16384 tokens of 12 heads of 128 x 128 in bfloat16 take 381 us, MFMA busy 23 %, and two waves
@@ -277,7 +319,8 @@ delta_grads_kernel(BwdArgs a) {
   __shared__ __attribute__((aligned(16))) double sG[kC];
   __shared__ __attribute__((aligned(16))) float sBeta[kC], sRk[kC], sRq[kC];
   __shared__ float sSe[8];
-  __shared__ float4 sDot[2][kC];
+  __shared__ float sDot[5][2][kC];  // k . u | k . E D | of the factor exp(G_i) | with qk_l2norm: k . dk | q . dq
+  __shared__ float sPair[8][kC];
   const DeltaGeom& g = a.g;
   int tid = threadIdx.x, lane = tid & 63, m = lane & 15, grp = lane >> 4;
   const int wave = wave_id(), tw = wave & 3, half = wave >> 2, d0 = half * KH * 16;  // token tile, first key column
@@ -309,6 +352,8 @@ delta_grads_kernel(BwdArgs a) {
     }
     __syncthreads();
     const double G = log_decay(g, a.in.g, c.t0, n, h, lane);
+    // (gates below the least one have no part in the outputs)
+    const uint64_t below = __ballot(lane < n && a.in.g[(c.t0 + static_cast<int64_t>(lane)) * g.gs + h] < kMinLogDecay);
     if (wave == 0) {
       sG[lane] = G;
       sBeta[lane] = lane < n ? load_beta<T>(g, a.in.beta, c.t0 + lane, h) : 0.f;
@@ -481,17 +526,58 @@ delta_grads_kernel(BwdArgs a) {
     __syncthreads();
     const double Gi = sG[ti];
     const float eG = exp_diff(Gi), eR = exp_diff(Gc - Gi), bi = sBeta[ti];
-    float kh = 0.f;
+    float kh = 0.f, us = 0.f, qs = 0.f;
 #pragma unroll
     for (int t = 0; t < KH; ++t) {
       accQ[t] *= g.scale * eG;
       accU[t] *= -eG;
       accK[t] *= eR;
-      const f32x4 x = sm.k.K.get4(ti, d0 + 16 * t + 4 * grp);
+      const f32x4 x = sm.k.K.get4(ti, d0 + 16 * t + 4 * grp), y = sm.k.Q.get4(ti, d0 + 16 * t + 4 * grp);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) kh = fmaf(accK[t][r], x[r], kh);
+      for (int r = 0; r < 4; ++r) {
+        kh = fmaf(accK[t][r], x[r], kh);
+        us = fmaf(accU[t][r], x[r], us);
+        qs = fmaf(accQ[t][r], y[r], qs);
+      }
       phase();
     }
+    // The decay between two tokens, from the earlier to the later, on all pairs; and dg's sums over them, of which the
+    // waves of the first half take those of q and k, the second half's those of k and k
+    {
+      const float own = half == 0 ? g.scale * rq : -bi * rk;
+      float before = 0.f;
+#pragma unroll
+      for (int jt = 0; jt < 4; ++jt) {
+        const int j0 = 16 * jt + 4 * grp;
+        f32x4 e;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) e[r] = exp_diff(j0 + r <= ti ? Gi - sG[j0 + r] : sG[j0 + r] - Gi);
+        UO[jt] *= e;
+        UX[jt] *= e;
+        if (jt == tw) {
+          ownO *= e;
+          ownX *= e;
+        }
+        phase();
+        if (jt <= tw) {
+          f32x4 W = z4;
+          int row = ti;  // (read anew for every tile: kept over them, the token's operands would spill)
+          asm volatile("" : "+v"(row));
+#pragma unroll
+          for (int s = 0; s < DKP / 32; ++s) {
+            W = mma<3>(sm.k.K.rows(16 * jt + m, s, grp), (half == 0 ? sm.k.Q : sm.k.K).rows(row, s, grp), W);
+            if constexpr (P == 3) phase();
+          }
+          const f32x4 rkj = *reinterpret_cast<const f32x4*>(&sRk[j0]);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) W[r] = j0 + r < ti ? W[r] * own * rkj[r] * (half == 0 ? UO : UX)[jt][r] : 0.f;
+          const f32x4 f = pairs_across(W, before, j0, ti, m, grp);
+          if (m < 4) sPair[wave][j0 + m] = m == 0 ? f[0] : m == 1 ? f[1] : m == 2 ? f[2] : f[3];
+        }
+        phase();
+      }
+    }
+    constexpr int KG = (P == 3 || GROUPED) && KH > 2 ? 2 : KH;  // column tiles whose operands are held at a time
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       f32x4 DO[2], DX[2], XD[2], OD[2];
@@ -504,33 +590,40 @@ delta_grads_kernel(BwdArgs a) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int j = j0 + r;
-          const float e = exp_diff(j <= ti ? Gi - sG[j] : sG[j] - Gi);  // from the earlier of the two to the later
-          DO[i][r] = j <= ti ? g.scale * rkj[r] * e * UO[jt][r] : 0.f;
-          DX[i][r] = j < ti ? -rkj[r] * e * UX[jt][r] : 0.f;
-          XD[i][r] = j > ti ? -bj[r] * rkj[r] * e * ux[r] : 0.f;
-          OD[i][r] = j >= ti ? g.scale * rqj[r] * e * uo[r] : 0.f;
+          DO[i][r] = j <= ti ? g.scale * rkj[r] * UO[jt][r] : 0.f;
+          DX[i][r] = j < ti ? -rkj[r] * UX[jt][r] : 0.f;
+          XD[i][r] = j > ti ? -bj[r] * rkj[r] * ux[r] : 0.f;
+          OD[i][r] = j >= ti ? g.scale * rqj[r] * uo[r] : 0.f;
         }
         phase();
       }
       const int j0 = 32 * ks + 4 * grp;
       if (2 * ks <= tw) {
         const Frag<3> f1 = split_tiles<3>(DO[0], DO[1]), f2 = split_tiles<3>(DX[0], DX[1]);
-        Frag<P> k[KH];
 #pragma unroll
-        for (int t = 0; t < KH; ++t) k[t] = sm.k.K.cols(d0 + 16 * t, j0, m);
-        mma_n<3>(k, f1, accQ);
-        mma_n<3>(k, f2, accU);
+        for (int t = 0; t < KH; t += KG) {
+          Frag<P> k[KG];
+#pragma unroll
+          for (int i = 0; i < KG; ++i) k[i] = sm.k.K.cols(d0 + 16 * (t + i), j0, m);
+          mma_n<3>(k, f1, accQ + t);
+          mma_n<3>(k, f2, accU + t);
+          if constexpr (KG < KH) phase();
+        }
       }
       phase();
       if (2 * ks + 1 >= tw) {
         const Frag<3> f1 = split_tiles<3>(XD[0], XD[1]), f2 = split_tiles<3>(OD[0], OD[1]);
-        Frag<P> k[KH];
 #pragma unroll
-        for (int t = 0; t < KH; ++t) k[t] = sm.k.K.cols(d0 + 16 * t, j0, m);
-        mma_n<3>(k, f1, accK);
+        for (int t = 0; t < KH; t += KG) {
+          Frag<P> k[KG];
 #pragma unroll
-        for (int t = 0; t < KH; ++t) k[t] = sm.k.Q.cols(d0 + 16 * t, j0, m);
-        mma_n<3>(k, f2, accK);
+          for (int i = 0; i < KG; ++i) k[i] = sm.k.K.cols(d0 + 16 * (t + i), j0, m);
+          mma_n<3>(k, f1, accK + t);
+#pragma unroll
+          for (int i = 0; i < KG; ++i) k[i] = sm.k.Q.cols(d0 + 16 * (t + i), j0, m);
+          mma_n<3>(k, f2, accK + t);
+          if constexpr (KG < KH) phase();
+        }
       }
       phase();
     }
@@ -542,8 +635,10 @@ delta_grads_kernel(BwdArgs a) {
       for (int r = 0; r < 4; ++r) {
         ku = fmaf(accU[t][r], x[r], ku);
         accK[t][r] = fmaf(bi, accU[t][r], accK[t][r]);
-        kd = fmaf(accK[t][r], x[r], kd);
-        qd = fmaf(accQ[t][r], y[r], qd);
+        if constexpr (!GROUPED) {
+          kd = fmaf(accK[t][r], x[r], kd);
+          qd = fmaf(accQ[t][r], y[r], qd);
+        }
       }
       if constexpr (GROUPED) {
         sumQ[t] += accQ[t];
@@ -552,25 +647,36 @@ delta_grads_kernel(BwdArgs a) {
       phase();
     }
     ku = sum_g(ku) * rk;
-    kd = sum_g(kd) * rk;
-    qd = sum_g(qd) * rq;
     kh = sum_g(kh) * rk;
-    if (grp == 0) sDot[half][ti] = make_float4(ku, kd, qd, kh);
+    us = sum_g(us) * rk;
+    qs = sum_g(qs) * rq;
+    if constexpr (!GROUPED) {
+      kd = sum_g(kd) * rk;
+      qd = sum_g(qd) * rq;
+    }
+    if (grp == 0) {
+      sDot[0][half][ti] = ku;
+      sDot[1][half][ti] = kh;
+      sDot[2][half][ti] = fmaf(bi, us, qs);
+      if constexpr (!GROUPED) {
+        sDot[3][half][ti] = kd;
+        sDot[4][half][ti] = qd;
+      }
+    }
     __syncthreads();
-    if (wave == 0) {  // lane = token, the last one first
-      const int t = 63 - lane;
-      const float4 x = sDot[0][t], y = sDot[1][t];
-      double s = static_cast<double>(x.z + y.z) - (x.y + y.y) + 2.f * sBeta[t] * (x.x + y.x), all = x.w + y.w;
-      s = wave_scan(s);
-      all = __shfl(wave_scan(all), 63);
-      double sums = 0.0;
+    if (wave == 0) {  // lane = token
+      const auto both = [&](int which, int t) { return sDot[which][0][t] + sDot[which][1][t]; };
+      const double to = __shfl_up(wave_scan(both(1, lane)), 1), from = __shfl(wave_scan(both(2, 63 - lane)), 63 - lane);
+      double sums = 0.0, s = 0.0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) sums += sSe[i];
-      all += static_cast<double>(exp_diff(Gc)) * sums;
-      if (t < n) a.b.dg[(c.t0 + static_cast<int64_t>(t)) * g.HV + h] = static_cast<float>(s + all);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s += (i & 3) >= lane / 16 ? sPair[i][lane] : 0.f;  // (waves of tokens behind it)
+      s += from + (lane > 0 ? to : 0.0) + static_cast<double>(exp_diff(Gc)) * sums;
+      if (lane < n) a.b.dg[(c.t0 + static_cast<int64_t>(lane)) * g.HV + h] = below >> lane & 1 ? 0.f : static_cast<float>(s);
     }
     if (half == 0 && grp == 0 && mine) {
-      const float db = xv + ku + sDot[1][ti].x;
+      const float db = xv + ku + sDot[0][1][ti];
       const int64_t i = row_t * g.HV + h;
       if (g.beta_f32)
         static_cast<float*>(a.b.dbeta)[i] = db;
@@ -602,12 +708,14 @@ delta_grads_kernel(BwdArgs a) {
       kd = sum_g(kd) * rk;
       qd = sum_g(qd) * rq;
       __syncthreads();
-      if (grp == 0) sDot[half][ti] = make_float4(0.f, kd, qd, 0.f);
+      if (grp == 0) {
+        sDot[3][half][ti] = kd;
+        sDot[4][half][ti] = qd;
+      }
       __syncthreads();
     }
-    const float4 x = sDot[0][ti], y = sDot[1][ti];
-    kd = (x.y + y.y) * rk;
-    qd = (x.z + y.z) * rq;
+    kd = (sDot[3][0][ti] + sDot[3][1][ti]) * rk;
+    qd = (sDot[4][0][ti] + sDot[4][1][ti]) * rq;
   }
   if (!mine) return;
   const int64_t out = (row_t * g.HK + hk) * g.DK;
