@@ -544,7 +544,13 @@ __device__ __forceinline__ double log_decay(const DeltaGeom& g, const float* gp,
   }
   return wave_scan(s);
 }
-__device__ __forceinline__ float exp_diff(double x) { return fast_exp2(static_cast<float>(x * 1.4426950408889634)); }
+// exp of it: the whole part of the binary exponent is set apart in 64 bits, so that what the transcendental unit gets
+// has the digits of a number below 1 (rounded whole, exp(-16) would be off by 7e-7 of itself)
+__device__ __forceinline__ float exp_diff(double x) {
+  const double t = x * 1.4426950408889634;
+  const float n = rintf(__builtin_amdgcn_fmed3f(static_cast<float>(t), -1000.f, 1000.f));
+  return ldexpf(fast_exp2(static_cast<float>(t - n)), static_cast<int>(n));
+}
 
 template <typename T>
 __device__ __forceinline__ float load_beta(const DeltaGeom& g, const void* beta, int64_t t, int h) {

@@ -76,3 +76,22 @@ def test_gates_below_the_least(cuda, dtype, HK, DK):
     want, mag = _gates(_off(lens), **a, initial=init, do=do, dfinal=df)
     _, factor = ref.reference(_off(lens), **{**a, "g": a["g"].clamp(min=-1e4)}, qk_l2norm=True, initial=init)
     assert bool(((got.double() - want).abs() <= 80 * factor * mag)[:, 1].all())
+
+
+@pytest.mark.parametrize("tokens", [1, 64, 70])
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_decays_have_the_digits_of_their_type(cuda, dtype, tokens):
+    """Nothing is written (beta 0): states and their gradients are multiplied by the decay alone, of a chunk at a time.
+    An exponential is off by a unit of 2^-23, its argument's fraction by 2^-26, a product by 2^-24: less than 2^-22 a chunk."""
+    total = torch.tensor([-0.01, -1.0, -5.0, -16.0, -33.0, -60.0, -80.0])
+    S = len(total)
+    lens = [tokens] * S
+    a, init, do, df = _inputs(lens, 1, 2, 16, 24, TYPES[dtype], 43)
+    a["g"][:] = (total / tokens).repeat_interleave(tokens)[:, None]
+    a["beta"].zero_()
+    got = _call(cuda, lens, a, init, 0 * do, df)
+    decay = a["g"].double().view(S, tokens, 2).sum(1).exp()[:, :, None, None]
+    for name, x in (("final", init), ("dinitial", df)):
+        want = decay * x.double()
+        err = ((got[name].detach().double().cpu() - want) / want).abs()
+        assert float(err.max()) <= 2.0 ** -22 * -(-tokens // 64), f"{name}: off by {float(err.max()):.3g} of the value"
