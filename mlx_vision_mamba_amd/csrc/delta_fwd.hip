@@ -43,8 +43,7 @@ template <typename T, int DKP, int NW, bool VEC, bool SAVE, bool AGG>
 __global__ void __launch_bounds__(64 * NW)
 delta_fwd_kernel(FwdArgs a) {
   constexpr int P = kRawParts<T>, KT = DKP / 16, KS = DKP / 32, NT = 64 * NW;
-  constexpr int ORD = P == 3 ? 3 : 2;  // of what only the outputs see: bfloat16 keeps 8 bits of them
-  constexpr int PP = AGG ? 0 : ORD;
+  constexpr int PP = AGG ? 0 : kTriParts;
   __shared__ __attribute__((aligned(16))) Tile<kC, DKP, P> sK;
   __shared__ __attribute__((aligned(16))) Tile<AGG ? 1 : kC, DKP, P> sQ;
   // float32 values go straight to the registers: with them the tiles would not fit
@@ -186,7 +185,7 @@ delta_fwd_kernel(FwdArgs a) {
         }
       const Frag<3> sf = split_tiles<3>(S[2 * ks], S[2 * ks + 1]);
       mma_n<3>(fk[ks & 1], sf, R);
-      if constexpr (!AGG) mma_t<ORD>(sf, fq[ks & 1], O);
+      if constexpr (!AGG) mma_t<3>(sf, fq[ks & 1], O);
 #pragma unroll
       for (int i = 4 * ks / KS; i < 4 * (ks + 1) / KS; ++i) load(ahead, i);
       phase();
@@ -209,7 +208,7 @@ delta_fwd_kernel(FwdArgs a) {
     mma_n<3>(t0f, rf[0], D);
     load(ahead, 4);
     phase();
-    Frag<ORD> p0f[4], p1f[2];
+    Frag<3> p0f[4], p1f[2];
     float dout[4];  // (the outputs' tiles have the token in the column)
     if constexpr (!AGG) {
       tri_tiles<0>(p0f, sTri, 1, 0, m, grp);
@@ -225,13 +224,13 @@ delta_fwd_kernel(FwdArgs a) {
 #pragma unroll
     for (int rt = 0; rt < 4; ++rt) up[rt] = dec_at(sDec, kDecUp, rt, grp);
     if constexpr (!AGG) {
-      const Frag<ORD> df[2] = {split_tiles<ORD>(D[0], D[1]), split_tiles<ORD>(D[2], D[3])};
+      const Frag<3> df[2] = {split_tiles<3>(D[0], D[1]), split_tiles<3>(D[2], D[3])};
 #pragma unroll
       for (int rt = 0; rt < 4; ++rt) O[rt] *= dout[rt];
       tri_tiles<2>(p1f, sTri, 1, 1, m, grp);
-      mma_t<ORD>(df[0], p0f, O);
+      mma_t<3>(df[0], p0f, O);
       phase();
-      mma_t<ORD>(df[1], p1f, O + 2);
+      mma_t<3>(df[1], p1f, O + 2);
     }
     constexpr int KG = KT < 4 ? KT : 4;  // row tiles of the state at a time
     Frag<P> fc[2][KG];

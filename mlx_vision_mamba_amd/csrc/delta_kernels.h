@@ -73,8 +73,8 @@ constexpr int kTriFrags = 6;                   // of 16 rows and 32 columns that
 constexpr int kTriParts = 3;
 constexpr int kTriFragments = 2 * kTriFrags * kTriParts * 64;
 constexpr int64_t kTriBytes = int64_t{kTriFragments} * 16;
-// where lane 0's fragment f of part p of the which-th triangle lies: the leading parts of the second come first,
-// so that a pass that needs no more of them reads one run
+// where lane 0's fragment f of part p of the which-th triangle lies: the second triangle last, so that a pass that
+// does without it reads one run
 constexpr int tri_index(int which, int p, int f) { return ((which * kTriParts + p) * kTriFrags + f) * 64; }
 
 inline int delta_dkp(int dk) { return dk <= 32 ? 32 : (dk <= 64 ? 64 : 128); }
