@@ -32,7 +32,7 @@ def _split(split_len):
     split_len = int(split_len)
     if split_len < 0 or split_len % 64:
         raise ValueError(f"split_len must be 0 or a multiple of 64; got {split_len}")
-    return split_len
+    return min(split_len, 2 ** 31 - 64)  # (of 32 bits beyond this; no sequence is longer)
 
 
 def gated_delta_rule_packed(q, k, v, g, beta, offsets=None, *, scale=None, qk_l2norm=False, initial_states=None,
