@@ -4,7 +4,7 @@
 //
 // Rows (one position a sample: the heads of a mixer): a power of two of lanes
 // takes a group, all its values in registers, so that x is read once: mean,
-// then variance from the registers.  A wave keeps its groups and their weights
+// then variance and what the mean was off by from the registers.  A wave keeps its groups and their weights
 // and walks rows; the backward sums the channels' gradients in registers on the
 // way and leaves one partial row a workgroup.  16384 rows of 12 gated groups of
 // 128 in bfloat16: 35 us forward (151 MB, 4.3 TB/s), 48 backward (252 MB, 5.2).
@@ -77,10 +77,30 @@ struct GnLanes {
   uint32_t blocks;     // waves abreast over a row's groups
 };
 
+// A mean, near + off, and 1 / sqrt(var + eps)
+struct GnMoments {
+  float near, off, rstd;
+};
+// Of values whose differences from `near`, a number as close to their mean as its sum's rounding allows, have the mean
+// `off` and the mean square `sq`: that rounding is taken out of both moments
+__device__ __forceinline__ GnMoments moments_of(float near, float off, float sq, float eps) {
+  const float var = fmaf(-off, off, sq);
+  return {near, off, 1.f / sqrtf((var < 0.f ? 0.f : var) + eps)};  // (NaN stays)
+}
+
 template <int V>
 __device__ __forceinline__ float group_sum(float v, int log2) {
   for (int o = 0; o < log2; ++o) v += __shfl_xor(v, 1 << o);
   return v;
+}
+// of two values, whose exchanges do not wait for each other
+__device__ __forceinline__ float2 group_sums(float a, float b, int log2) {
+  for (int o = 0; o < log2; ++o) {
+    const float x = __shfl_xor(a, 1 << o), y = __shfl_xor(b, 1 << o);
+    a += x;
+    b += y;
+  }
+  return make_float2(a, b);
 }
 
 // The weights and biases of columns c .. c + V - 1.  (float32 of any alignment: the card's wide loads ask for 4 bytes)
@@ -139,17 +159,20 @@ gn_rows_fwd_kernel(GnGeom g, GnPtr p, GnLanes ln, T* __restrict__ y, float2* __r
 #pragma unroll
       for (int j = 0; j < V; ++j) s += v[i][j] = ok ? to_f32(x[i].v[j]) : 0.f;
     }
-    const float mean = group_sum<V>(s, ln.log2) * inv;
-    s = 0.f;
+    const float near = group_sum<V>(s, ln.log2) * inv;
+    float q = s = 0.f;
 #pragma unroll
     for (int i = 0; i < PER; ++i)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        v[i][j] -= mean;
-        s = (l + (i << ln.log2)) * V < g.Cg ? fmaf(v[i][j], v[i][j], s) : s;
+        v[i][j] -= near;
+        const bool in = (l + (i << ln.log2)) * V < g.Cg;
+        s += in ? v[i][j] : 0.f;
+        q = in ? fmaf(v[i][j], v[i][j], q) : q;
       }
-    const float rstd = 1.f / sqrtf(group_sum<V>(s, ln.log2) * inv + g.eps);
-    if (on && l == 0 && stats != nullptr) stats[n * g.G + grp] = make_float2(mean, rstd);
+    const float2 dev = group_sums(s, q, ln.log2);
+    const GnMoments mo = moments_of(near, dev.x * inv, dev.y * inv, g.eps);
+    if (on && l == 0 && stats != nullptr) stats[n * g.G + grp] = make_float2(near + mo.off, mo.rstd);
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int c = (l + (i << ln.log2)) * V;
@@ -158,7 +181,7 @@ gn_rows_fwd_kernel(GnGeom g, GnPtr p, GnLanes ln, T* __restrict__ y, float2* __r
         Pack<T, V> out;
 #pragma unroll
         for (int j = 0; j < V; ++j)
-          out.v[j] = from_f32<T>(gn_out<SILU, GATE>(fmaf(v[i][j] * rstd, wt.w[i][j], wt.b[i][j]), GATE ? to_f32(z[i].v[j]) : 0.f));
+          out.v[j] = from_f32<T>(gn_out<SILU, GATE>(fmaf((v[i][j] - mo.off) * mo.rstd, wt.w[i][j], wt.b[i][j]), GATE ? to_f32(z[i].v[j]) : 0.f));
         store_pack(y + n * g.C + c0 + c, out);
       }
     }
@@ -269,8 +292,6 @@ gn_reduce_kernel(const float* part, int64_t nparts, int32_t C, float* dw, float*
   });
 }
 
-// ------------------------------------------------------------------- maps
-
 // ------------------------------------------------------------------- reductions of a workgroup
 
 // The sums over a workgroup's rows of each of its columns, (1 << log2) lanes of V columns a row: every
@@ -352,17 +373,19 @@ gn_tile_fwd_kernel(GnGeom g, GnPtr p, int log2, T* __restrict__ y, float2* __res
   for (int i = 0; i < PER; ++i)
 #pragma unroll
     for (int j = 0; j < V; ++j) s += a.ok && a.ri + i * a.RI < P ? to_f32(x[i].v[j]) : 0.f;
-  const float mean = workgroup_sum(s, 0.f, lds).x * inv;
-  s = 0.f;
+  const float near = workgroup_sum(s, 0.f, lds).x * inv;
+  float q = s = 0.f;
 #pragma unroll
   for (int i = 0; i < PER; ++i)
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const float d = a.ok && a.ri + i * a.RI < P ? to_f32(x[i].v[j]) - mean : 0.f;
-      s = fmaf(d, d, s);
+      const float d = a.ok && a.ri + i * a.RI < P ? to_f32(x[i].v[j]) - near : 0.f;
+      s += d;
+      q = fmaf(d, d, q);
     }
-  const float rstd = 1.f / sqrtf(workgroup_sum(s, 0.f, lds).x * inv + g.eps);
-  if (threadIdx.x == 0 && stats != nullptr) stats[a.n * g.G + a.grp] = make_float2(mean, rstd);
+  const float2 dev = workgroup_sum(s, q, lds);
+  const GnMoments mo = moments_of(near, dev.x * inv, dev.y * inv, g.eps);
+  if (threadIdx.x == 0 && stats != nullptr) stats[a.n * g.G + a.grp] = make_float2(near + mo.off, mo.rstd);
   T* yp = y + a.n * g.P * g.C + a.c;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
@@ -371,7 +394,7 @@ gn_tile_fwd_kernel(GnGeom g, GnPtr p, int log2, T* __restrict__ y, float2* __res
       Pack<T, V> out;
 #pragma unroll
       for (int j = 0; j < V; ++j)
-        out.v[j] = from_f32<T>(gn_out<SILU, GATE>(fmaf((to_f32(x[i].v[j]) - mean) * rstd, w[j], b[j]), GATE ? to_f32(z[i].v[j]) : 0.f));
+        out.v[j] = from_f32<T>(gn_out<SILU, GATE>(fmaf((to_f32(x[i].v[j]) - near - mo.off) * mo.rstd, w[j], b[j]), GATE ? to_f32(z[i].v[j]) : 0.f));
       store_pack(yp + static_cast<int64_t>(t) * g.C, out);
     }
   }
@@ -484,11 +507,15 @@ __device__ __forceinline__ GnAt gn_at(const GnGeom& g, const GnRun& r) {
   return a;
 }
 
-// Every channel's mean and sum of squared differences over a run.  Sums are taken around the mean of the run's first
-// rows, one for all threads, so that they add up without a division
+// A channel's values over a run: a number near their mean, what it is off by, and their squared differences' sum.  (The
+// mean as one float would have its rounding in it, of which a far mean's differences have few units.)
+struct GnPart {
+  float near, off, sq;
+};
+// Sums are taken around the mean of the run's first rows, one for all threads, so that they add up without a division
 template <typename T, int V>
 __global__ void __launch_bounds__(256)
-gn_stats_kernel(GnGeom g, GnPtr p, GnRun r, float2* __restrict__ part) {
+gn_stats_kernel(GnGeom g, GnPtr p, GnRun r, GnPart* __restrict__ part) {
   __shared__ float lds[4][64][V];
   const GnAt a = gn_at<V>(g, r);
   const bool ok = a.c < g.C;
@@ -530,7 +557,7 @@ gn_stats_kernel(GnGeom g, GnPtr p, GnRun r, float2* __restrict__ part) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const float m = s[j] * inv;
-      part[(a.n * r.runs + a.run) * g.C + a.c + j] = make_float2(piv[j] + m, fmaxf(q[j] - s[j] * m, 0.f));
+      part[(a.n * r.runs + a.run) * g.C + a.c + j] = {piv[j], m, fmaxf(q[j] - s[j] * m, 0.f)};
     }
 }
 
@@ -548,10 +575,11 @@ __device__ __forceinline__ double team_sum(double x, double* lds) {
   return x;
 }
 
-// W waves a group and sample (one, or the workgroup's four): its channels' partial statistics as one
+// W waves a group and sample (one, or the workgroup's four): its channels' partial statistics as one, for the backward
+// (unless NULL) and for the forward's last pass
 template <int W>
 __global__ void __launch_bounds__(256)
-gn_join_kernel(GnGeom g, GnRun r, const float2* __restrict__ part, float2* __restrict__ stats) {
+gn_join_kernel(GnGeom g, GnRun r, const GnPart* __restrict__ part, float2* __restrict__ stats, GnMoments* __restrict__ out) {
   __shared__ double lds[4];
   const int64_t item = static_cast<int64_t>(blockIdx.x) * (4 / W) + (W == 1 ? threadIdx.x >> 6 : 0);
   if (item >= g.N * g.G) return;  // (of four waves: all or none)
@@ -560,7 +588,7 @@ gn_join_kernel(GnGeom g, GnRun r, const float2* __restrict__ part, float2* __res
   // the mean of the means, then the squares around it
   const auto each = [&](auto f) {
     for (int i = threadIdx.x & (64 * W - 1); i < total; i += 256 * W) {
-      float2 v[4];
+      GnPart v[4];
       float cnt[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -575,29 +603,32 @@ gn_join_kernel(GnGeom g, GnRun r, const float2* __restrict__ part, float2* __res
   };
   const double count = static_cast<double>(g.P) * g.Cg;
   double m = 0.0, q = 0.0;
-  each([&](float2 v, float cnt) { m += static_cast<double>(v.x) * cnt; });
+  each([&](const GnPart& v, float cnt) { m += (static_cast<double>(v.near) + v.off) * cnt; });
   m = team_sum<W>(m, lds) / count;
-  each([&](float2 v, float cnt) {
-    const double d = v.x - m;
-    q += cnt > 0.f ? v.y + d * d * cnt : 0.0;
+  each([&](const GnPart& v, float cnt) {
+    const double d = v.near - m + v.off;
+    q += cnt > 0.f ? v.sq + d * d * cnt : 0.0;
   });
   q = team_sum<W>(q, lds) / count;
-  if ((threadIdx.x & (64 * W - 1)) == 0)
-    stats[item] = make_float2(static_cast<float>(m), static_cast<float>(1.0 / sqrt(q + g.eps)));
+  if ((threadIdx.x & (64 * W - 1)) == 0) {
+    const float mean = static_cast<float>(m), rstd = static_cast<float>(1.0 / sqrt(q + g.eps));
+    out[item] = {mean, static_cast<float>(m - mean), rstd};
+    if (stats != nullptr) stats[item] = make_float2(mean, rstd);
+  }
 }
 
 template <typename T, int V, bool SILU, bool GATE>
 __global__ void __launch_bounds__(256)
-gn_apply_kernel(GnGeom g, GnPtr p, GnRun r, const float2* __restrict__ stats, T* __restrict__ y) {
+gn_apply_kernel(GnGeom g, GnPtr p, GnRun r, const GnMoments* __restrict__ moments, T* __restrict__ y) {
   const GnAt a = gn_at<V>(g, r);
   if (a.c >= g.C) return;
   float mean[V], sc[V], b[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    const float2 st = stats[a.n * g.G + (a.c + j) / g.Cg];
-    mean[j] = st.x;
-    sc[j] = st.y * (p.w != nullptr ? p.w[a.c + j] : 1.f);
-    b[j] = p.b != nullptr ? p.b[a.c + j] : 0.f;
+    const GnMoments mo = moments[a.n * g.G + (a.c + j) / g.Cg];
+    mean[j] = mo.near;
+    sc[j] = mo.rstd * (p.w != nullptr ? p.w[a.c + j] : 1.f);
+    b[j] = fmaf(-mo.off, sc[j], p.b != nullptr ? p.b[a.c + j] : 0.f);
   }
   for (int64_t t0 = a.p0 + a.ri; t0 < a.p1; t0 += kAhead * a.RI) {
     Pack<T, V> x[kAhead], z[kAhead];
@@ -867,10 +898,10 @@ GnWs ws_of(const GnGeom& g, bool backward) {
     if (by_rows(g))
       part = backward ? static_cast<size_t>(row_blocks(g, lanes_of(g, V))) * row : 0;
     else
-      part = static_cast<size_t>(g.N) * run_of(g, V).runs * row;
+      part = static_cast<size_t>(g.N) * run_of(g, V).runs * (backward ? row : static_cast<size_t>(g.C) * sizeof(GnPart));
     w.part = std::max(w.part, align_up(part));
   }
-  w.stats = by_rows(g) ? 0 : align_up(static_cast<size_t>(g.N) * g.G * 8);
+  w.stats = by_rows(g) ? 0 : align_up(static_cast<size_t>(g.N) * g.G * (backward ? 8 : sizeof(GnMoments)));
   w.total = w.part + w.stats;
   return w;
 }
@@ -979,16 +1010,15 @@ int mvm_group_norm_fwd(const mvm_group_norm_desc* desc, const void* x, const flo
         });
     const GnRun r = run_of(g, V);
     const dim3 grid(static_cast<unsigned>(g.N * r.runs * r.cblocks));
-    float2* part = static_cast<float2*>(workspace);
-    float2* st = stats != nullptr ? reinterpret_cast<float2*>(stats)
-                                  : reinterpret_cast<float2*>(static_cast<char*>(workspace) + w.part);
+    GnPart* part = static_cast<GnPart*>(workspace);
+    GnMoments* mo = reinterpret_cast<GnMoments*>(static_cast<char*>(workspace) + w.part);
     hipLaunchKernelGGL((gn_stats_kernel<T, V>), grid, dim3(256), 0, s, g, p, r, part);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(wide_join(g, r) ? gn_join_kernel<4> : gn_join_kernel<1>, dim3(join_blocks(g, r)), dim3(256), 0, s, g, r,
-                       part, st);
+                       part, reinterpret_cast<float2*>(stats), mo);
     if ((e = hipGetLastError()) != hipSuccess) return e;
-    hipLaunchKernelGGL((gn_apply_kernel<T, V, SILU, GATE>), grid, dim3(256), 0, s, g, p, r, st, static_cast<T*>(y));
+    hipLaunchKernelGGL((gn_apply_kernel<T, V, SILU, GATE>), grid, dim3(256), 0, s, g, p, r, mo, static_cast<T*>(y));
     return hipGetLastError();
   });
   return hip_status(e, "mvm_group_norm_fwd launch");
