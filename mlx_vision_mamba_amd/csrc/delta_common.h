@@ -414,8 +414,10 @@ __device__ __forceinline__ f32x4 load4(const T* p, int c, int n, bool vec) {
   return v;
 }
 
-// 1 where sequence i starts from the state in row `row` of `states`, else 0.  (A scalar that selects by a product:
-// with conditions, of which one comes from a vector load, this toolchain lost a value on one of their paths.)
+// 1 where sequence i starts from the state in row `row` of `states`, else 0, for its users to multiply by.  (As `states
+// && row >= 0 && (!fresh || !fresh[i]) ? rows : 0` this toolchain leaves the copy of `rows` out of the edge behind the
+// load: a zero from before the conditions stays, and with flags no state is read.  A value that is set on both of that
+// condition's edges, as the mask in delta_step.hip, is not touched by it.)
 __device__ __forceinline__ int32_t seq_starts(const SeqGeom& g, int32_t i, int32_t row, const float* states) {
   const int32_t fresh = g.fresh != nullptr ? g.fresh[i] : 0;
   return (states != nullptr) & (row >= 0) & (__builtin_amdgcn_readfirstlane(fresh) == 0);
