@@ -219,6 +219,7 @@ struct ScanFn : Function<ScanFn> {
     return in_backward([&] { return grads(ctx, g); });
   }
   static variable_list grads(AutogradContext* ctx, const variable_list& g) {
+    check_captured_edges(g[0], "the selective scan");
     const auto sv = ctx->get_saved_variables();
     const bool flat = ctx->saved_data["flat"].toBool();
     const int64_t od = ctx->saved_data["out"].toInt();
@@ -475,6 +476,7 @@ struct ConvFn : Function<ConvFn> {
     return in_backward([&] { return grads(ctx, g); });
   }
   static variable_list grads(AutogradContext* ctx, const variable_list& g) {
+    check_captured_edges(g[0], "the causal conv");
     const auto sv = ctx->get_saved_variables();
     variable_list out;
     {
@@ -527,6 +529,7 @@ struct NormFn : Function<NormFn> {
   static variable_list grads(AutogradContext* ctx, const variable_list& g) {
     at::NoGradGuard no_grad;
     const auto sv = ctx->get_saved_variables();
+    check_captured_edges(sv[0], "the LayerNorm");
     const Tensor &x2 = sv[0], &w = sv[1];
     const int64_t R = x2.size(0), E = x2.size(1);
     const Tensor dy = g[0].reshape({R, E}).to(at::kFloat).contiguous();
@@ -651,6 +654,7 @@ struct InProjFn : Function<InProjFn> {
     return in_backward([&] { return grads(ctx, g); });
   }
   static variable_list grads(AutogradContext* ctx, const variable_list& g) {
+    check_captured_edges(g[0], "in_proj");
     const auto sv = ctx->get_saved_variables();
     const Tensor& W = sv[1];
     const int64_t O = W.size(0), E = W.size(1);
@@ -707,6 +711,7 @@ struct OutProjFn : Function<OutProjFn> {
     return in_backward([&] { return grads(ctx, g); });
   }
   static variable_list grads(AutogradContext* ctx, const variable_list& g) {
+    check_captured_edges(g[0], "out_proj");
     const auto sv = ctx->get_saved_variables();
     const Tensor& W = sv[1];
     const int64_t K = W.size(0), E = W.size(1), D = W.size(2);
@@ -782,7 +787,12 @@ struct DirectionParamsFn : Function<DirectionParamsFn> {
     for (const Tensor& b : bufs) out.push_back(b.view_as(b));
     return out;
   }
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    return in_backward([&] { return grads(ctx, g); });
+  }
+  static variable_list grads(AutogradContext* ctx, const variable_list& grads) {
+    for (const Tensor& g : grads)
+      if (g.defined()) check_captured_edges(g, "the directions' parameters");
     const int64_t nbuf = ctx->saved_data["nbuf"].toInt(), K = ctx->saved_data["K"].toInt();
     variable_list out(nbuf);
     for (const Tensor& g : grads) {
@@ -886,6 +896,7 @@ struct CoreFn : Function<CoreFn> {
     return in_backward([&] { return once_differentiable(grads(ctx, g), g, "the Mamba block's core"); });
   }
   static variable_list grads(AutogradContext* ctx, const variable_list& grads) {
+    check_captured_edges(grads[0], "the Mamba block's core");
     const auto sv = ctx->get_saved_variables();
     // refused at once, except where dt_proj is frozen: there the first
     // derivative was always given, and once_differentiable refuses the second

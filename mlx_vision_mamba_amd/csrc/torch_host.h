@@ -6,11 +6,13 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/extension.h>
 
 #include <algorithm>
 #include <initializer_list>
 #include <string>
+#include <unordered_set>
 #include <vector>
 
 #include "mvm_scan.h"
@@ -103,11 +105,11 @@ bool is_capturing(void* stream) {
          status == hipStreamCaptureStatusActive;
 }
 
-// In a Function's backward: while it is captured into a graph, what takes its gradients must be part of the capture or
-// join it.  A leaf's gradient accumulator, which an eager graph of the same leaf keeps alive, runs on the stream that
-// it was made on; the engine draws that stream into the capture, and waits for it again only where the accumulator
-// runs (backward(), not grad()).  The null stream cannot be drawn into one.  Either ends the process when the capture
-// ends: refused here.
+// In a Function's backward: while it is captured into a graph, what takes gradients from it, directly or through other
+// nodes, must be part of the capture or join it.  A leaf's gradient accumulator, which an eager graph of the same leaf
+// keeps alive, runs on the stream that it was made on; the engine draws that stream into the capture, and waits for it
+// again only where the accumulator runs (backward(), not grad()).  The null stream cannot be drawn into one.  Either
+// ends the process when the capture ends: refused here.
 void check_captured_edges(const Tensor& like, const char* what) {
   if (!is_capturing(stream_of(like))) return;
   const auto node = torch::autograd::get_current_node();
@@ -115,15 +117,31 @@ void check_captured_edges(const Tensor& like, const char* what) {
   const c10::Stream here = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(like.device().index()).unwrap();
   const auto* exec = torch::autograd::get_current_graph_task_exec_info();
   const bool accumulates = exec == nullptr || exec->empty();
-  for (size_t i = 0; i < node->num_outputs(); ++i) {
-    const auto& next = node->next_edge(i).function;
-    if (next == nullptr || !node->task_should_compute_output(i)) continue;
-    const auto s = next->stream();
-    if (!s.has_value() || *s == here || s->device() != here.device()) continue;
-    void* const other = c10::hip::HIPStreamMasqueradingAsCUDA(*s).stream();
-    if (is_capturing(other) || (other != nullptr && accumulates)) continue;
-    throw std::runtime_error(std::string("the backward of ") + what + " is captured into a graph, but an eager graph of "
-                             "its inputs is alive on another stream: delete that graph's outputs before the capture");
+  std::vector<const torch::autograd::Node*> todo{node.get()};
+  std::unordered_set<const torch::autograd::Node*> seen{node.get()};
+  while (!todo.empty()) {
+    const auto* from = todo.back();
+    todo.pop_back();
+    for (const auto& edge : from->next_edges()) {
+      torch::autograd::Node* next = edge.function.get();
+      if (next == nullptr || !seen.insert(next).second) continue;
+      bool runs = true;  // (else its gradient is handed out in front of it, or not asked for)
+      if (!accumulates) {
+        const auto info = exec->find(next);
+        if (info == exec->end() || !info->second.should_execute()) continue;
+        runs = info->second.needed_;
+      }
+      const auto s = next->stream();
+      if (s.has_value() && *s != here && s->device() == here.device()) {
+        void* const other = c10::hip::HIPStreamMasqueradingAsCUDA(*s).stream();
+        const bool waited_for = accumulates || (runs && next->num_outputs() > 0);
+        if (!is_capturing(other) && (other == nullptr || !waited_for))
+          throw std::runtime_error(std::string("the backward of ") + what + " is captured into a graph, but an eager graph "
+                                   "of its inputs is alive on another stream: delete that graph's outputs before the "
+                                   "capture");
+      }
+      if (runs) todo.push_back(next);
+    }
   }
 }
 

@@ -197,6 +197,7 @@ struct SeqScanFn : Function<SeqScanFn> {
     {
       at::NoGradGuard no_grad;
       const Tensor &u = sv[0], &delta = sv[1], &A = sv[2], &z = sv[6], &dbias = sv[7], &off = sv[9];
+      check_captured_edges(u, "the packed selective scan");
       const Seqs q = seqs_of("u", u, off);
       SeqScanArgs a = scan_args(q, u, delta, A, sv[3], sv[4], sv[5], z, dbias,
                                 {fl[0] != 0, fl[1] != 0, fl[2], fl[3]});
@@ -335,6 +336,7 @@ struct SeqConvFn : Function<SeqConvFn> {
     {
       at::NoGradGuard no_grad;
       const Tensor &x = sv[0], &w = sv[1], &b = sv[2], &off = sv[4];
+      check_captured_edges(x, "the packed causal conv");
       const Seqs q = seqs_of("x", x, off);
       SeqConvArgs a = conv_args(q, x, w, b);
       a.d.seq = seq_desc(q, q.nseq, Tensor(), Tensor());
