@@ -24,7 +24,8 @@
  *   gradients are contiguous.  States: (rows, value_heads, dk, dv) float32.
  *   Strides are at most 2^29 - 1 values, v_stride and value_heads * dv 2^25.
  *
- * g is taken as at least -10000 (exp of which is 0).  Products run over chunks
+ * g is taken as at least -10000 (exp of which is 0), below which its gradient
+ * is zero.  Products run over chunks
  * of 64 tokens: a value that is not finite makes its sequence's outputs
  * meaningless from the start of its chunk on, no other sequence's.
  */
@@ -66,11 +67,15 @@ typedef struct mvm_delta_desc {
 int mvm_delta_validate(const mvm_delta_desc* desc);
 
 /* float32 elements of the checkpoints that a forward leaves for a backward:
- * each chunk's initial state, the rows d_t, the chunk's triangles and decays. */
+ * each chunk's initial state, the rows d_t, the chunk's triangles and decays.
+ * (A head of 128 x 128: 2.1 KiB a token, about twice its q, k, v and o in
+ * bfloat16.) */
 int64_t mvm_delta_ckpt_elems(const mvm_delta_desc* desc);
 
-/* Workspace bytes: which = 0 forward, 1 backward.  The workspace must be
- * 256-byte aligned, the checkpoints 16-byte. */
+/* Workspace bytes: which = 0 forward, with or without checkpoints, 1 backward.
+ * The workspace must be 256-byte aligned, the checkpoints 16-byte.  (A head of
+ * 128 x 128: 0.6 KiB a token forward, 1.5 backward, and what the parts of the
+ * time axis leave each other.) */
 int64_t mvm_delta_workspace_bytes(const mvm_delta_desc* desc, int which);
 
 /* h0 (zero), h1 (not stored) and ckpt (no backward) may be NULL; h0 and h1 may

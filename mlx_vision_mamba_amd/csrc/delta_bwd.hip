@@ -8,7 +8,7 @@
 //   dS = e^Gc E + Q' diag(e^G) dO' - K' diag(beta e^G) X
 // the same chain of products as the forward's, with a wave keeping 16 columns
 // of E in registers.  It leaves X and every chunk's E.  (16384 tokens of 12 heads of
-// 128 x 128 in bfloat16: 137 us, as bound as the forward's.)
+// 128 x 128 in bfloat16: 136 us, as bound as the forward's.)
 //
 // Then every chunk and key head by itself (delta_grads_kernel), with M_ij =
 // exp(G_i - G_j):
@@ -301,8 +301,10 @@ __device__ __forceinline__ f32x4 pairs_across(const f32x4& W, float& before, int
 
 // Eight waves a chunk and key head: a wave has 16 tokens and half of the keys' columns; the small triangles of its
 // tokens are formed by both waves.  GROUPED: more than one value head a key head.
-// Bound by waits and issue: 16384 tokens of 12 heads of 128 x 128 in bfloat16 take 381 us, MFMA busy 23 %, and two waves
-// a SIMD that wait 45 % of their cycles; their 256 registers leave no room for a second workgroup.
+// Bound by waits and issue: 16384 tokens of 12 heads of 128 x 128 in bfloat16 take 416 us, MFMA busy 21 %, and two waves
+// a SIMD that wait 46 % of their cycles; their 256 registers leave no room for a second workgroup.  With keys shared, and
+// in float32, heads of more than 64 key values spill 116 to 340 bytes a lane, nearly all of it once a head, outside the
+// loop over the values' columns.
 template <typename T, int DKP, bool VEC, bool GROUPED>
 __global__ void __launch_bounds__(512)
 delta_grads_kernel(BwdArgs a) {

@@ -53,8 +53,8 @@ int check_stride(const char* name, int64_t stride) {
 // heads of bfloat16): a workgroup a compute unit, so passes take whole rounds of
 // them; a chunk of the parts' pass takes 0.7, a part's joining 0.2 to 0.75.
 // Measured on MI355X with 12 such heads, us forward whole / in parts: one
-// sequence of 32768 tokens 2986 / 640, of 8192 750 / 330; 6 of 2730 314 / 343; 16
-// of 512 95 / 177.
+// sequence of 32768 tokens 3122 / 588, of 8192 793 / 218; 6 of 2730 333 / 317; 16
+// of 512 96 / 162.
 constexpr int64_t kUnits = 256;
 
 void pick_parts(const mvm_delta_desc* d, mvm::DeltaGeom& g) {
@@ -83,8 +83,8 @@ void pick_parts(const mvm_delta_desc* d, mvm::DeltaGeom& g) {
 }
 
 // Waves of a workgroup of the passes along time: eight share a chunk's operands where the state has columns for them
-// and the card is full of them (bfloat16, 8191 tokens of 12 heads of 128 x 128: 122 us forward, 134 by four; but 2048
-// tokens of 4 heads 80, and 74 by four, whose chunks take less long).  Float32 operands are three parts, of which
+// and the card is full of them (bfloat16, 8191 tokens in 23 prompts of 12 heads of 128 x 128: 134 us, 141 by four; but 2048
+// tokens of 4 heads 100, and 91 by four, whose chunks take less long).  Float32 operands are three parts, of which
 // eight waves' registers spill (16384 tokens of 12 heads: 568 us forward, 354 by four).
 int pick_waves(const mvm_delta_desc* d, const mvm::DeltaGeom& g) {
   const int64_t items = (d->seq.tokens / mvm::kDeltaChunk + d->seq.nseq) * g.HV;

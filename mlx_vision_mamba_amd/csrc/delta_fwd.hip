@@ -15,8 +15,8 @@
 // the main pass starts each part from its own state.
 //
 // Bound by the chain of products of a chunk, 5.5-7 us for bfloat16 heads of 128 x
-// 128: 32768 tokens of 12 heads take 187 us in the main pass, MFMA busy 37 % with
-// two waves a SIMD, which wait to issue 42 % of their cycles.  Operands are read a
+// 128: 32768 tokens of 12 heads take 190 us in the main pass, MFMA busy 42 % with
+// two waves a SIMD, which wait to issue 41 % of their cycles.  Operands are read a
 // phase ahead and the next chunk's loads are spread over the phases: all at its
 // start took a quarter longer.
 #include "delta_common.h"

@@ -7,11 +7,11 @@
 // then variance and what the mean was off by from the registers.  A wave keeps its groups and their weights
 // and walks rows; the backward sums the channels' gradients in registers on the
 // way and leaves one partial row a workgroup.  16384 rows of 12 gated groups of
-// 128 in bfloat16: 35 us forward (151 MB, 4.3 TB/s), 48 backward (252 MB, 5.2).
+// 128 in bfloat16: 33 us forward (151 MB, 4.6 TB/s), 49 backward (252 MB, 5.2).
 //
 // Tiles (a sample's group of up to 8 16-byte accesses a thread): a workgroup
 // holds it, one launch a direction; 32 samples of 196 x 384 in 32 groups, float32:
-// 8 us forward, 12 backward, of which 5 are launch and first loads.
+// 7 us forward, 11 backward, of which 5 are launch and first loads.
 //
 // Maps: the values of a group do not fit, so x is read twice, the second time
 // from the last-level cache where it fits there.  One pass leaves every
@@ -20,7 +20,7 @@
 // around a mean of the run itself, and joined as mean and squares (Chan, Golub
 // and LeVeque, "Algorithms for computing the sample variance", 1983): a mean
 // far from zero costs no digits.  The backward has the same three passes, of the
-// sums of dn and dn xh.  4 maps of 50176 x 128 in bfloat16: 15 + 6 + 26 us, the
+// sums of dn and dn xh.  4 maps of 50176 x 128 in bfloat16: 14 + 6 + 26 us, the
 // last at 4.0 TB/s of reads from the cache and writes to memory.
 //
 // Statistics and sums are float32, those over runs float64; each output is
@@ -769,8 +769,8 @@ constexpr int64_t kMaxRows = int64_t{1} << 31;
 constexpr int64_t kMaxBlocks = (int64_t{1} << 24) - 8;  // of 256 threads, 2^32 a launch
 constexpr int kRowValues = 2048;        // of a group, held in registers by 64 lanes
 // waves that walk the rows forward: more of them load the weights more often, fewer leave loads unhidden (16384 rows of
-// 12 heads of 128: 1024 86 us, 2048 52, 4096 40, 16384 50, all with weights in 4-byte loads; 35 now); four times as
-// many where values come one by one (16384 rows of 1530: 36 us against 48)
+// 12 heads of 128: 1024 86 us, 2048 52, 4096 40, 16384 50, all with weights in 4-byte loads; 33 now); four times as
+// many where values come one by one (16384 rows of 1530 in 10 groups: 54 us against 67; in one, 117 against 103)
 constexpr int64_t kRowWaves = 4096;
 constexpr int64_t kTileRows = 8;        // of a thread, held in registers
 constexpr int64_t kPartRows = 512;      // partial rows of the channels' gradients
@@ -828,10 +828,9 @@ int64_t row_blocks(const GnGeom& g, const GnLanes& l) {
   return std::max<int64_t>(1, std::min(ceil_div(g.N, 4), std::max<int64_t>(1, kPartRows * 4 / l.blocks)));
 }
 
-// (32 samples of 196 x 384 in 32 groups, gated: 9.4 us forward and 16 backward against 15 and 28 in passes; 256 of them
-// 41 and 129 against 65 and 133)
 // A group in a workgroup's registers, for accesses of V values that groups start on: log2 of the lanes of a row and
-// the rows of a thread, 0 where it does not fit
+// the rows of a thread, 0 where it does not fit.  (32 samples of 196 x 384 in 32 groups, gated: 9.4 us forward and 14
+// backward, against 17 and 23 in passes; 256 of them 60 and 104, against 66 and 116)
 struct GnTile {
   int32_t log2 = 0, per = 0;
 };
@@ -1063,7 +1062,7 @@ int mvm_group_norm_bwd(const mvm_group_norm_desc* desc, const void* x, const flo
       if constexpr (V > 1)
         if (const GnTile t = tile_of(g, V); t.per > 0 && !(g.Cg == V && g.N * g.G > 8192)) {
           // (many groups of 16 bytes a row would take their lines several times: 1024 samples of 64 x 64 in 16 groups
-          // 58 us against 39 in passes; 8 of 1024 x 256 in 32 groups 14 against 22)
+          // 59 us against 28 in passes; 8 of 1024 x 256 in 32 groups 11 against 17)
           nparts = g.N;
           return with_tile(t, [&](auto per) {
             hipLaunchKernelGGL((gn_tile_bwd_kernel<T, V, decltype(per)::value, SILU, GATE>),

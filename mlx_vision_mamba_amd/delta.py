@@ -53,7 +53,9 @@ def gated_delta_rule_packed(q, k, v, g, beta, offsets=None, *, scale=None, qk_l2
     ``scale``: default D_k ** -0.5.  ``qk_l2norm``: q and k are first divided by
     sqrt(sum of squares + 1e-6).  initial_states (default zero) and
     final_states: (S, H_v, D_k, D_v), float32.  Gradients reach every argument,
-    final_states' gradient included; second derivatives are refused.
+    final_states' gradient included (g's is zero below -10000); second derivatives
+    are refused.  A call with gradients keeps, a token and value head, 2.1 KiB for
+    128 x 128 heads (the chunks' states) until its backward, which takes 1.5 to 1.8 more.
     ``max_len``: an upper bound of the lengths where the caller knows one; only
     the split over the time axis goes by it.  ``split_len``: 0, or a multiple of
     64 to set that split.  Values must be finite: one that is not makes its
