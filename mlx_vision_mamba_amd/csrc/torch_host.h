@@ -111,7 +111,7 @@ bool is_capturing(void* stream) {
 // again only where the accumulator runs (backward(), not grad()).  The null stream cannot be drawn into one.  Either
 // ends the process when the capture ends: refused here.
 void check_captured_edges(const Tensor& like, const char* what) {
-  if (!is_capturing(stream_of(like))) return;
+  if (!like.is_cuda() || !is_capturing(stream_of(like))) return;
   const auto node = torch::autograd::get_current_node();
   if (node == nullptr) return;
   const c10::Stream here = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(like.device().index()).unwrap();
